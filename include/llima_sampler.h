@@ -92,7 +92,7 @@ enum {
     LLIMA_E_CAPTURE = -6     /* a first call on a device made under stream capture */
 };
 
-enum { LLIMA_F32 = 0, LLIMA_BF16 = 1 };
+enum { LLIMA_F32 = 0, LLIMA_BF16 = 1, LLIMA_F16 = 2 /* norm and attention only */ };
 
 /* OR'ed into the LM head's logit_dtype together with LLIMA_BF16: out_logits
  * then points to bf16 [B][V] (uint16 bits) and receives each logit as the
@@ -419,6 +419,81 @@ int llima_lm_head_verify_tree_packed(const void* hidden, const void* packed, int
                                      const int32_t* retrieve_indices, const int32_t* candidates,
                                      int32_t n_paths, int32_t L, int32_t* out, void* workspace,
                                      size_t workspace_bytes, void* stream);
+
+/* The LM head over an 8-bit weight: values in e4m3 (OCP, largest 448) with an
+ * fp32 scale per block of 128.  No counterpart in the reference.
+ *
+ *   hidden  e4m3 [B][H],  hidden_scales fp32 [B][ceil(H/128)]
+ *   weight  e4m3 [V][H],  weight_scales fp32 [ceil(V/128)][ceil(H/128)]
+ *   sum[b][v] = sum over blocks kb of hidden_scales[b][kb] weight_scales[v/128][kb]
+ *               * sum over the block's k of hidden[b][k] weight[v][k]
+ *
+ * (fp32 products and sums), then everything as the entry points over a bf16
+ * weight: softcap, logit_dtype rounding, LLIMA_LOGITS_OUT_BF16, ids, values and
+ * logits (argmax), log-likelihoods (score), chain and tree verification.  A NaN
+ * value or scale makes the logits it enters NaN, which never win.  H is a
+ * multiple of 64, at most 65536; hidden and weight are 16-byte aligned.  B = 0
+ * launches nothing.  Batches above 128 rows go in passes.
+ * llima_add_rms_norm and llima_quantize_rows make the hidden rows,
+ * llima_lm_head_quantize the weight (or a checkpoint that stores it so). */
+size_t llima_lm_head_argmax_fp8_workspace_bytes(int32_t B, int32_t V);
+int llima_lm_head_argmax_fp8(const void* hidden, const float* hidden_scales, const void* weight,
+                             const float* weight_scales, int32_t B, int32_t H, int32_t V,
+                             float softcap, int32_t logit_dtype, int32_t* out_ids,
+                             float* out_vals, float* out_logits, void* workspace,
+                             size_t workspace_bytes, void* stream);
+size_t llima_lm_head_score_fp8_workspace_bytes(int32_t B, int32_t V);
+int llima_lm_head_score_fp8(const void* hidden, const float* hidden_scales, const void* weight,
+                            const float* weight_scales, int32_t B, int32_t H, int32_t V,
+                            float softcap, int32_t logit_dtype, const int32_t* targets,
+                            double* out_logprob, int32_t* out_is_greedy, void* workspace,
+                            size_t workspace_bytes, void* stream);
+size_t llima_lm_head_verify_greedy_fp8_workspace_bytes(int32_t B, int32_t D, int32_t V);
+int llima_lm_head_verify_greedy_fp8(const void* hidden, const float* hidden_scales,
+                                    const void* weight, const float* weight_scales, int32_t B,
+                                    int32_t D, int32_t H, int32_t V, float softcap,
+                                    int32_t logit_dtype, const int32_t* draft_ids,
+                                    int32_t* accepted_len, int32_t* emitted, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+size_t llima_lm_head_verify_tree_fp8_workspace_bytes(int32_t K, int32_t V);
+int llima_lm_head_verify_tree_fp8(const void* hidden, const float* hidden_scales,
+                                  const void* weight, const float* weight_scales, int32_t K,
+                                  int32_t H, int32_t V, float softcap, int32_t logit_dtype,
+                                  const int32_t* retrieve_indices, const int32_t* candidates,
+                                  int32_t n_paths, int32_t L, int32_t* out, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* An LM head weight bf16 [V][H] in 8 bits: per block of 128 x 128,
+ * m = max(max |w|, 2^-100), the scale m / 448 and the values e4m3(448 w / m)
+ * (to nearest, ties to even).  A block holding a NaN has that scale and NaN
+ * values; with an infinity the scale is infinite.  out [V][H] bytes, out_scales
+ * [ceil(V/128)][ceil(H/128)].  H a multiple of 64, at most 65536; weight and out
+ * 16-byte aligned. */
+int llima_lm_head_quantize(const void* weight, int32_t V, int32_t H, void* out,
+                           float* out_scales, void* stream);
+
+/* Hidden rows in 8 bits: per block of 128 of a row, as llima_lm_head_quantize's
+ * blocks.  x [B][H] of dtype LLIMA_BF16, LLIMA_F16 or LLIMA_F32, rows x_stride
+ * elements apart (rows and x 16-byte aligned); out [B][H] bytes (16-byte
+ * aligned), out_scales [B][ceil(H/128)].  H a multiple of 8, at most 65536. */
+int llima_quantize_rows(const void* x, int32_t dtype, int32_t B, int32_t H, int64_t x_stride,
+                        void* out, float* out_scales, void* stream);
+
+/* Root-mean-square norm with the residual's addition:
+ *   r = x + residual rounded to dtype (x itself when residual is NULL)
+ *   y = (r * f) * (weight + weight_offset),  f = fp32(1 / sqrt(mean(r^2) + eps))
+ * (the mean in 64 bits, y in fp32; weight_offset 1 for weights stored as the
+ * difference from 1).  out [B][H] is y rounded to dtype, or with out_scales
+ * e4m3 values and their scales as llima_quantize_rows makes them from y.
+ * out_residual [B][H] of dtype receives r (NULL: not written; needs residual; may
+ * be residual's own or x's buffer when their rows are contiguous).  x and residual
+ * rows x_stride and residual_stride elements apart; weight [H] of dtype; every
+ * pointer and row 16-byte aligned, scales excepted.  H a multiple of 8, at most
+ * 65536; eps >= 0.  No counterpart in the reference, whose norms run on the NPU. */
+int llima_add_rms_norm(const void* x, const void* residual, const void* weight, int32_t dtype,
+                       int32_t B, int32_t H, int64_t x_stride, int64_t residual_stride, float eps,
+                       float weight_offset, void* out, float* out_scales, void* out_residual,
+                       void* stream);
 
 /* Heap top-k of each of `rows` rows of `cols` values (row r at x + r*row_stride
  * elements), exactly as topk<T> (sima_lmm/devkit/cpp/utils.hpp:216-281):

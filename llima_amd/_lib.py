@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(HERE, "libllima_sampler.so")
 LLIMA_OK, LLIMA_E_INVAL, LLIMA_E_RANGE, LLIMA_E_HIP, LLIMA_E_WORKSPACE = 0, -1, -2, -3, -4
 LLIMA_E_SCRATCH = -5
 LLIMA_E_CAPTURE = -6
-LLIMA_F32, LLIMA_BF16 = 0, 1
+LLIMA_F32, LLIMA_BF16, LLIMA_F16 = 0, 1, 2
 LLIMA_LOGITS_OUT_BF16 = 0x100   # with LLIMA_BF16 in the LM head's logit_dtype: bf16 logits out
 ARGMAX_SPLIT_FIRST, ARGMAX_NEG_INF, ARGMAX_QUARTERS, ARGMAX_LOWEST = 0, 1, 2, 3
 MAX_SPLITS = 16
@@ -80,6 +80,26 @@ SIGNATURES = {
     "llima_lm_head_verify_tree_packed": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32,
                                                         ctypes.c_float, _i32, _vp, _vp, _i32,
                                                         _i32, _vp, _vp, _sz, _vp]),
+    "llima_lm_head_argmax_fp8_workspace_bytes": (_sz, [_i32, _i32]),
+    "llima_lm_head_argmax_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32,
+                                                ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _sz,
+                                                _vp]),
+    "llima_lm_head_score_fp8_workspace_bytes": (_sz, [_i32, _i32]),
+    "llima_lm_head_score_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32,
+                                               ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _sz,
+                                               _vp]),
+    "llima_lm_head_verify_greedy_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "llima_lm_head_verify_greedy_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
+                                                       ctypes.c_float, _i32, _vp, _vp, _vp, _vp,
+                                                       _sz, _vp]),
+    "llima_lm_head_verify_tree_fp8_workspace_bytes": (_sz, [_i32, _i32]),
+    "llima_lm_head_verify_tree_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32,
+                                                     ctypes.c_float, _i32, _vp, _vp, _i32, _i32,
+                                                     _vp, _vp, _sz, _vp]),
+    "llima_lm_head_quantize": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _vp]),
+    "llima_quantize_rows": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
+    "llima_add_rms_norm": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64,
+                                          ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _vp]),
     "llima_topk": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i64, _i32, _vp, _vp, _vp]),
     "llima_eagle3_tree_bytes": (_sz, [_i32, _i32]),
     "llima_eagle3_tree_split_bytes": (_sz, [_i32, _i32, _i32]),

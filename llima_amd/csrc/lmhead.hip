@@ -1172,6 +1172,8 @@ __global__ __launch_bounds__(LLIMA_WG) void lmh_pack(const uint16_t* weight, uin
     *(llima_u32x4*)(packed + p * 16) = v;
 }
 
+#include "lmhead_fp8.hpp"
+
 static size_t lmh_align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // Waves of the rows kernel (a whole number of workgroups): two 512-thread
@@ -1668,4 +1670,149 @@ extern "C" int llima_lm_head_verify_tree_packed(const void* hidden, const void* 
     hipStream_t st = (hipStream_t)stream;
     if ((st0 = lmh_run_packed<false>(P, (const uint8_t*)packed, st)) != LLIMA_OK) return st0;
     return lmh_launch_tree(P, retrieve_indices, candidates, n_paths, L, out, st);
+}
+
+// ------------------------------------------------------------------ 8-bit weight
+static int lmh8_check(const void* xq, const float* xs, const void* wq, const float* ws, int32_t B,
+                      int32_t H, int32_t V) {
+    if (B < 0 || H <= 0 || V <= 0 || H % LMH_KC != 0 || H > 65536) return LLIMA_E_INVAL;
+    if (!wq || !ws || (B > 0 && (!xq || !xs))) return LLIMA_E_INVAL;
+    if ((uintptr_t)wq % 16 || (B > 0 && (uintptr_t)xq % 16)) return LLIMA_E_INVAL;
+    return LLIMA_OK;
+}
+
+static int lmh8_slots(int V) { return (V + LMH_SLOT - 1) / LMH_SLOT; }
+
+static void lmh8_fill(Lmh8Params& Q, const void* xq, const float* xs, const void* wq,
+                      const float* ws, int32_t B, int32_t H, int32_t V, float softcap,
+                      int32_t logit_dtype) {
+    Q.xq = (const uint8_t*)xq;
+    Q.xs = xs;
+    Q.wq = (const uint8_t*)wq;
+    Q.ws = ws;
+    Q.NK = (H + 127) / 128;
+    Q.P.B = B; Q.P.H = H; Q.P.V = V;
+    Q.P.cap = softcap;
+    Q.P.round_bf16 = logit_dtype == LLIMA_BF16;
+}
+
+extern "C" size_t llima_lm_head_argmax_fp8_workspace_bytes(int32_t B, int32_t V) {
+    if (B <= 0 || V <= 0) return 0;
+    return lmh_ws_bytes(B, lmh8_slots(V), false);
+}
+
+extern "C" int llima_lm_head_argmax_fp8(const void* hidden, const float* hidden_scales,
+                                        const void* weight, const float* weight_scales, int32_t B,
+                                        int32_t H, int32_t V, float softcap, int32_t logit_dtype,
+                                        int32_t* out_ids, float* out_vals, float* out_logits,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+    int st0 = lmh8_check(hidden, hidden_scales, weight, weight_scales, B, H, V);
+    if (st0 != LLIMA_OK) return st0;
+    if (B > 0 && !out_ids) return LLIMA_E_INVAL;
+    int32_t logits_bf16 = 0;
+    if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
+    if (B == 0) return LLIMA_OK;
+    if (!workspace || workspace_bytes < llima_lm_head_argmax_fp8_workspace_bytes(B, V))
+        return LLIMA_E_WORKSPACE;
+    Lmh8Params Q = {};
+    lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, B, H, V, softcap, logit_dtype);
+    Q.P.out_logits = out_logits;
+    Q.P.keys = (uint64_t*)workspace;
+    Q.P.out_ids = out_ids;
+    Q.P.out_vals = out_vals;
+    Q.P.logits_bf16 = logits_bf16;
+    return lmh8_run<false>(Q, (hipStream_t)stream);
+}
+
+extern "C" size_t llima_lm_head_score_fp8_workspace_bytes(int32_t B, int32_t V) {
+    if (B <= 0 || V <= 0) return 0;
+    return lmh_ws_bytes(B, lmh8_slots(V), true);
+}
+
+extern "C" int llima_lm_head_score_fp8(const void* hidden, const float* hidden_scales,
+                                       const void* weight, const float* weight_scales, int32_t B,
+                                       int32_t H, int32_t V, float softcap, int32_t logit_dtype,
+                                       const int32_t* targets, double* out_logprob,
+                                       int32_t* out_is_greedy, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    int st0 = lmh8_check(hidden, hidden_scales, weight, weight_scales, B, H, V);
+    if (st0 != LLIMA_OK) return st0;
+    if (B > 0 && (!targets || !out_logprob || !out_is_greedy)) return LLIMA_E_INVAL;
+    if (logit_dtype & LLIMA_LOGITS_OUT_BF16) return LLIMA_E_INVAL;       // no logits output
+    int32_t logits_bf16 = 0;
+    if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
+    if (B == 0) return LLIMA_OK;
+    if (!workspace || workspace_bytes < llima_lm_head_score_fp8_workspace_bytes(B, V))
+        return LLIMA_E_WORKSPACE;
+    Lmh8Params Q = {};
+    lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, B, H, V, softcap, logit_dtype);
+    Q.P.targets = targets;
+    Q.P.out_logprob = out_logprob;
+    Q.P.out_greedy = out_is_greedy;
+    lmh_ws_split(Q.P, workspace, lmh8_slots(V));
+    return lmh8_run<true>(Q, (hipStream_t)stream);
+}
+
+extern "C" size_t llima_lm_head_verify_greedy_fp8_workspace_bytes(int32_t B, int32_t D, int32_t V) {
+    if (B <= 0 || D < 0 || (int64_t)B * (D + 1) > (int64_t)INT32_MAX) return 0;
+    const int32_t rows = B * (D + 1);
+    return lmh_verify_ws(llima_lm_head_argmax_fp8_workspace_bytes(rows, V), rows);
+}
+
+extern "C" int llima_lm_head_verify_greedy_fp8(const void* hidden, const float* hidden_scales,
+                                               const void* weight, const float* weight_scales,
+                                               int32_t B, int32_t D, int32_t H, int32_t V,
+                                               float softcap, int32_t logit_dtype,
+                                               const int32_t* draft_ids, int32_t* accepted_len,
+                                               int32_t* emitted, void* workspace,
+                                               size_t workspace_bytes, void* stream) {
+    int st0 = lmh_verify_check(B, D, draft_ids, accepted_len, emitted);
+    if (st0 != LLIMA_OK) return st0;
+    if (logit_dtype & LLIMA_LOGITS_OUT_BF16) return LLIMA_E_INVAL;       // no logits output
+    const int32_t rows = B * (D + 1);
+    if ((st0 = lmh8_check(hidden, hidden_scales, weight, weight_scales, rows, H, V)) != LLIMA_OK) return st0;
+    int32_t logits_bf16 = 0;
+    if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
+    if (B == 0) return LLIMA_OK;
+    if (!workspace || workspace_bytes < llima_lm_head_verify_greedy_fp8_workspace_bytes(B, D, V))
+        return LLIMA_E_WORKSPACE;
+    int32_t* ids = (int32_t*)((uint8_t*)workspace + llima_lm_head_argmax_fp8_workspace_bytes(rows, V));
+    Lmh8Params Q = {};
+    lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, rows, H, V, softcap, logit_dtype);
+    Q.P.keys = (uint64_t*)workspace;
+    Q.P.out_ids = ids;
+    hipStream_t st = (hipStream_t)stream;
+    if ((st0 = lmh8_run<false>(Q, st)) != LLIMA_OK) return st0;
+    return lmh_launch_chain(ids, draft_ids, accepted_len, emitted, B, D, st);
+}
+
+extern "C" size_t llima_lm_head_verify_tree_fp8_workspace_bytes(int32_t K, int32_t V) {
+    if (K <= 0) return 0;
+    return lmh_tree_ws(llima_lm_head_argmax_fp8_workspace_bytes(K, V), K);
+}
+
+extern "C" int llima_lm_head_verify_tree_fp8(const void* hidden, const float* hidden_scales,
+                                             const void* weight, const float* weight_scales,
+                                             int32_t K, int32_t H, int32_t V, float softcap,
+                                             int32_t logit_dtype, const int32_t* retrieve_indices,
+                                             const int32_t* candidates, int32_t n_paths, int32_t L,
+                                             int32_t* out, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
+    int st0 = lmh_tree_check(K, retrieve_indices, candidates, n_paths, L, out);
+    if (st0 != LLIMA_OK) return st0;
+    if (logit_dtype & LLIMA_LOGITS_OUT_BF16) return LLIMA_E_INVAL;       // no logits output
+    if ((st0 = lmh8_check(hidden, hidden_scales, weight, weight_scales, K, H, V)) != LLIMA_OK) return st0;
+    int32_t logits_bf16 = 0;
+    if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
+    if (!workspace || workspace_bytes < llima_lm_head_verify_tree_fp8_workspace_bytes(K, V))
+        return LLIMA_E_WORKSPACE;
+    uint8_t* rest = (uint8_t*)workspace + llima_lm_head_argmax_fp8_workspace_bytes(K, V);
+    Lmh8Params Q = {};
+    lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, K, H, V, softcap, logit_dtype);
+    Q.P.keys = (uint64_t*)workspace;
+    Q.P.out_ids = (int32_t*)rest;
+    Q.P.out_vals = (float*)(rest + lmh_align256((size_t)K * 4));
+    hipStream_t st = (hipStream_t)stream;
+    if ((st0 = lmh8_run<false>(Q, st)) != LLIMA_OK) return st0;
+    return lmh_launch_tree(Q.P, retrieve_indices, candidates, n_paths, L, out, st);
 }

@@ -25,6 +25,7 @@ ValueError / RuntimeError are raised for the same conditions.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -42,7 +43,8 @@ __all__ = [
     "sample", "verify_greedy", "resolve_draft_tokens", "verify_tree", "verify_rejection",
     "Workspace", "score_logits", "select_candidate_tokens", "argmax_gemma4_mtp_masked_rows",
     "argmax_gemma4_mtp_masked_row", "topk", "Eagle3DraftTree", "stop_mask", "stop_check",
-    "lm_head_argmax", "lm_head_pack", "PackedLmHead",
+    "lm_head_argmax", "lm_head_pack", "PackedLmHead", "Fp8LmHead", "Fp8Rows", "add_rms_norm",
+    "quantize_rows", "lm_head_quantize",
 ]
 
 
@@ -164,6 +166,45 @@ def _dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.bfloat16:
         return _lib.LLIMA_BF16
     raise ValueError(f"logits must be float32 or bfloat16, got {t.dtype}")
+
+
+def _scratch(device, kind: str, nbytes: int) -> torch.Tensor:
+    """Workspace.get, or under stream capture a buffer of the graph's own: graphs
+    captured on one stream may be replayed on several at once."""
+    if _capturing(device):
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    return Workspace.get(device, kind, nbytes)
+
+
+def _on(device):
+    """A context in which `device` is the current one (kernels are launched on the
+    current device; its stream has to be that device's)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+FLOAT_CODES = {torch.float32: _lib.LLIMA_F32, torch.bfloat16: _lib.LLIMA_BF16,
+               torch.float16: _lib.LLIMA_F16}
+
+
+def _rows16(x: torch.Tensor, name: str) -> torch.Tensor:
+    """x [..., H] as rows [B, H] that the kernels' 16-byte accesses can read: values of
+    a row adjacent, rows and the first row 16-byte aligned (copied when they are not)."""
+    if x.dim() == 0 or x.dtype not in FLOAT_CODES:
+        raise ValueError(f"{name} takes bfloat16, float16 or float32 rows")
+    _on_gpu(x)
+    H = x.shape[-1]
+    if H == 0 or H % 8 or H > 65536:
+        raise ValueError(f"{name} needs rows of a multiple of 8 values (at most 65536)")
+    x = x.reshape(-1, H)
+    e = x.element_size()
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < H) or x.stride(0) * e % 16:
+        x = x.contiguous()
+    if x.stride(0) * e % 16 or (x.shape[0] <= 1 and x.stride(0) < H):
+        x = x.as_strided((x.shape[0], H), (H, 1))
+    return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _on_gpu(*ts):
@@ -608,6 +649,253 @@ def lm_head_pack(weight: torch.Tensor) -> PackedLmHead:
     return PackedLmHead(data, V, H)
 
 
+E4M3_MAX = 448.0
+FP8_BLOCK = 128
+
+
+def _fp8_pair(values, scales, srows, name):
+    if values.dim() != 2 or values.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"{name}: values must be float8_e4m3fn and two-dimensional")
+    want = (srows, -(-values.shape[1] // FP8_BLOCK))
+    if scales.dtype != torch.float32 or tuple(scales.shape) != want:
+        raise ValueError(f"{name}: scales must be float32 {list(want)}")
+    _on_gpu(values, scales)
+    if values.device != scales.device:
+        raise ValueError(f"{name}: values and scales must be on one device")
+    v, s = values.contiguous(), scales.contiguous()
+    return (v if v.data_ptr() % 16 == 0 else v.clone()), s
+
+
+class Fp8Rows:
+    """Hidden rows in 8 bits: `values` float8_e4m3fn [B, H] and `scales` float32
+    [B, ceil(H/128)], one per 128 values of a row (a row is values * scales).
+    Made by add_rms_norm(out="fp8") and quantize_rows."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        self.values, self.scales = _fp8_pair(values, scales, values.shape[0], "Fp8Rows")
+
+
+class Fp8LmHead:
+    """An LM head weight in 8 bits: `values` float8_e4m3fn [V, H] and `scales`
+    float32 [ceil(V/128), ceil(H/128)], one per block of 128 x 128 (the weight is
+    values * scales), from lm_head_quantize or a checkpoint that stores it so.
+    The lm_head_* functions take it in the weight's place: the product reads
+    half of the bf16 weight's bytes.  H is a multiple of 64, at most 65536."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        self.values, self.scales = _fp8_pair(values, scales, -(-values.shape[0] // FP8_BLOCK),
+                                             "Fp8LmHead")
+        self.V, self.H = self.values.shape
+        if self.H % 64 or self.H > 65536 or self.H == 0 or self.V == 0:
+            raise ValueError("Fp8LmHead needs H a multiple of 64 (at most 65536)")
+
+
+def quantize_rows(x: torch.Tensor) -> Fp8Rows:
+    """Rows [..., H] (bf16, fp16 or fp32, H a multiple of 8) in 8 bits with a scale
+    per 128 values of a row: max = max(max |x|, 2^-100) of the block, the scale
+    max / 448 and the values e4m3(448 x / max) (llima_quantize_rows)."""
+    x = _rows16(x, "quantize_rows")
+    B, H = x.shape
+    q = Fp8Rows.__new__(Fp8Rows)
+    q.values = torch.empty((B, H), dtype=torch.float8_e4m3fn, device=x.device)
+    q.scales = torch.empty((B, -(-H // FP8_BLOCK)), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        check(lib().llima_quantize_rows(x.data_ptr(), FLOAT_CODES[x.dtype], B, H, x.stride(0),
+                                        q.values.data_ptr(), q.scales.data_ptr(),
+                                        _stream(x.device)), "llima_quantize_rows")
+    return q
+
+
+def lm_head_quantize(weight: torch.Tensor) -> Fp8LmHead:
+    """A bf16 [V, H] LM head weight in 8 bits with a scale per block of 128 x 128
+    (llima_lm_head_quantize; the blocks as quantize_rows')."""
+    if weight.dtype != torch.bfloat16 or weight.dim() != 2:
+        raise ValueError("lm_head_quantize takes a bf16 [V, H] weight")
+    _on_gpu(weight)
+    w = weight.contiguous()
+    w = w if w.data_ptr() % 16 == 0 else w.clone()
+    V, H = w.shape
+    q = torch.empty((V, H), dtype=torch.float8_e4m3fn, device=w.device)
+    s = torch.empty((-(-V // FP8_BLOCK), -(-H // FP8_BLOCK)), dtype=torch.float32, device=w.device)
+    with _on(w.device):
+        check(lib().llima_lm_head_quantize(w.data_ptr(), V, H, q.data_ptr(), s.data_ptr(),
+                                           _stream(w.device)), "llima_lm_head_quantize")
+    return Fp8LmHead(q, s)
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6, weight_offset: float = 0.0, out: str = "same"):
+    """The residual stream's addition and its root-mean-square norm
+    (llima_add_rms_norm): x [..., H] and residual (the same shape) in bf16, fp16 or
+    fp32, weight [H] of that type -> (y, new residual stream).  r = x + residual
+    rounded to the type (x when there is no residual), y = (r * f) * (weight +
+    weight_offset) with f = 1 / sqrt(mean(r^2) + eps); the second result is r, None
+    without a residual.  out "same" rounds y to the type; "fp8" returns Fp8Rows [rows,
+    H], 8-bit values with a scale per 128, as lm_head_* functions take them with an
+    Fp8LmHead.  H a multiple of 8, at most 65536."""
+    if out not in ("same", "fp8"):
+        raise ValueError("out must be 'same' or 'fp8'")
+    shape, H = x.shape, x.shape[-1] if x.dim() else 0
+    if weight.dim() != 1 or weight.shape[0] != H or weight.dtype != x.dtype:
+        raise ValueError("weight must be [H] of x's type")
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
+        raise ValueError("residual must have x's shape and type")
+    a = _rows16(x, "add_rms_norm")
+    b = None if residual is None else _rows16(residual, "add_rms_norm")
+    _on_gpu(weight)
+    w = weight.contiguous()
+    w = w if w.data_ptr() % 16 == 0 else w.clone()
+    dev = a.device
+    if w.device != dev or (b is not None and b.device != dev):
+        raise ValueError("add_rms_norm: tensors must be on one device")
+    B = a.shape[0]
+    if out == "fp8":
+        y = Fp8Rows.__new__(Fp8Rows)
+        y.values = torch.empty((B, H), dtype=torch.float8_e4m3fn, device=dev)
+        y.scales = torch.empty((B, -(-H // FP8_BLOCK)), dtype=torch.float32, device=dev)
+        o, sc = y.values, y.scales.data_ptr()
+    else:
+        y = o = torch.empty(shape, dtype=x.dtype, device=dev)
+        sc = None
+    r = None if b is None else torch.empty(shape, dtype=x.dtype, device=dev)
+    with _on(dev):
+        check(lib().llima_add_rms_norm(a.data_ptr(), _ptr(b), w.data_ptr(), FLOAT_CODES[x.dtype], B,
+                                       H, a.stride(0), 0 if b is None else b.stride(0), float(eps),
+                                       float(weight_offset), o.data_ptr(), sc, _ptr(r),
+                                       _stream(dev)), "llima_add_rms_norm")
+    return y, r
+
+
+def _fp8_hidden(hidden, head: Fp8LmHead, name: str) -> Fp8Rows:
+    """The hidden rows of a call over an Fp8LmHead: Fp8Rows as they are, bf16 rows
+    [rows, H] through quantize_rows."""
+    if isinstance(hidden, Fp8Rows):
+        x = hidden
+    else:
+        if hidden.dtype != torch.bfloat16:
+            raise ValueError(f"{name} takes bf16 hidden states or Fp8Rows with an Fp8LmHead")
+        if hidden.shape[-1] != head.H:
+            raise ValueError("hidden width differs from the weight's H")
+        x = quantize_rows(hidden)
+    if x.values.shape[1] != head.H:
+        raise ValueError("hidden width differs from the weight's H")
+    if x.values.device != head.values.device:
+        raise ValueError(f"{name}: hidden rows and weight must be on one device")
+    return x
+
+
+def _logit_dtype(logit_dtype: str, logits_out: str = "f32") -> int:
+    if logit_dtype not in ("bf16", "f32"):
+        raise ValueError("logit_dtype must be 'bf16' or 'f32'")
+    if logits_out not in ("bf16", "f32"):
+        raise ValueError("logits_out must be 'bf16' or 'f32'")
+    if logits_out == "bf16" and logit_dtype != "bf16":
+        raise ValueError("bf16 logits output needs logit_dtype 'bf16'")
+    return ((_lib.LLIMA_BF16 if logit_dtype == "bf16" else _lib.LLIMA_F32) |
+            (_lib.LLIMA_LOGITS_OUT_BF16 if logits_out == "bf16" else 0))
+
+
+def _head8(x: Fp8Rows, head: Fp8LmHead):
+    return (x.values.data_ptr(), x.scales.data_ptr(), head.values.data_ptr(),
+            head.scales.data_ptr())
+
+
+def _lm_head_argmax_fp8(hidden, head: Fp8LmHead, softcap, return_logits, logit_dtype, logits_out):
+    ld = _logit_dtype(logit_dtype, logits_out)
+    x = _fp8_hidden(hidden, head, "lm_head_argmax")
+    B, V, dev = x.values.shape[0], head.V, head.values.device
+    ids = torch.empty(B, dtype=torch.int32, device=dev)
+    vals = torch.empty(B, dtype=torch.float32, device=dev)
+    ldt = torch.bfloat16 if logits_out == "bf16" else torch.float32
+    logits = torch.empty((B, V), dtype=ldt, device=dev) if return_logits else None
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_argmax_fp8_workspace_bytes(B, V))
+    with _on(dev):
+        check(lib().llima_lm_head_argmax_fp8(*_head8(x, head), B, head.H, V, float(softcap), ld,
+                                             ids.data_ptr(), vals.data_ptr(), _ptr(logits),
+                                             ws.data_ptr(), ws.numel(), _stream(dev)),
+              "llima_lm_head_argmax_fp8")
+    return (ids, vals, logits) if return_logits else (ids, vals)
+
+
+def _lm_head_score_fp8(hidden, head: Fp8LmHead, target, softcap, logit_dtype):
+    single = not isinstance(hidden, Fp8Rows) and hidden.dim() == 1
+    ld = _logit_dtype(logit_dtype)
+    V, dev = head.V, head.values.device
+    if single:
+        t = int(target)
+        if t < 0 or t >= V:
+            raise RuntimeError(f"Target token id {t} is outside logits vocabulary size {V}")
+        tg = torch.full((1,), t, dtype=torch.int32, device=dev)
+    else:
+        tg = torch.as_tensor(target).to(device=dev, dtype=torch.int32).contiguous().reshape(-1)
+    rows = 1 if single else hidden.values.shape[0] if isinstance(hidden, Fp8Rows) else hidden.shape[0]
+    if tg.numel() != rows:
+        raise ValueError("one target per row is required")
+    in_range = None if single else _TargetCheck(tg)
+    x = _fp8_hidden(hidden, head, "lm_head_score")
+    B = x.values.shape[0]
+    lp = torch.empty(B, dtype=torch.float64, device=dev)
+    gr = torch.empty(B, dtype=torch.int32, device=dev)
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_score_fp8_workspace_bytes(B, V))
+    with _on(dev):
+        check(lib().llima_lm_head_score_fp8(*_head8(x, head), B, head.H, V, float(softcap), ld,
+                                            tg.data_ptr(), lp.data_ptr(), gr.data_ptr(),
+                                            ws.data_ptr(), ws.numel(), _stream(dev)),
+              "llima_lm_head_score_fp8")
+    if single:
+        return float(lp[0]), bool(gr[0] == 1)
+    greedy = gr == 1
+    in_range.wait(V)
+    return lp, greedy
+
+
+def _lm_head_verify_greedy_fp8(hidden, head: Fp8LmHead, draft_ids, softcap, logit_dtype):
+    ld = _logit_dtype(logit_dtype)
+    dev = head.values.device
+    dr = torch.as_tensor(draft_ids).to(device=dev, dtype=torch.int32).contiguous()
+    if dr.dim() != 2:
+        raise ValueError("draft_ids must be [B, D]")
+    B, D = dr.shape
+    rows = hidden.values.shape[0] if isinstance(hidden, Fp8Rows) else -1
+    if rows != B * (D + 1) and (rows >= 0 or hidden.dim() != 3 or tuple(hidden.shape[:2]) != (B, D + 1)):
+        raise ValueError("hidden must be [B, D+1, H], or Fp8Rows of B (D+1) rows")
+    x = _fp8_hidden(hidden, head, "lm_head_verify_greedy")
+    acc = torch.empty(B, dtype=torch.int32, device=dev)
+    em = torch.empty((B, D + 1), dtype=torch.int32, device=dev)
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_verify_greedy_fp8_workspace_bytes(B, D, head.V))
+    with _on(dev):
+        check(lib().llima_lm_head_verify_greedy_fp8(*_head8(x, head), B, D, head.H, head.V,
+                                                    float(softcap), ld, dr.data_ptr(),
+                                                    acc.data_ptr(), em.data_ptr(), ws.data_ptr(),
+                                                    ws.numel(), _stream(dev)),
+              "llima_lm_head_verify_greedy_fp8")
+    return acc, em
+
+
+def _lm_head_verify_tree_fp8(hidden, head: Fp8LmHead, retrieve_indices, candidates, softcap,
+                             logit_dtype):
+    ld = _logit_dtype(logit_dtype)
+    dev = head.values.device
+    if not isinstance(hidden, Fp8Rows) and hidden.dim() != 2:
+        raise ValueError("hidden must be [K, H] or Fp8Rows")
+    ri = retrieve_indices.to(device=dev, dtype=torch.int32).contiguous()
+    ca = candidates.to(device=dev, dtype=torch.int32).contiguous()
+    if ri.shape != ca.shape or ri.dim() != 2:
+        raise ValueError("retrieve_indices and candidates must both be [n_paths, L]")
+    P, L = ri.shape
+    x = _fp8_hidden(hidden, head, "lm_head_verify_tree")
+    K = x.values.shape[0]
+    out = torch.empty(3, dtype=torch.int32, device=dev)
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_verify_tree_fp8_workspace_bytes(K, head.V))
+    with _on(dev):
+        check(lib().llima_lm_head_verify_tree_fp8(*_head8(x, head), K, head.H, head.V,
+                                                  float(softcap), ld, ri.data_ptr(), ca.data_ptr(),
+                                                  P, L, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                                  _stream(dev)), "llima_lm_head_verify_tree_fp8")
+    o = out.tolist()
+    return o[0], o[1], o[2]
+
+
 def lm_head_argmax(hidden: torch.Tensor, weight, softcap: float = 0.0,
                    return_logits: bool = False, logit_dtype: str = "bf16",
                    logits_out: str = "f32"):
@@ -621,7 +909,11 @@ def lm_head_argmax(hidden: torch.Tensor, weight, softcap: float = 0.0,
     (with logit_dtype "bf16") returns the logits as a bfloat16 tensor, half
     the bytes of the float32 one and the same values, ready for sample().
     weight may be a PackedLmHead (lm_head_pack): the same logits, read in the
-    packed order (llima_lm_head_argmax_packed)."""
+    packed order (llima_lm_head_argmax_packed).
+    weight may also be an Fp8LmHead; hidden is then bf16 (put in 8 bits by
+    quantize_rows) or Fp8Rows (llima_lm_head_argmax_fp8)."""
+    if isinstance(weight, Fp8LmHead):
+        return _lm_head_argmax_fp8(hidden, weight, softcap, return_logits, logit_dtype, logits_out)
     x = hidden.reshape(1, -1) if hidden.dim() == 1 else hidden
     packed = isinstance(weight, PackedLmHead)
     if x.dtype != torch.bfloat16 or (not packed and weight.dtype != torch.bfloat16):
@@ -670,7 +962,11 @@ def lm_head_score(hidden: torch.Tensor, weight, target, softcap: float = 0.0,
     flags), or hidden [H] with an int target -> (float, bool).  The logits are
     lm_head_argmax's (the same softcap and logit_dtype); weight may be a
     PackedLmHead.  A target outside the vocabulary raises RuntimeError, and the
-    [B] results are ready in the order of the current stream, as score_logits'."""
+    [B] results are ready in the order of the current stream, as score_logits'.
+    weight may also be an Fp8LmHead; hidden is then bf16 (put in 8 bits by
+    quantize_rows) or Fp8Rows (llima_lm_head_score_fp8)."""
+    if isinstance(weight, Fp8LmHead):
+        return _lm_head_score_fp8(hidden, weight, target, softcap, logit_dtype)
     single = hidden.dim() == 1
     x = hidden.reshape(1, -1) if single else hidden
     packed = isinstance(weight, PackedLmHead)
@@ -724,7 +1020,11 @@ def lm_head_verify_greedy(hidden: torch.Tensor, weight, draft_ids: torch.Tensor,
     logits written (llima_lm_head_verify_greedy): hidden bf16 [B, D+1, H],
     draft_ids int [B, D] -> (accepted_len int32 [B], emitted int32 [B, D+1]),
     as verify_greedy over the logits lm_head_argmax would write (the same
-    softcap and logit_dtype).  weight may be a PackedLmHead."""
+    softcap and logit_dtype).  weight may be a PackedLmHead.
+    weight may also be an Fp8LmHead; hidden is then bf16 (put in 8 bits by
+    quantize_rows) or Fp8Rows (llima_lm_head_verify_greedy_fp8)."""
+    if isinstance(weight, Fp8LmHead):
+        return _lm_head_verify_greedy_fp8(hidden, weight, draft_ids, softcap, logit_dtype)
     if hidden.dim() != 3:
         raise ValueError("hidden must be [B, D+1, H]")
     B, D1, H = hidden.shape
@@ -774,7 +1074,12 @@ def lm_head_verify_tree(hidden: torch.Tensor, weight, retrieve_indices: torch.Te
     written (llima_lm_head_verify_tree): hidden bf16 [K, H] (the tree rows),
     retrieve_indices and candidates [n_paths, L] -> (best_candidate,
     accept_length, bonus_token), as verify_tree over the logits lm_head_argmax
-    would write.  weight may be a PackedLmHead."""
+    would write.  weight may be a PackedLmHead.
+    weight may also be an Fp8LmHead; hidden is then bf16 (put in 8 bits by
+    quantize_rows) or Fp8Rows (llima_lm_head_verify_tree_fp8)."""
+    if isinstance(weight, Fp8LmHead):
+        return _lm_head_verify_tree_fp8(hidden, weight, retrieve_indices, candidates, softcap,
+                                       logit_dtype)
     x = hidden.contiguous()
     packed = isinstance(weight, PackedLmHead)
     if x.dim() != 2 or x.dtype != torch.bfloat16 or (not packed and weight.dtype != torch.bfloat16):
