@@ -495,6 +495,85 @@ int llima_add_rms_norm(const void* x, const void* residual, const void* weight, 
                        float weight_offset, void* out, float* out_scales, void* out_residual,
                        void* stream);
 
+/* Attention of N drafted tokens per sequence over the sequence's cached tokens
+ * and, under a tree mask, each other.  No counterpart in the reference, whose
+ * attention runs on the NPU; the mask is the one its draft tree makes
+ * (sima_lmm/devkit/cpp/language_model_eagle3.cpp:808-1164), as
+ * llima_eagle3_tree_finish writes it.
+ *
+ *   out[b][n][h] = sum_j p_j v_j,  p = softmax over the visible j of scale q . k_j
+ *
+ * over the cache_lens[b] cached tokens, which every node sees, and the drafted
+ * tokens m with mask[b][n][m] != 0 (LLIMA_MASK_U8) or > 0 (LLIMA_MASK_F32); with
+ * mask NULL m <= n (a chain; N = 1 is a decode step).  Query head h reads key head
+ * h / (Hq / Hkv).  A row that sees nothing is 0.  What a row does not see does not
+ * reach it, NaN and infinities included.  Scores, softmax and sums are fp32; the
+ * weights are rounded to dtype for their product with v (the row's sum is not).
+ *
+ *   q, out [B][N][Hq][D],  k, v [B][N][Hkv][D] (the drafted tokens' own)
+ *   k_cache, v_cache [pages][page_size][Hkv][D]: sequence b's token j is token
+ *     j % page_size of page block_table[b][j / page_size] (max_blocks entries per
+ *     sequence); with block_table NULL page b is sequence b's (max_blocks 1, pages >= B)
+ *
+ * dtype LLIMA_BF16 or LLIMA_F16; D 64, 128 or 256, adjacent; every other stride is
+ * free, in elements, a multiple of 8, and not negative; base pointers and the
+ * workspace 16-byte aligned.  mask strides: batch (0: one mask for all) and row,
+ * columns adjacent.  N at most 1024, page_size * max_blocks + N at most 2^30.  A
+ * sequence whose length is outside [0, page_size * max_blocks], or which has a page
+ * outside [0, pages) among its cached tokens', gets NaN.  The order of the sums, and
+ * so the last bits, depend on the lengths of the whole batch, not on its timing. */
+enum { LLIMA_MASK_U8 = 0, LLIMA_MASK_F32 = 1 };
+typedef struct llima_tree_attention_args {
+    const void *q, *k, *v;
+    const void *k_cache, *v_cache;
+    void* out;
+    const int32_t* cache_lens;           /* [B], device */
+    const void* mask;                    /* or NULL */
+    const int32_t* block_table;          /* or NULL */
+    int64_t q_strides[3];                /* batch, token, head */
+    int64_t k_strides[3], v_strides[3], out_strides[3];
+    int64_t k_cache_strides[3];          /* page, token, head */
+    int64_t v_cache_strides[3];
+    int64_t mask_strides[2];
+    int64_t table_stride;
+    int32_t dtype, mask_dtype;
+    int32_t B, N, Hq, Hkv, D;
+    int32_t page_size, pages, max_blocks;
+    float scale;
+} llima_tree_attention_args;
+size_t llima_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq, int32_t Hkv,
+                                            int32_t D);
+int llima_tree_attention(const llima_tree_attention_args* args, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Keeps the accepted path of each sequence: in every layer, token
+ * cache_lens[b] + j of its cache becomes the keys and values of drafted token
+ * nodes[b][j], j < counts[b], and new_lens[b] = cache_lens[b] + counts[b].
+ *
+ *   k, v [layers][B][N][Hkv][D],  nodes [B][L],  counts, cache_lens, new_lens [B]
+ *   k_cache, v_cache [layers][pages][page_size][Hkv][D] and block_table as
+ *     llima_tree_attention's
+ *
+ * 16-bit values of any type, D a multiple of 8, strides as there (layer, batch or
+ * page, token, head).  A sequence with a count outside [0, L], a node outside [0, N),
+ * a length below 0, no room for its path or a page outside [0, pages) among those it
+ * would write is left as it is, and new_lens[b] is LLIMA_E_RANGE.  Nothing else of
+ * the cache is written.  new_lens may not be cache_lens; the caches may not overlap k
+ * or v, and no two sequences may write to one page's token. */
+typedef struct llima_tree_commit_args {
+    const void *k, *v;
+    void *k_cache, *v_cache;
+    const int32_t *nodes, *counts, *cache_lens, *block_table;
+    int32_t* new_lens;
+    int64_t k_strides[4], v_strides[4];  /* layer, batch, token, head */
+    int64_t k_cache_strides[4];          /* layer, page, token, head */
+    int64_t v_cache_strides[4];
+    int64_t nodes_stride, table_stride;
+    int32_t layers, B, N, L, Hkv, D;
+    int32_t page_size, pages, max_blocks;
+} llima_tree_commit_args;
+int llima_tree_commit(const llima_tree_commit_args* args, void* stream);
+
 /* Heap top-k of each of `rows` rows of `cols` values (row r at x + r*row_stride
  * elements), exactly as topk<T> (sima_lmm/devkit/cpp/utils.hpp:216-281):
  * a min-heap of the first k values, replaced at the root only by strictly

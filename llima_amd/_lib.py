@@ -15,6 +15,7 @@ LLIMA_OK, LLIMA_E_INVAL, LLIMA_E_RANGE, LLIMA_E_HIP, LLIMA_E_WORKSPACE = 0, -1, 
 LLIMA_E_SCRATCH = -5
 LLIMA_E_CAPTURE = -6
 LLIMA_F32, LLIMA_BF16, LLIMA_F16 = 0, 1, 2
+LLIMA_MASK_U8, LLIMA_MASK_F32 = 0, 1
 LLIMA_LOGITS_OUT_BF16 = 0x100   # with LLIMA_BF16 in the LM head's logit_dtype: bf16 logits out
 ARGMAX_SPLIT_FIRST, ARGMAX_NEG_INF, ARGMAX_QUARTERS, ARGMAX_LOWEST = 0, 1, 2, 3
 MAX_SPLITS = 16
@@ -100,6 +101,9 @@ SIGNATURES = {
     "llima_quantize_rows": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
     "llima_add_rms_norm": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64,
                                           ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _vp]),
+    "llima_tree_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "llima_tree_attention": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
+    "llima_tree_commit": (ctypes.c_int, [_vp, _vp]),
     "llima_topk": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i64, _i32, _vp, _vp, _vp]),
     "llima_eagle3_tree_bytes": (_sz, [_i32, _i32]),
     "llima_eagle3_tree_split_bytes": (_sz, [_i32, _i32, _i32]),
@@ -134,6 +138,31 @@ class SamplerConfigC(ctypes.Structure):
         ("presence_penalty_rows", ctypes.c_void_p),
         ("frequency_penalty_rows", ctypes.c_void_p),
     ]
+
+
+_i64x2, _i64x3, _i64x4 = _i64 * 2, _i64 * 3, _i64 * 4
+
+
+class TreeAttentionArgsC(ctypes.Structure):
+    """Mirror of llima_tree_attention_args."""
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "k_cache", "v_cache", "out", "cache_lens", "mask",
+                                    "block_table")] +
+                [(n, _i64x3) for n in ("q_strides", "k_strides", "v_strides", "out_strides",
+                                       "k_cache_strides", "v_cache_strides")] +
+                [("mask_strides", _i64x2), ("table_stride", _i64)] +
+                [(n, _i32) for n in ("dtype", "mask_dtype", "B", "N", "Hq", "Hkv", "D", "page_size",
+                                     "pages", "max_blocks")] + [("scale", ctypes.c_float)])
+
+
+class TreeCommitArgsC(ctypes.Structure):
+    """Mirror of llima_tree_commit_args."""
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_cache", "v_cache", "nodes", "counts", "cache_lens",
+                                    "block_table", "new_lens")] +
+                [(n, _i64x4) for n in ("k_strides", "v_strides", "k_cache_strides",
+                                       "v_cache_strides")] +
+                [("nodes_stride", _i64), ("table_stride", _i64)] +
+                [(n, _i32) for n in ("layers", "B", "N", "L", "Hkv", "D", "page_size", "pages",
+                                     "max_blocks")])
 
 
 _lib = None

@@ -1,0 +1,197 @@
+"""Attention of drafted tokens over a KV cache, and the commit of an accepted path.
+
+  tree_attention(q, k, v, k_cache, v_cache, cache_lens, tree_mask, block_table)
+  tree_commit(k, v, nodes, counts, k_cache, v_cache, cache_lens, block_table)
+
+The step of a draft tree around the token selection: the attention reads the mask
+that Eagle3DraftTree.finish makes, the commit keeps the path that verify_tree or
+lm_head_verify_tree accepted.  No counterpart in the reference, whose attention and
+caches are on the NPU.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .sampler import FLOAT_CODES, _on, _on_gpu, _ptr, _scratch, _stream
+
+__all__ = ["tree_attention", "tree_commit"]
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """[..., D] that 16-byte accesses can read: D adjacent, the other strides multiples
+    of 8 and not negative, 16-byte aligned (copied when it is not)."""
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0:
+        if not any([s % 8 for s in st[:-1]]):
+            return t
+        if not any([s % 8 and n > 1 for s, n in zip(st[:-1], t.shape[:-1])]):
+            return t.as_strided(t.shape, [0 if n <= 1 else s for s, n in zip(st[:-1], t.shape[:-1])] + [1])
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _in_place(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A cache as the kernels can use it where it is (it is never copied)."""
+    h = _heads(t)
+    if h.data_ptr() != t.data_ptr():
+        raise ValueError(f"{name}: head values must be adjacent, other strides multiples of 8, "
+                         "and the first 16-byte aligned")
+    return h
+
+
+def _cache(k_cache, v_cache, Hkv, D, dtype, block_table, B, dev):
+    """Checks of a cache [..., page_size, Hkv, D] and its table -> (page size, pages, blocks per
+    sequence, table)."""
+    for t in (k_cache, v_cache):
+        if t.dtype != dtype or tuple(t.shape[-2:]) != (Hkv, D) or t.shape != k_cache.shape:
+            raise ValueError("k_cache and v_cache must both be [..., tokens, Hkv, D] of k's type")
+    pages, page = k_cache.shape[-4], k_cache.shape[-3]
+    if page == 0:
+        raise ValueError("the cache has no room for a token")
+    if block_table is None:
+        if pages != B:
+            raise ValueError("without a block table the cache must be [B, tokens, Hkv, D]")
+        return page, pages, 1, None
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype != torch.int32:
+        raise ValueError("block_table must be int32 [B, blocks]")
+    if block_table.device != dev:
+        raise ValueError("block_table must be on the cache's device")
+    t = block_table if block_table.stride(1) == 1 or block_table.shape[1] == 1 else block_table.contiguous()
+    if t.shape[1] and page * t.shape[1] > 1 << 30:
+        raise ValueError("a sequence's blocks hold more than 2^30 tokens")
+    return page, pages, t.shape[1], t
+
+
+def _ints(t: torch.Tensor, B: int, name: str, dev) -> torch.Tensor:
+    if tuple(t.shape) != (B,) or t.dtype != torch.int32 or t.device != dev:
+        raise ValueError(f"{name} must be int32 [{B}] on the cache's device")
+    return t.contiguous()
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor, cache_lens: torch.Tensor,
+                   tree_mask: Optional[torch.Tensor] = None,
+                   block_table: Optional[torch.Tensor] = None,
+                   scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of N drafted tokens of B sequences over the sequences' caches and, under the
+    tree mask, over each other (llima_tree_attention) -> [B, N, Hq, D] of q's type.
+
+    q [B, N, Hq, D], k and v [B, N, Hkv, D] (the drafted tokens' own, not in the cache yet;
+    Hq a multiple of Hkv), bf16 or fp16, D 64, 128 or 256.  k_cache, v_cache: [B, tokens, Hkv,
+    D], or pages [pages, page_size, Hkv, D] with block_table int32 [B, blocks]; cache_lens
+    int32 [B]: the cached tokens, which every node sees.  tree_mask [N, N] or [B, N, N],
+    bool (or uint8, nonzero) or float32 (above 0, as Eagle3DraftTree.finish's): node n sees
+    drafted token m where mask[n, m]; None: m <= n, the chain of drafts, or with N = 1 a
+    decode step.  A row that sees nothing is 0; a sequence with a length or a page out of
+    range is NaN.  scale defaults to D^-0.5.  Strides are free where values of a head are
+    adjacent (head-major caches as transposed views).  Nothing waits for the device, and the
+    call can be captured into a graph."""
+    if q.dim() != 4 or k.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("q [B, N, Hq, D], k and v [B, N, Hkv, D] and 4-dimensional caches are needed")
+    B, N, Hq, D = q.shape
+    Hkv = k.shape[2]
+    if tuple(k.shape) != (B, N, Hkv, D) or v.shape != k.shape:
+        raise ValueError("k and v must be [B, N, Hkv, D] with q's B, N and D")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must be bfloat16 or float16, of one type")
+    if D not in (64, 128, 256):
+        raise ValueError("the head size must be 64, 128 or 256")
+    if N == 0 or N > 1024 or Hkv == 0 or Hq == 0 or Hq % Hkv or Hq > 1024:
+        raise ValueError("1 to 1024 drafted tokens and query heads, a multiple of the key heads, are supported")
+    _on_gpu(q, k, v, k_cache, v_cache, cache_lens, tree_mask, block_table)
+    dev = q.device
+    if not (k.device == v.device == k_cache.device == v_cache.device == dev):
+        raise ValueError("tree_attention: tensors must be on one device")
+    page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, q.dtype, block_table, B, dev)
+    lens = _ints(cache_lens, B, "cache_lens", dev)
+    a = _lib.TreeAttentionArgsC()
+    mask = tree_mask
+    if mask is not None:
+        if tuple(mask.shape) not in ((N, N), (B, N, N)) or mask.device != dev:
+            raise ValueError("tree_mask must be [N, N] or [B, N, N] on q's device")
+        if mask.dtype not in (torch.bool, torch.uint8, torch.float32):
+            raise ValueError("tree_mask must be bool, uint8 or float32")
+        if mask.stride(-1) != 1:
+            mask = mask.contiguous()
+        a.mask_dtype = _lib.LLIMA_MASK_F32 if mask.dtype == torch.float32 else _lib.LLIMA_MASK_U8
+        a.mask_strides[:] = (mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    kc, vc = _in_place(k_cache, "k_cache"), _in_place(v_cache, "v_cache")
+    out = torch.empty((B, N, Hq, D), dtype=q.dtype, device=dev)
+    if B == 0:
+        return out
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("k_cache", kc), ("v_cache", vc)):
+        setattr(a, name, t.data_ptr())
+        getattr(a, name + "_strides")[:] = t.stride()[:3]
+    a.cache_lens, a.mask = lens.data_ptr(), _ptr(mask)
+    a.block_table = None if table is None else table.data_ptr() or lens.data_ptr()   # (no blocks: not read)
+    a.table_stride = 0 if table is None else table.stride(0)
+    a.dtype = FLOAT_CODES[q.dtype]
+    a.B, a.N, a.Hq, a.Hkv, a.D = B, N, Hq, Hkv, D
+    a.page_size, a.pages, a.max_blocks = page, pages, blocks
+    a.scale = D ** -0.5 if scale is None else float(scale)
+    ws = _scratch(dev, "tree_attention", lib().llima_tree_attention_workspace_bytes(B, N, Hq, Hkv, D))
+    with _on(dev):
+        check(lib().llima_tree_attention(ctypes.byref(a), ws.data_ptr(), ws.numel(), _stream(dev)),
+              "llima_tree_attention")
+    return out
+
+
+def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: torch.Tensor,
+                k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens: torch.Tensor,
+                block_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Keeps the accepted path of each sequence in its cache, in place (llima_tree_commit), and
+    returns the new lengths int32 [B]: token cache_lens[b] + j becomes drafted token
+    nodes[b, j], j < counts[b].
+
+    k, v [B, N, Hkv, D] or, for every layer at once, [layers, B, N, Hkv, D], with caches
+    [B, tokens, Hkv, D] or [pages, page_size, Hkv, D] (and the layers' dimension in front);
+    bf16 or fp16, D a multiple of 8.  nodes int32 [B, L], counts int32 [B] (a row of
+    Eagle3DraftTree's retrieve indices and the accept length + 1; arange and accepted_len + 1
+    for a chain).  A sequence with a count, node, length or page out of range, or no room for
+    its path, is left as it is and its new length is -2 (LLIMA_E_RANGE).  Nothing waits
+    for the device, and the call can be captured into a graph."""
+    if k.dim() == 4:
+        if k_cache.dim() != 4 or v_cache.dim() != 4 or v.dim() != 4:
+            raise ValueError("k and v [B, N, Hkv, D] need 4-dimensional caches")
+        k, v, k_cache, v_cache = k[None], v[None], k_cache[None], v_cache[None]
+    if k.dim() != 5 or k_cache.dim() != 5 or v_cache.dim() != 5:
+        raise ValueError("k and v must be [B, N, Hkv, D] or [layers, B, N, Hkv, D], the caches likewise")
+    layers, B, N, Hkv, D = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("k and v must have one shape and type, bfloat16 or float16")
+    if k_cache.shape[0] != layers or v_cache.shape[0] != layers:
+        raise ValueError("k, v and the caches must have the same number of layers")
+    if N == 0 or Hkv == 0 or D == 0 or D % 8 or layers == 0 or layers > 65535:
+        raise ValueError("1 to 65535 layers, tokens, and heads of a multiple of 8 values are needed")
+    if nodes.dim() != 2 or nodes.shape[0] != B or nodes.shape[1] == 0 or nodes.dtype != torch.int32:
+        raise ValueError("nodes must be int32 [B, L], L at least 1")
+    _on_gpu(k, v, nodes, counts, k_cache, v_cache, cache_lens, block_table)
+    dev = k.device
+    if not (v.device == k_cache.device == v_cache.device == nodes.device == dev):
+        raise ValueError("tree_commit: tensors must be on one device")
+    page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, k.dtype, block_table, B, dev)
+    counts, lens = _ints(counts, B, "counts", dev), _ints(cache_lens, B, "cache_lens", dev)
+    nodes = nodes if nodes.stride(1) == 1 or nodes.shape[1] == 1 else nodes.contiguous()
+    k, v = _heads(k), _heads(v)
+    kc, vc = _in_place(k_cache, "k_cache"), _in_place(v_cache, "v_cache")
+    new = torch.empty(B, dtype=torch.int32, device=dev)
+    if B == 0:
+        return new
+    a = _lib.TreeCommitArgsC()
+    for name, t in (("k", k), ("v", v), ("k_cache", kc), ("v_cache", vc)):
+        setattr(a, name, t.data_ptr())
+        getattr(a, name + "_strides")[:] = t.stride()[:4]
+    a.nodes, a.counts, a.cache_lens = nodes.data_ptr(), counts.data_ptr(), lens.data_ptr()
+    a.new_lens = new.data_ptr()
+    a.block_table = None if table is None else table.data_ptr() or lens.data_ptr()   # (no blocks: not read)
+    a.nodes_stride, a.table_stride = nodes.stride(0), 0 if table is None else table.stride(0)
+    a.layers, a.B, a.N, a.L, a.Hkv, a.D = layers, B, N, nodes.shape[1], Hkv, D
+    a.page_size, a.pages, a.max_blocks = page, pages, blocks
+    with _on(dev):
+        check(lib().llima_tree_commit(ctypes.byref(a), _stream(dev)), "llima_tree_commit")
+    return new

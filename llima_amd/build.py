@@ -24,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libllima_sampler.so")
 SOURCES = ["argmax.hip", "sample.hip", "verify.hip", "score.hip", "lmhead.hip", "tree.hip", "stop.hip",
-           "norm.hip"]
+           "norm.hip", "attention.hip"]
 HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "lmhead_fp8.hpp"),
            os.path.join(ROOT, "include", "llima_sampler.h")]
 ARCH = os.environ.get("LLIMA_OFFLOAD_ARCH", "gfx950")

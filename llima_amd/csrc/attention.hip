@@ -1,0 +1,690 @@
+// attention.hip -- attention of drafted tokens over a KV cache under a tree mask,
+// and the commit of an accepted path into the cache (gfx950).
+//
+//   out[b][n][h] = sum_j p_j v_j,  p = softmax over the visible j of scale q . k_j
+//
+// Keys 0 .. len_b - 1 of sequence b are its cached tokens (every drafted token
+// sees them), keys len_b + m its N drafted tokens, of which node n sees those with
+// mask[b][n][m].  A row that sees nothing is 0.
+//
+// One pass over the keys with the running maximum and sum of the softmax (fp32,
+// base 2).  The products are taken transposed: S^T = K Q^T has a query row in
+// each lane's column, so that a row's maximum and sum are one lane's (and its
+// partner's, lane ^ 32) and the rescaling is a scalar per lane; the lane's 16
+// sums of a block of 32 keys are at once the operand of O^T = V^T P^T, whose key
+// order is the one the lane holds (16 s + e % 4 + 8 (e / 4) + 4 g for element e of
+// half g), and V is read from LDS through the transposing loads in that order.
+// P is rounded to the cache's type for that product (by 2^-8 of a weight at most
+// in bf16, 2^-11 in fp16: the precision of the values it multiplies); the row's
+// sum takes the weights before the rounding.  In fp16 the weights carry a factor
+// of 2^10, so that they become subnormal below 2^-24 of the row's largest.
+//
+// Bound: reading K and V once for all N Hq / Hkv rows of a key head.
+#include "common.hpp"
+#include "../../include/llima_sampler.h"
+
+namespace llima {
+
+struct AttnParams {
+    const void *q, *k, *v, *kc, *vc;
+    void* out;
+    const int32_t* lens;                                     // [B]
+    const void* mask;                                        // [B][N][N] or null (m <= n)
+    const int32_t* table;                                    // [B][max_blocks] or null
+    float* part_o;                                           // [slots][Hkv][R][D]
+    float2* part_ml;                                         // [slots][Hkv][R]
+    int64_t qs[3], ks[3], vs[3], os[3];                      // batch, token and head strides (elements)
+    int64_t kcs[3], vcs[3];                                  // page, token and head strides
+    int64_t ms[2];                                           // mask: batch and row strides
+    int64_t ts;                                              // table row stride
+    int64_t cap;                                             // tokens a sequence has room for
+    int32_t mask_f32;
+    int32_t B, N, Hq, Hkv, G, R;                             // R = N G rows of a key head
+    int32_t page, pages;                                     // tokens of a page; pages of the cache
+    uint32_t page_mul, page_shift;                           // j / page = j page_mul >> page_shift, j < 2^30
+    int32_t slots, ntarget;                                  // key chunks: at most, and wished for
+    int32_t RG, RT;                                          // row groups, row tiles of a group
+    float scale2;                                            // scale log2(e)
+};
+
+#define AT_KEYS (1 << 30)              // keys of a sequence at most
+#define AT_TAB 1024                    // table entries of a chunk kept in LDS
+
+__device__ __forceinline__ uint32_t at_page(const AttnParams& P, int j) {
+    return (uint32_t)(((uint64_t)(uint32_t)j * P.page_mul) >> P.page_shift);
+}
+
+typedef float at_acc __attribute__((ext_vector_type(16)));
+typedef short at_s4 __attribute__((ext_vector_type(4)));
+typedef short at_s8 __attribute__((ext_vector_type(8)));
+
+template <int DT> __device__ __forceinline__ at_acc at_mfma(at_s8 a, at_s8 b, at_acc c) {
+    if constexpr (DT == LLIMA_BF16) {
+        typedef __bf16 t8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
+    } else {
+        typedef _Float16 t8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
+    }
+}
+
+// Two fp32 rounded to the type (to nearest, ties to even).
+template <int DT> __device__ __forceinline__ uint32_t at_pack(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 v = {a, b};
+    if constexpr (DT == LLIMA_BF16) {
+        typedef __bf16 t2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
+    } else {
+        typedef _Float16 t2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
+    }
+}
+
+template <int DT> __device__ __forceinline__ float at_f32(uint16_t h) {
+    if constexpr (DT == LLIMA_BF16) return __uint_as_float((uint32_t)h << 16);
+    else return (float)__builtin_bit_cast(_Float16, h);
+}
+
+// Exponent all ones: an infinity or NaN of the type.
+template <int DT> __device__ __forceinline__ bool at_special(uint16_t h) {
+    constexpr uint32_t e = DT == LLIMA_BF16 ? 0x7F80u : 0x7C00u;
+    return (h & e) == e;
+}
+
+// Sequence b's cached length; a length outside [0, cap] is 0 and bad.
+__device__ __forceinline__ int at_len(const AttnParams& P, int b, bool& bad) {
+    const int l = P.lens[b];
+    bad = l < 0 || l > P.cap;
+    return bad ? 0 : l;
+}
+
+// The partition of all sequences' keys into chunks of one length, a multiple
+// of T: as long as gives at most P.ntarget + B chunks (a sequence's last may be
+// short).  Finds slot's sequence and the chunk's place in it; first is the
+// sequence's first slot.  False past the last chunk.  Every lane of a wave
+// calls it and gets the same.
+template <int T>
+__device__ __forceinline__ int at_chunk(const AttnParams& P) {
+    const int lane = (int)lane_id();
+    int64_t total = 0;
+    for (int b0 = 0; b0 < P.B; b0 += 64) {
+        bool bad;
+        if (b0 + lane < P.B) total += at_len(P, b0 + lane, bad) + P.N;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
+    int64_t c = (total + P.ntarget - 1) / P.ntarget;
+    c = c < AT_KEYS ? c : AT_KEYS;
+    return (int)((c + T - 1) / T) * T;
+}
+
+__device__ __forceinline__ bool at_find(const AttnParams& P, int chunk, int slot, int& b, int& first) {
+    const int lane = (int)lane_id();
+    int before = 0;
+    for (int b0 = 0; b0 < P.B; b0 += 64) {
+        bool bad;
+        const bool in = b0 + lane < P.B;
+        const int n = in ? (at_len(P, in ? b0 + lane : 0, bad) + P.N + chunk - 1) / chunk : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(incl, o, 64);
+            incl += lane >= o ? up : 0;
+        }
+        const uint64_t past = ballot(in && before + incl > slot);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            b = b0 + l;
+            first = before + __shfl(incl - n, l, 64);
+            return true;
+        }
+        before += __shfl(incl, 63, 64);
+    }
+    return false;
+}
+
+__device__ __forceinline__ void at_dma(const void* src, uint8_t* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void at_wait_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// One workgroup: NW waves over one chunk of a sequence's keys, one key head and
+// a group of up to NW / KW row tiles (32 rows each).  Keys come in tiles of T,
+// requested straight into a ring of S stages; KW waves share a row tile and take
+// half of a tile's keys each (KW = 2), or one takes all.
+template <int DT, int D, int NW, int KW, int T, int S>
+__global__ __launch_bounds__(64 * NW) void tree_attn(AttnParams P) {
+    constexpr int U = D / 8;                                 // 16-byte units of a key row
+    constexpr int KQ = 64 / U;                               // keys per 1 KB request
+    constexpr int NQ = (T / KQ + NW - 1) / NW;               // requests per wave and tile, K and V each
+    constexpr int TB = T * D * 2;                            // bytes of a tile of K or V
+    constexpr int KPW = T / 32 / KW;                         // 32-key blocks per wave
+    static_assert(T / KQ % NW == 0 || NQ == 1, "requests split evenly");
+    static_assert(KPW >= 1, "a block per wave");
+    // one array: with several the compiler waits for every request before each LDS read
+    __shared__ __align__(1024) uint8_t sm[S * 2 * TB + 4 * AT_TAB + 16];
+    int32_t* const tab = (int32_t*)(sm + S * 2 * TB);
+    uint32_t* const flag = (uint32_t*)(sm + S * 2 * TB + 4 * AT_TAB);   // a bad page or length; special values
+    const int t = (int)threadIdx.x, lane = t & 63, g = lane >> 5, r = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int rw = wave / KW, kw = wave % KW;
+    const int h = (int)(blockIdx.x % (uint32_t)P.Hkv), rg = (int)(blockIdx.x / (uint32_t)P.Hkv % (uint32_t)P.RG);
+    const int slot = (int)(blockIdx.x / (uint32_t)(P.Hkv * P.RG));
+    const int chunk = at_chunk<T>(P);
+    int b, first;
+    if (!at_find(P, chunk, slot, b, first)) return;          // uniform
+    b = __builtin_amdgcn_readfirstlane(b);
+    first = __builtin_amdgcn_readfirstlane(first);
+    bool bad;
+    const int len = __builtin_amdgcn_readfirstlane(at_len(P, b, bad));
+    const int nkeys = len + P.N, nchunk = (nkeys + chunk - 1) / chunk;
+    const int j0 = (slot - first) * chunk, j1 = j0 + chunk < nkeys ? j0 + chunk : nkeys;
+    const int ntile = (j1 - j0 + T - 1) / T;
+    if (t == 0) { flag[0] = bad ? 1u : 0u; flag[1] = 0u; }
+    // the chunk's table entries
+    const int jc = j1 < len ? j1 : len;                      // its cached keys end here
+    const uint32_t e0 = P.table ? at_page(P, j0) : 0u;
+    const int ne = P.table && jc > j0 ? (int)(at_page(P, jc - 1) - e0) + 1 : 0;
+    const bool in_lds = ne <= AT_TAB;                        // uniform
+    if (in_lds)
+        for (int i = t; i < ne; i += 64 * NW) tab[i] = P.table[b * P.ts + e0 + i];
+    // the wave's rows: node n and query head of row tile rw
+    const int row = (rg * P.RT + rw) * 32 + r;
+    const bool active = rw < P.RT && (rg * P.RT + rw) * 32 < P.R;   // uniform: the wave has rows
+    const int rc = row < P.R ? row : P.R - 1;
+    const int n = rc / P.G, hq = h * P.G + rc % P.G;
+    at_s8 qf[D / 16];
+    {
+        const uint16_t* qp = (const uint16_t*)P.q + b * P.qs[0] + n * P.qs[1] + hq * P.qs[2] + g * 8;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) qf[s] = *(const at_s8*)(qp + s * 16);
+    }
+    // requests: the lane's key of request i of a tile and its 16-byte unit
+    const int kq = lane / U, unit = lane % U;
+    auto key_at = [&](int tile, int i) {                     // a key of the chunk (past its end: the last)
+        const int j = j0 + tile * T + (wave + NW * i) * KQ + kq;
+        return j < j1 ? j : j1 - 1;
+    };
+    bool miss = false;
+    auto issue = [&](int tile, int st) {
+        uint8_t* const sk = sm + st * 2 * TB;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int qi = wave + NW * i;                    // request of the tile
+            if (T / KQ % NW == 0 || qi < T / KQ) {           // uniform
+                const int kt = qi * KQ + kq;                 // the key's place in the tile
+                const int j = key_at(tile, i);
+                const uint16_t *kp, *vp;
+                if (j < len) {
+                    int64_t p = b, o = j;
+                    if (P.table) {                           // uniform
+                        const uint32_t e = at_page(P, j);
+                        o = j - (int)e * P.page;
+                        int pi;
+                        if (in_lds) {                        // uniform
+                            pi = tab[e - e0];
+                        } else {
+                            pi = P.table[b * P.ts + e];
+                            __builtin_amdgcn_s_waitcnt(LLIMA_WAITCNT_VM0);
+                        }
+                        if (pi < 0 || pi >= P.pages) { pi = 0; miss = true; }
+                        p = pi;
+                    }
+                    kp = (const uint16_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2];
+                    vp = (const uint16_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2];
+                } else {
+                    kp = (const uint16_t*)P.k + b * P.ks[0] + (j - len) * P.ks[1] + h * P.ks[2];
+                    vp = (const uint16_t*)P.v + b * P.vs[0] + (j - len) * P.vs[1] + h * P.vs[2];
+                }
+                at_dma(kp + ((unit ^ (kt & (U - 1) & 15)) * 8), sk + qi * 1024);
+                at_dma(vp + ((unit ^ ((kt & 3) << 2 & (U - 1))) * 8), sk + TB + qi * 1024);
+            }
+        }
+    };
+    at_acc o[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+    if (ne > 0) __syncthreads();                             // uniform
+#pragma unroll
+    for (int e = 0; e < S - 1; ++e) issue(e < ntile ? e : ntile - 1, e);
+    for (int tile = 0; tile < ntile; ++tile) {
+        at_wait_barrier<(S - 2) * 2 * NQ>();                 // the tile has landed, and the last one is read
+        {
+            const int nt = tile + S - 1;                     // past the last: the last again, into a free stage
+            issue(nt < ntile ? nt : ntile - 1, nt % S);
+        }
+        uint8_t* const sk = sm + (tile % S) * 2 * TB;
+        const int jt = j0 + tile * T;
+        const bool tail = jt + T > len;                      // uniform: drafted keys, or past the end
+        if (tail) {
+            // Values that not every row sees: rows past the end become 0, and so
+            // do infinities and NaN of drafted tokens (0 times them would be NaN
+            // for the rows that do not see them; at the end they are added to the
+            // rows that do).
+            for (int p = t; p < T * U; p += 64 * NW) {
+                const int kt = p / U, j = jt + kt;
+                llima_u32x4* const at = (llima_u32x4*)(sk + TB + p * 16);
+                llima_u32x4 x = *at;
+                bool put = j >= j1;
+                if (put) x = (llima_u32x4){0u, 0u, 0u, 0u};
+                if (!put && j >= len) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t w = x[e];
+                        if (at_special<DT>((uint16_t)w)) { w &= 0xFFFF0000u; put = true; flag[1] = 1u; }
+                        if (at_special<DT>((uint16_t)(w >> 16))) { w &= 0xFFFFu; put = true; flag[1] = 1u; }
+                        x[e] = w;
+                    }
+                }
+                if (put) *at = x;
+            }
+            __syncthreads();
+        }
+        if (!active) continue;                               // uniform (the barriers are above)
+        at_acc s[KPW];
+#pragma unroll
+        for (int kb = 0; kb < KPW; ++kb) {
+            const int kt = (kw * KPW + kb) * 32 + r;         // the lane's key row of the K operand
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                const at_s8 kf = *(const at_s8*)(sk + kt * (D * 2) + (((2 * d + g) ^ (kt & (U - 1) & 15)) << 4));
+                s[kb] = at_mfma<DT>(kf, qf[d], s[kb]);
+            }
+        }
+        float mt = -__builtin_inff();
+#pragma unroll
+        for (int kb = 0; kb < KPW; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float x = s[kb][i] * P.scale2;
+                if (tail) {                                  // uniform
+                    const int j = jt + (kw * KPW + kb) * 32 + (i & 3) + 8 * (i >> 2) + 4 * g;
+                    bool see = j < len;
+                    if (!see && j < j1) {
+                        const int mm = j - len;
+                        if (!P.mask) see = mm <= n;
+                        else if (P.mask_f32) see = ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
+                        else see = ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
+                    }
+                    x = see ? x : -__builtin_inff();
+                }
+                s[kb][i] = x;
+                mt = __builtin_fmaxf(mt, x);
+            }
+        mt = __builtin_fmaxf(mt, __shfl_xor(mt, 32, 64));
+        const float mn = __builtin_fmaxf(m, mt);
+        const float mu = mn > -__builtin_inff() ? mn : 0.0f;
+        const float mup = DT == LLIMA_F16 ? mu - 10.0f : mu;
+        if (__any(mn > m)) {                                 // else the factor is 1 for every row
+            const float a = __builtin_amdgcn_exp2f(m - mu);
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= a;
+            m = mn;
+        }
+#pragma unroll
+        for (int kb = 0; kb < KPW; ++kb) {
+            float ls = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] - mup);
+                ls += s[kb][i];
+            }
+            l += ls;
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {                 // 16 keys of the block
+                uint32_t pw[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pw[e] = at_pack<DT>(s[kb][8 * st + 2 * e], s[kb][8 * st + 2 * e + 1]);
+                const at_s8 pf = __builtin_bit_cast(at_s8, (llima_u32x4){pw[0], pw[1], pw[2], pw[3]});
+                // element e of half g is key 16 st + e % 4 + 8 (e / 4) + 4 g: a
+                // transposing load takes 4 keys by 16 columns from 16 lanes
+                const int kk = (kw * KPW + kb) * 32 + st * 16 + 4 * g + (lane >> 2 & 3);
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    const int c8 = d * 8 + (lane >> 4 & 1) * 4 + (lane & 3);      // 8-byte piece of the row
+                    auto vload = [&](int key) {
+                        const uint8_t* a = sk + TB + key * (D * 2) + (((c8 >> 1) ^ ((key & 3) << 2 & (U - 1))) << 4) + (c8 & 1) * 8;
+                        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)a);
+                    };
+                    const at_s4 v0 = vload(kk), v1 = vload(kk + 8);
+                    const at_s8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[d] = at_mfma<DT>(vf, pf, o[d]);
+                }
+            }
+        }
+    }
+    if (miss) flag[0] = 1u;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no request outlives this
+    __syncthreads();
+    l += __shfl_xor(l, 32, 64);
+    if constexpr (KW > 1) {                                  // the second half of the keys joins the first
+        float* const red = (float*)sm + (size_t)rw * 64 * (D / 2 + 2);
+        if (active && kw == 1) {
+            red[lane] = m;
+            red[64 + lane] = l;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) red[(2 + d * 16 + i) * 64 + lane] = o[d][i];
+        }
+        __syncthreads();
+        if (kw == 1) return;
+        if (active) {
+            const float m2 = red[lane], mn = __builtin_fmaxf(m, m2), mu = mn > -__builtin_inff() ? mn : 0.0f;
+            const float a = __builtin_amdgcn_exp2f(m - mu), a2 = __builtin_amdgcn_exp2f(m2 - mu);
+            m = mn;
+            l = l * a + red[64 + lane] * a2;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * a + red[(2 + d * 16 + i) * 64 + lane] * a2;
+        }
+    }
+    if (!active || row >= P.R) return;
+    if (flag[1]) {                                          // infinities and NaN of drafted tokens in this chunk
+        for (int mm = (j0 > len ? j0 : len) - len; mm < j1 - len; ++mm) {
+            bool see;
+            if (!P.mask) see = mm <= n;
+            else if (P.mask_f32) see = ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
+            else see = ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
+            if (!see) continue;
+            const uint16_t* vp = (const uint16_t*)P.v + b * P.vs[0] + mm * P.vs[1] + h * P.vs[2];
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint16_t x = vp[d * 32 + (i & 3) + 8 * (i >> 2) + 4 * g];
+                    if (at_special<DT>(x)) o[d][i] += at_f32<DT>(x);
+                }
+        }
+    }
+    if (flag[0]) l = __builtin_nanf("");
+    if (nchunk == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing seen: 0
+        uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + 4 * g;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(uint2*)(op + d * 32 + 2 * i) = make_uint2(at_pack<DT>(o[d][i] * inv, o[d][i + 1] * inv),
+                                                            at_pack<DT>(o[d][i + 2] * inv, o[d][i + 3] * inv));
+    } else {
+        const size_t at = ((size_t)slot * P.Hkv + h) * P.R + row;
+        if (g == 0) P.part_ml[at] = make_float2(m, l);
+        float* op = P.part_o + at * D + 4 * g;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(float4*)(op + d * 32 + 2 * i) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+    }
+}
+
+// Joins the chunks of each row: a wave per (sequence, node, query head).
+template <int DT, int D, int T>
+__global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
+    constexpr int E = D / 64;                                // values per lane
+    const int lane = (int)lane_id(), chunk = at_chunk<T>(P);
+    const int64_t w = (int64_t)blockIdx.x * LLIMA_WAVES + wave_id();
+    if (w >= (int64_t)P.B * P.N * P.Hq) return;
+    const int b = (int)(w / (P.N * P.Hq)), n = (int)(w / P.Hq % P.N), hq = (int)(w % P.Hq);
+    // the sequence's first chunk
+    int first = 0;
+    for (int i = lane; i < b; i += 64) {
+        bool bad;
+        first += (at_len(P, i, bad) + P.N + chunk - 1) / chunk;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
+    bool bad;
+    const int nchunk = (at_len(P, b, bad) + P.N + chunk - 1) / chunk;
+    if (nchunk <= 1) return;
+    const int h = hq / P.G, row = n * P.G + hq % P.G;
+    const size_t step = (size_t)P.Hkv * P.R, at0 = ((size_t)first * P.Hkv + h) * P.R + row;
+    float m = -__builtin_inff(), l = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    // the greatest maximum first (a lane per chunk), then one pass of weighted sums
+    for (int c = lane; c < nchunk; c += 64) m = __builtin_fmaxf(m, P.part_ml[at0 + c * step].x);
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, x, 64));
+    const float mu = m > -__builtin_inff() ? m : 0.0f;
+#pragma unroll 4
+    for (int c = 0; c < nchunk; ++c) {
+        const float2 ml = P.part_ml[at0 + c * step];
+        const float a = __builtin_amdgcn_exp2f(ml.x - mu);
+        l += ml.y * a;
+        const float* po = P.part_o + (at0 + c * step) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += po[e] * a;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + lane * E;
+    if constexpr (E == 1) op[0] = (uint16_t)at_pack<DT>(o[0] * inv, 0.0f);
+#pragma unroll
+    for (int e = 0; e + 1 < E; e += 2) *(uint32_t*)(op + e) = at_pack<DT>(o[e] * inv, o[e + 1] * inv);
+}
+
+struct CommitParams {
+    const uint8_t *k, *v;
+    uint8_t *kc, *vc;
+    const int32_t *nodes, *counts, *lens, *table;
+    int32_t* new_lens;
+    int64_t ks[4], vs[4];                                    // layer, batch, node and head strides (bytes)
+    int64_t kcs[4], vcs[4];                                  // layer, page, token and head strides
+    int64_t ns, ts, cap;
+    int32_t B, N, L, Hkv, U;                                 // U: 16-byte units of a head's row
+    int32_t page, pages;
+};
+
+// One workgroup per (path place, sequence, layer): checks the sequence's path
+// and room (every workgroup of a sequence comes to the same answer), then
+// copies one token's K and V rows.
+__global__ __launch_bounds__(LLIMA_WG) void tree_commit(CommitParams P) {
+    const int j = (int)(blockIdx.x % (uint32_t)P.L), b = (int)(blockIdx.x / (uint32_t)P.L), t = (int)threadIdx.x;
+    const int64_t layer = blockIdx.y;
+    const int len = P.lens[b], cnt = P.counts[b];
+    bool ok = len >= 0 && cnt >= 0 && cnt <= P.L && len <= P.cap && (int64_t)len + cnt <= P.cap;
+    if (ok) {
+        bool all = true;
+        for (int i = t & 63; i < cnt; i += 64) {
+            const int node = P.nodes[b * P.ns + i];
+            all = all && node >= 0 && node < P.N;
+            if (P.table) {
+                const int p = P.table[b * P.ts + (uint32_t)(len + i) / (uint32_t)P.page];
+                all = all && p >= 0 && p < P.pages;
+            }
+        }
+        ok = __all(all);
+    }
+    if (j == 0 && layer == 0 && t == 0) P.new_lens[b] = ok ? len + cnt : LLIMA_E_RANGE;
+    if (!ok || j >= cnt) return;                             // uniform
+    const int64_t node = P.nodes[b * P.ns + j];
+    int64_t p = b, o = len + j;
+    if (P.table) {
+        p = P.table[b * P.ts + (uint32_t)(len + j) / (uint32_t)P.page];
+        o = (uint32_t)(len + j) % (uint32_t)P.page;
+    }
+    const int n = P.Hkv * P.U;
+    for (int i = t; i < 2 * n; i += LLIMA_WG) {
+        const bool isv = i >= n;
+        const int e = isv ? i - n : i, h = e / P.U, u = e % P.U;
+        const int64_t* fs = isv ? P.vs : P.ks;
+        const int64_t* ts = isv ? P.vcs : P.kcs;
+        const uint8_t* src = (isv ? P.v : P.k) + layer * fs[0] + b * fs[1] + node * fs[2] + h * fs[3] + u * 16;
+        uint8_t* dst = (isv ? P.vc : P.kc) + layer * ts[0] + p * ts[1] + o * ts[2] + h * ts[3] + u * 16;
+        *(llima_u32x4*)dst = *(const llima_u32x4*)src;
+    }
+}
+
+// Key chunks wished for: enough workgroups to fill the device twice.
+static int at_ntarget(int Hkv, int RG) {
+    const int n = 512 / (Hkv * RG);
+    return n < 1 ? 1 : n;
+}
+
+static int at_row_tiles(int R, int& RG) {                    // row tiles of a group, groups
+    const int rt = (R + 31) / 32;
+    RG = (rt + 7) / 8;
+    return (rt + RG - 1) / RG;
+}
+
+template <int DT, int D>
+static void at_launch(const AttnParams& P, hipStream_t st) {
+    const dim3 g((uint32_t)P.slots * P.RG * P.Hkv);
+    constexpr int T = D == 256 ? 32 : 64, KW = D == 256 ? 1 : 2;
+    constexpr int S2 = D == 64 ? 4 : 2, S8 = 4;
+    if (P.RT <= (KW == 2 ? 1 : 2)) hipLaunchKernelGGL((tree_attn<DT, D, 2, KW, T, S2>), g, dim3(128), 0, st, P);
+    else if (P.RT <= (KW == 2 ? 2 : 4)) hipLaunchKernelGGL((tree_attn<DT, D, 4, KW, T, S2>), g, dim3(256), 0, st, P);
+    else if (KW == 2 && P.RT <= 4) hipLaunchKernelGGL((tree_attn<DT, D, 8, KW, T, S8>), g, dim3(512), 0, st, P);
+    else hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8>), g, dim3(512), 0, st, P);
+    const int64_t rows = (int64_t)P.B * P.N * P.Hq;
+    hipLaunchKernelGGL((tree_attn_join<DT, D, T>), dim3((uint32_t)((rows + LLIMA_WAVES - 1) / LLIMA_WAVES)),
+                       dim3(LLIMA_WG), 0, st, P);
+}
+
+template <int DT>
+static int at_dispatch(const AttnParams& P, int D, hipStream_t st) {
+    if (D == 64) at_launch<DT, 64>(P, st);
+    else if (D == 128) at_launch<DT, 128>(P, st);
+    else at_launch<DT, 256>(P, st);
+    return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
+}
+
+}  // namespace llima
+
+using namespace llima;
+
+static bool at_sizes_ok(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D) {
+    if (B < 0 || N <= 0 || N > 1024 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq > 1024) return false;
+    if (D != 64 && D != 128 && D != 256) return false;
+    return (int64_t)B * N * Hq <= (1 << 28);
+}
+
+static void at_plan(AttnParams& P) {
+    P.R = P.N * P.G;
+    P.RT = at_row_tiles(P.R, P.RG);
+    P.ntarget = at_ntarget(P.Hkv, P.RG);
+    P.slots = P.ntarget + P.B;
+}
+
+extern "C" size_t llima_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq,
+                                                       int32_t Hkv, int32_t D) {
+    if (B <= 0 || !at_sizes_ok(B, N, Hq, Hkv, D)) return 0;
+    AttnParams P = {};
+    P.B = B; P.N = N; P.Hkv = Hkv; P.G = Hq / Hkv;
+    at_plan(P);
+    const size_t rows = (size_t)P.slots * Hkv * P.R;
+    return (rows * D * sizeof(float) + 255) / 256 * 256 + rows * sizeof(float2);
+}
+
+// Strides are multiples of 8 elements (16 bytes), so every row is aligned as
+// its base pointer is.
+static bool at_strides_ok(const int64_t* s, int n) {
+    for (int i = 0; i < n; ++i)
+        if (s[i] < 0 || s[i] % 8 != 0) return false;
+    return true;
+}
+
+extern "C" int llima_tree_attention(const llima_tree_attention_args* a, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    if (!a || !at_sizes_ok(a->B, a->N, a->Hq, a->Hkv, a->D)) return LLIMA_E_INVAL;
+    if (a->dtype != LLIMA_BF16 && a->dtype != LLIMA_F16) return LLIMA_E_INVAL;
+    if (!(a->scale == a->scale) || __builtin_isinf(a->scale)) return LLIMA_E_INVAL;
+    if (a->page_size <= 0 || a->pages < 0 || a->max_blocks < 0) return LLIMA_E_INVAL;
+    if (!a->block_table && (a->pages < a->B || a->max_blocks != 1)) return LLIMA_E_INVAL;
+    if ((int64_t)a->page_size * a->max_blocks + a->N > AT_KEYS) return LLIMA_E_INVAL;
+    if (a->mask_dtype != LLIMA_MASK_U8 && a->mask_dtype != LLIMA_MASK_F32) return LLIMA_E_INVAL;
+    if (!at_strides_ok(a->q_strides, 3) || !at_strides_ok(a->k_strides, 3) || !at_strides_ok(a->v_strides, 3) ||
+        !at_strides_ok(a->out_strides, 3) || !at_strides_ok(a->k_cache_strides, 3) ||
+        !at_strides_ok(a->v_cache_strides, 3))
+        return LLIMA_E_INVAL;
+    if (a->mask && (a->mask_strides[0] < 0 || a->mask_strides[1] < 0)) return LLIMA_E_INVAL;
+    if (a->block_table && a->table_stride < 0) return LLIMA_E_INVAL;
+    if (a->B == 0) return LLIMA_OK;
+    const bool cached = a->pages > 0 && a->max_blocks > 0;   // else no sequence may have a cached token
+    if (!a->q || !a->k || !a->v || !a->out || !a->cache_lens || (cached && (!a->k_cache || !a->v_cache)))
+        return LLIMA_E_INVAL;
+    const void* ptrs[] = {a->q, a->k, a->v, a->out, a->k_cache, a->v_cache};
+    for (const void* p : ptrs)
+        if ((uintptr_t)p % 16) return LLIMA_E_INVAL;
+    if (!workspace || workspace_bytes < llima_tree_attention_workspace_bytes(a->B, a->N, a->Hq, a->Hkv, a->D))
+        return LLIMA_E_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return LLIMA_E_INVAL;
+    AttnParams P = {};
+    P.q = a->q; P.k = a->k; P.v = a->v; P.kc = a->k_cache; P.vc = a->v_cache; P.out = a->out;
+    P.lens = a->cache_lens; P.mask = a->mask; P.table = a->block_table;
+    for (int i = 0; i < 3; ++i) {
+        P.qs[i] = a->q_strides[i]; P.ks[i] = a->k_strides[i]; P.vs[i] = a->v_strides[i];
+        P.os[i] = a->out_strides[i]; P.kcs[i] = a->k_cache_strides[i]; P.vcs[i] = a->v_cache_strides[i];
+    }
+    P.ms[0] = a->mask_strides[0]; P.ms[1] = a->mask_strides[1];
+    P.ts = a->table_stride;
+    P.cap = cached ? (int64_t)a->page_size * a->max_blocks : 0;
+    P.mask_f32 = a->mask_dtype == LLIMA_MASK_F32;
+    P.B = a->B; P.N = a->N; P.Hq = a->Hq; P.Hkv = a->Hkv; P.G = a->Hq / a->Hkv;
+    P.page = a->page_size; P.pages = a->pages;
+    // l = ceil(log2 page): mul = ceil(2^(30 + l) / page) <= 2^31 + 1 exceeds the
+    // quotient by less than page / 2^(30 + l) <= 2^-30 of j
+    uint32_t l = 0;
+    while ((1ll << l) < P.page) ++l;
+    P.page_mul = (uint32_t)(((1ull << (30 + l)) + P.page - 1) / (uint64_t)P.page);
+    P.page_shift = 30 + l;
+    P.scale2 = a->scale * 1.44269504088896340736f;
+    at_plan(P);
+    const size_t rows = (size_t)P.slots * P.Hkv * P.R;
+    P.part_o = (float*)workspace;
+    P.part_ml = (float2*)((uint8_t*)workspace + (rows * a->D * sizeof(float) + 255) / 256 * 256);
+    return a->dtype == LLIMA_BF16 ? at_dispatch<LLIMA_BF16>(P, a->D, (hipStream_t)stream)
+                                  : at_dispatch<LLIMA_F16>(P, a->D, (hipStream_t)stream);
+}
+
+extern "C" int llima_tree_commit(const llima_tree_commit_args* a, void* stream) {
+    if (!a || a->layers <= 0 || a->layers > 65535 || a->B < 0 || a->N <= 0 || a->L <= 0 || a->Hkv <= 0 || a->D <= 0)
+        return LLIMA_E_INVAL;
+    if (a->D % 8 != 0 || a->D > 65536 || a->Hkv > 65536 || (int64_t)a->Hkv * a->D > (1 << 24)) return LLIMA_E_INVAL;
+    if (a->page_size <= 0 || a->pages < 0 || a->max_blocks < 0) return LLIMA_E_INVAL;
+    if (!a->block_table && (a->pages < a->B || a->max_blocks != 1)) return LLIMA_E_INVAL;
+    if ((int64_t)a->page_size * a->max_blocks > (int64_t)INT32_MAX) return LLIMA_E_INVAL;
+    if ((int64_t)a->B * a->L > (int64_t)INT32_MAX) return LLIMA_E_INVAL;
+    if (!at_strides_ok(a->k_strides, 4) || !at_strides_ok(a->v_strides, 4) || !at_strides_ok(a->k_cache_strides, 4) ||
+        !at_strides_ok(a->v_cache_strides, 4) || a->nodes_stride < 0 || (a->block_table && a->table_stride < 0))
+        return LLIMA_E_INVAL;
+    if (a->B == 0) return LLIMA_OK;
+    const bool cached = a->pages > 0 && a->max_blocks > 0;
+    if (!a->nodes || !a->counts || !a->cache_lens || !a->new_lens) return LLIMA_E_INVAL;
+    if (!a->k || !a->v || (cached && (!a->k_cache || !a->v_cache))) return LLIMA_E_INVAL;
+    const void* ptrs[] = {a->k, a->v, a->k_cache, a->v_cache};
+    for (const void* p : ptrs)
+        if ((uintptr_t)p % 16) return LLIMA_E_INVAL;
+    CommitParams P = {};
+    P.k = (const uint8_t*)a->k; P.v = (const uint8_t*)a->v;
+    P.kc = (uint8_t*)a->k_cache; P.vc = (uint8_t*)a->v_cache;
+    P.nodes = a->nodes; P.counts = a->counts; P.lens = a->cache_lens; P.table = a->block_table;
+    P.new_lens = a->new_lens;
+    for (int i = 0; i < 4; ++i) {
+        P.ks[i] = 2 * a->k_strides[i]; P.vs[i] = 2 * a->v_strides[i];
+        P.kcs[i] = 2 * a->k_cache_strides[i]; P.vcs[i] = 2 * a->v_cache_strides[i];
+    }
+    P.ns = a->nodes_stride; P.ts = a->table_stride;
+    P.cap = a->pages > 0 ? (int64_t)a->page_size * a->max_blocks : 0;
+    P.B = a->B; P.N = a->N; P.L = a->L; P.Hkv = a->Hkv; P.U = a->D / 8;
+    P.page = a->page_size; P.pages = a->pages;
+    hipLaunchKernelGGL(tree_commit, dim3((uint32_t)(a->B * a->L), (uint32_t)a->layers), dim3(LLIMA_WG), 0,
+                       (hipStream_t)stream, P);
+    return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
+}

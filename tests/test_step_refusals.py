@@ -95,3 +95,102 @@ def test_python_refuses_on_host_tensors_and_shapes():
                  lambda: llima_amd.Fp8LmHead(x.to(F8), torch.zeros(2, 1))):
         with pytest.raises(ValueError):
             call()
+
+
+def attention_args(**kw):
+    from llima_amd import _lib
+    a = _lib.TreeAttentionArgsC()
+    for n in ("q", "k", "v", "k_cache", "v_cache", "out", "cache_lens", "mask", "block_table"):
+        setattr(a, n, 4096)
+    for n in ("q_strides", "k_strides", "v_strides", "out_strides", "k_cache_strides", "v_cache_strides"):
+        getattr(a, n)[:] = (4096, 512, 128)
+    a.mask_strides[:] = (16, 4)
+    a.table_stride = 8
+    for n, x in dict(dtype=1, mask_dtype=0, B=2, N=4, Hq=8, Hkv=4, D=128, page_size=16, pages=20, max_blocks=8,
+                     scale=0.1).items():
+        setattr(a, n, x)
+    for n, x in kw.items():
+        if isinstance(x, tuple):
+            getattr(a, n)[:] = x
+        else:
+            setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=0), dict(dtype=3), dict(B=-1), dict(N=0), dict(N=1025), dict(Hq=0), dict(Hq=9), dict(Hkv=0),
+    dict(Hq=1028), dict(D=96), dict(D=0), dict(page_size=0), dict(pages=-1), dict(max_blocks=-1),
+    dict(block_table=None), dict(block_table=None, max_blocks=1, pages=1), dict(scale=float("nan")),
+    dict(scale=float("inf")), dict(mask_dtype=2), dict(q_strides=(4096, 512, 129)), dict(k_strides=(-8, 512, 128)),
+    dict(out_strides=(4, 512, 128)), dict(k_cache_strides=(4096, 511, 128)), dict(mask_strides=(-1, 4)),
+    dict(table_stride=-1), dict(q=None), dict(q=4104), dict(k=None), dict(v=4100), dict(out=None), dict(cache_lens=None),
+    dict(k_cache=None), dict(v_cache=4097), dict(page_size=1 << 28, max_blocks=4), dict(B=1 << 20, N=1024)])
+def test_attention_refuses(bad):
+    a = attention_args(**bad)
+    assert L().llima_tree_attention(ctypes.byref(a), P, BIG << 10, None) == -1
+
+
+def test_attention_workspace_and_empty_batch():
+    l = L()
+    a = attention_args()
+    need = l.llima_tree_attention_workspace_bytes(2, 4, 8, 4, 128)
+    assert need > 0 and l.llima_tree_attention_workspace_bytes(2, 4, 8, 4, 96) == 0
+    assert l.llima_tree_attention(ctypes.byref(a), N, need, None) == -4
+    assert l.llima_tree_attention(ctypes.byref(a), P, need - 1, None) == -4
+    assert l.llima_tree_attention(ctypes.byref(a), ctypes.c_void_p(24), need, None) == -1
+    assert l.llima_tree_attention(None, P, need, None) == -1
+    a = attention_args(B=0, q=None, k=None, v=None, out=None, cache_lens=None)
+    assert l.llima_tree_attention(ctypes.byref(a), N, 0, None) == 0
+
+
+def commit_args(**kw):
+    from llima_amd import _lib
+    a = _lib.TreeCommitArgsC()
+    for n in ("k", "v", "k_cache", "v_cache", "nodes", "counts", "cache_lens", "block_table", "new_lens"):
+        setattr(a, n, 4096)
+    for n in ("k_strides", "v_strides", "k_cache_strides", "v_cache_strides"):
+        getattr(a, n)[:] = (65536, 4096, 512, 128)
+    a.nodes_stride, a.table_stride = 3, 8
+    for n, x in dict(layers=2, B=2, N=4, L=3, Hkv=4, D=128, page_size=16, pages=20, max_blocks=8).items():
+        setattr(a, n, x)
+    for n, x in kw.items():
+        if isinstance(x, tuple):
+            getattr(a, n)[:] = x
+        else:
+            setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("bad", [
+    dict(layers=0), dict(layers=65536), dict(B=-1), dict(N=0), dict(L=0), dict(Hkv=0), dict(D=0), dict(D=12), dict(D=131072),
+    dict(page_size=0), dict(pages=-1), dict(max_blocks=-1), dict(block_table=None), dict(k=None), dict(v=None),
+    dict(k_cache=None), dict(v_cache=4104), dict(k=4104), dict(nodes=None), dict(counts=None), dict(cache_lens=None),
+    dict(new_lens=None), dict(k_strides=(65536, 4096, 512, 4)), dict(v_cache_strides=(65536, -8, 512, 128)),
+    dict(nodes_stride=-1), dict(table_stride=-1), dict(page_size=1 << 30, max_blocks=2), dict(B=1 << 20, L=1 << 12)])
+def test_commit_refuses(bad):
+    assert L().llima_tree_commit(ctypes.byref(commit_args(**bad)), None) == -1
+    assert L().llima_tree_commit(None, None) == -1
+
+
+def test_commit_of_no_sequences():
+    a = commit_args(B=0, k=None, v=None, nodes=None, counts=None, cache_lens=None, new_lens=None)
+    assert L().llima_tree_commit(ctypes.byref(a), None) == 0
+
+
+def test_python_attention_refuses():
+    import llima_amd
+    bf = torch.bfloat16
+    q, k = torch.zeros(2, 3, 8, 64, dtype=bf), torch.zeros(2, 3, 4, 64, dtype=bf)
+    c, n = torch.zeros(2, 10, 4, 64, dtype=bf), torch.zeros(2, dtype=torch.int32)
+    f, g = llima_amd.tree_attention, llima_amd.tree_commit
+    p, m = torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    for call in (lambda: f(q, k, k, c, c, n), lambda: f(q[0], k, k, c, c, n), lambda: f(q[:1], k, k, c, c, n),
+                 lambda: f(q, k, k[:, :2], c, c, n), lambda: f(q.float(), k, k, c, c, n), lambda: f(q, k.half(), k, c, c, n),
+                 lambda: f(q[..., :32], k[..., :32], k[..., :32], c, c, n), lambda: f(q[:, :, :6], k, k, c, c, n),
+                 lambda: f(q[:, :0], k[:, :0], k[:, :0], c, c, n), lambda: g(k, k, p, m, c, c, n),
+                 lambda: g(k, k[:, :2], p, m, c, c, n), lambda: g(k, k, p[:, :0], m, c, c, n),
+                 lambda: g(k, k, p.long(), m, c, c, n), lambda: g(k[None], k[None], p, m, c, c, n),
+                 lambda: g(k.float(), k.float(), p, m, c, c, n), lambda: g(k[0], k[0], p, m, c, c, n),
+                 lambda: g(k[None].expand(2, 2, 3, 4, 64), k[None].expand(2, 2, 3, 4, 64), p, m, c[None], c[None], n)):
+        with pytest.raises(ValueError):
+            call()
