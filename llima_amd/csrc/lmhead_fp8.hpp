@@ -5,13 +5,25 @@
 //   s[b][v] = sum over kb of (xs[b][kb] ws[v / 128][kb]) p,
 //   p       = sum over the block's k of xq[b][k] wq[v][k]
 //
-// p is one block's sum in the matrix core (products of e4m3 values are exact in
-// fp32), scaled and added in fp32; then softcap, rounding and argmax as the
-// bf16 head (lmh_logit).  xq [B][H] and xs [B][NK] are a hidden row's values
+// p is one block's sum in the matrix core, scaled and added in fp32; then
+// softcap, rounding and argmax as the bf16 head (lmh_logit).  The values go into
+// the matrix core as bf16, which holds every e4m3 value: its 8-bit instructions
+// are twice as fast but drop low bits of the products when they add them (128
+// products of values from N(0, 60^2): off by 2^-16 of the terms' magnitude at
+// most, by 2^-12 where one product in 64 is 2^11 times the others; the bf16
+// instructions 2^-25 and 2^-22), which is not a sum in 32 bits.  xq [B][H] and xs [B][NK] are a hidden row's values
 // and scales, wq [V][H] and ws [ceil(V/128)][NK] the weight's, NK = ceil(H/128).
 #pragma once
 
-typedef int lmh8_i8 __attribute__((ext_vector_type(8)));
+// Eight e4m3 values as bf16 (exact; NaN stays NaN).
+__device__ __forceinline__ lmh_b8 lmh8_wide(uint32_t lo, uint32_t hi) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+    const b2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+    const b2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return (lmh_b8){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
 
 struct Lmh8Params {
     LmhParams P;
@@ -105,8 +117,8 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[32]
 // row % 16 (the request's source address does it): fragment reads have no bank
 // conflicts.  The weight is the MFMA's row operand: lane (r, g) has for hidden
 // row r the sums of 32 of the tile's 64 vocab rows (the lane with the other g
-// the others).  k order within a block: step s takes pieces 4 s + g, 4 s + 2 + g
-// of 16 ids, for both operands.
+// the others).  k order within a block: piece e of 16 ids of half g is ids
+// 32 e + 16 g .. + 15, its halves two steps, for both operands.
 //
 // 512 contiguous bytes per row: read 128 bytes at a time (a tile of 256 rows)
 // the weight streams at 4.8 TB/s, this way at 5.6 to 5.9 (0.53 GB, requests alone).
@@ -185,22 +197,29 @@ __global__ __launch_bounds__(256, 2) void lmh8_rows(Lmh8Params Q, int b0, int nb
             const int kb = c * 4 + ks * KB + j;
             if (kb < NK) {                                   // uniform
                 const bool half = kb * 128 + 64 >= H;        // uniform: H % 128 == 64, the last block
+                lmh_acc p[2];
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const int row = v * 32 + r;
-                    auto frag = [&](int p) {
-                        return *(const llima_u32x4*)(wb + row * LMH8_W + ((((ks * KB + j) * 8 + 2 * p + g) ^ (row & 15)) << 4));
-                    };
-                    auto op = [](llima_u32x4 a, llima_u32x4 b) {
-                        return (lmh8_i8){(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
-                    };
-                    lmh_acc p = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                    p = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(op(frag(0), frag(1)), op(hx[j][0], hx[j][1]), p, 0, 0, 0, 0, 0, 0);
-                    if (!half)
-                        p = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(op(frag(2), frag(3)), op(hx[j][2], hx[j][3]), p, 0, 0, 0, 0, 0, 0);
+                for (int v = 0; v < 2; ++v)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[v][i] = __builtin_fmaf(p[i], sc[j], acc[v][i]);
+                    for (int i = 0; i < 16; ++i) p[v][i] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (e < 2 || !half) {
+                        const llima_u32x4 x = hx[j][e];
+                        const lmh_b8 x0 = lmh8_wide(x.x, x.y), x1 = lmh8_wide(x.z, x.w);
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            const int row = v * 32 + r;
+                            const llima_u32x4 w = *(const llima_u32x4*)(wb + row * LMH8_W + ((((ks * KB + j) * 8 + 2 * e + g) ^ (row & 15)) << 4));
+                            p[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lmh8_wide(w.x, w.y), x0, p[v], 0, 0, 0);
+                            p[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lmh8_wide(w.z, w.w), x1, p[v], 0, 0, 0);
+                        }
+                    }
                 }
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[v][i] = __builtin_fmaf(p[v][i], sc[j], acc[v][i]);
             }
         }
         if (++c == nch) {                                    // uniform: the tile is summed

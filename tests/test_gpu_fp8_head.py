@@ -3,6 +3,8 @@
 Tolerance of a logit: the e4m3 products are exact in fp32, so a logit carries at most 128 roundings
 within a block, two of the scales, and one per block's addition, each at most 2^-23 of the sum of
 the terms' magnitudes (2^-24 where the matrix core rounds to nearest): (130 + NK) 2^-23 of it.
+These bounds add up; roundings of either sign do not, so the whole of many logits is off by far
+less (test_error_of_many_logits).
 """
 import pytest
 import torch
@@ -66,6 +68,26 @@ def test_logits_and_ids(gpu, B, H, V):
     assert torch.equal(l3, logits.to(torch.bfloat16)) and torch.equal(v3, l3.amax(1).float())
     first = torch.where(l3 == l3.amax(1, keepdim=True), torch.arange(V, device=gpu), V).amin(1)
     assert torch.equal(i3.long(), first)
+
+
+@pytest.mark.parametrize("B", [1, 60, 128, 200])
+def test_error_of_many_logits(gpu, B):
+    """Roundings of either sign: the root mean square over many logits is within 2^-24 sqrt(130 + NK) of the terms'
+    magnitude each, also where one product of a block is 2^11 times the others and cancels in pairs."""
+    import llima_amd
+    H, V = 1024, 2000
+    xq, xs, wq, ws = make(B, H, V, 21, gpu)
+    for spread in (False, True):
+        if spread:
+            x = xq.float() / 2048.0
+            x[:, ::64] *= 2048.0
+            xq = x.to(F8)
+        ref, tol = definition(xq, xs, wq, ws)
+        _, _, logits = llima_amd.lm_head_argmax(llima_amd.Fp8Rows(xq, xs), llima_amd.Fp8LmHead(wq, ws),
+                                                return_logits=True, logit_dtype="f32")
+        mag = tol / ((130 + 8) * 2.0 ** -23)
+        rel = ((logits.double() - ref) / mag).square().mean().sqrt()
+        assert rel < 2.0 ** -24 * 138 ** 0.5
 
 
 @pytest.mark.parametrize("B", [1, 40, 100, 140, 260])
