@@ -188,25 +188,26 @@ __device__ __forceinline__ void lmh8_barrier() {
 // the weight streams at 4.8 TB/s, this way at 5.6 to 5.9 (0.53 GB, requests alone).
 #define LMH8_W 512                     // bytes of a row per chunk
 #define LMH8_NV 64                     // vocab rows per tile
-#define LMH8_S 4                       // chunks of the ring
 
-template <int CG, bool SC>
-__global__ __launch_bounds__(512) void lmh8_rows(Lmh8Params Q, int b0, int nb) {
-    constexpr int KS = 4 / CG;                               // waves that share a column group
+template <int CG, int NC, int S, bool SC>
+__global__ __launch_bounds__(64 * (NC + 4)) void lmh8_rows(Lmh8Params Q, int b0, int nb) {
+    constexpr int KS = NC / CG;                              // waves that share a column group
     constexpr int KB = 4 / KS;                               // blocks of a chunk per wave
-    constexpr int SB = LMH8_NV * LMH8_W, S = LMH8_S;         // bytes of a slot
+    constexpr int SB = LMH8_NV * LMH8_W;                     // bytes of a slot
     constexpr int NX = 32 / KS;                              // a lane's sums of a finished slot
-    constexpr int RED = KS > 1 ? 4 * (KS - 1) * NX * 64 * 4 : 0;
+    constexpr int RED = NC * (KS - 1) * NX * 64 * 4;         // the exchanged sums
+    static_assert(KS * CG == NC && KS <= 4 && S * SB + RED <= 163840, "shape");
     __shared__ __align__(1024) uint8_t sm[S * SB + RED];
     const LmhParams& P = Q.P;
     const int t = (int)threadIdx.x, lane = t & 63, g = lane >> 5, r = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int H = P.H, V = P.V, NK = Q.NK, nch = (H + LMH8_W - 1) / LMH8_W;
     const int ntile = (V + LMH8_NV - 1) / LMH8_NV, G = (int)gridDim.x;
+    const int rot = (int)(blockIdx.x >> 3) % nch;            // the tiles' first chunk
     const int ntot = (ntile - 1 - (int)blockIdx.x) / G * nch + nch;   // the workgroup's chunks (grid <= ntile)
-    if (wave >= 4) {
-        const int wq = wave - 4;
-        int tw = (int)blockIdx.x, cw = 0, sw = 0;
+    if (wave >= NC) {
+        const int wq = wave - NC;
+        int tw = (int)blockIdx.x, cw = rot, sw = 0;
         auto issue = [&]() {                                 // the next chunk; past the last one, that again
             const uint8_t* base = Q.wq + (size_t)tw * LMH8_NV * H + cw * LMH8_W;
             const int left = V - 1 - tw * LMH8_NV;           // the tile's last row
@@ -218,10 +219,8 @@ __global__ __launch_bounds__(512) void lmh8_rows(Lmh8Params Q, int b0, int nb) {
                         sm + sw * SB + (wq + 4 * q) * 1024);
             }
             sw = sw + 1 == S ? 0 : sw + 1;
-            if (++cw == nch) {
-                if (tw + G < ntile) { tw += G; cw = 0; }
-                else cw = nch - 1;
-            }
+            cw = cw + 1 == nch ? 0 : cw + 1;
+            if (cw == rot && tw + G < ntile) tw += G;        // past its last tile: that again
         };
 #pragma unroll
         for (int i = 0; i < S - 1; ++i) issue();
@@ -252,19 +251,20 @@ __global__ __launch_bounds__(512) void lmh8_rows(Lmh8Params Q, int b0, int nb) {
 #pragma unroll
         for (int p = 0; p < 4; ++p) hx[j][p] = *(const llima_u32x4*)(xf + (size_t)kc * 4096 + p * 1024);
     };
-    int tile = (int)blockIdx.x, c = 0, slot = 0;
+    int tile = (int)blockIdx.x, c = rot, slot = 0;
     float acc[2][16];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < KB; ++j) load(tile, 0, j);
+    for (int j = 0; j < KB; ++j) load(tile, rot, j);
     asm volatile("s_barrier" ::: "memory");
     for (int it = 0; it < ntot; ++it) {
         const uint8_t* wb = sm + slot * SB;
-        const bool end = c + 1 == nch;                       // uniform: the tile's last chunk
-        const int cn = end ? 0 : c + 1, tn = end && tile + G < ntile ? tile + G : tile;
+        const int cn = c + 1 == nch ? 0 : c + 1;
+        const bool end = cn == rot;                          // uniform: the tile's last chunk
+        const int tn = end && tile + G < ntile ? tile + G : tile;
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
             const int kb = c * 4 + ks * KB + j;
@@ -343,7 +343,12 @@ __global__ __launch_bounds__(512) void lmh8_rows(Lmh8Params Q, int b0, int nb) {
 }
 
 // Vocab rows per key slot: a wave finishes 64 / KS rows of a tile.
-static int lmh8_slot_rows(int nb) { return nb <= 32 ? 16 : nb <= 64 ? 32 : 64; }
+#ifndef LMH8_C2
+#define LMH8_C2 8, 3
+#define LMH8_T2 768
+#define LMH8_R2 16
+#endif
+static int lmh8_slot_rows(int nb) { return nb <= 32 ? 16 : nb <= 64 ? LMH8_R2 : 32; }
 
 template <bool SC>
 static int lmh8_run(Lmh8Params& Q, hipStream_t st) {
@@ -355,9 +360,9 @@ static int lmh8_run(Lmh8Params& Q, hipStream_t st) {
     hipLaunchKernelGGL(lmh8_order, dim3((uint32_t)Q.NK, (uint32_t)((P.B + 31) / 32)), dim3(LLIMA_WG), 0, st, Q);
     for (int b0 = 0; b0 < P.B; b0 += 128) {
         const int nb = P.B - b0 < 128 ? P.B - b0 : 128;
-        if (per <= 32) hipLaunchKernelGGL((lmh8_rows<1, SC>), g, dim3(512), 0, st, Q, b0, nb);
-        else if (per <= 64) hipLaunchKernelGGL((lmh8_rows<2, SC>), g, dim3(512), 0, st, Q, b0, nb);
-        else hipLaunchKernelGGL((lmh8_rows<4, SC>), g, dim3(512), 0, st, Q, b0, nb);
+        if (per <= 32) hipLaunchKernelGGL((lmh8_rows<1, 4, 4, SC>), g, dim3(512), 0, st, Q, b0, nb);
+        else if (per <= 64) hipLaunchKernelGGL((lmh8_rows<2, LMH8_C2, SC>), g, dim3(LMH8_T2), 0, st, Q, b0, nb);
+        else hipLaunchKernelGGL((lmh8_rows<4, 8, 4, SC>), g, dim3(768), 0, st, Q, b0, nb);
     }
     if (SC) hipLaunchKernelGGL(lmh_score_finish, dim3((uint32_t)P.B), dim3(LLIMA_WG), 0, st, P);
     else hipLaunchKernelGGL(lmh_finish, dim3((uint32_t)P.B), dim3(LLIMA_WG), 0, st, P);
