@@ -436,27 +436,26 @@ int llima_lm_head_verify_tree_packed(const void* hidden, const void* packed, int
  * launches nothing.  Batches above 128 rows go in passes.
  * llima_add_rms_norm and llima_quantize_rows make the hidden rows,
  * llima_lm_head_quantize the weight (or a checkpoint that stores it so). */
-size_t llima_lm_head_argmax_fp8_workspace_bytes(int32_t B, int32_t H, int32_t V);
+size_t llima_lm_head_argmax_fp8_workspace_bytes(int32_t B, int32_t V);
 int llima_lm_head_argmax_fp8(const void* hidden, const float* hidden_scales, const void* weight,
                              const float* weight_scales, int32_t B, int32_t H, int32_t V,
                              float softcap, int32_t logit_dtype, int32_t* out_ids,
                              float* out_vals, float* out_logits, void* workspace,
                              size_t workspace_bytes, void* stream);
-size_t llima_lm_head_score_fp8_workspace_bytes(int32_t B, int32_t H, int32_t V);
+size_t llima_lm_head_score_fp8_workspace_bytes(int32_t B, int32_t V);
 int llima_lm_head_score_fp8(const void* hidden, const float* hidden_scales, const void* weight,
                             const float* weight_scales, int32_t B, int32_t H, int32_t V,
                             float softcap, int32_t logit_dtype, const int32_t* targets,
                             double* out_logprob, int32_t* out_is_greedy, void* workspace,
                             size_t workspace_bytes, void* stream);
-size_t llima_lm_head_verify_greedy_fp8_workspace_bytes(int32_t B, int32_t D, int32_t H,
-                                                       int32_t V);
+size_t llima_lm_head_verify_greedy_fp8_workspace_bytes(int32_t B, int32_t D, int32_t V);
 int llima_lm_head_verify_greedy_fp8(const void* hidden, const float* hidden_scales,
                                     const void* weight, const float* weight_scales, int32_t B,
                                     int32_t D, int32_t H, int32_t V, float softcap,
                                     int32_t logit_dtype, const int32_t* draft_ids,
                                     int32_t* accepted_len, int32_t* emitted, void* workspace,
                                     size_t workspace_bytes, void* stream);
-size_t llima_lm_head_verify_tree_fp8_workspace_bytes(int32_t K, int32_t H, int32_t V);
+size_t llima_lm_head_verify_tree_fp8_workspace_bytes(int32_t K, int32_t V);
 int llima_lm_head_verify_tree_fp8(const void* hidden, const float* hidden_scales,
                                   const void* weight, const float* weight_scales, int32_t K,
                                   int32_t H, int32_t V, float softcap, int32_t logit_dtype,

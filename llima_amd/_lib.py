@@ -81,19 +81,19 @@ SIGNATURES = {
     "llima_lm_head_verify_tree_packed": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32,
                                                         ctypes.c_float, _i32, _vp, _vp, _i32,
                                                         _i32, _vp, _vp, _sz, _vp]),
-    "llima_lm_head_argmax_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "llima_lm_head_argmax_fp8_workspace_bytes": (_sz, [_i32, _i32]),
     "llima_lm_head_argmax_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32,
                                                 ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _sz,
                                                 _vp]),
-    "llima_lm_head_score_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "llima_lm_head_score_fp8_workspace_bytes": (_sz, [_i32, _i32]),
     "llima_lm_head_score_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32,
                                                ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _sz,
                                                _vp]),
-    "llima_lm_head_verify_greedy_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "llima_lm_head_verify_greedy_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "llima_lm_head_verify_greedy_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
                                                        ctypes.c_float, _i32, _vp, _vp, _vp, _vp,
                                                        _sz, _vp]),
-    "llima_lm_head_verify_tree_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "llima_lm_head_verify_tree_fp8_workspace_bytes": (_sz, [_i32, _i32]),
     "llima_lm_head_verify_tree_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32,
                                                      ctypes.c_float, _i32, _vp, _vp, _i32, _i32,
                                                      _vp, _vp, _sz, _vp]),

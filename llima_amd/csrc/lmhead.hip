@@ -1681,11 +1681,6 @@ static int lmh8_check(const void* xq, const float* xs, const void* wq, const flo
     return LLIMA_OK;
 }
 
-static int lmh8_slots(int B, int V) {
-    const int n = lmh8_slot_rows(B < 128 ? B : 128);
-    return (V + n - 1) / n;
-}
-
 static void lmh8_fill(Lmh8Params& Q, const void* xq, const float* xs, const void* wq,
                       const float* ws, int32_t B, int32_t H, int32_t V, float softcap,
                       int32_t logit_dtype) {
@@ -1699,20 +1694,9 @@ static void lmh8_fill(Lmh8Params& Q, const void* xq, const float* xs, const void
     Q.P.round_bf16 = logit_dtype == LLIMA_BF16;
 }
 
-// Room for the ordered hidden rows and their scales, in whole groups of 32.
-static size_t lmh8_order_bytes(int32_t B, int32_t H) {
-    const size_t blocks = (size_t)((B + 31) / 32) * ((H + 127) / 128);
-    return blocks * (4096 + 128);
-}
-
-static void lmh8_place(Lmh8Params& Q, void* at) {
-    Q.frag = (uint8_t*)at;
-    Q.fs = (float*)(Q.frag + (size_t)((Q.P.B + 31) / 32) * Q.NK * 4096);
-}
-
-extern "C" size_t llima_lm_head_argmax_fp8_workspace_bytes(int32_t B, int32_t H, int32_t V) {
-    if (B <= 0 || V <= 0 || H <= 0 || H > 65536) return 0;
-    return lmh_ws_bytes(B, lmh8_slots(B, V), false) + lmh8_order_bytes(B, H);
+extern "C" size_t llima_lm_head_argmax_fp8_workspace_bytes(int32_t B, int32_t V) {
+    if (B <= 0 || V <= 0) return 0;
+    return lmh_ws_bytes(B, lmh8_slots(B, V), false);
 }
 
 extern "C" int llima_lm_head_argmax_fp8(const void* hidden, const float* hidden_scales,
@@ -1726,22 +1710,21 @@ extern "C" int llima_lm_head_argmax_fp8(const void* hidden, const float* hidden_
     int32_t logits_bf16 = 0;
     if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
     if (B == 0) return LLIMA_OK;
-    if (!workspace || workspace_bytes < llima_lm_head_argmax_fp8_workspace_bytes(B, H, V))
+    if (!workspace || workspace_bytes < llima_lm_head_argmax_fp8_workspace_bytes(B, V))
         return LLIMA_E_WORKSPACE;
     Lmh8Params Q = {};
     lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, B, H, V, softcap, logit_dtype);
     Q.P.out_logits = out_logits;
     Q.P.keys = (uint64_t*)workspace;
-    lmh8_place(Q, (uint8_t*)workspace + lmh_ws_bytes(B, lmh8_slots(B, V), false));
     Q.P.out_ids = out_ids;
     Q.P.out_vals = out_vals;
     Q.P.logits_bf16 = logits_bf16;
     return lmh8_run<false>(Q, (hipStream_t)stream);
 }
 
-extern "C" size_t llima_lm_head_score_fp8_workspace_bytes(int32_t B, int32_t H, int32_t V) {
-    if (B <= 0 || V <= 0 || H <= 0 || H > 65536) return 0;
-    return lmh_ws_bytes(B, lmh8_slots(B, V), true) + lmh8_order_bytes(B, H);
+extern "C" size_t llima_lm_head_score_fp8_workspace_bytes(int32_t B, int32_t V) {
+    if (B <= 0 || V <= 0) return 0;
+    return lmh_ws_bytes(B, lmh8_slots(B, V), true);
 }
 
 extern "C" int llima_lm_head_score_fp8(const void* hidden, const float* hidden_scales,
@@ -1757,7 +1740,7 @@ extern "C" int llima_lm_head_score_fp8(const void* hidden, const float* hidden_s
     int32_t logits_bf16 = 0;
     if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
     if (B == 0) return LLIMA_OK;
-    if (!workspace || workspace_bytes < llima_lm_head_score_fp8_workspace_bytes(B, H, V))
+    if (!workspace || workspace_bytes < llima_lm_head_score_fp8_workspace_bytes(B, V))
         return LLIMA_E_WORKSPACE;
     Lmh8Params Q = {};
     lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, B, H, V, softcap, logit_dtype);
@@ -1765,15 +1748,13 @@ extern "C" int llima_lm_head_score_fp8(const void* hidden, const float* hidden_s
     Q.P.out_logprob = out_logprob;
     Q.P.out_greedy = out_is_greedy;
     lmh_ws_split(Q.P, workspace, lmh8_slots(B, V));
-    lmh8_place(Q, (uint8_t*)workspace + lmh_ws_bytes(B, lmh8_slots(B, V), true));
     return lmh8_run<true>(Q, (hipStream_t)stream);
 }
 
-extern "C" size_t llima_lm_head_verify_greedy_fp8_workspace_bytes(int32_t B, int32_t D, int32_t H,
-                                                                 int32_t V) {
+extern "C" size_t llima_lm_head_verify_greedy_fp8_workspace_bytes(int32_t B, int32_t D, int32_t V) {
     if (B <= 0 || D < 0 || (int64_t)B * (D + 1) > (int64_t)INT32_MAX) return 0;
     const int32_t rows = B * (D + 1);
-    return lmh_verify_ws(llima_lm_head_argmax_fp8_workspace_bytes(rows, H, V), rows);
+    return lmh_verify_ws(llima_lm_head_argmax_fp8_workspace_bytes(rows, V), rows);
 }
 
 extern "C" int llima_lm_head_verify_greedy_fp8(const void* hidden, const float* hidden_scales,
@@ -1791,22 +1772,21 @@ extern "C" int llima_lm_head_verify_greedy_fp8(const void* hidden, const float* 
     int32_t logits_bf16 = 0;
     if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
     if (B == 0) return LLIMA_OK;
-    if (!workspace || workspace_bytes < llima_lm_head_verify_greedy_fp8_workspace_bytes(B, D, H, V))
+    if (!workspace || workspace_bytes < llima_lm_head_verify_greedy_fp8_workspace_bytes(B, D, V))
         return LLIMA_E_WORKSPACE;
-    int32_t* ids = (int32_t*)((uint8_t*)workspace + llima_lm_head_argmax_fp8_workspace_bytes(rows, H, V));
+    int32_t* ids = (int32_t*)((uint8_t*)workspace + llima_lm_head_argmax_fp8_workspace_bytes(rows, V));
     Lmh8Params Q = {};
     lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, rows, H, V, softcap, logit_dtype);
     Q.P.keys = (uint64_t*)workspace;
-    lmh8_place(Q, (uint8_t*)workspace + lmh_ws_bytes(rows, lmh8_slots(rows, V), false));
     Q.P.out_ids = ids;
     hipStream_t st = (hipStream_t)stream;
     if ((st0 = lmh8_run<false>(Q, st)) != LLIMA_OK) return st0;
     return lmh_launch_chain(ids, draft_ids, accepted_len, emitted, B, D, st);
 }
 
-extern "C" size_t llima_lm_head_verify_tree_fp8_workspace_bytes(int32_t K, int32_t H, int32_t V) {
+extern "C" size_t llima_lm_head_verify_tree_fp8_workspace_bytes(int32_t K, int32_t V) {
     if (K <= 0) return 0;
-    return lmh_tree_ws(llima_lm_head_argmax_fp8_workspace_bytes(K, H, V), K);
+    return lmh_tree_ws(llima_lm_head_argmax_fp8_workspace_bytes(K, V), K);
 }
 
 extern "C" int llima_lm_head_verify_tree_fp8(const void* hidden, const float* hidden_scales,
@@ -1822,13 +1802,12 @@ extern "C" int llima_lm_head_verify_tree_fp8(const void* hidden, const float* hi
     if ((st0 = lmh8_check(hidden, hidden_scales, weight, weight_scales, K, H, V)) != LLIMA_OK) return st0;
     int32_t logits_bf16 = 0;
     if ((st0 = lmh_check_dtype(softcap, &logit_dtype, &logits_bf16)) != LLIMA_OK) return st0;
-    if (!workspace || workspace_bytes < llima_lm_head_verify_tree_fp8_workspace_bytes(K, H, V))
+    if (!workspace || workspace_bytes < llima_lm_head_verify_tree_fp8_workspace_bytes(K, V))
         return LLIMA_E_WORKSPACE;
-    uint8_t* rest = (uint8_t*)workspace + llima_lm_head_argmax_fp8_workspace_bytes(K, H, V);
+    uint8_t* rest = (uint8_t*)workspace + llima_lm_head_argmax_fp8_workspace_bytes(K, V);
     Lmh8Params Q = {};
     lmh8_fill(Q, hidden, hidden_scales, weight, weight_scales, K, H, V, softcap, logit_dtype);
     Q.P.keys = (uint64_t*)workspace;
-    lmh8_place(Q, (uint8_t*)workspace + lmh_ws_bytes(K, lmh8_slots(K, V), false));
     Q.P.out_ids = (int32_t*)rest;
     Q.P.out_vals = (float*)(rest + lmh_align256((size_t)K * 4));
     hipStream_t st = (hipStream_t)stream;

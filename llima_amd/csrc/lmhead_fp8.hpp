@@ -31,27 +31,8 @@ struct Lmh8Params {
     const float* xs;
     const uint8_t* wq;
     const float* ws;
-    uint8_t* frag;                                           // hidden rows in operand order (lmh8_order)
-    float* fs;                                               // and their scales
     int32_t NK;
 };
-
-// The hidden rows in the order the MFMAs read them, so that a wave's load is 1 KB
-// of adjacent memory (read from the rows themselves, 32 pieces of 32 bytes, they
-// and not the weight bound the product: B = 64, H = 4096, V = 128256 147 us): per
-// group of 32 rows and block of 128 ids the pieces e < 4, lane (r, g)'s 16 bytes
-// being ids 32 e + 16 g .. of row r; then the block's 32 scales, one per row.
-// Rows past the batch repeat its last one, ids past H are 0.
-__global__ __launch_bounds__(LLIMA_WG) void lmh8_order(Lmh8Params Q) {
-    const int kb = (int)blockIdx.x, rg = (int)blockIdx.y, t = (int)threadIdx.x;
-    const int H = Q.P.H, B = Q.P.B, lane = t & 63, m = rg * 32 + (lane & 31), mc = m < B ? m : B - 1;
-    const int h = kb * 128 + (t >> 6) * 32 + (lane >> 5) * 16;
-    llima_u32x4 v = {0u, 0u, 0u, 0u};
-    if (h < H) v = *(const llima_u32x4*)(Q.xq + (size_t)mc * H + h);
-    const size_t block = (size_t)rg * Q.NK + kb;
-    *(llima_u32x4*)(Q.frag + (block * 256 + t) * 16) = v;
-    if (t < 32) Q.fs[block * 32 + t] = Q.xs[(size_t)mc * Q.NK + kb];
-}
 
 // NX sums of one lane as the argmax sees them (lmh_logit), in place.
 template <int NX>
@@ -76,14 +57,22 @@ __device__ __forceinline__ void lmh8_logits(const LmhParams& P, float (&x)[NX]) 
     }
 }
 
-// One slot (2 NX vocab rows from n) of one hidden row per lane pair (r, 0), (r, 1):
-// x[k] of lane half g is row (k / 16) 32 + (k / 4 % 4) 8 + 4 g + k % 4 of the
-// slot.  Writes the logits when asked, the slot's key, and with SC its sum and
-// the target's logit.  b: the hidden row (row false: none).
+// What a lane keeps of its hidden row over the tiles of its wave: the best key
+// (both lanes of the pair the same), and with SC the sum of exp(logit - m), m
+// its greatest non-NaN logit (each lane its own half of the rows).
+struct Lmh8Best {
+    uint64_t key;
+    float m, s;
+};
+
+// 2 NX vocab rows from n of one hidden row per lane pair (r, 0), (r, 1): x[k]
+// of lane half g is row n + (k / 16) 32 + (k / 4 % 4) 8 + 4 g + k % 4.  Writes the
+// logits when asked, and with SC the target's logit.  b: the hidden row (row
+// false: none); end: the first row that is not the tile's.
 template <int NX, bool SC>
-__device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX], int b, bool row,
-                                              int n, int g) {
-    const int left = P.V - n;                                // <= 0: the slot is past the vocabulary
+__device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX], Lmh8Best& B, int b,
+                                              bool row, int n, int end, int g) {
+    const int left = end - n;                                // <= 0: nothing
     auto col = [&](int k) { return (k >> 4) * 32 + (k >> 2 & 3) * 8 + 4 * g + (k & 3); };
     lmh8_logits<NX>(P, x);
     if (P.out_logits) {                                      // uniform
@@ -116,7 +105,7 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
             }
         }
     }
-    if (left < 2 * NX) {                                     // uniform: rows past the vocabulary
+    if (left < 2 * NX) {                                     // uniform: rows past the tile
 #pragma unroll
         for (int k = 0; k < NX; ++k) x[k] = col(k) < left ? x[k] : __builtin_nanf("");
     }
@@ -124,6 +113,7 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
     float best = lmh_max3(x[0], x[1], x[1]);
 #pragma unroll
     for (int k = 2; k < NX; k += 2) best = lmh_max3(best, x[k], x[k + 1]);
+    const float own = best;
     best = lmh_max3(best, __shfl_xor(best, 32, 64), best);
     int at = 255;
 #pragma unroll
@@ -131,22 +121,22 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
     at = at == 255 ? 255 : at + 4 * g;
     const int other = __shfl_xor(at, 32, 64);
     at = at < other ? at : other;
-    const size_t slot = (size_t)b * P.NW + n / (2 * NX);
-    if (row && g == 0)
-        P.keys[slot] = at < 255 ? ((uint64_t)f32_key(best) << 32) | (uint32_t)~(uint32_t)(n + at) : 0ull;
+    const uint64_t key = at < 255 ? ((uint64_t)f32_key(best) << 32) | (uint32_t)~(uint32_t)(n + at) : 0ull;
+    B.key = key > B.key ? key : B.key;
     if constexpr (SC) {
         const int32_t tg = row ? P.targets[b] : -1;
         if (left < 2 * NX) {                                 // uniform
 #pragma unroll
             for (int k = 0; k < NX; ++k) x[k] = col(k) < left ? x[k] : -__builtin_inff();
         }
-        const float mw = best > -__builtin_inff() ? best : 0.0f;
+        const float mn = own > B.m ? own : B.m;              // (own NaN: all of them, the sum becomes NaN)
+        const float mw = mn > -__builtin_inff() ? mn : 0.0f;
         float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < NX; ++k) e[k & 3] += __builtin_amdgcn_exp2f((x[k] - mw) * LMH_LOG2E);
-        float s = (e[0] + e[1]) + (e[2] + e[3]);
-        s += __shfl_xor(s, 32, 64);
-        if (row && g == 0) P.sums[slot] = s;
+        const float old = B.m > -__builtin_inff() ? B.s * __builtin_amdgcn_exp2f((B.m - mw) * LMH_LOG2E) : B.s;
+        B.s = old + ((e[0] + e[1]) + (e[2] + e[3]));
+        B.m = mn;
         const int ts = tg >= 0 ? tg - n : -1;                // the target's column of the slot
         const bool hit = ts >= 0 && ts < 2 * NX && ts < left && (ts >> 2 & 1) == g;
         if (__any(hit)) {
@@ -158,211 +148,214 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
     }
 }
 
-// A barrier of the workgroup that waits for the wave's LDS accesses and for no
-// other request.
-__device__ __forceinline__ void lmh8_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
-// lmh8_rows: up to 32 CG hidden rows.  A workgroup (one per CU) takes tiles of
-// 64 vocab rows (tile, tile + grid, ...) through k in chunks of 512 ids: a
-// chunk is 512 contiguous bytes of each of 64 weight rows, in a ring of LMH8_S LDS
-// slots (32 KB).  Four waves request the chunks straight into LDS, four
-// multiply: requests return in order, so a wave that also loaded hidden rows
-// would wait for the weight's whenever it waits for those.  CG waves take a group
-// of 32 hidden rows each, KS = 4 / CG waves share a group and split a chunk's
-// four blocks of 128 between them, so that a wave's hidden values are its own:
-// it loads them from L2 into registers, each block of the next chunk when that
-// of this one is used.  At a tile's end the waves of a group exchange their
-// sums through LDS and each finishes 64 / KS of the tile's rows (a key slot),
-// while the ring fills up.
+// lmh8_tiles: up to 32 CWV MB hidden rows in a pass.  A workgroup of eight waves
+// (two per SIMD: one alone issues a vector instruction every nine cycles, two
+// together every 4.6), one workgroup per CU, takes tiles of 256 vocab rows (tile,
+// tile + grid, ...), RWV waves along the vocab rows (VB blocks of 32 each) and CWV
+// along the hidden rows (MB blocks of 32).  k goes in steps of one block of 128
+// ids: 128 bytes of each weight row and of each hidden row are requested
+// straight into a ring of S LDS slots.  LDS rows are 128 bytes with their 16-byte
+// columns exchanged by row / 2 (the request's source address does it): fragment
+// reads have no bank conflicts.  The scales are loaded a step ahead, before the
+// requests, so that waiting for them leaves those in flight (with requests made by
+// global loads the compiler takes them to return in any order and waits for all).  A step's values are read, converted and
+// multiplied piece by piece (piece e of half g: ids 32 e + 16 g .. + 15, its halves two
+// MFMAs), its sums scaled and added to the tile's.  The weight is the MFMA's
+// row operand: lane (r, g) has, for hidden row r of a block, half of a wave's vocab rows
+// (the lane with the other g the other half).
 //
-// LDS rows are 512 bytes with their 16-byte columns exchanged by row % 16 (the
-// request's source address does it): fragment reads have no bank conflicts.
-// The weight is the MFMA's row operand: lane (r, g) has for hidden row r the
-// sums of half of a slot's rows (the lane with the other g the others).  k order
-// within a block: piece e of 16 ids of half g is ids 32 e + 16 g .. + 15, its
-// halves two steps, for both operands.
+// A tile's steps start at another block in each workgroup of an XCD: all at the
+// first one read the same 128 bytes of every 4 KB, which is a part of the memory
+// channels (the weight of 0.53 GB, requests alone: 110 us, started apart 88).
 //
-// 512 contiguous bytes per row: read 128 bytes at a time (a tile of 256 rows)
-// the weight streams at 4.8 TB/s, this way at 5.6 to 5.9 (0.53 GB, requests alone).
-#define LMH8_W 512                     // bytes of a row per chunk
-#define LMH8_NV 64                     // vocab rows per tile
+// Bound: reading the weight up to 128 rows; a batch of more goes in passes of 128.
+#define LMH8_NV 256                    // vocab rows per tile
+#define LMH8_CUS 256                   // workgroups: one per CU (its LDS)
 
-template <int CG, int NC, int S, bool SC>
-__global__ __launch_bounds__(64 * (NC + 4)) void lmh8_rows(Lmh8Params Q, int b0, int nb) {
-    constexpr int KS = NC / CG;                              // waves that share a column group
-    constexpr int KB = 4 / KS;                               // blocks of a chunk per wave
-    constexpr int SB = LMH8_NV * LMH8_W;                     // bytes of a slot
-    constexpr int NX = 32 / KS;                              // a lane's sums of a finished slot
-    constexpr int RED = NC * (KS - 1) * NX * 64 * 4;         // the exchanged sums
-    static_assert(KS * CG == NC && KS <= 4 && S * SB + RED <= 163840, "shape");
-    __shared__ __align__(1024) uint8_t sm[S * SB + RED];
+template <int RWV, int VB, int CWV, int MB, int S, bool SC>
+__global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) {
+    constexpr int NM = 32 * CWV * MB;                        // hidden rows of the pass
+    constexpr int LW = LMH8_NV / 64;                         // 1 KB requests per wave and step: weight,
+    constexpr int LX = NM >= 64 ? NM / 64 : 1;               // hidden rows (NM = 32: half of the waves' again)
+    constexpr int WB = LMH8_NV * 128, SB = WB + NM * 128;    // bytes of a slot
+    static_assert(RWV * CWV == 8 && RWV * VB * 32 == LMH8_NV && S >= 2 && S * SB <= 163840, "shape");
+    __shared__ __align__(1024) uint8_t sm[S * SB];
     const LmhParams& P = Q.P;
     const int t = (int)threadIdx.x, lane = t & 63, g = lane >> 5, r = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int H = P.H, V = P.V, NK = Q.NK, nch = (H + LMH8_W - 1) / LMH8_W;
-    const int ntile = (V + LMH8_NV - 1) / LMH8_NV, G = (int)gridDim.x;
-    const int rot = (int)(blockIdx.x >> 3) % nch;            // the tiles' first chunk
-    const int ntot = (ntile - 1 - (int)blockIdx.x) / G * nch + nch;   // the workgroup's chunks (grid <= ntile)
-    if (wave >= NC) {
-        const int wq = wave - NC;
-        int tw = (int)blockIdx.x, cw = rot, sw = 0;
-        auto issue = [&]() {                                 // the next chunk; past the last one, that again
-            const uint8_t* base = Q.wq + (size_t)tw * LMH8_NV * H + cw * LMH8_W;
-            const int left = V - 1 - tw * LMH8_NV;           // the tile's last row
+    const int wr = wave % RWV, wc = wave / RWV;
+    const int H = P.H, V = P.V, NK = Q.NK, G = (int)gridDim.x;
+    const int ntile = (V + LMH8_NV - 1) / LMH8_NV;           // grid <= ntile
+    const int rot = (int)(blockIdx.x >> 3) % NK;             // the tiles' first block
+    const int ntot = ((ntile - 1 - (int)blockIdx.x) / G + 1) * NK;   // the workgroup's steps
+    // The request stream: a tile and a block of it.  Through buffer descriptors:
+    // rows past the vocabulary or the batch lie outside them and read as 0, as
+    // does what the last row's last block has past H (other rows read the next
+    // row's there; it is not used).
+    uint32_t ow[LW], ox[LX];                                 // the lane's row and column of its requests
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const int row = 2 * (wq + 4 * q) + (lane >> 5), pos = lane & 31;
-                const int col = (pos ^ (row & 15)) * 16;     // bytes past H read the chunk's first ones
-                lmh_dma(base, (uint32_t)(row < left ? row : left) * (uint32_t)H + (uint32_t)(cw * LMH8_W + col < H ? col : 0),
-                        sm + sw * SB + (wq + 4 * q) * 1024);
-            }
-            sw = sw + 1 == S ? 0 : sw + 1;
-            cw = cw + 1 == nch ? 0 : cw + 1;
-            if (cw == rot && tw + G < ntile) tw += G;        // past its last tile: that again
-        };
-#pragma unroll
-        for (int i = 0; i < S - 1; ++i) issue();
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 2) * 8) : "memory");   // chunk 0 has landed
-        for (int i = 0, c = 0; i < ntot; ++i) {
-            issue();                                         // into the slot read before the last barrier
-            if (++c == nch) {
-                c = 0;
-                if (KS > 1) asm volatile("s_barrier" ::: "memory");
-            }
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 2) * 8) : "memory");   // chunk i + 1 has
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // no request outlives the workgroup
-        return;
+    for (int q = 0; q < LW; ++q) {
+        const int row = 8 * (wave + 8 * q) + (lane >> 3);
+        ow[q] = (uint32_t)row * (uint32_t)H + (uint32_t)(((lane & 7) ^ (row >> 1 & 7)) * 16);
     }
-    const int cg = wave % CG, ks = wave / CG;
-    const int m = cg * 32 + r;                               // the lane's hidden row of the pass
-    const int mc = m < nb ? m : nb - 1;                      // rows past the batch repeat the last one
-    const size_t block0 = (size_t)((b0 >> 5) + (cg * 32 < nb ? cg : 0)) * NK;   // the group's first block
-    const uint8_t* const xf = Q.frag + block0 * 4096 + lane * 16;
-    const float* const xsf = Q.fs + block0 * 32 + r;
-    llima_u32x4 hx[KB][4];
-    float sx[KB], sw[KB];
-    auto load = [&](int tile, int c, int j) {                // block j of the wave in chunk c of tile
-        const int kb = c * 4 + ks * KB + j, kc = kb < NK ? kb : 0;
-        sx[j] = xsf[kc * 32];
-        sw[j] = Q.ws[(size_t)(tile >> 1) * NK + kc];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) hx[j][p] = *(const llima_u32x4*)(xf + (size_t)kc * 4096 + p * 1024);
+    for (int q = 0; q < LX; ++q) {
+        const int row = 8 * ((wave + 8 * q) % (NM / 8)) + (lane >> 3);
+        ox[q] = (uint32_t)row * (uint32_t)H + (uint32_t)(((lane & 7) ^ (row >> 1 & 7)) * 16);
+    }
+    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(Q.xq + (size_t)b0 * H), 0, nb * H, 0x00027000);
+    int tw = (int)blockIdx.x, cw = rot, sw = 0;
+    auto issue = [&]() {
+        const int rows = V - tw * LMH8_NV < LMH8_NV ? V - tw * LMH8_NV : LMH8_NV;
+        const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(Q.wq + (size_t)tw * LMH8_NV * H), 0, rows * H, 0x00027000);
+        uint8_t* const at = sm + sw * SB;
+#pragma unroll
+        for (int q = 0; q < LX; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(at + WB + ((wave + 8 * q) % (NM / 8)) * 1024),
+                                                     16, (int)ox[q], cw * 128, 0, 0);
+#pragma unroll
+        for (int q = 0; q < LW; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(at + (wave + 8 * q) * 1024),
+                                                     16, (int)ow[q], cw * 128, 0, 0);
+        sw = sw + 1 == S ? 0 : sw + 1;
+        cw = cw + 1 == NK ? 0 : cw + 1;
+        if (cw == rot && tw + G < ntile) tw += G;            // past its last tile: that again
+    };
+    int m[MB], mc[MB];                                       // the lane's hidden rows of the pass
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        m[i] = (wc * MB + i) * 32 + r;
+        mc[i] = m[i] < nb ? m[i] : nb - 1;
+    }
+    float sx[MB], swt;                                       // the next step's scales
+    auto load_s = [&](int tile, int c) {
+        const int vb = tile * 2 + (wr * VB * 32) / 128;      // the block of 128 vocab rows of the wave
+        swt = Q.ws[(size_t)(vb * 128 < V ? vb : 0) * NK + c];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) sx[i] = Q.xs[(size_t)(b0 + mc[i]) * NK + c];
     };
     int tile = (int)blockIdx.x, c = rot, slot = 0;
-    float acc[2][16];
+    float acc[MB][VB][16];
+    Lmh8Best best[MB];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < MB; ++i) {
+        best[i] = {0ull, -__builtin_inff(), 0.0f};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
+        for (int v = 0; v < VB; ++v)
 #pragma unroll
-    for (int j = 0; j < KB; ++j) load(tile, rot, j);
-    asm volatile("s_barrier" ::: "memory");
+            for (int k = 0; k < 16; ++k) acc[i][v][k] = 0.0f;
+    }
+    load_s(tile, c);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue();
+    const uint32_t rl = (uint32_t)(r * 128), rz = (uint32_t)(r >> 1 & 7);
     for (int it = 0; it < ntot; ++it) {
-        const uint8_t* wb = sm + slot * SB;
-        const int cn = c + 1 == nch ? 0 : c + 1;
-        const bool end = cn == rot;                          // uniform: the tile's last chunk
+        lmh_wait_barrier<(S - 2) * (LW + LX)>();             // the step's values have landed, the last one's are read
+        const int cn = c + 1 == NK ? 0 : c + 1;
+        const bool end = cn == rot;                          // uniform: the tile's last step
         const int tn = end && tile + G < ntile ? tile + G : tile;
+        float sc[MB];
 #pragma unroll
-        for (int j = 0; j < KB; ++j) {
-            const int kb = c * 4 + ks * KB + j;
-            if (kb < NK) {                                   // uniform
-                const bool half = kb * 128 + 64 >= H;        // uniform: H % 128 == 64, the last block
-                lmh_acc p[2];
-#pragma unroll
-                for (int v = 0; v < 2; ++v)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) p[v][i] = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (e < 2 || !half) {
-                        const llima_u32x4 x = hx[j][e];
-                        const lmh_b8 x0 = lmh8_wide(x.x, x.y), x1 = lmh8_wide(x.z, x.w);
-#pragma unroll
-                        for (int v = 0; v < 2; ++v) {
-                            const int row = v * 32 + r;
-                            const llima_u32x4 w = *(const llima_u32x4*)(wb + row * LMH8_W + ((((ks * KB + j) * 8 + 2 * e + g) ^ (row & 15)) << 4));
-                            p[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lmh8_wide(w.x, w.y), x0, p[v], 0, 0, 0);
-                            p[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lmh8_wide(w.z, w.w), x1, p[v], 0, 0, 0);
-                        }
-                    }
-                }
-                const float sc = sx[j] * sw[j];
-#pragma unroll
-                for (int v = 0; v < 2; ++v)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[v][i] = __builtin_fmaf(p[v][i], sc, acc[v][i]);
-            }
-            load(tn, cn, j);
+        for (int i = 0; i < MB; ++i) {
+            sc[i] = sx[i] * swt;
+            asm volatile("" : "+v"(sc[i]));                  // now: later, the next scales would need a copy, and that a wait
         }
-        if (end) {                                           // uniform
-            float x[NX];
-            if constexpr (KS > 1) {
-                // wave ks keeps sums ks NX .. + NX - 1 of its 32 and gives the others to their waves
-                float* red = (float*)(sm + S * SB);
+        load_s(tn, cn);
+        __builtin_amdgcn_sched_barrier(0);                   // before the requests: waited for without them
+        issue();
+        const uint8_t* wb = sm + slot * SB + wr * VB * 4096;
+        const uint8_t* xb = sm + slot * SB + WB + wc * MB * 4096;
+        const bool half = c * 128 + 64 >= H;                 // uniform: H % 128 == 64, the last block
+        lmh_acc p[MB][VB];
 #pragma unroll
-                for (int d = 1; d < KS; ++d) {
-                    const int to = (ks + d) % KS;
-                    float* w = red + (((to * CG + cg) * (KS - 1) + d - 1) * NX) * 64 + lane;
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-                    for (int i = 0; i < NX; ++i) {
-                        float v = 0.0f;
+            for (int v = 0; v < VB; ++v)
 #pragma unroll
-                        for (int q = 0; q < KS; ++q) v = to == q ? acc[(q * NX + i) >> 4][(q * NX + i) & 15] : v;
-                        w[i * 64] = v;
-                    }
+                for (int k = 0; k < 16; ++k) p[i][v][k] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e < 2 || !half) {
+                const uint32_t o = rl + ((((uint32_t)(2 * e + g)) ^ rz) << 4);
+                lmh_b8 w0[VB], w1[VB];
+#pragma unroll
+                for (int v = 0; v < VB; ++v) {
+                    const llima_u32x4 w = *(const llima_u32x4*)(wb + v * 4096 + o);
+                    w0[v] = lmh8_wide(w.x, w.y);
+                    w1[v] = lmh8_wide(w.z, w.w);
                 }
-                lmh8_barrier();
 #pragma unroll
-                for (int i = 0; i < NX; ++i) {
-                    float v = 0.0f;
+                for (int i = 0; i < MB; ++i) {
+                    const llima_u32x4 x = *(const llima_u32x4*)(xb + i * 4096 + o);
+                    const lmh_b8 x0 = lmh8_wide(x.x, x.y), x1 = lmh8_wide(x.z, x.w);
 #pragma unroll
-                    for (int q = 0; q < KS; ++q) v = ks == q ? acc[(q * NX + i) >> 4][(q * NX + i) & 15] : v;
+                    for (int v = 0; v < VB; ++v) p[i][v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w0[v], x0, p[i][v], 0, 0, 0);
 #pragma unroll
-                    for (int d = 1; d < KS; ++d) v += red[(((ks * CG + cg) * (KS - 1) + d - 1) * NX + i) * 64 + lane];
-                    x[i] = v;
+                    for (int v = 0; v < VB; ++v) p[i][v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w1[v], x1, p[i][v], 0, 0, 0);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < NX; ++i) x[i] = acc[i >> 4][i & 15];
             }
-            const int n = tile * LMH8_NV + ks * 2 * NX;
-            if (n < V) lmh8_slot_out<NX, SC>(P, x, b0 + mc, m < nb, n, g);   // uniform
+        }
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
+            for (int v = 0; v < VB; ++v)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[i][v][k] = __builtin_fmaf(p[i][v][k], sc[i], acc[i][v][k]);
+        if (end) {                                           // uniform
+            const int n = tile * LMH8_NV + wr * VB * 32;
+            if (n < V) {                                     // uniform
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+                    float x[16 * VB];
+#pragma unroll
+                    for (int k = 0; k < 16 * VB; ++k) x[k] = acc[i][k >> 4][k & 15];
+                    lmh8_slot_out<16 * VB, SC>(P, x, best[i], b0 + mc[i], m[i] < nb, n, V, g);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int v = 0; v < VB; ++v)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) acc[i][v][k] = 0.0f;
         }
         c = cn;
         tile = tn;
         slot = slot + 1 == S ? 0 : slot + 1;
-        lmh8_barrier();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no request outlives the workgroup
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const size_t at = (size_t)(b0 + mc[i]) * P.NW + blockIdx.x * RWV + wr;
+        if constexpr (SC) {                                  // the two lanes' sums under the pair's maximum
+            const float mo = __shfl_xor(best[i].m, 32, 64), so = __shfl_xor(best[i].s, 32, 64);
+            const float mn = mo > best[i].m ? mo : best[i].m, mw = mn > -__builtin_inff() ? mn : 0.0f;
+            auto under = [&](float m, float s) { return m > -__builtin_inff() ? s * __builtin_amdgcn_exp2f((m - mw) * LMH_LOG2E) : s; };
+            if (m[i] < nb && g == 0) P.sums[at] = under(best[i].m, best[i].s) + under(mo, so);
+        }
+        if (m[i] < nb && g == 0) P.keys[at] = best[i].key;
     }
 }
 
-// Vocab rows per key slot: a wave finishes 64 / KS rows of a tile.
-#ifndef LMH8_C2
-#define LMH8_C2 8, 3
-#define LMH8_T2 768
-#define LMH8_R2 16
-#endif
-static int lmh8_slot_rows(int nb) { return nb <= 32 ? 16 : nb <= 64 ? LMH8_R2 : 32; }
+static int lmh8_groups(int V) {
+    const int ntile = (V + LMH8_NV - 1) / LMH8_NV;
+    return ntile < LMH8_CUS ? ntile : LMH8_CUS;
+}
+
+// Key slots per hidden row: one per wave along the vocab rows.
+static int lmh8_slots(int B, int V) { return lmh8_groups(V) * (B <= 32 ? 8 : 4); }
 
 template <bool SC>
 static int lmh8_run(Lmh8Params& Q, hipStream_t st) {
     LmhParams& P = Q.P;
-    const int ntile = (P.V + LMH8_NV - 1) / LMH8_NV;
-    const int per = P.B < 128 ? P.B : 128;                   // rows per pass, one slot size for all
-    P.NW = (P.V + lmh8_slot_rows(per) - 1) / lmh8_slot_rows(per);
-    const dim3 g((uint32_t)(ntile < LMH_CUS ? ntile : LMH_CUS));
-    hipLaunchKernelGGL(lmh8_order, dim3((uint32_t)Q.NK, (uint32_t)((P.B + 31) / 32)), dim3(LLIMA_WG), 0, st, Q);
+    P.NW = lmh8_slots(P.B, P.V);
+    const dim3 g((uint32_t)lmh8_groups(P.V)), blk(512);
     for (int b0 = 0; b0 < P.B; b0 += 128) {
         const int nb = P.B - b0 < 128 ? P.B - b0 : 128;
-        if (per <= 32) hipLaunchKernelGGL((lmh8_rows<1, 4, 4, SC>), g, dim3(512), 0, st, Q, b0, nb);
-        else if (per <= 64) hipLaunchKernelGGL((lmh8_rows<2, LMH8_C2, SC>), g, dim3(LMH8_T2), 0, st, Q, b0, nb);
-        else hipLaunchKernelGGL((lmh8_rows<4, 8, 4, SC>), g, dim3(768), 0, st, Q, b0, nb);
+        if (P.B <= 32) hipLaunchKernelGGL((lmh8_tiles<8, 1, 1, 1, 4, SC>), g, blk, 0, st, Q, b0, nb);
+        else if (nb <= 64) hipLaunchKernelGGL((lmh8_tiles<4, 2, 2, 1, 4, SC>), g, blk, 0, st, Q, b0, nb);
+        else hipLaunchKernelGGL((lmh8_tiles<4, 2, 2, 2, 3, SC>), g, blk, 0, st, Q, b0, nb);
     }
     if (SC) hipLaunchKernelGGL(lmh_score_finish, dim3((uint32_t)P.B), dim3(LLIMA_WG), 0, st, P);
     else hipLaunchKernelGGL(lmh_finish, dim3((uint32_t)P.B), dim3(LLIMA_WG), 0, st, P);

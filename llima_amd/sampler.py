@@ -808,7 +808,7 @@ def _lm_head_argmax_fp8(hidden, head: Fp8LmHead, softcap, return_logits, logit_d
     vals = torch.empty(B, dtype=torch.float32, device=dev)
     ldt = torch.bfloat16 if logits_out == "bf16" else torch.float32
     logits = torch.empty((B, V), dtype=ldt, device=dev) if return_logits else None
-    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_argmax_fp8_workspace_bytes(B, head.H, V))
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_argmax_fp8_workspace_bytes(B, V))
     with _on(dev):
         check(lib().llima_lm_head_argmax_fp8(*_head8(x, head), B, head.H, V, float(softcap), ld,
                                              ids.data_ptr(), vals.data_ptr(), _ptr(logits),
@@ -836,7 +836,7 @@ def _lm_head_score_fp8(hidden, head: Fp8LmHead, target, softcap, logit_dtype):
     B = x.values.shape[0]
     lp = torch.empty(B, dtype=torch.float64, device=dev)
     gr = torch.empty(B, dtype=torch.int32, device=dev)
-    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_score_fp8_workspace_bytes(B, head.H, V))
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_score_fp8_workspace_bytes(B, V))
     with _on(dev):
         check(lib().llima_lm_head_score_fp8(*_head8(x, head), B, head.H, V, float(softcap), ld,
                                             tg.data_ptr(), lp.data_ptr(), gr.data_ptr(),
@@ -862,7 +862,7 @@ def _lm_head_verify_greedy_fp8(hidden, head: Fp8LmHead, draft_ids, softcap, logi
     x = _fp8_hidden(hidden, head, "lm_head_verify_greedy")
     acc = torch.empty(B, dtype=torch.int32, device=dev)
     em = torch.empty((B, D + 1), dtype=torch.int32, device=dev)
-    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_verify_greedy_fp8_workspace_bytes(B, D, head.H, head.V))
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_verify_greedy_fp8_workspace_bytes(B, D, head.V))
     with _on(dev):
         check(lib().llima_lm_head_verify_greedy_fp8(*_head8(x, head), B, D, head.H, head.V,
                                                     float(softcap), ld, dr.data_ptr(),
@@ -886,7 +886,7 @@ def _lm_head_verify_tree_fp8(hidden, head: Fp8LmHead, retrieve_indices, candidat
     x = _fp8_hidden(hidden, head, "lm_head_verify_tree")
     K = x.values.shape[0]
     out = torch.empty(3, dtype=torch.int32, device=dev)
-    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_verify_tree_fp8_workspace_bytes(K, head.H, head.V))
+    ws = _scratch(dev, "lm_head_fp8", lib().llima_lm_head_verify_tree_fp8_workspace_bytes(K, head.V))
     with _on(dev):
         check(lib().llima_lm_head_verify_tree_fp8(*_head8(x, head), K, head.H, head.V,
                                                   float(softcap), ld, ri.data_ptr(), ca.data_ptr(),

@@ -73,8 +73,8 @@ def test_fp8_score_and_verification_refuse():
     assert t(P, P, P, P, 0, 64, 100, 0.0, 1, P, P, 2, 3, P, P, BIG, None) == -1
     assert t(P, P, P, P, 4, 64, 100, 0.0, 1, P, P, 0, 3, P, P, BIG, None) == -1
     assert t(P, P, P, P, 4, 64, 100, 0.0, 1, P, P, 2, 3, P, P, 0, None) == -4
-    assert l.llima_lm_head_argmax_fp8_workspace_bytes(0, 64, 10) == 0
-    assert l.llima_lm_head_argmax_fp8_workspace_bytes(3, 64, 65) >= 3 * 2 * 8
+    assert l.llima_lm_head_argmax_fp8_workspace_bytes(0, 10) == 0
+    assert l.llima_lm_head_argmax_fp8_workspace_bytes(3, 65) >= 3 * 8
 
 
 def test_python_refuses_on_host_tensors_and_shapes():
