@@ -267,41 +267,51 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
         const uint8_t* wb = sm + slot * SB + wr * VB * 4096;
         const uint8_t* xb = sm + slot * SB + WB + wc * MB * 4096;
         const bool half = c * 128 + 64 >= H;                 // uniform: H % 128 == 64, the last block
-        lmh_acc p[MB][VB];
+        // NE pieces of the block (two in the last one when H % 128 == 64); each
+        // read one ahead of its conversion
+        auto block = [&](auto ne) __attribute__((always_inline)) {
+            constexpr int NE = decltype(ne)::value;
+            lmh_acc p[MB][VB];
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int v = 0; v < VB; ++v)
+                for (int v = 0; v < VB; ++v)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) p[i][v][k] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (e < 2 || !half) {
+                    for (int k = 0; k < 16; ++k) p[i][v][k] = 0.0f;
+            llima_u32x4 w[2][VB], x[2][MB];
+            auto read = [&](int e) {
                 const uint32_t o = rl + ((((uint32_t)(2 * e + g)) ^ rz) << 4);
-                lmh_b8 w0[VB], w1[VB];
 #pragma unroll
-                for (int v = 0; v < VB; ++v) {
-                    const llima_u32x4 w = *(const llima_u32x4*)(wb + v * 4096 + o);
-                    w0[v] = lmh8_wide(w.x, w.y);
-                    w1[v] = lmh8_wide(w.z, w.w);
-                }
+                for (int v = 0; v < VB; ++v) w[e & 1][v] = *(const llima_u32x4*)(wb + v * 4096 + o);
 #pragma unroll
-                for (int i = 0; i < MB; ++i) {
-                    const llima_u32x4 x = *(const llima_u32x4*)(xb + i * 4096 + o);
-                    const lmh_b8 x0 = lmh8_wide(x.x, x.y), x1 = lmh8_wide(x.z, x.w);
+                for (int i = 0; i < MB; ++i) x[e & 1][i] = *(const llima_u32x4*)(xb + i * 4096 + o);
+            };
+            read(0);
 #pragma unroll
-                    for (int v = 0; v < VB; ++v) p[i][v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w0[v], x0, p[i][v], 0, 0, 0);
+            for (int e = 0; e < NE; ++e) {
+                if (e + 1 < NE) read(e + 1);
 #pragma unroll
-                    for (int v = 0; v < VB; ++v) p[i][v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w1[v], x1, p[i][v], 0, 0, 0);
+                for (int q = 0; q < 2; ++q) {
+                    lmh_b8 wv[VB], xv[MB];
+#pragma unroll
+                    for (int v = 0; v < VB; ++v) wv[v] = q ? lmh8_wide(w[e & 1][v].z, w[e & 1][v].w) : lmh8_wide(w[e & 1][v].x, w[e & 1][v].y);
+#pragma unroll
+                    for (int i = 0; i < MB; ++i) xv[i] = q ? lmh8_wide(x[e & 1][i].z, x[e & 1][i].w) : lmh8_wide(x[e & 1][i].x, x[e & 1][i].y);
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+#pragma unroll
+                        for (int v = 0; v < VB; ++v) p[i][v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[v], xv[i], p[i][v], 0, 0, 0);
                 }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int v = 0; v < VB; ++v)
+                for (int v = 0; v < VB; ++v)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) acc[i][v][k] = __builtin_fmaf(p[i][v][k], sc[i], acc[i][v][k]);
+                    for (int k = 0; k < 16; ++k) acc[i][v][k] = __builtin_fmaf(p[i][v][k], sc[i], acc[i][v][k]);
+        };
+        if (half) block(std::integral_constant<int, 2>{});
+        else block(std::integral_constant<int, 4>{});
         if (end) {                                           // uniform
             const int n = tile * LMH8_NV + wr * VB * 32;
             if (n < V) {                                     // uniform
