@@ -20,6 +20,8 @@
 // of 2^10, so that they become subnormal below 2^-24 of the row's largest.
 //
 // Bound: reading K and V once for all N Hq / Hkv rows of a key head.
+#include <type_traits>
+
 #include "common.hpp"
 #include "../../include/llima_sampler.h"
 
@@ -48,7 +50,6 @@ struct AttnParams {
 };
 
 #define AT_KEYS (1 << 30)              // keys of a sequence at most
-#define AT_TAB 1024                    // table entries of a chunk kept in LDS
 
 __device__ __forceinline__ uint32_t at_page(const AttnParams& P, int j) {
     return (uint32_t)(((uint64_t)(uint32_t)j * P.page_mul) >> P.page_shift);
@@ -101,16 +102,14 @@ __device__ __forceinline__ int at_len(const AttnParams& P, int b, bool& bad) {
 
 // The partition of all sequences' keys into chunks of one length, a multiple
 // of T: as long as gives at most P.ntarget + B chunks (a sequence's last may be
-// short).  Finds slot's sequence and the chunk's place in it; first is the
-// sequence's first slot.  False past the last chunk.  Every lane of a wave
-// calls it and gets the same.
+// short).  Every lane of a wave calls these and gets the same.
 template <int T>
-__device__ __forceinline__ int at_chunk(const AttnParams& P) {
+__device__ __forceinline__ int at_chunk(const AttnParams& P, int len0) {
     const int lane = (int)lane_id();
-    int64_t total = 0;
-    for (int b0 = 0; b0 < P.B; b0 += 64) {
+    int64_t total = lane < P.B ? len0 + P.N : 0;             // len0: sequence lane's length
+    for (int b = 64 + lane; b < P.B; b += 64) {
         bool bad;
-        if (b0 + lane < P.B) total += at_len(P, b0 + lane, bad) + P.N;
+        total += at_len(P, b, bad) + P.N;
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
@@ -119,13 +118,16 @@ __device__ __forceinline__ int at_chunk(const AttnParams& P) {
     return (int)((c + T - 1) / T) * T;
 }
 
-__device__ __forceinline__ bool at_find(const AttnParams& P, int chunk, int slot, int& b, int& first) {
+// slot's sequence, its length and its first slot; false past the last chunk.
+__device__ __forceinline__ bool at_find(const AttnParams& P, int chunk, int slot, int len0, int& b,
+                                        int& first, int& len) {
     const int lane = (int)lane_id();
     int before = 0;
     for (int b0 = 0; b0 < P.B; b0 += 64) {
         bool bad;
         const bool in = b0 + lane < P.B;
-        const int n = in ? (at_len(P, in ? b0 + lane : 0, bad) + P.N + chunk - 1) / chunk : 0;
+        const int ln = !in ? 0 : b0 ? at_len(P, b0 + lane, bad) : len0;
+        const int n = in ? (ln + P.N + chunk - 1) / chunk : 0;
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -136,10 +138,11 @@ __device__ __forceinline__ bool at_find(const AttnParams& P, int chunk, int slot
         if (past) {
             const int l = __builtin_ctzll(past);
             b = b0 + l;
-            first = before + __shfl(incl - n, l, 64);
+            first = before + (int)readlane((uint32_t)(incl - n), l);
+            len = (int)readlane((uint32_t)ln, l);
             return true;
         }
-        before += __shfl(incl, 63, 64);
+        before += (int)readlane((uint32_t)incl, 63);
     }
     return false;
 }
@@ -158,138 +161,139 @@ __device__ __forceinline__ void at_wait_barrier() {
 // a group of up to NW / KW row tiles (32 rows each).  Keys come in tiles of T,
 // requested straight into a ring of S stages; KW waves share a row tile and take
 // half of a tile's keys each (KW = 2), or one takes all.
-template <int DT, int D, int NW, int KW, int T, int S>
-__global__ __launch_bounds__(64 * NW) void tree_attn(AttnParams P) {
+//
+// Tiles of cached keys alone: a request takes 64 / (D / 8) keys, which lie in one
+// page (contiguous caches and pages of a multiple of 8), so that its address is
+// the wave's and comes from the scalar unit; GEN, for other page sizes and
+// strides, computes one per lane.  The tiles after them, which hold drafted keys
+// or end the chunk, come one at a time with the mask.
+template <int DT, int D, int NW, int KW, int T, int S, bool GEN>
+__global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_attn(AttnParams P) {
     constexpr int U = D / 8;                                 // 16-byte units of a key row
     constexpr int KQ = 64 / U;                               // keys per 1 KB request
     constexpr int NQ = (T / KQ + NW - 1) / NW;               // requests per wave and tile, K and V each
     constexpr int TB = T * D * 2;                            // bytes of a tile of K or V
     constexpr int KPW = T / 32 / KW;                         // 32-key blocks per wave
-    static_assert(T / KQ % NW == 0 || NQ == 1, "requests split evenly");
+    static_assert(T / KQ % NW == 0, "requests split evenly");
     static_assert(KPW >= 1, "a block per wave");
-    // one array: with several the compiler waits for every request before each LDS read
-    __shared__ __align__(1024) uint8_t sm[S * 2 * TB + 4 * AT_TAB + 16];
-    int32_t* const tab = (int32_t*)(sm + S * 2 * TB);
-    uint32_t* const flag = (uint32_t*)(sm + S * 2 * TB + 4 * AT_TAB);   // a bad page or length; special values
+    __shared__ __align__(1024) uint8_t sm[S * 2 * TB + 16];
+    uint32_t* const flag = (uint32_t*)(sm + S * 2 * TB);     // a bad page or length; special values
     const int t = (int)threadIdx.x, lane = t & 63, g = lane >> 5, r = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int rw = wave / KW, kw = wave % KW;
     const int h = (int)(blockIdx.x % (uint32_t)P.Hkv), rg = (int)(blockIdx.x / (uint32_t)P.Hkv % (uint32_t)P.RG);
     const int slot = (int)(blockIdx.x / (uint32_t)(P.Hkv * P.RG));
-    const int chunk = at_chunk<T>(P);
-    int b, first;
-    if (!at_find(P, chunk, slot, b, first)) return;          // uniform
+    bool bad = false;
+    const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
+    const int chunk = __builtin_amdgcn_readfirstlane(at_chunk<T>(P, len0));
+    int b, first, len;
+    if (!at_find(P, chunk, slot, len0, b, first, len)) return;   // uniform
     b = __builtin_amdgcn_readfirstlane(b);
     first = __builtin_amdgcn_readfirstlane(first);
-    bool bad;
-    const int len = __builtin_amdgcn_readfirstlane(at_len(P, b, bad));
+    len = __builtin_amdgcn_readfirstlane(len);
     const int nkeys = len + P.N, nchunk = (nkeys + chunk - 1) / chunk;
     const int j0 = (slot - first) * chunk, j1 = j0 + chunk < nkeys ? j0 + chunk : nkeys;
-    const int ntile = (j1 - j0 + T - 1) / T;
-    if (t == 0) { flag[0] = bad ? 1u : 0u; flag[1] = 0u; }
-    // the chunk's table entries
-    const int jc = j1 < len ? j1 : len;                      // its cached keys end here
-    const uint32_t e0 = P.table ? at_page(P, j0) : 0u;
-    const int ne = P.table && jc > j0 ? (int)(at_page(P, jc - 1) - e0) + 1 : 0;
-    const bool in_lds = ne <= AT_TAB;                        // uniform
-    if (in_lds)
-        for (int i = t; i < ne; i += 64 * NW) tab[i] = P.table[b * P.ts + e0 + i];
+    const int jc = j1 < len ? j1 : len;                      // the chunk's cached keys end here
+    const int nfull = jc > j0 ? (jc - j0) / T : 0;           // tiles of cached keys alone
+    if (t == 0) {
+        bool wrong;
+        at_len(P, b, wrong);
+        flag[0] = wrong ? 1u : 0u;
+        flag[1] = 0u;
+    }
     // the wave's rows: node n and query head of row tile rw
     const int row = (rg * P.RT + rw) * 32 + r;
     const bool active = rw < P.RT && (rg * P.RT + rw) * 32 < P.R;   // uniform: the wave has rows
     const int rc = row < P.R ? row : P.R - 1;
     const int n = rc / P.G, hq = h * P.G + rc % P.G;
+    // requests: the lane's key of a request and its 16-byte unit of K and V
+    const int kq = lane / U, unit = lane % U;
+    bool miss = false;
+    // a page of the sequence (uniform): the page's number, or 0 and a miss
+    auto page_of = [&](int j) {
+        const __attribute__((address_space(4))) int32_t* tab = (const __attribute__((address_space(4))) int32_t*)(P.table + b * P.ts);
+        return tab[at_page(P, j)];
+    };
+    int pg[NQ];
+    auto lookup = [&](int tile) {
+        if (!GEN && P.table) {                               // uniform
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) pg[i] = page_of(j0 + tile * T + (wave + NW * i) * KQ);
+        }
+    };
+    auto at_k = [&](int i) { return (uint32_t)((unit ^ (((wave + NW * i) * KQ + kq) & (U - 1) & 15)) * 16); };
+    auto at_v = [&](int i) { return (uint32_t)((unit ^ ((((wave + NW * i) * KQ + kq) & 3) << 2 & (U - 1))) * 16); };
+    // one key's rows, by lane: cached key or drafted token j
+    auto issue_key = [&](int i, int j, uint8_t* sk) {
+        const uint16_t *kp, *vp;
+        if (j < len) {
+            int64_t p = b, o = j;
+            if (P.table) {                                   // uniform
+                const uint32_t e = at_page(P, j);
+                o = j - (int)e * P.page;
+                int pi = P.table[b * P.ts + e];
+                if (pi < 0 || pi >= P.pages) { pi = 0; miss = true; }
+                p = pi;
+            }
+            kp = (const uint16_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2];
+            vp = (const uint16_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2];
+        } else {
+            kp = (const uint16_t*)P.k + b * P.ks[0] + (j - len) * P.ks[1] + h * P.ks[2];
+            vp = (const uint16_t*)P.v + b * P.vs[0] + (j - len) * P.vs[1] + h * P.vs[2];
+        }
+        at_dma((const uint8_t*)kp + at_k(i), sk + (wave + NW * i) * 1024);
+        at_dma((const uint8_t*)vp + at_v(i), sk + TB + (wave + NW * i) * 1024);
+    };
+    uint32_t ok[NQ], ov[NQ];
+    if constexpr (!GEN) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            ok[i] = (uint32_t)kq * (uint32_t)(2 * P.kcs[1]) + at_k(i);
+            ov[i] = (uint32_t)kq * (uint32_t)(2 * P.vcs[1]) + at_v(i);
+        }
+    }
+    auto issue = [&](int tile, int st) {                     // a tile of cached keys
+        uint8_t* const sk = sm + st * 2 * TB;
+        if constexpr (GEN) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) issue_key(i, j0 + tile * T + (wave + NW * i) * KQ + kq, sk);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const int j = j0 + tile * T + (wave + NW * i) * KQ;
+                int p = b, o = j;
+                if (P.table) {                               // uniform
+                    p = pg[i];
+                    o = j - (int)at_page(P, j) * P.page;
+                    const bool out = p < 0 || p >= P.pages;
+                    miss |= out;
+                    p = out ? 0 : p;
+                }
+                const uint16_t* kb = (const uint16_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2];
+                const uint16_t* vb = (const uint16_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2];
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)kb, 0, 0x7FFFFFFF, 0x00027000),
+                    (__attribute__((address_space(3))) void*)(sk + (wave + NW * i) * 1024), 16, (int)ok[i], 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)vb, 0, 0x7FFFFFFF, 0x00027000),
+                    (__attribute__((address_space(3))) void*)(sk + TB + (wave + NW * i) * 1024), 16, (int)ov[i], 0, 0, 0);
+            }
+        }
+    };
     at_s8 qf[D / 16];
     {
         const uint16_t* qp = (const uint16_t*)P.q + b * P.qs[0] + n * P.qs[1] + hq * P.qs[2] + g * 8;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) qf[s] = *(const at_s8*)(qp + s * 16);
     }
-    // requests: the lane's key of request i of a tile and its 16-byte unit
-    const int kq = lane / U, unit = lane % U;
-    auto key_at = [&](int tile, int i) {                     // a key of the chunk (past its end: the last)
-        const int j = j0 + tile * T + (wave + NW * i) * KQ + kq;
-        return j < j1 ? j : j1 - 1;
-    };
-    bool miss = false;
-    auto issue = [&](int tile, int st) {
-        uint8_t* const sk = sm + st * 2 * TB;
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int qi = wave + NW * i;                    // request of the tile
-            if (T / KQ % NW == 0 || qi < T / KQ) {           // uniform
-                const int kt = qi * KQ + kq;                 // the key's place in the tile
-                const int j = key_at(tile, i);
-                const uint16_t *kp, *vp;
-                if (j < len) {
-                    int64_t p = b, o = j;
-                    if (P.table) {                           // uniform
-                        const uint32_t e = at_page(P, j);
-                        o = j - (int)e * P.page;
-                        int pi;
-                        if (in_lds) {                        // uniform
-                            pi = tab[e - e0];
-                        } else {
-                            pi = P.table[b * P.ts + e];
-                            __builtin_amdgcn_s_waitcnt(LLIMA_WAITCNT_VM0);
-                        }
-                        if (pi < 0 || pi >= P.pages) { pi = 0; miss = true; }
-                        p = pi;
-                    }
-                    kp = (const uint16_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2];
-                    vp = (const uint16_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2];
-                } else {
-                    kp = (const uint16_t*)P.k + b * P.ks[0] + (j - len) * P.ks[1] + h * P.ks[2];
-                    vp = (const uint16_t*)P.v + b * P.vs[0] + (j - len) * P.vs[1] + h * P.vs[2];
-                }
-                at_dma(kp + ((unit ^ (kt & (U - 1) & 15)) * 8), sk + qi * 1024);
-                at_dma(vp + ((unit ^ ((kt & 3) << 2 & (U - 1))) * 8), sk + TB + qi * 1024);
-            }
-        }
-    };
     at_acc o[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
-    if (ne > 0) __syncthreads();                             // uniform
-#pragma unroll
-    for (int e = 0; e < S - 1; ++e) issue(e < ntile ? e : ntile - 1, e);
-    for (int tile = 0; tile < ntile; ++tile) {
-        at_wait_barrier<(S - 2) * 2 * NQ>();                 // the tile has landed, and the last one is read
-        {
-            const int nt = tile + S - 1;                     // past the last: the last again, into a free stage
-            issue(nt < ntile ? nt : ntile - 1, nt % S);
-        }
-        uint8_t* const sk = sm + (tile % S) * 2 * TB;
-        const int jt = j0 + tile * T;
-        const bool tail = jt + T > len;                      // uniform: drafted keys, or past the end
-        if (tail) {
-            // Values that not every row sees: rows past the end become 0, and so
-            // do infinities and NaN of drafted tokens (0 times them would be NaN
-            // for the rows that do not see them; at the end they are added to the
-            // rows that do).
-            for (int p = t; p < T * U; p += 64 * NW) {
-                const int kt = p / U, j = jt + kt;
-                llima_u32x4* const at = (llima_u32x4*)(sk + TB + p * 16);
-                llima_u32x4 x = *at;
-                bool put = j >= j1;
-                if (put) x = (llima_u32x4){0u, 0u, 0u, 0u};
-                if (!put && j >= len) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t w = x[e];
-                        if (at_special<DT>((uint16_t)w)) { w &= 0xFFFF0000u; put = true; flag[1] = 1u; }
-                        if (at_special<DT>((uint16_t)(w >> 16))) { w &= 0xFFFFu; put = true; flag[1] = 1u; }
-                        x[e] = w;
-                    }
-                }
-                if (put) *at = x;
-            }
-            __syncthreads();
-        }
-        if (!active) continue;                               // uniform (the barriers are above)
+    // The products and the softmax of a staged tile.  see(j): whether the lane's
+    // row sees the tile's key j; ALL: it sees every one.
+    auto math = [&](const uint8_t* sk, auto all, auto see) __attribute__((always_inline)) {
+        constexpr bool ALL = decltype(all)::value;
         at_acc s[KPW];
 #pragma unroll
         for (int kb = 0; kb < KPW; ++kb) {
@@ -308,17 +312,7 @@ __global__ __launch_bounds__(64 * NW) void tree_attn(AttnParams P) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float x = s[kb][i] * P.scale2;
-                if (tail) {                                  // uniform
-                    const int j = jt + (kw * KPW + kb) * 32 + (i & 3) + 8 * (i >> 2) + 4 * g;
-                    bool see = j < len;
-                    if (!see && j < j1) {
-                        const int mm = j - len;
-                        if (!P.mask) see = mm <= n;
-                        else if (P.mask_f32) see = ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
-                        else see = ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
-                    }
-                    x = see ? x : -__builtin_inff();
-                }
+                if constexpr (!ALL) x = see((kw * KPW + kb) * 32 + (i & 3) + 8 * (i >> 2) + 4 * g) ? x : -__builtin_inff();
                 s[kb][i] = x;
                 mt = __builtin_fmaxf(mt, x);
             }
@@ -366,6 +360,63 @@ __global__ __launch_bounds__(64 * NW) void tree_attn(AttnParams P) {
                 }
             }
         }
+    };
+    auto seen = [&](int mm) {                                // the lane's row sees drafted token mm
+        if (!P.mask) return mm <= n;
+        if (P.mask_f32) return ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
+        return ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
+    };
+    if (nfull > 0) {                                         // uniform
+        lookup(0);
+#pragma unroll
+        for (int e = 0; e < S - 1; ++e) {                    // past the last tile: that again, which nobody reads
+            issue(e < nfull ? e : nfull - 1, e);
+            lookup(e + 1 < nfull ? e + 1 : nfull - 1);
+        }
+        for (int tile = 0; tile < nfull; ++tile) {
+            at_wait_barrier<(S - 2) * 2 * NQ>();             // the tile has landed, and the last one is read
+            const int nt = tile + S - 1;
+            issue(nt < nfull ? nt : nfull - 1, nt % S);
+            lookup(nt + 1 < nfull ? nt + 1 : nfull - 1);
+            if (active) math(sm + (tile % S) * 2 * TB, std::integral_constant<bool, true>{}, [](int) { return true; });
+        }
+        at_wait_barrier<0>();                                // the ring is free
+    }
+    // The rest, one tile at a time in the first stage.
+    for (int jt = j0 + nfull * T; jt < j1; jt += T) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int j = jt + (wave + NW * i) * KQ + kq;    // past the chunk's end: its last key
+            issue_key(i, j < j1 ? j : j1 - 1, sm);
+        }
+        at_wait_barrier<0>();
+        // Values that not every row sees: rows past the end become 0, and so do
+        // infinities and NaN of drafted tokens (0 times them would be NaN for the
+        // rows that do not see them; at the end they are added to the rows that do).
+        for (int p = t; p < T * U; p += 64 * NW) {
+            const int j = jt + p / U;
+            llima_u32x4* const at = (llima_u32x4*)(sm + TB + p * 16);
+            llima_u32x4 x = *at;
+            bool put = j >= j1;
+            if (put) x = (llima_u32x4){0u, 0u, 0u, 0u};
+            if (!put && j >= len) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t w = x[e];
+                    if (at_special<DT>((uint16_t)w)) { w &= 0xFFFF0000u; put = true; flag[1] = 1u; }
+                    if (at_special<DT>((uint16_t)(w >> 16))) { w &= 0xFFFFu; put = true; flag[1] = 1u; }
+                    x[e] = w;
+                }
+            }
+            if (put) *at = x;
+        }
+        __syncthreads();
+        if (active)
+            math(sm, std::integral_constant<bool, false>{}, [&](int k) {
+                const int j = jt + k;
+                return j < len || (j < j1 && seen(j - len));
+            });
+        __syncthreads();
     }
     if (miss) flag[0] = 1u;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no request outlives this
@@ -373,6 +424,7 @@ __global__ __launch_bounds__(64 * NW) void tree_attn(AttnParams P) {
     l += __shfl_xor(l, 32, 64);
     if constexpr (KW > 1) {                                  // the second half of the keys joins the first
         float* const red = (float*)sm + (size_t)rw * 64 * (D / 2 + 2);
+        static_assert(NW / KW * 64 * (D / 2 + 2) * 4 <= S * 2 * TB, "room for the second halves");
         if (active && kw == 1) {
             red[lane] = m;
             red[64 + lane] = l;
@@ -395,13 +447,9 @@ __global__ __launch_bounds__(64 * NW) void tree_attn(AttnParams P) {
         }
     }
     if (!active || row >= P.R) return;
-    if (flag[1]) {                                          // infinities and NaN of drafted tokens in this chunk
+    if (flag[1]) {                                           // infinities and NaN of drafted tokens in this chunk
         for (int mm = (j0 > len ? j0 : len) - len; mm < j1 - len; ++mm) {
-            bool see;
-            if (!P.mask) see = mm <= n;
-            else if (P.mask_f32) see = ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
-            else see = ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
-            if (!see) continue;
+            if (!seen(mm)) continue;
             const uint16_t* vp = (const uint16_t*)P.v + b * P.vs[0] + mm * P.vs[1] + h * P.vs[2];
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
@@ -438,19 +486,19 @@ __global__ __launch_bounds__(64 * NW) void tree_attn(AttnParams P) {
 template <int DT, int D, int T>
 __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
     constexpr int E = D / 64;                                // values per lane
-    const int lane = (int)lane_id(), chunk = at_chunk<T>(P);
+    const int lane = (int)lane_id();
+    bool bad;
+    const int chunk = at_chunk<T>(P, lane < P.B ? at_len(P, lane, bad) : 0);
     const int64_t w = (int64_t)blockIdx.x * LLIMA_WAVES + wave_id();
     if (w >= (int64_t)P.B * P.N * P.Hq) return;
     const int b = (int)(w / (P.N * P.Hq)), n = (int)(w / P.Hq % P.N), hq = (int)(w % P.Hq);
     // the sequence's first chunk
     int first = 0;
     for (int i = lane; i < b; i += 64) {
-        bool bad;
         first += (at_len(P, i, bad) + P.N + chunk - 1) / chunk;
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
-    bool bad;
     const int nchunk = (at_len(P, b, bad) + P.N + chunk - 1) / chunk;
     if (nchunk <= 1) return;
     const int h = hq / P.G, row = n * P.G + hq % P.G;
@@ -543,15 +591,21 @@ static int at_row_tiles(int R, int& RG) {                    // row tiles of a g
     return (rt + RG - 1) / RG;
 }
 
-template <int DT, int D>
+template <int DT, int D, bool GEN>
 static void at_launch(const AttnParams& P, hipStream_t st) {
     const dim3 g((uint32_t)P.slots * P.RG * P.Hkv);
-    constexpr int T = D == 256 ? 32 : 64, KW = D == 256 ? 1 : 2;
-    constexpr int S2 = D == 64 ? 4 : 2, S8 = 4;
-    if (P.RT <= (KW == 2 ? 1 : 2)) hipLaunchKernelGGL((tree_attn<DT, D, 2, KW, T, S2>), g, dim3(128), 0, st, P);
-    else if (P.RT <= (KW == 2 ? 2 : 4)) hipLaunchKernelGGL((tree_attn<DT, D, 4, KW, T, S2>), g, dim3(256), 0, st, P);
-    else if (KW == 2 && P.RT <= 4) hipLaunchKernelGGL((tree_attn<DT, D, 8, KW, T, S8>), g, dim3(512), 0, st, P);
-    else hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8>), g, dim3(512), 0, st, P);
+    constexpr int T = D == 256 ? 32 : 64, K2 = D == 256 ? 1 : 2;
+    constexpr int S2 = D == 64 ? 4 : 2, S4 = D == 256 ? 4 : S2, S8 = 4;
+    if (P.RT <= (K2 == 2 ? 1 : 2)) {
+        hipLaunchKernelGGL((tree_attn<DT, D, 2, K2, T, S2, GEN>), g, dim3(128), 0, st, P);
+    } else if (P.RT <= 4) {
+        if constexpr (K2 == 2) {
+            if (P.RT <= 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 2, T, S4, GEN>), g, dim3(256), 0, st, P);
+        }
+        if (K2 == 1 || P.RT > 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 1, T, S4, GEN>), g, dim3(256), 0, st, P);
+    } else {
+        hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8, GEN>), g, dim3(512), 0, st, P);
+    }
     const int64_t rows = (int64_t)P.B * P.N * P.Hq;
     hipLaunchKernelGGL((tree_attn_join<DT, D, T>), dim3((uint32_t)((rows + LLIMA_WAVES - 1) / LLIMA_WAVES)),
                        dim3(LLIMA_WG), 0, st, P);
@@ -559,9 +613,11 @@ static void at_launch(const AttnParams& P, hipStream_t st) {
 
 template <int DT>
 static int at_dispatch(const AttnParams& P, int D, hipStream_t st) {
-    if (D == 64) at_launch<DT, 64>(P, st);
-    else if (D == 128) at_launch<DT, 128>(P, st);
-    else at_launch<DT, 256>(P, st);
+    // a request's keys (8 at most) lie in one page and within 2^31 bytes
+    const bool gen = (P.table && P.page % 8 != 0) || P.kcs[1] > (1 << 26) || P.vcs[1] > (1 << 26);
+    if (D == 64) gen ? at_launch<DT, 64, true>(P, st) : at_launch<DT, 64, false>(P, st);
+    else if (D == 128) gen ? at_launch<DT, 128, true>(P, st) : at_launch<DT, 128, false>(P, st);
+    else gen ? at_launch<DT, 256, true>(P, st) : at_launch<DT, 256, false>(P, st);
     return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
 }
 
