@@ -44,15 +44,25 @@ struct AttnParams {
     int32_t B, N, Hq, Hkv, G, R;                             // R = N G rows of a key head
     int32_t page, pages;                                     // tokens of a page; pages of the cache
     uint32_t page_mul, page_shift;                           // j / page = j page_mul >> page_shift, j < 2^30
-    int32_t slots, ntarget;                                  // key chunks: at most, and wished for
+    int32_t slots, parts;                                    // partial sums per key head at most; shares of the keys
     int32_t RG, RT;                                          // row groups, row tiles of a group
-    float scale2;                                            // scale log2(e)
+    float scale2;                                            // |scale| log2(e)
+    int32_t flip;                                            // scale < 0
+    int32_t mode;                                            // AT_TILE, AT_REQUEST or AT_LANE
 };
 
 #define AT_KEYS (1 << 30)              // keys of a sequence at most
+#define AT_TILE 0
+#define AT_REQUEST 1
+#define AT_LANE 2
 
 __device__ __forceinline__ uint32_t at_page(const AttnParams& P, int j) {
     return (uint32_t)(((uint64_t)(uint32_t)j * P.page_mul) >> P.page_shift);
+}
+
+__device__ __forceinline__ uint64_t readfirstlane64(uint64_t v) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+           (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
 }
 
 typedef float at_acc __attribute__((ext_vector_type(16)));
@@ -100,49 +110,58 @@ __device__ __forceinline__ int at_len(const AttnParams& P, int b, bool& bad) {
     return bad ? 0 : l;
 }
 
-// The partition of all sequences' keys into chunks of one length, a multiple
-// of T: as long as gives at most P.ntarget + B chunks (a sequence's last may be
-// short).  Every lane of a wave calls these and gets the same.
+// The partition of the keys: each sequence's are tiles of T, all sequences'
+// tiles stand in a row, and P.parts workgroups (per key head and row group)
+// take equal shares of it.  A share may hold parts of several sequences; part x
+// of sequence b leaves its sums in slot x + b, which no other pair has.
+// at_tiles: sequence b's tiles; at_share: the length of a share (every lane of
+// a wave calls it and gets the same).  len0: the length of sequence lane.
+// A sequence counts for AT_EXTRA tiles more than it has, at its end: the time that
+// its mask, its sums' exchange and the next sequence's start take.
+#define AT_EXTRA 3
 template <int T>
-__device__ __forceinline__ int at_chunk(const AttnParams& P, int len0) {
+__device__ __forceinline__ int at_tiles(const AttnParams& P, int len) { return (len + P.N + T - 1) / T + AT_EXTRA; }
+
+template <int T>
+__device__ __forceinline__ int64_t at_share(const AttnParams& P, int len0) {
     const int lane = (int)lane_id();
-    int64_t total = lane < P.B ? len0 + P.N : 0;             // len0: sequence lane's length
+    int64_t total = lane < P.B ? at_tiles<T>(P, len0) : 0;
     for (int b = 64 + lane; b < P.B; b += 64) {
         bool bad;
-        total += at_len(P, b, bad) + P.N;
+        total += at_tiles<T>(P, at_len(P, b, bad));
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
-    int64_t c = (total + P.ntarget - 1) / P.ntarget;
-    c = c < AT_KEYS ? c : AT_KEYS;
-    return (int)((c + T - 1) / T) * T;
+    return (total + P.parts - 1) / P.parts;
 }
 
-// slot's sequence, its length and its first slot; false past the last chunk.
-__device__ __forceinline__ bool at_find(const AttnParams& P, int chunk, int slot, int len0, int& b,
-                                        int& first, int& len) {
+// The sequence that has tile `at` of the row, its length, and its first tile's
+// place in the row; false past the last tile.
+template <int T>
+__device__ __forceinline__ bool at_find(const AttnParams& P, int64_t at, int len0, int& b, int& len,
+                                        int64_t& first) {
     const int lane = (int)lane_id();
-    int before = 0;
+    int64_t before = 0;
     for (int b0 = 0; b0 < P.B; b0 += 64) {
         bool bad;
         const bool in = b0 + lane < P.B;
         const int ln = !in ? 0 : b0 ? at_len(P, b0 + lane, bad) : len0;
-        const int n = in ? (ln + P.N + chunk - 1) / chunk : 0;
-        int incl = n;
+        const int64_t n = in ? at_tiles<T>(P, ln) : 0;
+        int64_t incl = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(incl, o, 64);
+            const int64_t up = __shfl_up(incl, o, 64);
             incl += lane >= o ? up : 0;
         }
-        const uint64_t past = ballot(in && before + incl > slot);
+        const uint64_t past = ballot(in && before + incl > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             b = b0 + l;
-            first = before + (int)readlane((uint32_t)(incl - n), l);
+            first = before + (int64_t)readlane64((uint64_t)(incl - n), l);
             len = (int)readlane((uint32_t)ln, l);
             return true;
         }
-        before += (int)readlane((uint32_t)incl, 63);
+        before += (int64_t)readlane64((uint64_t)incl, 63);
     }
     return false;
 }
@@ -157,18 +176,18 @@ __device__ __forceinline__ void at_wait_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// One workgroup: NW waves over one chunk of a sequence's keys, one key head and
-// a group of up to NW / KW row tiles (32 rows each).  Keys come in tiles of T,
-// requested straight into a ring of S stages; KW waves share a row tile and take
-// half of a tile's keys each (KW = 2), or one takes all.
+// One workgroup: NW waves over one share of the keys, one key head and a group of
+// up to NW / KW row tiles (32 rows each).  Keys come in tiles of T, requested straight into a ring of S stages; KW waves share a row tile and
+// take half of a tile's keys each (KW = 2), or one takes all.
 //
-// Tiles of cached keys alone: a request takes 64 / (D / 8) keys, which lie in one
-// page (contiguous caches and pages of a multiple of 8), so that its address is
-// the wave's and comes from the scalar unit; GEN, for other page sizes and
-// strides, computes one per lane.  The tiles after them, which hold drafted keys
-// or end the chunk, come one at a time with the mask.
-template <int DT, int D, int NW, int KW, int T, int S, bool GEN>
+// Tiles of cached keys alone are requested by mode: a tile lies in one page
+// (contiguous caches and pages of a multiple of 64), its address is the wave's
+// and comes from the scalar unit; or each request does (its 8 keys at most: pages of
+// a multiple of 8); or every lane computes its own.  The tiles after them, which hold drafted keys
+// or end a part, come one at a time with the mask.
+template <int DT, int D, int NW, int KW, int T, int S>
 __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_attn(AttnParams P) {
+#ifdef __HIP_DEVICE_COMPILE__                               // (the host pass drops the launch stub over the descriptors)
     constexpr int U = D / 8;                                 // 16-byte units of a key row
     constexpr int KQ = 64 / U;                               // keys per 1 KB request
     constexpr int NQ = (T / KQ + NW - 1) / NW;               // requests per wave and tile, K and V each
@@ -182,19 +201,28 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int rw = wave / KW, kw = wave % KW;
     const int h = (int)(blockIdx.x % (uint32_t)P.Hkv), rg = (int)(blockIdx.x / (uint32_t)P.Hkv % (uint32_t)P.RG);
-    const int slot = (int)(blockIdx.x / (uint32_t)(P.Hkv * P.RG));
+    const int part = (int)(blockIdx.x / (uint32_t)(P.Hkv * P.RG));
     bool bad = false;
     const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
-    const int chunk = __builtin_amdgcn_readfirstlane(at_chunk<T>(P, len0));
-    int b, first, len;
-    if (!at_find(P, chunk, slot, len0, b, first, len)) return;   // uniform
+    const int64_t share = (int64_t)readfirstlane64((uint64_t)at_share<T>(P, len0));
+    const int64_t end = (part + 1) * share;
+    for (int64_t from = part * share; from < end;) {         // the share's sequences
+    int b, len;
+    int64_t first;
+    if (!at_find<T>(P, from, len0, b, len, first)) return;   // uniform: past the last tile
     b = __builtin_amdgcn_readfirstlane(b);
-    first = __builtin_amdgcn_readfirstlane(first);
     len = __builtin_amdgcn_readfirstlane(len);
-    const int nkeys = len + P.N, nchunk = (nkeys + chunk - 1) / chunk;
-    const int j0 = (slot - first) * chunk, j1 = j0 + chunk < nkeys ? j0 + chunk : nkeys;
-    const int jc = j1 < len ? j1 : len;                      // the chunk's cached keys end here
+    first = (int64_t)readfirstlane64((uint64_t)first);
+    const int nkeys = len + P.N;
+    const int64_t last = first + at_tiles<T>(P, len), upto = last < end ? last : end;
+    const int64_t je = (upto - first) * T;
+    const int j0 = (int)(from - first) * T, j1 = je < nkeys ? (int)je : nkeys;
+    const bool whole = from == first && upto >= last - AT_EXTRA;   // the sequence has no other part
+    from = upto;
+    if (j0 >= nkeys) continue;                               // uniform: nothing of it but the extra tiles
+    const int jc = j1 < len ? j1 : len;                      // the part's cached keys end here
     const int nfull = jc > j0 ? (jc - j0) / T : 0;           // tiles of cached keys alone
+    __syncthreads();                                         // (the sequence before is done with LDS)
     if (t == 0) {
         bool wrong;
         at_len(P, b, wrong);
@@ -209,18 +237,6 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
     // requests: the lane's key of a request and its 16-byte unit of K and V
     const int kq = lane / U, unit = lane % U;
     bool miss = false;
-    // a page of the sequence (uniform): the page's number, or 0 and a miss
-    auto page_of = [&](int j) {
-        const __attribute__((address_space(4))) int32_t* tab = (const __attribute__((address_space(4))) int32_t*)(P.table + b * P.ts);
-        return tab[at_page(P, j)];
-    };
-    int pg[NQ];
-    auto lookup = [&](int tile) {
-        if (!GEN && P.table) {                               // uniform
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) pg[i] = page_of(j0 + tile * T + (wave + NW * i) * KQ);
-        }
-    };
     auto at_k = [&](int i) { return (uint32_t)((unit ^ (((wave + NW * i) * KQ + kq) & (U - 1) & 15)) * 16); };
     auto at_v = [&](int i) { return (uint32_t)((unit ^ ((((wave + NW * i) * KQ + kq) & 3) << 2 & (U - 1))) * 16); };
     // one key's rows, by lane: cached key or drafted token j
@@ -244,45 +260,72 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         at_dma((const uint8_t*)kp + at_k(i), sk + (wave + NW * i) * 1024);
         at_dma((const uint8_t*)vp + at_v(i), sk + TB + (wave + NW * i) * 1024);
     };
-    uint32_t ok[NQ], ov[NQ];
-    if constexpr (!GEN) {
+    // the page of key j (uniform), by the scalar unit
+    auto page_of = [&](int j) {
+        const __attribute__((address_space(4))) int32_t* tab = (const __attribute__((address_space(4))) int32_t*)(P.table + b * P.ts);
+        return tab[at_page(P, j)];
+    };
+    auto base_of = [&](const void* c, const int64_t (&cs)[3], int p, int o) {
+        return (void*)((const uint16_t*)c + p * cs[0] + o * cs[1] + h * cs[2]);
+    };
+    uint32_t ok[NQ], ov[NQ];                                 // the lane's offsets within a tile
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            ok[i] = (uint32_t)kq * (uint32_t)(2 * P.kcs[1]) + at_k(i);
-            ov[i] = (uint32_t)kq * (uint32_t)(2 * P.vcs[1]) + at_v(i);
-        }
+    for (int i = 0; i < NQ; ++i) {
+        const uint32_t key = (uint32_t)((wave + NW * i) * KQ + kq);
+        ok[i] = key * (uint32_t)(2 * P.kcs[1]) + at_k(i);
+        ov[i] = key * (uint32_t)(2 * P.vcs[1]) + at_v(i);
     }
+    auto place = [&](int j, int pi, int& p, int& o) {        // cached key j's page and place in it
+        p = b;
+        o = j;
+        if (P.table) {                                       // uniform
+            o = j - (int)at_page(P, j) * P.page;
+            const bool out = pi < 0 || pi >= P.pages;
+            miss |= out;
+            p = out ? 0 : pi;
+        }
+    };
+    int pg = 0;                                              // the page of the next tile to request
+    auto lookup = [&](int tile) {
+        if (P.mode == AT_TILE && P.table && tile < nfull) pg = page_of(j0 + tile * T);   // uniform
+    };
     auto issue = [&](int tile, int st) {                     // a tile of cached keys
         uint8_t* const sk = sm + st * 2 * TB;
-        if constexpr (GEN) {
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) issue_key(i, j0 + tile * T + (wave + NW * i) * KQ + kq, sk);
-        } else {
+        const int jt = j0 + tile * T;
+        if (P.mode == AT_TILE) {                             // uniform
+            int p, o;
+            place(jt, pg, p, o);
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(base_of(P.kc, P.kcs, p, o), 0, 0x7FFFFFFF, 0x00027000);
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(base_of(P.vc, P.vcs, p, o), 0, 0x7FFFFFFF, 0x00027000);
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
-                const int j = j0 + tile * T + (wave + NW * i) * KQ;
-                int p = b, o = j;
-                if (P.table) {                               // uniform
-                    p = pg[i];
-                    o = j - (int)at_page(P, j) * P.page;
-                    const bool out = p < 0 || p >= P.pages;
-                    miss |= out;
-                    p = out ? 0 : p;
-                }
-                const uint16_t* kb = (const uint16_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2];
-                const uint16_t* vb = (const uint16_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2];
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)kb, 0, 0x7FFFFFFF, 0x00027000),
-                    (__attribute__((address_space(3))) void*)(sk + (wave + NW * i) * 1024), 16, (int)ok[i], 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)vb, 0, 0x7FFFFFFF, 0x00027000),
-                    (__attribute__((address_space(3))) void*)(sk + TB + (wave + NW * i) * 1024), 16, (int)ov[i], 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(sk + (wave + NW * i) * 1024), 16, (int)ok[i], 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(sk + TB + (wave + NW * i) * 1024), 16, (int)ov[i], 0, 0, 0);
             }
+        } else if (P.mode == AT_REQUEST) {                   // uniform
+#pragma unroll 1
+            for (int i = 0; i < NQ; ++i) {
+                const int j = jt + (wave + NW * i) * KQ;
+                int p, o;
+                place(j, P.table ? page_of(j) : 0, p, o);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(base_of(P.kc, P.kcs, p, o), 0, 0x7FFFFFFF, 0x00027000),
+                    (__attribute__((address_space(3))) void*)(sk + (wave + NW * i) * 1024), 16, (int)((uint32_t)kq * (uint32_t)(2 * P.kcs[1]) + at_k(i)), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(base_of(P.vc, P.vcs, p, o), 0, 0x7FFFFFFF, 0x00027000),
+                    (__attribute__((address_space(3))) void*)(sk + TB + (wave + NW * i) * 1024), 16, (int)((uint32_t)kq * (uint32_t)(2 * P.vcs[1]) + at_v(i)), 0, 0, 0);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < NQ; ++i) issue_key(i, jt + (wave + NW * i) * KQ + kq, sk);
         }
     };
     at_s8 qf[D / 16];
     {
         const uint16_t* qp = (const uint16_t*)P.q + b * P.qs[0] + n * P.qs[1] + hq * P.qs[2] + g * 8;
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) qf[s] = *(const at_s8*)(qp + s * 16);
+        for (int s = 0; s < D / 16; ++s) {                   // a negative scale's sign goes to q
+            qf[s] = *(const at_s8*)(qp + s * 16);
+            if (P.flip) qf[s] ^= (short)0x8000;              // uniform
+        }
     }
     at_acc o[D / 32];
 #pragma unroll
@@ -290,9 +333,9 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
-    // The products and the softmax of a staged tile.  see(j): whether the lane's
+    // The products and the softmax of a staged tile.  Bit j of bits: the lane's
     // row sees the tile's key j; ALL: it sees every one.
-    auto math = [&](const uint8_t* sk, auto all, auto see) __attribute__((always_inline)) {
+    auto math = [&](const uint8_t* sk, auto all, uint64_t bits) __attribute__((always_inline)) {
         constexpr bool ALL = decltype(all)::value;
         at_acc s[KPW];
 #pragma unroll
@@ -311,12 +354,15 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         for (int kb = 0; kb < KPW; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float x = s[kb][i] * P.scale2;
-                if constexpr (!ALL) x = see((kw * KPW + kb) * 32 + (i & 3) + 8 * (i >> 2) + 4 * g) ? x : -__builtin_inff();
-                s[kb][i] = x;
-                mt = __builtin_fmaxf(mt, x);
+                if constexpr (!ALL) {
+                    const float x = s[kb][i] * P.scale2;
+                    const uint32_t w = (uint32_t)(bits >> ((kw * KPW + kb) * 32)) >> (4 * g);
+                    s[kb][i] = w >> ((i & 3) + 8 * (i >> 2)) & 1u ? x : -__builtin_inff();
+                }
+                mt = __builtin_fmaxf(mt, s[kb][i]);
             }
         mt = __builtin_fmaxf(mt, __shfl_xor(mt, 32, 64));
+        if constexpr (ALL) mt *= P.scale2;                   // scale2 >= 0
         const float mn = __builtin_fmaxf(m, mt);
         const float mu = mn > -__builtin_inff() ? mn : 0.0f;
         const float mup = DT == LLIMA_F16 ? mu - 10.0f : mu;
@@ -334,7 +380,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
             float ls = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] - mup);
+                s[kb][i] = __builtin_amdgcn_exp2f(ALL ? __builtin_fmaf(s[kb][i], P.scale2, -mup) : s[kb][i] - mup);
                 ls += s[kb][i];
             }
             l += ls;
@@ -366,36 +412,59 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         if (P.mask_f32) return ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
         return ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
     };
-    if (nfull > 0) {                                         // uniform
-        lookup(0);
-#pragma unroll
-        for (int e = 0; e < S - 1; ++e) {                    // past the last tile: that again, which nobody reads
-            issue(e < nfull ? e : nfull - 1, e);
-            lookup(e + 1 < nfull ? e + 1 : nfull - 1);
+    const int ntile = (j1 - j0 + T - 1) / T;
+    // a tile of the part; past the last one that again, which nobody reads
+    auto request = [&](int tile, int st) {
+        const int tl = tile < ntile ? tile : ntile - 1;
+        if (tl < nfull) {                                    // uniform
+            issue(tl, st);
+        } else {
+            uint8_t* const sk = sm + st * 2 * TB;
+#pragma unroll 1
+            for (int i = 0; i < NQ; ++i) {
+                const int j = j0 + tl * T + (wave + NW * i) * KQ + kq;   // past the part's end: its last key
+                issue_key(i, j < j1 ? j : j1 - 1, sk);
+            }
         }
-        for (int tile = 0; tile < nfull; ++tile) {
-            at_wait_barrier<(S - 2) * 2 * NQ>();             // the tile has landed, and the last one is read
-            const int nt = tile + S - 1;
-            issue(nt < nfull ? nt : nfull - 1, nt % S);
-            lookup(nt + 1 < nfull ? nt + 1 : nfull - 1);
-            if (active) math(sm + (tile % S) * 2 * TB, std::integral_constant<bool, true>{}, [](int) { return true; });
-        }
-        at_wait_barrier<0>();                                // the ring is free
+        if (tile + 1 < nfull) lookup(tile + 1);
+    };
+    lookup(0);
+#pragma unroll 1
+    for (int e = 0; e < S - 1; ++e) request(e, e);
+    int tile = 0;
+    for (; tile < nfull; ++tile) {
+        at_wait_barrier<(S - 2) * 2 * NQ>();                 // the tile has landed, and the last one is read
+        request(tile + S - 1, (tile + S - 1) % S);
+        if (active) math(sm + (tile % S) * 2 * TB, std::integral_constant<bool, true>{}, 0ull);
     }
-    // The rest, one tile at a time in the first stage.
-    for (int jt = j0 + nfull * T; jt < j1; jt += T) {
+    for (; tile < ntile; ++tile) {                           // the tiles with a mask
+        const int jt = j0 + tile * T, je = jt + T < j1 ? jt + T : j1;
+        uint8_t* const sk = sm + (tile % S) * 2 * TB;
+        uint64_t bits = 0;
+        if (active) {                                        // uniform
+            // the cached keys, and with no mask the drafted ones up to n
+            auto below = [&](int j) {                        // the tile's keys below j
+                const int c = j - jt;
+                return c <= 0 ? 0ull : c >= 64 ? ~0ull : (1ull << c) - 1;
+            };
+            bits = below(P.mask ? (len < je ? len : je) : (len + n + 1 < je ? len + n + 1 : je));
+            if (P.mask)                                      // uniform
+                for (int j = jt > len ? jt : len; j < je; j += 8) {
+                    bool v[8];
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int j = jt + (wave + NW * i) * KQ + kq;    // past the chunk's end: its last key
-            issue_key(i, j < j1 ? j : j1 - 1, sm);
+                    for (int e = 0; e < 8; ++e) v[e] = seen((j + e < je ? j + e : je - 1) - len);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) bits |= j + e < je && v[e] ? 1ull << (j + e - jt) : 0ull;
+                }
         }
-        at_wait_barrier<0>();
+        at_wait_barrier<(S - 2) * 2 * NQ>();
+        request(tile + S - 1, (tile + S - 1) % S);
         // Values that not every row sees: rows past the end become 0, and so do
         // infinities and NaN of drafted tokens (0 times them would be NaN for the
         // rows that do not see them; at the end they are added to the rows that do).
         for (int p = t; p < T * U; p += 64 * NW) {
             const int j = jt + p / U;
-            llima_u32x4* const at = (llima_u32x4*)(sm + TB + p * 16);
+            llima_u32x4* const at = (llima_u32x4*)(sk + TB + p * 16);
             llima_u32x4 x = *at;
             bool put = j >= j1;
             if (put) x = (llima_u32x4){0u, 0u, 0u, 0u};
@@ -410,13 +479,8 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
             }
             if (put) *at = x;
         }
-        __syncthreads();
-        if (active)
-            math(sm, std::integral_constant<bool, false>{}, [&](int k) {
-                const int j = jt + k;
-                return j < len || (j < j1 && seen(j - len));
-            });
-        __syncthreads();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (active) math(sk, std::integral_constant<bool, false>{}, bits);
     }
     if (miss) flag[0] = 1u;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no request outlives this
@@ -434,8 +498,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
                 for (int i = 0; i < 16; ++i) red[(2 + d * 16 + i) * 64 + lane] = o[d][i];
         }
         __syncthreads();
-        if (kw == 1) return;
-        if (active) {
+        if (active && kw == 0) {
             const float m2 = red[lane], mn = __builtin_fmaxf(m, m2), mu = mn > -__builtin_inff() ? mn : 0.0f;
             const float a = __builtin_amdgcn_exp2f(m - mu), a2 = __builtin_amdgcn_exp2f(m2 - mu);
             m = mn;
@@ -446,22 +509,23 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
                 for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * a + red[(2 + d * 16 + i) * 64 + lane] * a2;
         }
     }
-    if (!active || row >= P.R) return;
-    if (flag[1]) {                                           // infinities and NaN of drafted tokens in this chunk
+    if (!active || row >= P.R || kw != 0) continue;
+    if (flag[1]) {                                           // infinities and NaN of drafted tokens in this part
         for (int mm = (j0 > len ? j0 : len) - len; mm < j1 - len; ++mm) {
-            if (!seen(mm)) continue;
+            if (!seen(mm)) continue;                         // (of the loop over mm)
             const uint16_t* vp = (const uint16_t*)P.v + b * P.vs[0] + mm * P.vs[1] + h * P.vs[2];
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint16_t x = vp[d * 32 + (i & 3) + 8 * (i >> 2) + 4 * g];
-                    if (at_special<DT>(x)) o[d][i] += at_f32<DT>(x);
+                for (int i = 0; i < 16; i += 4) {
+                    const uint2 w = *(const uint2*)(vp + d * 32 + 2 * i + 4 * g);
+                    auto add = [&](int e, uint32_t x) { o[d][e] += at_special<DT>((uint16_t)x) ? at_f32<DT>((uint16_t)x) : 0.0f; };
+                    add(i, w.x); add(i + 1, w.x >> 16); add(i + 2, w.y); add(i + 3, w.y >> 16);
                 }
         }
     }
     if (flag[0]) l = __builtin_nanf("");
-    if (nchunk == 1) {
+    if (whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing seen: 0
         uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + 4 * g;
 #pragma unroll
@@ -471,7 +535,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
                 *(uint2*)(op + d * 32 + 2 * i) = make_uint2(at_pack<DT>(o[d][i] * inv, o[d][i + 1] * inv),
                                                             at_pack<DT>(o[d][i + 2] * inv, o[d][i + 3] * inv));
     } else {
-        const size_t at = ((size_t)slot * P.Hkv + h) * P.R + row;
+        const size_t at = ((size_t)(part + b) * P.Hkv + h) * P.R + row;
         if (g == 0) P.part_ml[at] = make_float2(m, l);
         float* op = P.part_o + at * D + 4 * g;
 #pragma unroll
@@ -480,39 +544,40 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
             for (int i = 0; i < 16; i += 4)
                 *(float4*)(op + d * 32 + 2 * i) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
     }
+    }
+#endif
 }
 
-// Joins the chunks of each row: a wave per (sequence, node, query head).
+// Joins the parts of each row: a wave per (sequence, node, query head).
 template <int DT, int D, int T>
 __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
     constexpr int E = D / 64;                                // values per lane
     const int lane = (int)lane_id();
-    bool bad;
-    const int chunk = at_chunk<T>(P, lane < P.B ? at_len(P, lane, bad) : 0);
     const int64_t w = (int64_t)blockIdx.x * LLIMA_WAVES + wave_id();
     if (w >= (int64_t)P.B * P.N * P.Hq) return;
     const int b = (int)(w / (P.N * P.Hq)), n = (int)(w / P.Hq % P.N), hq = (int)(w % P.Hq);
-    // the sequence's first chunk
-    int first = 0;
-    for (int i = lane; i < b; i += 64) {
-        first += (at_len(P, i, bad) + P.N + chunk - 1) / chunk;
-    }
+    bool bad;
+    const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
+    const int64_t share = at_share<T>(P, len0);
+    int64_t first = lane < b ? at_tiles<T>(P, len0) : 0;     // the sequence's first tile
+    for (int i = 64 + lane; i < b; i += 64) first += at_tiles<T>(P, at_len(P, i, bad));
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
-    const int nchunk = (at_len(P, b, bad) + P.N + chunk - 1) / chunk;
-    if (nchunk <= 1) return;
+    const int64_t last = first + at_tiles<T>(P, b < 64 ? (int)readlane((uint32_t)len0, (uint32_t)b) : at_len(P, b, bad)) - 1 - AT_EXTRA;
+    const int x0 = (int)(first / share), np = (int)(last / share) - x0 + 1;
+    if (np <= 1) return;
     const int h = hq / P.G, row = n * P.G + hq % P.G;
-    const size_t step = (size_t)P.Hkv * P.R, at0 = ((size_t)first * P.Hkv + h) * P.R + row;
+    const size_t step = (size_t)P.Hkv * P.R, at0 = ((size_t)(x0 + b) * P.Hkv + h) * P.R + row;
     float m = -__builtin_inff(), l = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    // the greatest maximum first (a lane per chunk), then one pass of weighted sums
-    for (int c = lane; c < nchunk; c += 64) m = __builtin_fmaxf(m, P.part_ml[at0 + c * step].x);
+    // the greatest maximum first (a lane per part), then one pass of weighted sums
+    for (int c = lane; c < np; c += 64) m = __builtin_fmaxf(m, P.part_ml[at0 + c * step].x);
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, x, 64));
     const float mu = m > -__builtin_inff() ? m : 0.0f;
-#pragma unroll 4
-    for (int c = 0; c < nchunk; ++c) {
+#pragma unroll 8
+    for (int c = 0; c < np; ++c) {
         const float2 ml = P.part_ml[at0 + c * step];
         const float a = __builtin_amdgcn_exp2f(ml.x - mu);
         l += ml.y * a;
@@ -579,9 +644,10 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_commit(CommitParams P) {
     }
 }
 
-// Key chunks wished for: enough workgroups to fill the device twice.
-static int at_ntarget(int Hkv, int RG) {
-    const int n = 512 / (Hkv * RG);
+// Shares of the keys: as many workgroups as the device holds at a time, two per
+// CU, or one of those that take more than half of its LDS.
+static int at_parts(int Hkv, int RG, int RT, int D) {
+    const int n = (RT > 4 || (D == 256 && RT > 2) ? 256 : 512) / (Hkv * RG);
     return n < 1 ? 1 : n;
 }
 
@@ -591,20 +657,20 @@ static int at_row_tiles(int R, int& RG) {                    // row tiles of a g
     return (rt + RG - 1) / RG;
 }
 
-template <int DT, int D, bool GEN>
+template <int DT, int D>
 static void at_launch(const AttnParams& P, hipStream_t st) {
-    const dim3 g((uint32_t)P.slots * P.RG * P.Hkv);
+    const dim3 g((uint32_t)P.parts * P.RG * P.Hkv);
     constexpr int T = D == 256 ? 32 : 64, K2 = D == 256 ? 1 : 2;
     constexpr int S2 = D == 64 ? 4 : 2, S4 = D == 256 ? 4 : S2, S8 = 4;
     if (P.RT <= (K2 == 2 ? 1 : 2)) {
-        hipLaunchKernelGGL((tree_attn<DT, D, 2, K2, T, S2, GEN>), g, dim3(128), 0, st, P);
+        hipLaunchKernelGGL((tree_attn<DT, D, 2, K2, T, S2>), g, dim3(128), 0, st, P);
     } else if (P.RT <= 4) {
         if constexpr (K2 == 2) {
-            if (P.RT <= 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 2, T, S4, GEN>), g, dim3(256), 0, st, P);
+            if (P.RT <= 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 2, T, S4>), g, dim3(256), 0, st, P);
         }
-        if (K2 == 1 || P.RT > 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 1, T, S4, GEN>), g, dim3(256), 0, st, P);
+        if (K2 == 1 || P.RT > 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 1, T, S4>), g, dim3(256), 0, st, P);
     } else {
-        hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8, GEN>), g, dim3(512), 0, st, P);
+        hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8>), g, dim3(512), 0, st, P);
     }
     const int64_t rows = (int64_t)P.B * P.N * P.Hq;
     hipLaunchKernelGGL((tree_attn_join<DT, D, T>), dim3((uint32_t)((rows + LLIMA_WAVES - 1) / LLIMA_WAVES)),
@@ -613,11 +679,9 @@ static void at_launch(const AttnParams& P, hipStream_t st) {
 
 template <int DT>
 static int at_dispatch(const AttnParams& P, int D, hipStream_t st) {
-    // a request's keys (8 at most) lie in one page and within 2^31 bytes
-    const bool gen = (P.table && P.page % 8 != 0) || P.kcs[1] > (1 << 26) || P.vcs[1] > (1 << 26);
-    if (D == 64) gen ? at_launch<DT, 64, true>(P, st) : at_launch<DT, 64, false>(P, st);
-    else if (D == 128) gen ? at_launch<DT, 128, true>(P, st) : at_launch<DT, 128, false>(P, st);
-    else gen ? at_launch<DT, 256, true>(P, st) : at_launch<DT, 256, false>(P, st);
+    if (D == 64) at_launch<DT, 64>(P, st);
+    else if (D == 128) at_launch<DT, 128>(P, st);
+    else at_launch<DT, 256>(P, st);
     return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
 }
 
@@ -631,11 +695,11 @@ static bool at_sizes_ok(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D
     return (int64_t)B * N * Hq <= (1 << 28);
 }
 
-static void at_plan(AttnParams& P) {
+static void at_plan(AttnParams& P, int D) {
     P.R = P.N * P.G;
     P.RT = at_row_tiles(P.R, P.RG);
-    P.ntarget = at_ntarget(P.Hkv, P.RG);
-    P.slots = P.ntarget + P.B;
+    P.parts = at_parts(P.Hkv, P.RG, P.RT, D);
+    P.slots = P.parts + P.B;
 }
 
 extern "C" size_t llima_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq,
@@ -643,7 +707,7 @@ extern "C" size_t llima_tree_attention_workspace_bytes(int32_t B, int32_t N, int
     if (B <= 0 || !at_sizes_ok(B, N, Hq, Hkv, D)) return 0;
     AttnParams P = {};
     P.B = B; P.N = N; P.Hkv = Hkv; P.G = Hq / Hkv;
-    at_plan(P);
+    at_plan(P, D);
     const size_t rows = (size_t)P.slots * Hkv * P.R;
     return (rows * D * sizeof(float) + 255) / 256 * 256 + rows * sizeof(float2);
 }
@@ -700,8 +764,13 @@ extern "C" int llima_tree_attention(const llima_tree_attention_args* a, void* wo
     while ((1ll << l) < P.page) ++l;
     P.page_mul = (uint32_t)(((1ull << (30 + l)) + P.page - 1) / (uint64_t)P.page);
     P.page_shift = 30 + l;
-    P.scale2 = a->scale * 1.44269504088896340736f;
-    at_plan(P);
+    P.scale2 = __builtin_fabsf(a->scale) * 1.44269504088896340736f;
+    P.flip = a->scale < 0.0f;
+    // offsets within a tile (64 keys) or a request have 31 bits
+    const int64_t ts = P.kcs[1] > P.vcs[1] ? P.kcs[1] : P.vcs[1];
+    P.mode = ts <= (1 << 23) && (!P.table || P.page % 64 == 0) ? AT_TILE
+           : ts <= (1 << 26) && (!P.table || P.page % 8 == 0) ? AT_REQUEST : AT_LANE;
+    at_plan(P, a->D);
     const size_t rows = (size_t)P.slots * P.Hkv * P.R;
     P.part_o = (float*)workspace;
     P.part_ml = (float2*)((uint8_t*)workspace + (rows * a->D * sizeof(float) + 255) / 256 * 256);
