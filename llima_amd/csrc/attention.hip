@@ -56,8 +56,17 @@ struct AttnParams {
 #define AT_REQUEST 1
 #define AT_LANE 2
 
-__device__ __forceinline__ uint32_t at_page(const AttnParams& P, int j) {
-    return (uint32_t)(((uint64_t)(uint32_t)j * P.page_mul) >> P.page_shift);
+__device__ __forceinline__ uint32_t at_page(uint32_t mul, uint32_t shift, int j) {
+    return (uint32_t)(((uint64_t)(uint32_t)j * mul) >> shift);
+}
+
+// The kernel's arguments, loaded anew where they are used: held in registers
+// from the start, those of the parts that run seldom push out the others.
+typedef const __attribute__((address_space(4))) AttnParams* AttnArgs;
+__device__ __forceinline__ AttnArgs at_args() {
+    AttnArgs a = (AttnArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return a;
 }
 
 __device__ __forceinline__ uint64_t readfirstlane64(uint64_t v) {
@@ -125,6 +134,8 @@ __device__ __forceinline__ int at_tiles(const AttnParams& P, int len) { return (
 template <int T>
 __device__ __forceinline__ int64_t at_share(const AttnParams& P, int len0) {
     const int lane = (int)lane_id();
+    if (P.B == 1)                                            // uniform; a step of one stream waits for this
+        return ((uint32_t)__builtin_amdgcn_readfirstlane(at_tiles<T>(P, len0)) + (uint32_t)P.parts - 1u) / (uint32_t)P.parts;
     int64_t total = lane < P.B ? at_tiles<T>(P, len0) : 0;
     for (int b = 64 + lane; b < P.B; b += 64) {
         bool bad;
@@ -141,6 +152,12 @@ template <int T>
 __device__ __forceinline__ bool at_find(const AttnParams& P, int64_t at, int len0, int& b, int& len,
                                         int64_t& first) {
     const int lane = (int)lane_id();
+    if (P.B == 1) {                                          // uniform
+        b = 0;
+        len = __builtin_amdgcn_readfirstlane(len0);
+        first = 0;
+        return at < at_tiles<T>(P, len);
+    }
     int64_t before = 0;
     for (int b0 = 0; b0 < P.B; b0 += 64) {
         bool bad;
@@ -184,8 +201,8 @@ __device__ __forceinline__ void at_wait_barrier() {
 // (contiguous caches and pages of a multiple of 64), its address is the wave's
 // and comes from the scalar unit; or each request does (its 8 keys at most: pages of
 // a multiple of 8); or every lane computes its own.  The tiles after them, which hold drafted keys
-// or end a part, come one at a time with the mask.
-template <int DT, int D, int NW, int KW, int T, int S>
+// or end a part, are requested by key and have the mask.  GEN: the last two modes.
+template <int DT, int D, int NW, int KW, int T, int S, bool GEN>
 __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_attn(AttnParams P) {
 #ifdef __HIP_DEVICE_COMPILE__                               // (the host pass drops the launch stub over the descriptors)
     constexpr int U = D / 8;                                 // 16-byte units of a key row
@@ -245,7 +262,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         if (j < len) {
             int64_t p = b, o = j;
             if (P.table) {                                   // uniform
-                const uint32_t e = at_page(P, j);
+                const uint32_t e = at_page(P.page_mul, P.page_shift, j);
                 o = j - (int)e * P.page;
                 int pi = P.table[b * P.ts + e];
                 if (pi < 0 || pi >= P.pages) { pi = 0; miss = true; }
@@ -263,7 +280,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
     // the page of key j (uniform), by the scalar unit
     auto page_of = [&](int j) {
         const __attribute__((address_space(4))) int32_t* tab = (const __attribute__((address_space(4))) int32_t*)(P.table + b * P.ts);
-        return tab[at_page(P, j)];
+        return tab[at_page(P.page_mul, P.page_shift, j)];
     };
     auto base_of = [&](const void* c, const int64_t (&cs)[3], int p, int o) {
         return (void*)((const uint16_t*)c + p * cs[0] + o * cs[1] + h * cs[2]);
@@ -279,7 +296,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         p = b;
         o = j;
         if (P.table) {                                       // uniform
-            o = j - (int)at_page(P, j) * P.page;
+            o = j - (int)at_page(P.page_mul, P.page_shift, j) * P.page;
             const bool out = pi < 0 || pi >= P.pages;
             miss |= out;
             p = out ? 0 : pi;
@@ -287,12 +304,12 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
     };
     int pg = 0;                                              // the page of the next tile to request
     auto lookup = [&](int tile) {
-        if (P.mode == AT_TILE && P.table && tile < nfull) pg = page_of(j0 + tile * T);   // uniform
+        if (!GEN && P.table && tile < nfull) pg = page_of(j0 + tile * T);   // uniform
     };
     auto issue = [&](int tile, int st) {                     // a tile of cached keys
         uint8_t* const sk = sm + st * 2 * TB;
         const int jt = j0 + tile * T;
-        if (P.mode == AT_TILE) {                             // uniform
+        if constexpr (!GEN) {
             int p, o;
             place(jt, pg, p, o);
             const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(base_of(P.kc, P.kcs, p, o), 0, 0x7FFFFFFF, 0x00027000);
@@ -462,7 +479,8 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         // Values that not every row sees: rows past the end become 0, and so do
         // infinities and NaN of drafted tokens (0 times them would be NaN for the
         // rows that do not see them; at the end they are added to the rows that do).
-        for (int p = t; p < T * U; p += 64 * NW) {
+        const int clean = jc - jt > 0 ? jc - jt : 0;         // the tile's cached keys
+        for (int p = clean * U + t; p < T * U; p += 64 * NW) {
             const int j = jt + p / U;
             llima_u32x4* const at = (llima_u32x4*)(sk + TB + p * 16);
             llima_u32x4 x = *at;
@@ -510,10 +528,11 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         }
     }
     if (!active || row >= P.R || kw != 0) continue;
+    const AttnArgs A = at_args();
     if (flag[1]) {                                           // infinities and NaN of drafted tokens in this part
         for (int mm = (j0 > len ? j0 : len) - len; mm < j1 - len; ++mm) {
             if (!seen(mm)) continue;                         // (of the loop over mm)
-            const uint16_t* vp = (const uint16_t*)P.v + b * P.vs[0] + mm * P.vs[1] + h * P.vs[2];
+            const uint16_t* vp = (const uint16_t*)A->v + b * A->vs[0] + mm * A->vs[1] + h * A->vs[2];
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -527,7 +546,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
     if (flag[0]) l = __builtin_nanf("");
     if (whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing seen: 0
-        uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + 4 * g;
+        uint16_t* op = (uint16_t*)A->out + b * A->os[0] + n * A->os[1] + hq * A->os[2] + 4 * g;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -535,9 +554,9 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
                 *(uint2*)(op + d * 32 + 2 * i) = make_uint2(at_pack<DT>(o[d][i] * inv, o[d][i + 1] * inv),
                                                             at_pack<DT>(o[d][i + 2] * inv, o[d][i + 3] * inv));
     } else {
-        const size_t at = ((size_t)(part + b) * P.Hkv + h) * P.R + row;
-        if (g == 0) P.part_ml[at] = make_float2(m, l);
-        float* op = P.part_o + at * D + 4 * g;
+        const size_t at = ((size_t)(part + b) * A->Hkv + h) * A->R + row;
+        if (g == 0) A->part_ml[at] = make_float2(m, l);
+        float* op = A->part_o + at * D + 4 * g;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -548,24 +567,32 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
 #endif
 }
 
-// Joins the parts of each row: a wave per (sequence, node, query head).
-template <int DT, int D, int T>
+// Joins the parts of each row (a sequence's node and query head), WPR waves a
+// row, which take every WPR-th part each in rounds of 8 loads.  Four waves where rows
+// are few (512 rows of 44 parts 7.4 -> 6.0 us), one where they fill the device
+// (12288 rows: 33 us with four, 11 with one).
+template <int DT, int D, int T, int WPR>
 __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
     constexpr int E = D / 64;                                // values per lane
-    const int lane = (int)lane_id();
-    const int64_t w = (int64_t)blockIdx.x * LLIMA_WAVES + wave_id();
-    if (w >= (int64_t)P.B * P.N * P.Hq) return;
-    const int b = (int)(w / (P.N * P.Hq)), n = (int)(w / P.Hq % P.N), hq = (int)(w % P.Hq);
+    static_assert(WPR == 1 || WPR == LLIMA_WAVES, "one row or four to a workgroup");
+    __shared__ float so[WPR][D], sl[WPR];
+    const int lane = (int)lane_id(), sub = (int)wave_id() % WPR;
+    const int w = (int)(blockIdx.x * (LLIMA_WAVES / WPR) + wave_id() / WPR);
+    if (w >= P.B * P.N * P.Hq) return;                       // (WPR = 1)
+    const int b = w / (P.N * P.Hq), n = w / P.Hq % P.N, hq = w % P.Hq;
     bool bad;
     const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
     const int64_t share = at_share<T>(P, len0);
-    int64_t first = lane < b ? at_tiles<T>(P, len0) : 0;     // the sequence's first tile
-    for (int i = 64 + lane; i < b; i += 64) first += at_tiles<T>(P, at_len(P, i, bad));
+    int64_t first = 0;                                       // the sequence's first tile
+    if (b > 0) {                                             // uniform
+        first = lane < b ? at_tiles<T>(P, len0) : 0;
+        for (int i = 64 + lane; i < b; i += 64) first += at_tiles<T>(P, at_len(P, i, bad));
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
+        for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
+    }
     const int64_t last = first + at_tiles<T>(P, b < 64 ? (int)readlane((uint32_t)len0, (uint32_t)b) : at_len(P, b, bad)) - 1 - AT_EXTRA;
     const int x0 = (int)(first / share), np = (int)(last / share) - x0 + 1;
-    if (np <= 1) return;
+    if (np <= 1) return;                                     // the same for a row's waves
     const int h = hq / P.G, row = n * P.G + hq % P.G;
     const size_t step = (size_t)P.Hkv * P.R, at0 = ((size_t)(x0 + b) * P.Hkv + h) * P.R + row;
     float m = -__builtin_inff(), l = 0.0f, o[E];
@@ -576,20 +603,47 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, x, 64));
     const float mu = m > -__builtin_inff() ? m : 0.0f;
-#pragma unroll 8
-    for (int c = 0; c < np; ++c) {
-        const float2 ml = P.part_ml[at0 + c * step];
-        const float a = __builtin_amdgcn_exp2f(ml.x - mu);
-        l += ml.y * a;
-        const float* po = P.part_o + (at0 + c * step) * D + lane * E;
+    for (int c0 = sub; c0 < np; c0 += 8 * WPR) {
+        float2 ml[8];
+        float po[8][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += po[e] * a;
+        for (int i = 0; i < 8; ++i) {
+            const int c = c0 + i * WPR;
+            const size_t at = at0 + (c < np ? c : c0) * step;
+            ml[i] = P.part_ml[at];
+#pragma unroll
+            for (int e = 0; e < E; ++e) po[i][e] = P.part_o[at * D + lane * E + e];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (c0 + i * WPR < np) {                         // uniform
+                const float a = __builtin_amdgcn_exp2f(ml[i].x - mu);
+                l += ml[i].y * a;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += po[i][e] * a;
+            }
+        }
+    }
+    if constexpr (WPR > 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) so[sub][lane * E + e] = o[e];
+        if (lane == 0) sl[sub] = l;
+        __syncthreads();
+        if (sub != 0) return;
+        l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int d = lane * E + e;
+            o[e] = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + lane * E;
-    if constexpr (E == 1) op[0] = (uint16_t)at_pack<DT>(o[0] * inv, 0.0f);
 #pragma unroll
-    for (int e = 0; e + 1 < E; e += 2) *(uint32_t*)(op + e) = at_pack<DT>(o[e] * inv, o[e + 1] * inv);
+    for (int e = 0; e < E; ++e) o[e] *= inv;
+    uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + lane * E;
+    if constexpr (E == 1) op[0] = (uint16_t)at_pack<DT>(o[0], 0.0f);
+#pragma unroll
+    for (int e = 0; e + 1 < E; e += 2) *(uint32_t*)(op + e) = at_pack<DT>(o[e], o[e + 1]);
 }
 
 struct CommitParams {
@@ -657,31 +711,32 @@ static int at_row_tiles(int R, int& RG) {                    // row tiles of a g
     return (rt + RG - 1) / RG;
 }
 
-template <int DT, int D>
+template <int DT, int D, bool GEN>
 static void at_launch(const AttnParams& P, hipStream_t st) {
     const dim3 g((uint32_t)P.parts * P.RG * P.Hkv);
     constexpr int T = D == 256 ? 32 : 64, K2 = D == 256 ? 1 : 2;
     constexpr int S2 = D == 64 ? 4 : 2, S4 = D == 256 ? 4 : S2, S8 = 4;
     if (P.RT <= (K2 == 2 ? 1 : 2)) {
-        hipLaunchKernelGGL((tree_attn<DT, D, 2, K2, T, S2>), g, dim3(128), 0, st, P);
+        hipLaunchKernelGGL((tree_attn<DT, D, 2, K2, T, S2, GEN>), g, dim3(128), 0, st, P);
     } else if (P.RT <= 4) {
         if constexpr (K2 == 2) {
-            if (P.RT <= 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 2, T, S4>), g, dim3(256), 0, st, P);
+            if (P.RT <= 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 2, T, S4, GEN>), g, dim3(256), 0, st, P);
         }
-        if (K2 == 1 || P.RT > 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 1, T, S4>), g, dim3(256), 0, st, P);
+        if (K2 == 1 || P.RT > 2) hipLaunchKernelGGL((tree_attn<DT, D, 4, 1, T, S4, GEN>), g, dim3(256), 0, st, P);
     } else {
-        hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8>), g, dim3(512), 0, st, P);
+        hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8, GEN>), g, dim3(512), 0, st, P);
     }
     const int64_t rows = (int64_t)P.B * P.N * P.Hq;
-    hipLaunchKernelGGL((tree_attn_join<DT, D, T>), dim3((uint32_t)((rows + LLIMA_WAVES - 1) / LLIMA_WAVES)),
-                       dim3(LLIMA_WG), 0, st, P);
+    if (rows <= 2048) hipLaunchKernelGGL((tree_attn_join<DT, D, T, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, P);
+    else hipLaunchKernelGGL((tree_attn_join<DT, D, T, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, P);
 }
 
 template <int DT>
 static int at_dispatch(const AttnParams& P, int D, hipStream_t st) {
-    if (D == 64) at_launch<DT, 64>(P, st);
-    else if (D == 128) at_launch<DT, 128>(P, st);
-    else at_launch<DT, 256>(P, st);
+    const bool gen = P.mode != AT_TILE;
+    if (D == 64) gen ? at_launch<DT, 64, true>(P, st) : at_launch<DT, 64, false>(P, st);
+    else if (D == 128) gen ? at_launch<DT, 128, true>(P, st) : at_launch<DT, 128, false>(P, st);
+    else gen ? at_launch<DT, 256, true>(P, st) : at_launch<DT, 256, false>(P, st);
     return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
 }
 
