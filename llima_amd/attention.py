@@ -10,14 +10,13 @@ caches are on the NPU.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional
 
 import torch
 
 from . import _lib
 from ._lib import check, lib
-from .sampler import FLOAT_CODES, _on, _on_gpu, _ptr, _scratch, _stream
+from .sampler import FLOAT_CODES, _on, _on_gpu, _scratch, _stream
 
 __all__ = ["tree_attention", "tree_commit"]
 
@@ -25,6 +24,8 @@ __all__ = ["tree_attention", "tree_commit"]
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """[..., D] that 16-byte accesses can read: D adjacent, the other strides multiples
     of 8 and not negative, 16-byte aligned (copied when it is not)."""
+    if t.is_contiguous() and t.shape[-1] % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
     st = t.stride()
     if st[-1] == 1 and t.data_ptr() % 16 == 0:
         if not any([s % 8 for s in st[:-1]]):
@@ -37,7 +38,7 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
 def _in_place(t: torch.Tensor, name: str) -> torch.Tensor:
     """A cache as the kernels can use it where it is (it is never copied)."""
     h = _heads(t)
-    if h.data_ptr() != t.data_ptr():
+    if h is not t and h.data_ptr() != t.data_ptr():
         raise ValueError(f"{name}: head values must be adjacent, other strides multiples of 8, "
                          "and the first 16-byte aligned")
     return h
@@ -108,8 +109,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
         raise ValueError("tree_attention: tensors must be on one device")
     page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, q.dtype, block_table, B, dev)
     lens = _ints(cache_lens, B, "cache_lens", dev)
-    a = _lib.TreeAttentionArgsC()
-    mask = tree_mask
+    mask, mask_dtype, ms = tree_mask, _lib.LLIMA_MASK_U8, (0, 0)
     if mask is not None:
         if tuple(mask.shape) not in ((N, N), (B, N, N)) or mask.device != dev:
             raise ValueError("tree_mask must be [N, N] or [B, N, N] on q's device")
@@ -117,27 +117,25 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
             raise ValueError("tree_mask must be bool, uint8 or float32")
         if mask.stride(-1) != 1:
             mask = mask.contiguous()
-        a.mask_dtype = _lib.LLIMA_MASK_F32 if mask.dtype == torch.float32 else _lib.LLIMA_MASK_U8
-        a.mask_strides[:] = (mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
+        if mask.dtype == torch.float32:
+            mask_dtype = _lib.LLIMA_MASK_F32
+        ms = (mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
     q, k, v = _heads(q), _heads(k), _heads(v)
     kc, vc = _in_place(k_cache, "k_cache"), _in_place(v_cache, "v_cache")
     out = torch.empty((B, N, Hq, D), dtype=q.dtype, device=dev)
     if B == 0:
         return out
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("k_cache", kc), ("v_cache", vc)):
-        setattr(a, name, t.data_ptr())
-        getattr(a, name + "_strides")[:] = t.stride()[:3]
-    a.cache_lens, a.mask = lens.data_ptr(), _ptr(mask)
-    a.block_table = None if table is None else table.data_ptr() or lens.data_ptr()   # (no blocks: not read)
-    a.table_stride = 0 if table is None else table.stride(0)
-    a.dtype = FLOAT_CODES[q.dtype]
-    a.B, a.N, a.Hq, a.Hkv, a.D = B, N, Hq, Hkv, D
-    a.page_size, a.pages, a.max_blocks = page, pages, blocks
-    a.scale = D ** -0.5 if scale is None else float(scale)
-    ws = _scratch(dev, "tree_attention", lib().llima_tree_attention_workspace_bytes(B, N, Hq, Hkv, D))
+    L = lib()
+    ws = _scratch(dev, "tree_attention", L.llima_tree_attention_workspace_bytes(B, N, Hq, Hkv, D))
+    # a table of no blocks is not read
+    tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
+    a = _lib.TREE_ATTENTION_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), lens.data_ptr(),
+        0 if mask is None else mask.data_ptr(), tp, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+        *out.stride()[:3], *kc.stride()[:3], *vc.stride()[:3], *ms, ts, FLOAT_CODES[q.dtype], mask_dtype, B, N, Hq,
+        Hkv, D, page, pages, blocks, D ** -0.5 if scale is None else float(scale))
     with _on(dev):
-        check(lib().llima_tree_attention(ctypes.byref(a), ws.data_ptr(), ws.numel(), _stream(dev)),
-              "llima_tree_attention")
+        check(L.llima_tree_attention(a, ws.data_ptr(), ws.numel(), _stream(dev)), "llima_tree_attention")
     return out
 
 
@@ -182,16 +180,11 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     new = torch.empty(B, dtype=torch.int32, device=dev)
     if B == 0:
         return new
-    a = _lib.TreeCommitArgsC()
-    for name, t in (("k", k), ("v", v), ("k_cache", kc), ("v_cache", vc)):
-        setattr(a, name, t.data_ptr())
-        getattr(a, name + "_strides")[:] = t.stride()[:4]
-    a.nodes, a.counts, a.cache_lens = nodes.data_ptr(), counts.data_ptr(), lens.data_ptr()
-    a.new_lens = new.data_ptr()
-    a.block_table = None if table is None else table.data_ptr() or lens.data_ptr()   # (no blocks: not read)
-    a.nodes_stride, a.table_stride = nodes.stride(0), 0 if table is None else table.stride(0)
-    a.layers, a.B, a.N, a.L, a.Hkv, a.D = layers, B, N, nodes.shape[1], Hkv, D
-    a.page_size, a.pages, a.max_blocks = page, pages, blocks
+    tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
+    a = _lib.TREE_COMMIT_ARGS.pack(
+        k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), nodes.data_ptr(), counts.data_ptr(), lens.data_ptr(),
+        tp, new.data_ptr(), *k.stride()[:4], *v.stride()[:4], *kc.stride()[:4], *vc.stride()[:4], nodes.stride(0), ts,
+        layers, B, N, nodes.shape[1], Hkv, D, page, pages, blocks)
     with _on(dev):
-        check(lib().llima_tree_commit(ctypes.byref(a), _stream(dev)), "llima_tree_commit")
+        check(lib().llima_tree_commit(a, _stream(dev)), "llima_tree_commit")
     return new

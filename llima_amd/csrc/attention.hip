@@ -658,12 +658,12 @@ struct CommitParams {
     int32_t page, pages;
 };
 
-// One workgroup per (path place, sequence, layer): checks the sequence's path
-// and room (every workgroup of a sequence comes to the same answer), then
-// copies one token's K and V rows.
-__global__ __launch_bounds__(LLIMA_WG) void tree_commit(CommitParams P) {
+// One workgroup per path place, sequence and `per` layers (8 at most): checks
+// the sequence's path and room (every workgroup of a sequence comes to the same
+// answer), then copies one token's K and V rows, all layers' loads in flight together.
+__global__ __launch_bounds__(LLIMA_WG) void tree_commit(CommitParams P, int layers, int per) {
     const int j = (int)(blockIdx.x % (uint32_t)P.L), b = (int)(blockIdx.x / (uint32_t)P.L), t = (int)threadIdx.x;
-    const int64_t layer = blockIdx.y;
+    const int l0 = (int)blockIdx.y * per, nl = layers - l0 < per ? layers - l0 : per;
     const int len = P.lens[b], cnt = P.counts[b];
     bool ok = len >= 0 && cnt >= 0 && cnt <= P.L && len <= P.cap && (int64_t)len + cnt <= P.cap;
     if (ok) {
@@ -678,7 +678,7 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_commit(CommitParams P) {
         }
         ok = __all(all);
     }
-    if (j == 0 && layer == 0 && t == 0) P.new_lens[b] = ok ? len + cnt : LLIMA_E_RANGE;
+    if (j == 0 && l0 == 0 && t == 0) P.new_lens[b] = ok ? len + cnt : LLIMA_E_RANGE;
     if (!ok || j >= cnt) return;                             // uniform
     const int64_t node = P.nodes[b * P.ns + j];
     int64_t p = b, o = len + j;
@@ -692,9 +692,15 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_commit(CommitParams P) {
         const int e = isv ? i - n : i, h = e / P.U, u = e % P.U;
         const int64_t* fs = isv ? P.vs : P.ks;
         const int64_t* ts = isv ? P.vcs : P.kcs;
-        const uint8_t* src = (isv ? P.v : P.k) + layer * fs[0] + b * fs[1] + node * fs[2] + h * fs[3] + u * 16;
-        uint8_t* dst = (isv ? P.vc : P.kc) + layer * ts[0] + p * ts[1] + o * ts[2] + h * ts[3] + u * 16;
-        *(llima_u32x4*)dst = *(const llima_u32x4*)src;
+        const uint8_t* src = (isv ? P.v : P.k) + l0 * fs[0] + b * fs[1] + node * fs[2] + h * fs[3] + u * 16;
+        uint8_t* dst = (isv ? P.vc : P.kc) + l0 * ts[0] + p * ts[1] + o * ts[2] + h * ts[3] + u * 16;
+        llima_u32x4 x[8];
+#pragma unroll
+        for (int l = 0; l < 8; ++l)
+            if (l < nl) x[l] = *(const llima_u32x4*)(src + l * fs[0]);   // uniform
+#pragma unroll
+        for (int l = 0; l < 8; ++l)
+            if (l < nl) *(llima_u32x4*)(dst + l * ts[0]) = x[l];
     }
 }
 
@@ -864,7 +870,10 @@ extern "C" int llima_tree_commit(const llima_tree_commit_args* a, void* stream) 
     P.cap = a->pages > 0 ? (int64_t)a->page_size * a->max_blocks : 0;
     P.B = a->B; P.N = a->N; P.L = a->L; P.Hkv = a->Hkv; P.U = a->D / 8;
     P.page = a->page_size; P.pages = a->pages;
-    hipLaunchKernelGGL(tree_commit, dim3((uint32_t)(a->B * a->L), (uint32_t)a->layers), dim3(LLIMA_WG), 0,
-                       (hipStream_t)stream, P);
+    // a layer to a workgroup where there are few, 8 where they fill the device
+    // (64 paths in 32 layers: 36 us with one)
+    const int per = (int64_t)a->B * a->L * a->layers <= 2048 ? 1 : 8;
+    hipLaunchKernelGGL(tree_commit, dim3((uint32_t)(a->B * a->L), (uint32_t)((a->layers + per - 1) / per)),
+                       dim3(LLIMA_WG), 0, (hipStream_t)stream, P, a->layers, per);
     return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
 }

@@ -348,9 +348,12 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
     }
 }
 
+// Workgroups: as many as give each the same number of tiles but for one (a
+// last turn of a few workgroups does not draw the memory's rate; fewer that run to
+// the end together do).
 static int lmh8_groups(int V) {
-    const int ntile = (V + LMH8_NV - 1) / LMH8_NV;
-    return ntile < LMH8_CUS ? ntile : LMH8_CUS;
+    const int ntile = (V + LMH8_NV - 1) / LMH8_NV, turns = (ntile + LMH8_CUS - 1) / LMH8_CUS;
+    return (ntile + turns - 1) / turns;
 }
 
 // Key slots per hidden row: one per wave along the vocab rows.

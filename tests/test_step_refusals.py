@@ -194,3 +194,17 @@ def test_python_attention_refuses():
                  lambda: g(k[None].expand(2, 2, 3, 4, 64), k[None].expand(2, 2, 3, 4, 64), p, m, c[None], c[None], n)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_packed_arguments_are_the_structures():
+    """The byte layouts that the Python calls pack are those of the C structures, field by field."""
+    from llima_amd import _lib
+    for fmt, cls in ((_lib.TREE_ATTENTION_ARGS, _lib.TreeAttentionArgsC), (_lib.TREE_COMMIT_ARGS, _lib.TreeCommitArgsC)):
+        assert fmt.size == ctypes.sizeof(cls)
+        n = sum(getattr(t, "_length_", 1) for _, t in cls._fields_)
+        a = cls.from_buffer_copy(fmt.pack(*range(1, n + 1)))
+        got = []
+        for name, t in cls._fields_:
+            v = getattr(a, name)
+            got += list(v) if hasattr(t, "_length_") else [v]
+        assert got == list(range(1, n + 1))
