@@ -389,3 +389,18 @@ def test_commit_without_layers_dimension_and_with_views(gpu):
     with pytest.raises(ValueError):                          # a cache that would have to be copied
         llima_amd.tree_commit(k, v, nodes, lens, torch.zeros(2, 30, 2, 65, device=gpu, dtype=torch.bfloat16)[..., 1:],
                               vc, lens)
+
+
+@pytest.mark.parametrize("page", [0, 64, 24, 7])
+@pytest.mark.parametrize("N,Hq,Hkv", [(3, 4, 2), (11, 8, 2), (20, 4, 1), (30, 8, 2), (33, 8, 2), (64, 16, 4), (65, 16, 2)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_kernel(gpu, dtype, D, N, Hq, Hkv, page):
+    """Every number of row tiles in a workgroup (1, 2, 3, 4, 5, 8, and more than one group of them) with every way of
+    addressing the cache, short and longer sequences together, with and without a mask."""
+    import llima_amd
+    lens = [0, 130, 700, 63]
+    s, g = make(gpu, 4, N, Hq, Hkv, D, lens, page, dtype, seed=N + D)
+    mask = tree_mask(g, 4, N).to(gpu)
+    check(llima_amd.tree_attention(tree_mask=mask, **s), s, mask)
+    check(llima_amd.tree_attention(scale=-0.05, **s), s, scale=-0.05)
