@@ -252,7 +252,7 @@ __global__ __launch_bounds__(LLIMA_WG) void fp8_blocks(const uint16_t* w, uint8_
 template <int DT, int NWV, bool Q8, bool NORM>
 static void nrm_launch_np(const NormParams& P, hipStream_t st) {
     const int np = (P.H / 8 + 64 * NWV - 1) / (64 * NWV);
-    const dim3 g((uint32_t)P.B), blk(64 * NWV);
+    const dim3 g((uint32_t)P.B), blk(64 * NWV);              // B <= NRM_ROWS
     switch (np) {
         case 1: hipLaunchKernelGGL((rms_rows<DT, NWV, 1, Q8, NORM>), g, blk, 0, st, P); break;
         case 2: hipLaunchKernelGGL((rms_rows<DT, NWV, 2, Q8, NORM>), g, blk, 0, st, P); break;
@@ -262,9 +262,22 @@ static void nrm_launch_np(const NormParams& P, hipStream_t st) {
     }
 }
 
+// A launch holds fewer than 2^32 threads.
+#define NRM_ROWS (1 << 23)
+
 template <int DT, bool Q8, bool NORM>
 static int nrm_launch(const NormParams& P, hipStream_t st) {
-    nrm_launch_np<DT, 4, Q8, NORM>(P, st);
+    const size_t e = NormType<DT>::E, row = (size_t)P.H * e;
+    for (int64_t b0 = 0; b0 < P.B; b0 += NRM_ROWS) {
+        NormParams Q = P;
+        Q.B = P.B - b0 < NRM_ROWS ? (int)(P.B - b0) : NRM_ROWS;
+        Q.x = (const uint8_t*)P.x + b0 * P.x_stride * (int64_t)e;
+        if (P.residual) Q.residual = (const uint8_t*)P.residual + b0 * P.res_stride * (int64_t)e;
+        if (P.out_residual) Q.out_residual = (uint8_t*)P.out_residual + b0 * row;
+        Q.out = (uint8_t*)P.out + b0 * (Q8 ? (size_t)P.H : row);
+        if (Q8) Q.scales = P.scales + b0 * P.NK;
+        nrm_launch_np<DT, 4, Q8, NORM>(Q, st);
+    }
     return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
 }
 

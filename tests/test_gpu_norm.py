@@ -193,3 +193,23 @@ def test_lm_head_quantize_is_its_formula(gpu, V, H):
     q = (p * 448.0 / top).to(F8).view(nv * 128, nh * 128)[:V, :H]
     same(got.values, q)
     same(got.scales, (top / 448.0)[:, 0, :, 0])
+
+
+def test_more_rows_than_a_launch_holds(gpu):
+    """2^24 + 3 rows of 8: three launches, the rows around their edges, and nothing left out."""
+    import llima_amd
+    B, H = (1 << 24) + 3, 8
+    g = torch.Generator().manual_seed(5)
+    base = torch.randn(4099, H, generator=g).to(gpu, torch.bfloat16)
+    x = base.repeat(B // 4099 + 1, 1)[:B].contiguous()
+    w = torch.randn(H, generator=g).to(gpu, torch.bfloat16)
+    y, r = llima_amd.add_rms_norm(x, w, x)
+    y0, r0 = llima_amd.add_rms_norm(base, w, base)
+    for got, want in ((y, y0), (r, r0)):
+        n = B // 4099 * 4099
+        assert torch.equal(got[:n].view(-1, 4099, H), want[None].expand(n // 4099, 4099, H))
+        assert torch.equal(got[n:], want[:B - n])
+    q, q0 = llima_amd.quantize_rows(x), llima_amd.quantize_rows(base)
+    at = torch.tensor([0, (1 << 23) - 1, 1 << 23, (1 << 24) - 1, 1 << 24, B - 1], device=gpu)
+    assert torch.equal(q.values[at].view(torch.uint8), q0.values[at % 4099].view(torch.uint8))
+    assert torch.equal(q.scales[at], q0.scales[at % 4099])
