@@ -44,6 +44,17 @@ def _in_place(t: torch.Tensor, name: str) -> torch.Tensor:
     return h
 
 
+def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the spans of memory from the first to the last value of two tensors meet."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or not a.numel() or not b.numel():
+        return False
+
+    def end(t):
+        return t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    return pa < end(b) and pb < end(a)
+
+
 def _cache(k_cache, v_cache, Hkv, D, dtype, block_table, B, dev):
     """Checks of a cache [..., page_size, Hkv, D] and its table -> (page size, pages, blocks per
     sequence, table)."""
@@ -150,9 +161,9 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     [B, tokens, Hkv, D] or [pages, page_size, Hkv, D] (and the layers' dimension in front);
     bf16 or fp16, D a multiple of 8.  nodes int32 [B, L], counts int32 [B] (a row of
     Eagle3DraftTree's retrieve indices and the accept length + 1; arange and accepted_len + 1
-    for a chain).  A sequence with a count, node, length or page out of range, or no room for
-    its path, is left as it is and its new length is -2 (LLIMA_E_RANGE).  Nothing waits
-    for the device, and the call can be captured into a graph."""
+    for a chain).  k and v do not overlap the caches.  A sequence with a count, node, length or
+    page out of range, or no room for its path, is left as it is and its new length is -2
+    (LLIMA_E_RANGE).  Nothing waits for the device, and the call can be captured into a graph."""
     if k.dim() == 4:
         if k_cache.dim() != 4 or v_cache.dim() != 4 or v.dim() != 4:
             raise ValueError("k and v [B, N, Hkv, D] need 4-dimensional caches")
@@ -177,6 +188,8 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     nodes = nodes if nodes.stride(1) == 1 or nodes.shape[1] == 1 else nodes.contiguous()
     k, v = _heads(k), _heads(v)
     kc, vc = _in_place(k_cache, "k_cache"), _in_place(v_cache, "v_cache")
+    if _shared(k, kc) or _shared(k, vc) or _shared(v, kc) or _shared(v, vc):
+        raise ValueError("tree_commit: k and v must not overlap the caches (copy them first)")
     new = torch.empty(B, dtype=torch.int32, device=dev)
     if B == 0:
         return new

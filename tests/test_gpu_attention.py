@@ -404,3 +404,21 @@ def test_every_kernel(gpu, dtype, D, N, Hq, Hkv, page):
     mask = tree_mask(g, 4, N).to(gpu)
     check(llima_amd.tree_attention(tree_mask=mask, **s), s, mask)
     check(llima_amd.tree_attention(scale=-0.05, **s), s, scale=-0.05)
+
+
+def test_commit_refuses_keys_inside_the_cache(gpu):
+    """Drafted tokens kept in the cache itself: copies in no order would read what others wrote."""
+    import llima_amd
+    buf = torch.randn(2, 2, 40, 4, 64, device=gpu).to(torch.bfloat16)      # K and V in one allocation
+    kc, vc = buf[0], buf[1]
+    nodes = torch.tensor([[0, 2], [1, 2]], dtype=torch.int32, device=gpu)
+    counts = torch.tensor([2, 2], dtype=torch.int32, device=gpu)
+    lens = torch.tensor([10, 10], dtype=torch.int32, device=gpu)
+    before = buf.clone()
+    for k, v in ((kc[:, 10:13], vc[:, 10:13]), (vc[:, 10:13], vc[:, 10:13])):
+        with pytest.raises(ValueError, match="overlap"):
+            llima_amd.tree_commit(k, v, nodes, counts, kc, vc, lens)
+    assert torch.equal(buf, before)
+    k, v = kc[:, 10:13].clone(), vc[:, 10:13].clone()
+    assert llima_amd.tree_commit(k, v, nodes, counts, kc, vc, lens).tolist() == [12, 12]
+    assert torch.equal(kc[0, 11], k[0, 2]) and torch.equal(vc[1, 10], v[1, 1])
