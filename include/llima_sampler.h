@@ -69,6 +69,10 @@
  *                            _argmax_lm_head_rows + resolve_draft_tokens, no logits
  *   llima_lm_head_verify_tree(_packed) <- the EAGLE3 tree step's LM head + verify
  *                            argmax + tree_decoding + evaluate_posterior, no logits
+ * Without a counterpart (the reference compiles these for its NPU): the LM head
+ * over an 8-bit weight (llima_lm_head_*_fp8, llima_lm_head_quantize), and the
+ * verification step around the selection: llima_add_rms_norm, llima_quantize_rows,
+ * llima_tree_attention, llima_tree_commit.
  */
 #ifndef LLIMA_SAMPLER_H
 #define LLIMA_SAMPLER_H
@@ -518,7 +522,8 @@ int llima_add_rms_norm(const void* x, const void* residual, const void* weight, 
  * dtype LLIMA_BF16 or LLIMA_F16; D 64, 128 or 256, adjacent; every other stride is
  * free, in elements, a multiple of 8, and not negative; base pointers and the
  * workspace 16-byte aligned.  mask strides: batch (0: one mask for all) and row,
- * columns adjacent.  N at most 1024, page_size * max_blocks + N at most 2^30.  A
+ * columns adjacent.  N and Hq at most 1024, B N Hq below 2^26, page_size *
+ * max_blocks + N at most 2^30.  A
  * sequence whose length is outside [0, page_size * max_blocks], or which has a page
  * outside [0, pages) among its cached tokens', gets NaN.  The order of the sums, and
  * so the last bits, depend on the lengths of the whole batch, not on its timing. */
@@ -554,7 +559,7 @@ int llima_tree_attention(const llima_tree_attention_args* args, void* workspace,
  *   k_cache, v_cache [layers][pages][page_size][Hkv][D] and block_table as
  *     llima_tree_attention's
  *
- * 16-bit values of any type, D a multiple of 8, strides as there (layer, batch or
+ * 16-bit values of any type, D a multiple of 8, B L below 2^24, strides as there (layer, batch or
  * page, token, head).  A sequence with a count outside [0, L], a node outside [0, N),
  * a length below 0, no room for its path or a page outside [0, pages) among those it
  * would write is left as it is, and new_lens[b] is LLIMA_E_RANGE.  Nothing else of

@@ -753,7 +753,7 @@ using namespace llima;
 static bool at_sizes_ok(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D) {
     if (B < 0 || N <= 0 || N > 1024 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq > 1024) return false;
     if (D != 64 && D != 128 && D != 256) return false;
-    return (int64_t)B * N * Hq <= (1 << 28);
+    return (int64_t)B * N * Hq < (1 << 26);                  // (the join's launch: fewer than 2^32 threads)
 }
 
 static void at_plan(AttnParams& P, int D) {
@@ -846,7 +846,7 @@ extern "C" int llima_tree_commit(const llima_tree_commit_args* a, void* stream) 
     if (a->page_size <= 0 || a->pages < 0 || a->max_blocks < 0) return LLIMA_E_INVAL;
     if (!a->block_table && (a->pages < a->B || a->max_blocks != 1)) return LLIMA_E_INVAL;
     if ((int64_t)a->page_size * a->max_blocks > (int64_t)INT32_MAX) return LLIMA_E_INVAL;
-    if ((int64_t)a->B * a->L > (int64_t)INT32_MAX) return LLIMA_E_INVAL;
+    if ((int64_t)a->B * a->L >= (1 << 24)) return LLIMA_E_INVAL;   // (the launch: fewer than 2^32 threads)
     if (!at_strides_ok(a->k_strides, 4) || !at_strides_ok(a->v_strides, 4) || !at_strides_ok(a->k_cache_strides, 4) ||
         !at_strides_ok(a->v_cache_strides, 4) || a->nodes_stride < 0 || (a->block_table && a->table_stride < 0))
         return LLIMA_E_INVAL;

@@ -208,3 +208,11 @@ def test_packed_arguments_are_the_structures():
             v = getattr(a, name)
             got += list(v) if hasattr(t, "_length_") else [v]
         assert got == list(range(1, n + 1))
+
+
+def test_batches_past_one_launch_are_refused():
+    a = attention_args(B=1 << 19, N=16)                      # 2^26 rows
+    assert L().llima_tree_attention(ctypes.byref(a), P, BIG << 20, None) == -1
+    assert L().llima_tree_attention_workspace_bytes(1 << 19, 16, 8, 4, 128) == 0
+    assert L().llima_tree_attention_workspace_bytes((1 << 19) - 1, 16, 8, 4, 128) > 0
+    assert L().llima_tree_commit(ctypes.byref(commit_args(B=1 << 20, L=1 << 4)), None) == -1
