@@ -188,6 +188,32 @@ __device__ __forceinline__ void at_dma(const void* src, uint8_t* dst) {
                                      (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
+// Keys KEY + (0 .. 3, 8 .. 11) + 4 g of every block of 32 columns, by the transposing
+// loads from the lane's places.  In one piece with their wait: as builtins, the
+// compiler waits for all the requests into LDS before them.
+template <int D, int KEY>
+__device__ __forceinline__ void at_vread(const uint32_t (&a)[4], at_s4 (&v)[D / 32][2]) {
+    constexpr int K0 = KEY * D * 2, K1 = (KEY + 8) * D * 2;
+    if constexpr (D == 64) {
+        asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+                     "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+                     : "v"(a[0]), "v"(a[1]), "n"(K0), "n"(K1));
+    } else {
+#pragma unroll
+        for (int d = 0; d < D / 32; d += 4)
+            asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                         "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                         "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                         "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                         "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(v[d][0]), "=&v"(v[d][1]), "=&v"(v[d + 1][0]), "=&v"(v[d + 1][1]),
+                           "=&v"(v[d + 2][0]), "=&v"(v[d + 2][1]), "=&v"(v[d + 3][0]), "=&v"(v[d + 3][1])
+                         : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(K0 + d * 64), "n"(K1 + d * 64));
+    }
+}
+
 template <int N>
 __device__ __forceinline__ void at_wait_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
@@ -356,15 +382,34 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
         constexpr bool ALL = decltype(all)::value;
         at_acc s[KPW];
 #pragma unroll
-        for (int kb = 0; kb < KPW; ++kb) {
-            const int kt = (kw * KPW + kb) * 32 + r;         // the lane's key row of the K operand
+        for (int kb = 0; kb < KPW; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+        // four pieces of K at a time, read while the four before are multiplied
+        constexpr int NG = KPW * D / 64;
+        at_s8 kf[2][4];
+        auto kread = [&](int e) {
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-                const at_s8 kf = *(const at_s8*)(sk + kt * (D * 2) + (((2 * d + g) ^ (kt & (U - 1) & 15)) << 4));
-                s[kb] = at_mfma<DT>(kf, qf[d], s[kb]);
+            for (int i = 0; i < 4; ++i) {
+                const int kt = (kw * KPW + e * 4 / (D / 16)) * 32 + r, d = e * 4 % (D / 16) + i;   // the lane's key row
+                kf[e & 1][i] = *(const at_s8*)(sk + kt * (D * 2) + (((2 * d + g) ^ (r & (U - 1) & 15)) << 4));
             }
+        };
+        kread(0);
+#pragma unroll
+        for (int e = 0; e < NG; ++e) {
+            if (e + 1 < NG) kread(e + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[e * 4 / (D / 16)] = at_mfma<DT>(kf[e & 1][i], qf[e * 4 % (D / 16) + i], s[e * 4 / (D / 16)]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        uint32_t va[4];                                      // V: the lane's places of four column blocks
+        {
+            const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)sk + TB +
+                                  (uint32_t)((kw * KPW * 32 + 4 * g + (lane >> 2 & 3)) * (D * 2) + (lane >> 4 & 1) * 32 + (lane & 3) * 8);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) va[d] = base + (uint32_t)(((d * 4) ^ ((lane >> 2 & 3) << 2 & (U - 1))) * 16);
         }
         float mt = -__builtin_inff();
 #pragma unroll
@@ -409,18 +454,14 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
                 const at_s8 pf = __builtin_bit_cast(at_s8, (llima_u32x4){pw[0], pw[1], pw[2], pw[3]});
                 // element e of half g is key 16 st + e % 4 + 8 (e / 4) + 4 g: a
                 // transposing load takes 4 keys by 16 columns from 16 lanes
-                const int kk = (kw * KPW + kb) * 32 + st * 16 + 4 * g + (lane >> 2 & 3);
+                at_s4 v[D / 32][2];
+                if (kb == 0 && st == 0) at_vread<D, 0>(va, v);
+                else if (kb == 0) at_vread<D, 16>(va, v);
+                else if (st == 0) at_vread<D, 32>(va, v);
+                else at_vread<D, 48>(va, v);
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    const int c8 = d * 8 + (lane >> 4 & 1) * 4 + (lane & 3);      // 8-byte piece of the row
-                    auto vload = [&](int key) {
-                        const uint8_t* a = sk + TB + key * (D * 2) + (((c8 >> 1) ^ ((key & 3) << 2 & (U - 1))) << 4) + (c8 & 1) * 8;
-                        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)a);
-                    };
-                    const at_s4 v0 = vload(kk), v1 = vload(kk + 8);
-                    const at_s8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = at_mfma<DT>(vf, pf, o[d]);
-                }
+                for (int d = 0; d < D / 32; ++d)
+                    o[d] = at_mfma<DT>(__builtin_shufflevector(v[d][0], v[d][1], 0, 1, 2, 3, 4, 5, 6, 7), pf, o[d]);
             }
         }
     };
