@@ -19,7 +19,13 @@
 // sum takes the weights before the rounding.  In fp16 the weights carry a factor
 // of 2^10, so that they become subnormal below 2^-24 of the row's largest.
 //
-// Bound: reading K and V once for all N Hq / Hkv rows of a key head.
+// Bound: reading K and V once for all N Hq / Hkv rows of a key head.  Up to 128 such
+// rows the loop over the tiles runs at the memory's rate (16 nodes, 4 query heads per key
+// head: 8 x 16384 tokens 537 MB in 125 us, twice as many sequences 215: 5.9 TB/s for what
+// is added, and as long with the products left out); some 25 us are the call's start, the
+// masked tile, the partial sums and the join.  From five row tiles on the waves' chain
+// of LDS reads, product, softmax and product bounds (4 x 131072 tokens, 33 nodes: 2.15 GB in
+// 555 us, requests alone 408).
 #include <type_traits>
 
 #include "common.hpp"
@@ -126,8 +132,10 @@ __device__ __forceinline__ int at_len(const AttnParams& P, int b, bool& bad) {
 // at_tiles: sequence b's tiles; at_share: the length of a share (every lane of
 // a wave calls it and gets the same).  len0: the length of sequence lane.
 // A sequence counts for AT_EXTRA tiles more than it has, at its end: the time that
-// its mask, its sums' exchange and the next sequence's start take.
-#define AT_EXTRA 3
+// its mask, its sums' exchange and the next sequence's start take (3 / 6 / 8: 24 ragged
+// sequences of up to 16384 tokens, 16 nodes, 151 / 140 / 140 us; 48 of up to 3000, one
+// node, 75 / 67 / 62; 100 of up to 500 49 / 52 / 59).
+#define AT_EXTRA 6
 template <int T>
 __device__ __forceinline__ int at_tiles(const AttnParams& P, int len) { return (len + P.N + T - 1) / T + AT_EXTRA; }
 
@@ -220,8 +228,13 @@ __device__ __forceinline__ void at_wait_barrier() {
 }
 
 // One workgroup: NW waves over one share of the keys, one key head and a group of
-// up to NW / KW row tiles (32 rows each).  Keys come in tiles of T, requested straight into a ring of S stages; KW waves share a row tile and
-// take half of a tile's keys each (KW = 2), or one takes all.
+// up to NW / KW row tiles (32 rows each).  Keys come in tiles of T, requested straight
+// into a ring of S stages; KW waves share a row tile and take half of a tile's keys each
+// (KW = 2), or one takes all.  Two workgroups per CU with two stages of 64 keys each: one
+// with four stages leaves the products alone on a SIMD (16 nodes over 8 x 16384 tokens 127
+// -> 148 us), a third stage for K alone has nothing more to hide (127 -> 129).  Five and
+// six row tiles take the eight waves too: twelve with halves of the keys need more
+// registers than they have (33 nodes 590 -> 700 us).
 //
 // Tiles of cached keys alone are requested by mode: a tile lies in one page
 // (contiguous caches and pages of a multiple of 64), its address is the wave's
