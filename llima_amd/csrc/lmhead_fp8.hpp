@@ -348,12 +348,12 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
     }
 }
 
-// Workgroups: as many as give each the same number of tiles but for one (a
-// last turn of a few workgroups does not draw the memory's rate; fewer that run to
-// the end together do).
+// Workgroups: one per CU, or per tile where there are fewer.  (As many as give
+// each the same number of tiles: 151936 rows, B = 64, 142 us with 198 of them, 138
+// with 256.)
 static int lmh8_groups(int V) {
-    const int ntile = (V + LMH8_NV - 1) / LMH8_NV, turns = (ntile + LMH8_CUS - 1) / LMH8_CUS;
-    return (ntile + turns - 1) / turns;
+    const int ntile = (V + LMH8_NV - 1) / LMH8_NV;
+    return ntile < LMH8_CUS ? ntile : LMH8_CUS;
 }
 
 // Key slots per hidden row: one per wave along the vocab rows.
