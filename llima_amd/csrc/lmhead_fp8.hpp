@@ -11,8 +11,9 @@
 // are twice as fast but drop low bits of the products when they add them (128
 // products of values from N(0, 60^2): off by 2^-16 of the terms' magnitude at
 // most, by 2^-12 where one product in 64 is 2^11 times the others; the bf16
-// instructions 2^-25 and 2^-22), which is not a sum in 32 bits.  xq [B][H] and xs [B][NK] are a hidden row's values
-// and scales, wq [V][H] and ws [ceil(V/128)][NK] the weight's, NK = ceil(H/128).
+// instructions 2^-25 and 2^-22), which is not a sum in 32 bits.  xq [B][H] and
+// xs [B][NK] are a hidden row's values and scales, wq [V][H] and ws [ceil(V/128)][NK]
+// the weight's, NK = ceil(H/128).
 #pragma once
 
 // Eight e4m3 values as bf16 (exact; NaN stays NaN).
@@ -158,17 +159,24 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
 // columns exchanged by row / 2 (the request's source address does it): fragment
 // reads have no bank conflicts.  The scales are loaded a step ahead, before the
 // requests, so that waiting for them leaves those in flight (with requests made by
-// global loads the compiler takes them to return in any order and waits for all).  A step's values are read, converted and
-// multiplied piece by piece (piece e of half g: ids 32 e + 16 g .. + 15, its halves two
-// MFMAs), its sums scaled and added to the tile's.  The weight is the MFMA's
-// row operand: lane (r, g) has, for hidden row r of a block, half of a wave's vocab rows
-// (the lane with the other g the other half).
+// global loads the compiler takes them to return in any order and waits for all).  A
+// step's values are read, converted and multiplied piece by piece (piece e of half g:
+// ids 32 e + 16 g .. + 15, its halves two MFMAs), its sums scaled and added to the
+// tile's.  The weight is the MFMA's row operand: lane (r, g) has, for hidden row r of a
+// block, half of a wave's vocab rows (the lane with the other g the other half).
 //
 // A tile's steps start at another block in each workgroup of an XCD: all at the
 // first one read the same 128 bytes of every 4 KB, which is a part of the memory
 // channels (the weight of 0.53 GB, requests alone: 110 us, started apart 88).
 //
-// Bound: reading the weight up to 128 rows; a batch of more goes in passes of 128.
+// Shapes <RWV, VB, CWV, MB, S>: <8, 1, 1, 1, 4> up to 32 rows, <4, 2, 2, 1, 4> up to 64,
+// <4, 2, 2, 2, 3> up to 128, and larger batches in passes of 128.  The waves' split along the
+// hidden rows halves what each converts of the weight; along the vocab rows alone
+// (8 waves) the LDS reads bound (64 / 128 rows 130 / 199 us against 101 / 151).
+//
+// Bound: reading the weight up to 64 rows (H 4096, V 128256, 0.53 GB: 1 row 92 us,
+// 32 rows 96, 64 101; the requests alone 88), from 128 on (151, 500 rows 600) the issue of
+// the vector instructions that widen, scale and add.
 #define LMH8_NV 256                    // vocab rows per tile
 #define LMH8_CUS 256                   // workgroups: one per CU (its LDS)
 

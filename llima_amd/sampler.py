@@ -19,6 +19,8 @@ the buffers handed to it (inputs must already be on the GPU).
   topk(x, k)                          utils.hpp:216-281
   stop_check(tokens, stop_mask, V)    language_model.cpp:643-671 (the decode loops' stop rule)
   Eagle3DraftTree                     language_model_eagle3.cpp:808-1164 (topk_generate's selection)
+  add_rms_norm, quantize_rows,        no reference counterpart: the residual's addition and norm, and
+  Fp8LmHead, lm_head_quantize         the LM head over an 8-bit weight
 
 Errors: the reference throws std::invalid_argument / std::runtime_error; here
 ValueError / RuntimeError are raised for the same conditions.
