@@ -639,7 +639,7 @@ class PackedLmHead:
 def lm_head_pack(weight: torch.Tensor) -> PackedLmHead:
     """Prepack a bf16 [V, H] LM head weight (H a multiple of 256) for
     lm_head_argmax (llima_lm_head_pack)."""
-    if weight.dtype != torch.bfloat16 or weight.dim() != 2:
+    if isinstance(weight, Fp8LmHead) or weight.dtype != torch.bfloat16 or weight.dim() != 2:
         raise ValueError("lm_head_pack takes a bf16 [V, H] weight")
     w = weight.contiguous()
     V, H = w.shape
@@ -768,6 +768,11 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
                                        float(weight_offset), o.data_ptr(), sc, _ptr(r),
                                        _stream(dev)), "llima_add_rms_norm")
     return y, r
+
+
+def _bf16_rows(hidden) -> None:
+    if isinstance(hidden, Fp8Rows):
+        raise ValueError("Fp8Rows are for an Fp8LmHead (lm_head_quantize); a bf16 weight takes bf16 rows")
 
 
 def _fp8_hidden(hidden, head: Fp8LmHead, name: str) -> Fp8Rows:
@@ -918,6 +923,7 @@ def lm_head_argmax(hidden: torch.Tensor, weight, softcap: float = 0.0,
     quantize_rows) or Fp8Rows (llima_lm_head_argmax_fp8)."""
     if isinstance(weight, Fp8LmHead):
         return _lm_head_argmax_fp8(hidden, weight, softcap, return_logits, logit_dtype, logits_out)
+    _bf16_rows(hidden)
     x = hidden.reshape(1, -1) if hidden.dim() == 1 else hidden
     packed = isinstance(weight, PackedLmHead)
     if x.dtype != torch.bfloat16 or (not packed and weight.dtype != torch.bfloat16):
@@ -971,6 +977,7 @@ def lm_head_score(hidden: torch.Tensor, weight, target, softcap: float = 0.0,
     quantize_rows) or Fp8Rows (llima_lm_head_score_fp8)."""
     if isinstance(weight, Fp8LmHead):
         return _lm_head_score_fp8(hidden, weight, target, softcap, logit_dtype)
+    _bf16_rows(hidden)
     single = hidden.dim() == 1
     x = hidden.reshape(1, -1) if single else hidden
     packed = isinstance(weight, PackedLmHead)
@@ -1029,6 +1036,7 @@ def lm_head_verify_greedy(hidden: torch.Tensor, weight, draft_ids: torch.Tensor,
     quantize_rows) or Fp8Rows (llima_lm_head_verify_greedy_fp8)."""
     if isinstance(weight, Fp8LmHead):
         return _lm_head_verify_greedy_fp8(hidden, weight, draft_ids, softcap, logit_dtype)
+    _bf16_rows(hidden)
     if hidden.dim() != 3:
         raise ValueError("hidden must be [B, D+1, H]")
     B, D1, H = hidden.shape
@@ -1084,6 +1092,7 @@ def lm_head_verify_tree(hidden: torch.Tensor, weight, retrieve_indices: torch.Te
     if isinstance(weight, Fp8LmHead):
         return _lm_head_verify_tree_fp8(hidden, weight, retrieve_indices, candidates, softcap,
                                        logit_dtype)
+    _bf16_rows(hidden)
     x = hidden.contiguous()
     packed = isinstance(weight, PackedLmHead)
     if x.dim() != 2 or x.dtype != torch.bfloat16 or (not packed and weight.dtype != torch.bfloat16):

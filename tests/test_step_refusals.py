@@ -216,3 +216,17 @@ def test_batches_past_one_launch_are_refused():
     assert L().llima_tree_attention_workspace_bytes(1 << 19, 16, 8, 4, 128) == 0
     assert L().llima_tree_attention_workspace_bytes((1 << 19) - 1, 16, 8, 4, 128) > 0
     assert L().llima_tree_commit(ctypes.byref(commit_args(B=1 << 20, L=1 << 4)), None) == -1
+
+
+def test_8_bit_rows_need_an_8_bit_weight():
+    import llima_amd
+    x = llima_amd.Fp8Rows.__new__(llima_amd.Fp8Rows)          # (the constructor refuses host tensors)
+    x.values, x.scales = torch.zeros(2, 64).to(torch.float8_e4m3fn), torch.zeros(2, 1)
+    h = llima_amd.Fp8LmHead.__new__(llima_amd.Fp8LmHead)
+    h.values, h.scales, h.V, h.H = torch.zeros(100, 64).to(torch.float8_e4m3fn), torch.zeros(1, 1), 100, 64
+    w, i = torch.zeros(100, 64, dtype=torch.bfloat16), torch.zeros(2, 2, dtype=torch.int32)
+    for call in (lambda: llima_amd.lm_head_argmax(x, w), lambda: llima_amd.lm_head_score(x, w, i[0]),
+                 lambda: llima_amd.lm_head_verify_greedy(x, w, i[:1, :1]),
+                 lambda: llima_amd.lm_head_verify_tree(x, w, i, i), lambda: llima_amd.lm_head_pack(h)):
+        with pytest.raises(ValueError, match="bf16"):
+            call()
