@@ -775,6 +775,13 @@ def _bf16_rows(hidden) -> None:
         raise ValueError("Fp8Rows are for an Fp8LmHead (lm_head_quantize); a bf16 weight takes bf16 rows")
 
 
+def _fp8_rows_only(hidden) -> None:
+    """Refuses hidden states with more than one leading dimension, as the heads over a bf16
+    weight do (quantize_rows would make rows of all of them)."""
+    if not isinstance(hidden, Fp8Rows) and hidden.dim() not in (1, 2):
+        raise ValueError("hidden must be [H], [rows, H] or Fp8Rows")
+
+
 def _fp8_hidden(hidden, head: Fp8LmHead, name: str) -> Fp8Rows:
     """The hidden rows of a call over an Fp8LmHead: Fp8Rows as they are, bf16 rows
     [rows, H] through quantize_rows."""
@@ -827,6 +834,7 @@ def _lm_head_argmax_fp8(hidden, head: Fp8LmHead, softcap, return_logits, logit_d
 
 
 def _lm_head_score_fp8(hidden, head: Fp8LmHead, target, softcap, logit_dtype):
+    _fp8_rows_only(hidden)
     single = not isinstance(hidden, Fp8Rows) and hidden.dim() == 1
     ld = _logit_dtype(logit_dtype)
     V, dev = head.V, head.values.device

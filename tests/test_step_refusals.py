@@ -230,3 +230,20 @@ def test_8_bit_rows_need_an_8_bit_weight():
                  lambda: llima_amd.lm_head_verify_tree(x, w, i, i), lambda: llima_amd.lm_head_pack(h)):
         with pytest.raises(ValueError, match="bf16"):
             call()
+
+
+def host_head():
+    """An 8-bit head on the host (the constructor refuses host tensors): H 64, V 100."""
+    import llima_amd
+    h = llima_amd.Fp8LmHead.__new__(llima_amd.Fp8LmHead)
+    h.values, h.scales, h.V, h.H = torch.zeros(100, 64).to(torch.float8_e4m3fn), torch.zeros(1, 1), 100, 64
+    return h
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 64), (2, 1, 64), (1, 1, 2, 64), ()])
+def test_scoring_over_an_8_bit_head_takes_rows(shape):
+    """Two targets for [2, 3, H]: one target per leading index is not one per row, and the rows past them would be scored
+    against what lies behind the targets."""
+    import llima_amd
+    with pytest.raises(ValueError, match="hidden must be"):
+        llima_amd.lm_head_score(torch.zeros(shape, dtype=torch.bfloat16), host_head(), torch.tensor([1, 2]))
