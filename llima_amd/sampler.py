@@ -817,6 +817,7 @@ def _head8(x: Fp8Rows, head: Fp8LmHead):
 
 
 def _lm_head_argmax_fp8(hidden, head: Fp8LmHead, softcap, return_logits, logit_dtype, logits_out):
+    _fp8_rows_only(hidden)
     ld = _logit_dtype(logit_dtype, logits_out)
     x = _fp8_hidden(hidden, head, "lm_head_argmax")
     B, V, dev = x.values.shape[0], head.V, head.values.device

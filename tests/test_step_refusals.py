@@ -247,3 +247,15 @@ def test_scoring_over_an_8_bit_head_takes_rows(shape):
     import llima_amd
     with pytest.raises(ValueError, match="hidden must be"):
         llima_amd.lm_head_score(torch.zeros(shape, dtype=torch.bfloat16), host_head(), torch.tensor([1, 2]))
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 64), (1, 1, 64), ()])
+def test_argmax_over_an_8_bit_head_takes_rows(shape):
+    """As over a bf16 weight: rows or one row, not rows of rows flattened."""
+    import llima_amd
+    x = torch.zeros(shape, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="hidden must be"):
+        llima_amd.lm_head_argmax(x, host_head())
+    if x.dim():
+        with pytest.raises(ValueError):
+            llima_amd.lm_head_argmax(x, torch.zeros(100, 64, dtype=torch.bfloat16))
