@@ -435,7 +435,9 @@ int llima_lm_head_verify_tree_packed(const void* hidden, const void* packed, int
  * (fp32 products and sums), then everything as the entry points over a bf16
  * weight: softcap, logit_dtype rounding, LLIMA_LOGITS_OUT_BF16, ids, values and
  * logits (argmax), log-likelihoods (score), chain and tree verification.  A NaN
- * value or scale makes the logits it enters NaN, which never win.  H is a
+ * value or scale makes the logits it enters NaN, which never win.  The order of a
+ * sum depends on H and on whether the batch has more than 64 rows, not on the vocab row
+ * or the hidden row: equal rows under equal scales have equal logits, and the lower id wins.  H is a
  * multiple of 64, at most 65536; hidden and weight are 16-byte aligned.  B = 0
  * launches nothing.  Batches above 128 rows go in passes.
  * llima_add_rms_norm and llima_quantize_rows make the hidden rows,

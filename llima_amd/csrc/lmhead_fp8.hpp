@@ -165,9 +165,18 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
 // tile's.  The weight is the MFMA's row operand: lane (r, g) has, for hidden row r of a
 // block, half of a wave's vocab rows (the lane with the other g the other half).
 //
-// A tile's steps start at another block in each workgroup of an XCD: all at the
-// first one read the same 128 bytes of every 4 KB, which is a part of the memory
-// channels (the weight of 0.53 GB, requests alone: 110 us, started apart 88).
+// The order of a sum may not depend on where its vocab row lies, or equal rows would get
+// logits that differ in their last bits and the greater id could win.  But workgroups that
+// all start their tiles at the first block of k read the same 128 bytes of every 4 KB, which
+// is a part of the memory channels.  So the blocks stand in 2^K groups, each summed from its
+// first block on, and the groups' sums are added in pairs, then the pairs': every order
+// q ^ rot of the groups adds the same two values in one order or the other, and workgroups
+// start at different groups.  K = 2 from H = 4096 on, up to 64 rows (V 128256, from block 0 /
+// K = 2: 1 row of 4096 ids 114 / 94 us, 64 rows 123 / 112, 1 row of 8192 230 / 181).  Narrower
+// rows lie apart by themselves (V 152064, 3584 ids, 1 row 105 / 107, 64 rows 125 / 129; V 32000,
+// 512 ids 9.6 / 10.4), and above 64 rows the waiting sums' registers are not there (K = 1 at
+// 128 rows: 154 -> 176 us) and reading bounds less: K = 0, from block 0 on, the last pass of
+// such a batch too.
 //
 // Shapes <RWV, VB, CWV, MB, S>: <8, 1, 1, 1, 4> up to 32 rows, <4, 2, 2, 1, 4> up to 64,
 // <4, 2, 2, 2, 3> up to 128, and larger batches in passes of 128.  The waves' split along the
@@ -180,7 +189,7 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
 #define LMH8_NV 256                    // vocab rows per tile
 #define LMH8_CUS 256                   // workgroups: one per CU (its LDS)
 
-template <int RWV, int VB, int CWV, int MB, int S, bool SC>
+template <int RWV, int VB, int CWV, int MB, int S, int K, bool SC>
 __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) {
     constexpr int NM = 32 * CWV * MB;                        // hidden rows of the pass
     constexpr int LW = LMH8_NV / 64;                         // 1 KB requests per wave and step: weight,
@@ -194,8 +203,9 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
     const int wr = wave % RWV, wc = wave / RWV;
     const int H = P.H, V = P.V, NK = Q.NK, G = (int)gridDim.x;
     const int ntile = (V + LMH8_NV - 1) / LMH8_NV;           // grid <= ntile
-    const int rot = (int)(blockIdx.x >> 3) % NK;             // the tiles' first block
-    const int ntot = ((ntile - 1 - (int)blockIdx.x) / G + 1) * NK;   // the workgroup's steps
+    constexpr int NG = 1 << K;                               // groups of blocks; NK >= NG
+    const int rot = (int)(blockIdx.x >> 3) & (NG - 1);       // they are taken in the order q ^ rot
+    auto start = [&](int q) { return (q * NK) >> K; };       // group q's first block
     // The request stream: a tile and a block of it.  Through buffer descriptors:
     // rows past the vocabulary or the batch lie outside them and read as 0, as
     // does what the last row's last block has past H (other rows read the next
@@ -212,7 +222,7 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
         ox[q] = (uint32_t)row * (uint32_t)H + (uint32_t)(((lane & 7) ^ (row >> 1 & 7)) * 16);
     }
     const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(Q.xq + (size_t)b0 * H), 0, nb * H, 0x00027000);
-    int tw = (int)blockIdx.x, cw = rot, sw = 0;
+    int tw = (int)blockIdx.x, qw = 0, cw = start(rot), ew = start(rot + 1), sw = 0;
     auto issue = [&]() {
         const int rows = V - tw * LMH8_NV < LMH8_NV ? V - tw * LMH8_NV : LMH8_NV;
         const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(Q.wq + (size_t)tw * LMH8_NV * H), 0, rows * H, 0x00027000);
@@ -226,8 +236,14 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(at + (wave + 8 * q) * 1024),
                                                      16, (int)ow[q], cw * 128, 0, 0);
         sw = sw + 1 == S ? 0 : sw + 1;
-        cw = cw + 1 == NK ? 0 : cw + 1;
-        if (cw == rot && tw + G < ntile) tw += G;            // past its last tile: that again
+        if (++cw == ew) {                                    // uniform
+            if (++qw == NG) {
+                qw = 0;
+                if (tw + G < ntile) tw += G;                 // past its last tile: that again
+            }
+            cw = start(qw ^ rot);
+            ew = start((qw ^ rot) + 1);
+        }
     };
     int m[MB], mc[MB];                                       // the lane's hidden rows of the pass
 #pragma unroll
@@ -242,7 +258,7 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
 #pragma unroll
         for (int i = 0; i < MB; ++i) sx[i] = Q.xs[(size_t)(b0 + mc[i]) * NK + c];
     };
-    int tile = (int)blockIdx.x, c = rot, slot = 0;
+    int slot = 0;
     float acc[MB][VB][16];
     Lmh8Best best[MB];
 #pragma unroll
@@ -253,94 +269,117 @@ __global__ __launch_bounds__(512) void lmh8_tiles(Lmh8Params Q, int b0, int nb) 
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][v][k] = 0.0f;
     }
-    load_s(tile, c);
+    load_s((int)blockIdx.x, start(rot));
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) issue();
     const uint32_t rl = (uint32_t)(r * 128), rz = (uint32_t)(r >> 1 & 7);
-    for (int it = 0; it < ntot; ++it) {
-        lmh_wait_barrier<(S - 2) * (LW + LX)>();             // the step's values have landed, the last one's are read
-        const int cn = c + 1 == NK ? 0 : c + 1;
-        const bool end = cn == rot;                          // uniform: the tile's last step
-        const int tn = end && tile + G < ntile ? tile + G : tile;
-        float sc[MB];
+    for (int tile = (int)blockIdx.x; tile < ntile; tile += G) {
+        float low[K > 0 ? K : 1][MB][VB][16];                // sums of groups that wait for their counterpart
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-            sc[i] = sx[i] * swt;
-            asm volatile("" : "+v"(sc[i]));                  // now: later, the next scales would need a copy, and that a wait
-        }
-        load_s(tn, cn);
-        __builtin_amdgcn_sched_barrier(0);                   // before the requests: waited for without them
-        issue();
-        const uint8_t* wb = sm + slot * SB + wr * VB * 4096;
-        const uint8_t* xb = sm + slot * SB + WB + wc * MB * 4096;
-        const bool half = c * 128 + 64 >= H;                 // uniform: H % 128 == 64, the last block
-        // NE pieces of the block (two in the last one when H % 128 == 64); each
-        // read one ahead of its conversion
-        auto block = [&](auto ne) __attribute__((always_inline)) {
-            constexpr int NE = decltype(ne)::value;
-            lmh_acc p[MB][VB];
+        for (int q = 0; q < NG; ++q) {
+            const int ce = start((q ^ rot) + 1);
+            const bool over = q + 1 == NG;                   // (compile time) the step after is the next tile's
+            const int cnext = over ? start(rot) : start((q + 1) ^ rot);
+            const int tnext = over && tile + G < ntile ? tile + G : tile;
+            for (int c = start(q ^ rot); c < ce; ++c) {
+                lmh_wait_barrier<(S - 2) * (LW + LX)>();     // the step's values have landed, the last one's are read
+                const int cn = c + 1 < ce ? c + 1 : cnext, tn = c + 1 < ce ? tile : tnext;
+                float sc[MB];
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int v = 0; v < VB; ++v)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) p[i][v][k] = 0.0f;
-            llima_u32x4 w[2][VB], x[2][MB];
-            auto read = [&](int e) {
-                const uint32_t o = rl + ((((uint32_t)(2 * e + g)) ^ rz) << 4);
-#pragma unroll
-                for (int v = 0; v < VB; ++v) w[e & 1][v] = *(const llima_u32x4*)(wb + v * 4096 + o);
-#pragma unroll
-                for (int i = 0; i < MB; ++i) x[e & 1][i] = *(const llima_u32x4*)(xb + i * 4096 + o);
-            };
-            read(0);
-#pragma unroll
-            for (int e = 0; e < NE; ++e) {
-                if (e + 1 < NE) read(e + 1);
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    lmh_b8 wv[VB], xv[MB];
-#pragma unroll
-                    for (int v = 0; v < VB; ++v) wv[v] = q ? lmh8_wide(w[e & 1][v].z, w[e & 1][v].w) : lmh8_wide(w[e & 1][v].x, w[e & 1][v].y);
-#pragma unroll
-                    for (int i = 0; i < MB; ++i) xv[i] = q ? lmh8_wide(x[e & 1][i].z, x[e & 1][i].w) : lmh8_wide(x[e & 1][i].x, x[e & 1][i].y);
+                for (int i = 0; i < MB; ++i) {
+                    sc[i] = sx[i] * swt;
+                    asm volatile("" : "+v"(sc[i]));          // now: later, the next scales would need a copy, and that a wait
+                }
+                load_s(tn, cn);
+                __builtin_amdgcn_sched_barrier(0);           // before the requests: waited for without them
+                issue();
+                const uint8_t* wb = sm + slot * SB + wr * VB * 4096;
+                const uint8_t* xb = sm + slot * SB + WB + wc * MB * 4096;
+                const bool half = c * 128 + 64 >= H;         // uniform: H % 128 == 64, the last block
+                // NE pieces of the block (two in the last one when H % 128 == 64); each
+                // read one ahead of its conversion
+                auto block = [&](auto ne) __attribute__((always_inline)) {
+                    constexpr int NE = decltype(ne)::value;
+                    lmh_acc p[MB][VB];
 #pragma unroll
                     for (int i = 0; i < MB; ++i)
 #pragma unroll
-                        for (int v = 0; v < VB; ++v) p[i][v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[v], xv[i], p[i][v], 0, 0, 0);
+                        for (int v = 0; v < VB; ++v)
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) p[i][v][k] = 0.0f;
+                    llima_u32x4 w[2][VB], x[2][MB];
+                    auto read = [&](int e) {
+                        const uint32_t o = rl + ((((uint32_t)(2 * e + g)) ^ rz) << 4);
+#pragma unroll
+                        for (int v = 0; v < VB; ++v) w[e & 1][v] = *(const llima_u32x4*)(wb + v * 4096 + o);
+#pragma unroll
+                        for (int i = 0; i < MB; ++i) x[e & 1][i] = *(const llima_u32x4*)(xb + i * 4096 + o);
+                    };
+                    read(0);
+#pragma unroll
+                    for (int e = 0; e < NE; ++e) {
+                        if (e + 1 < NE) read(e + 1);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            lmh_b8 wv[VB], xv[MB];
+#pragma unroll
+                            for (int v = 0; v < VB; ++v) wv[v] = q ? lmh8_wide(w[e & 1][v].z, w[e & 1][v].w) : lmh8_wide(w[e & 1][v].x, w[e & 1][v].y);
+#pragma unroll
+                            for (int i = 0; i < MB; ++i) xv[i] = q ? lmh8_wide(x[e & 1][i].z, x[e & 1][i].w) : lmh8_wide(x[e & 1][i].x, x[e & 1][i].y);
+#pragma unroll
+                            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                                for (int v = 0; v < VB; ++v) p[i][v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[v], xv[i], p[i][v], 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+#pragma unroll
+                        for (int v = 0; v < VB; ++v)
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) acc[i][v][k] = __builtin_fmaf(p[i][v][k], sc[i], acc[i][v][k]);
+                };
+                if (half) block(std::integral_constant<int, 2>{});
+                else block(std::integral_constant<int, 4>{});
+                slot = slot + 1 == S ? 0 : slot + 1;
+            }
+            if constexpr (K > 0) {                           // a pair of groups, then a pair of pairs
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if ((q & ((1 << k) - 1)) != (1 << k) - 1) continue;      // (compile time)
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+#pragma unroll
+                        for (int v = 0; v < VB; ++v)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) {
+                                if (q >> k & 1) {
+                                    acc[i][v][x] += low[k][i][v][x];
+                                } else {
+                                    low[k][i][v][x] = acc[i][v][x];
+                                    acc[i][v][x] = 0.0f;
+                                }
+                            }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int v = 0; v < VB; ++v)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) acc[i][v][k] = __builtin_fmaf(p[i][v][k], sc[i], acc[i][v][k]);
-        };
-        if (half) block(std::integral_constant<int, 2>{});
-        else block(std::integral_constant<int, 4>{});
-        if (end) {                                           // uniform
-            const int n = tile * LMH8_NV + wr * VB * 32;
-            if (n < V) {                                     // uniform
-#pragma unroll
-                for (int i = 0; i < MB; ++i) {
-                    float x[16 * VB];
-#pragma unroll
-                    for (int k = 0; k < 16 * VB; ++k) x[k] = acc[i][k >> 4][k & 15];
-                    lmh8_slot_out<16 * VB, SC>(P, x, best[i], b0 + mc[i], m[i] < nb, n, V, g);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int v = 0; v < VB; ++v)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) acc[i][v][k] = 0.0f;
         }
-        c = cn;
-        tile = tn;
-        slot = slot + 1 == S ? 0 : slot + 1;
+        const int n = tile * LMH8_NV + wr * VB * 32;
+        if (n < V) {                                         // uniform
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                float x[16 * VB];
+#pragma unroll
+                for (int k = 0; k < 16 * VB; ++k) x[k] = acc[i][k >> 4][k & 15];
+                lmh8_slot_out<16 * VB, SC>(P, x, best[i], b0 + mc[i], m[i] < nb, n, V, g);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int v = 0; v < VB; ++v)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[i][v][k] = 0.0f;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no request outlives the workgroup
 #pragma unroll
@@ -372,11 +411,14 @@ static int lmh8_run(Lmh8Params& Q, hipStream_t st) {
     LmhParams& P = Q.P;
     P.NW = lmh8_slots(P.B, P.V);
     const dim3 g((uint32_t)lmh8_groups(P.V)), blk(512);
+    const bool apart = P.H >= 4096 && P.B <= 64;              // K = 2
     for (int b0 = 0; b0 < P.B; b0 += 128) {
         const int nb = P.B - b0 < 128 ? P.B - b0 : 128;
-        if (P.B <= 32) hipLaunchKernelGGL((lmh8_tiles<8, 1, 1, 1, 4, SC>), g, blk, 0, st, Q, b0, nb);
-        else if (nb <= 64) hipLaunchKernelGGL((lmh8_tiles<4, 2, 2, 1, 4, SC>), g, blk, 0, st, Q, b0, nb);
-        else hipLaunchKernelGGL((lmh8_tiles<4, 2, 2, 2, 3, SC>), g, blk, 0, st, Q, b0, nb);
+        if (P.B <= 32 && apart) hipLaunchKernelGGL((lmh8_tiles<8, 1, 1, 1, 4, 2, SC>), g, blk, 0, st, Q, b0, nb);
+        else if (P.B <= 32) hipLaunchKernelGGL((lmh8_tiles<8, 1, 1, 1, 4, 0, SC>), g, blk, 0, st, Q, b0, nb);
+        else if (apart) hipLaunchKernelGGL((lmh8_tiles<4, 2, 2, 1, 4, 2, SC>), g, blk, 0, st, Q, b0, nb);
+        else if (nb <= 64) hipLaunchKernelGGL((lmh8_tiles<4, 2, 2, 1, 4, 0, SC>), g, blk, 0, st, Q, b0, nb);
+        else hipLaunchKernelGGL((lmh8_tiles<4, 2, 2, 2, 3, 0, SC>), g, blk, 0, st, Q, b0, nb);
     }
     if (SC) hipLaunchKernelGGL(lmh_score_finish, dim3((uint32_t)P.B), dim3(LLIMA_WG), 0, st, P);
     else hipLaunchKernelGGL(lmh_finish, dim3((uint32_t)P.B), dim3(LLIMA_WG), 0, st, P);

@@ -255,3 +255,29 @@ def test_two_graphs_on_one_stream_have_their_own_scratch(gpu):
         for (gr, out, _, _), e in zip(graphs, eager):
             assert torch.equal(out[0], e[0]) and torch.equal(out[1], e[1])
         llima_amd.lm_head_argmax(llima_amd.Fp8Rows(*a[:2]), llima_amd.Fp8LmHead(*a[2:]))
+
+
+@pytest.mark.parametrize("B", [1, 32, 33, 64, 65, 128, 140, 200])
+@pytest.mark.parametrize("H", [64, 320, 512, 1984, 4096])
+def test_equal_rows_have_equal_logits(gpu, B, H):
+    """Equal weight rows under equal scales, 256 rows apart over the whole vocabulary: the same bits wherever a row lies, so
+    the lowest id wins; a part of the vocabulary gives the whole's logits, and equal hidden rows of a batch equal ones."""
+    import llima_amd
+    T = 36
+    xq, xs, wq, ws = make(B, H, 256, B + H, gpu)
+    xq.view(torch.uint8)[-1], xs[-1] = xq.view(torch.uint8)[0], xs[0]
+    rows = llima_amd.Fp8Rows(xq, xs)
+    whole = llima_amd.Fp8LmHead(wq.view(torch.uint8).repeat(T, 1).view(F8), ws.repeat(T, 1))
+    for ld in ("f32", "bf16"):
+        ids, vals, logits = llima_amd.lm_head_argmax(rows, whole, return_logits=True, logit_dtype=ld)
+        first = logits[:, :256]
+        assert torch.equal(logits.view(B, T, 256), first[:, None].expand(B, T, 256))
+        assert torch.equal(logits[0], logits[-1])
+        lowest = torch.where(first == first.amax(1, keepdim=True), torch.arange(256, device=gpu), 256).amin(1)
+        assert torch.equal(ids.long(), lowest)
+        part = llima_amd.lm_head_argmax(rows, llima_amd.Fp8LmHead(wq, ws), return_logits=True, logit_dtype=ld)
+        assert torch.equal(part[2], first) and torch.equal(part[0], ids) and torch.equal(part[1], vals)
+        _, greedy = llima_amd.lm_head_score(rows, whole, ids, logit_dtype=ld)
+        assert greedy.all()
+        _, greedy = llima_amd.lm_head_score(rows, whole, ids + 256 * (T - 1), logit_dtype=ld)
+        assert not greedy.any()
