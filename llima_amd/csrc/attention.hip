@@ -51,6 +51,7 @@ struct AttnParams {
     int32_t page, pages;                                     // tokens of a page; pages of the cache
     uint32_t page_mul, page_shift;                           // j / page = j page_mul >> page_shift, j < 2^30
     int32_t slots, parts;                                    // partial sums per key head at most; shares of the keys
+    int32_t pairs;                                           // partial sums stand two to a share (at_slot)
     int32_t RG, RT;                                          // row groups, row tiles of a group
     float scale2;                                            // |scale| log2(e)
     int32_t flip;                                            // scale < 0
@@ -127,8 +128,8 @@ __device__ __forceinline__ int at_len(const AttnParams& P, int b, bool& bad) {
 
 // The partition of the keys: each sequence's are tiles of T, all sequences'
 // tiles stand in a row, and P.parts workgroups (per key head and row group)
-// take equal shares of it.  A share may hold parts of several sequences; part x
-// of sequence b leaves its sums in slot x + b, which no other pair has.
+// take equal shares of it.  A share may hold parts of several sequences (at_slot:
+// where a part leaves its sums).
 // at_tiles: sequence b's tiles; at_share: the length of a share (every lane of
 // a wave calls it and gets the same).  len0: the length of sequence lane.
 // A sequence counts for AT_EXTRA tiles more than it has, at its end: the time that
@@ -152,6 +153,14 @@ __device__ __forceinline__ int64_t at_share(const AttnParams& P, int len0) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
     return (total + P.parts - 1) / P.parts;
+}
+
+// The slot of the partial sums that share x has of sequence b (begins: from the
+// sequence's first tile on).  Slot x + b is one that no other pair has; with more
+// sequences than shares, two slots to a share: its first sequence may come from the
+// share before, its last may go on in the next, and the others it has whole.
+__device__ __forceinline__ int at_slot(int pairs, int x, int b, bool begins) {
+    return pairs ? 2 * x + (begins ? 1 : 0) : x + b;
 }
 
 // The sequence that has tile `at` of the row, its length, and its first tile's
@@ -608,7 +617,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
                 *(uint2*)(op + d * 32 + 2 * i) = make_uint2(at_pack<DT>(o[d][i] * inv, o[d][i + 1] * inv),
                                                             at_pack<DT>(o[d][i + 2] * inv, o[d][i + 3] * inv));
     } else {
-        const size_t at = ((size_t)(part + b) * A->Hkv + h) * A->R + row;
+        const size_t at = ((size_t)at_slot(A->pairs, part, b, j0 == 0) * A->Hkv + h) * A->R + row;
         if (g == 0) A->part_ml[at] = make_float2(m, l);
         float* op = A->part_o + at * D + 4 * g;
 #pragma unroll
@@ -648,12 +657,15 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
     const int x0 = (int)(first / share), np = (int)(last / share) - x0 + 1;
     if (np <= 1) return;                                     // the same for a row's waves
     const int h = hq / P.G, row = n * P.G + hq % P.G;
-    const size_t step = (size_t)P.Hkv * P.R, at0 = ((size_t)(x0 + b) * P.Hkv + h) * P.R + row;
+    const size_t slot = (size_t)P.Hkv * P.R, step = P.pairs ? 2 * slot : slot;
+    const size_t at1 = (size_t)at_slot(P.pairs, x0 + 1, b, false) * slot + (size_t)h * P.R + row;
+    const size_t at0 = (size_t)at_slot(P.pairs, x0, b, true) * slot + (size_t)h * P.R + row;
+    auto place = [&](int c) { return c == 0 ? at0 : at1 + (size_t)(c - 1) * step; };
     float m = -__builtin_inff(), l = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
     // the greatest maximum first (a lane per part), then one pass of weighted sums
-    for (int c = lane; c < np; c += 64) m = __builtin_fmaxf(m, P.part_ml[at0 + c * step].x);
+    for (int c = lane; c < np; c += 64) m = __builtin_fmaxf(m, P.part_ml[place(c)].x);
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, x, 64));
     const float mu = m > -__builtin_inff() ? m : 0.0f;
@@ -663,7 +675,7 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int c = c0 + i * WPR;
-            const size_t at = at0 + (c < np ? c : c0) * step;
+            const size_t at = place(c < np ? c : c0);
             ml[i] = P.part_ml[at];
 #pragma unroll
             for (int e = 0; e < E; ++e) po[i][e] = P.part_o[at * D + lane * E + e];
@@ -814,7 +826,8 @@ static void at_plan(AttnParams& P, int D) {
     P.R = P.N * P.G;
     P.RT = at_row_tiles(P.R, P.RG);
     P.parts = at_parts(P.Hkv, P.RG, P.RT, D);
-    P.slots = P.parts + P.B;
+    P.pairs = P.parts < P.B;
+    P.slots = P.pairs ? 2 * P.parts : P.parts + P.B;
 }
 
 extern "C" size_t llima_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq,

@@ -422,3 +422,25 @@ def test_commit_refuses_keys_inside_the_cache(gpu):
     k, v = kc[:, 10:13].clone(), vc[:, 10:13].clone()
     assert llima_amd.tree_commit(k, v, nodes, counts, kc, vc, lens).tolist() == [12, 12]
     assert torch.equal(kc[0, 11], k[0, 2]) and torch.equal(vc[1, 10], v[1, 1])
+
+
+@pytest.mark.parametrize("B,N,Hq,Hkv,D,page", [(40, 1, 64, 64, 64, 0), (21, 3, 128, 64, 64, 16), (30, 40, 64, 8, 128, 64),
+                                               (33, 2, 512, 512, 64, 0), (18, 9, 48, 24, 256, 5)])
+def test_more_sequences_than_shares(gpu, monkeypatch, B, N, Hq, Hkv, D, page):
+    """Batches above the number of shares, where partial sums stand two to a share: sequences that begin, end and lie inside a
+    share, or span several, and nothing written past the workspace's size."""
+    import llima_amd
+    from llima_amd import attention
+    lens = [(7 * b * b) % 500 for b in range(B)]
+    lens[3], lens[B // 2], lens[B - 1] = 9000, 0, 4000
+    s, g = make(gpu, B, N, Hq, Hkv, D, lens, page, seed=B)
+    bufs = []
+
+    def scratch(dev, kind, nbytes):
+        bufs.append((torch.full((nbytes + 4096,), 0x7F, dtype=torch.uint8, device=dev), nbytes))
+        return bufs[-1][0][:nbytes]
+    monkeypatch.setattr(attention, "_scratch", scratch)
+    mask = tree_mask(g, B, N).to(gpu)
+    check(llima_amd.tree_attention(tree_mask=mask, **s), s, mask)
+    buf, n = bufs[0]
+    assert (buf[n:] == 0x7F).all()

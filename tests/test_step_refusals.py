@@ -259,3 +259,13 @@ def test_argmax_over_an_8_bit_head_takes_rows(shape):
     if x.dim():
         with pytest.raises(ValueError):
             llima_amd.lm_head_argmax(x, torch.zeros(100, 64, dtype=torch.bfloat16))
+
+
+def test_attention_workspace_is_bounded_by_the_shares():
+    """A share of the keys leaves the parts of two sequences at most, its first and its last: the workspace stops growing with
+    the batch (8 key heads of 264 rows: two row groups, 16 shares)."""
+    l = L()
+    size = [l.llima_tree_attention_workspace_bytes(B, 33, 64, 8, 128) for B in (1, 8, 16, 32, 64, 1024, 4096)]
+    row = 33 * 64 * (128 + 2) * 4
+    assert size[0] < size[1] <= 2 * size[0]
+    assert size[3:] == [size[3]] * 4 and size[3] <= 64 * row + 256
