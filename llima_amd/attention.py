@@ -45,14 +45,27 @@ def _in_place(t: torch.Tensor, name: str) -> torch.Tensor:
 
 
 def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the spans of memory from the first to the last value of two tensors meet."""
-    pa, pb = a.data_ptr(), b.data_ptr()
-    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or not a.numel() or not b.numel():
+    """Whether two tensors may have memory in common: False where their strides show that they
+    have none.  Either the spans from their first to their last value do not meet, or, for one of
+    the strides, the places of a's values modulo that stride (an interval) are not those of b's,
+    as in views that differ in one index or range of a dimension of a larger tensor."""
+    if not a.numel() or not b.numel():
         return False
 
-    def end(t):
-        return t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    return pa < end(b) and pb < end(a)
+    def span(t, period=0):
+        return t.element_size() * (1 + sum([(n - 1) * s for n, s in zip(t.shape, t.stride())
+                                            if not period or s * t.element_size() % period]))
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa >= pb + span(b) or pb >= pa + span(a):
+        return False
+    for t in (a, b):
+        for n, s in zip(t.shape, t.stride()):
+            period = s * t.element_size()
+            if n > 1 and period:
+                d = (pb - pa) % period
+                if d >= span(a, period) and period - d >= span(b, period):
+                    return False
+    return True
 
 
 def _cache(k_cache, v_cache, Hkv, D, dtype, block_table, B, dev):
@@ -161,9 +174,10 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     [B, tokens, Hkv, D] or [pages, page_size, Hkv, D] (and the layers' dimension in front);
     bf16 or fp16, D a multiple of 8.  nodes int32 [B, L], counts int32 [B] (a row of
     Eagle3DraftTree's retrieve indices and the accept length + 1; arange and accepted_len + 1
-    for a chain).  k and v do not overlap the caches.  A sequence with a count, node, length or
-    page out of range, or no room for its path, is left as it is and its new length is -2
-    (LLIMA_E_RANGE).  Nothing waits for the device, and the call can be captured into a graph."""
+    for a chain).  k and v may stand beside the caches in one storage, but not in them.  A
+    sequence with a count, node, length or page out of range, or no room for its path, is left
+    as it is and its new length is -2 (LLIMA_E_RANGE).  Nothing waits for the device, and the
+    call can be captured into a graph."""
     if k.dim() == 4:
         if k_cache.dim() != 4 or v_cache.dim() != 4 or v.dim() != 4:
             raise ValueError("k and v [B, N, Hkv, D] need 4-dimensional caches")

@@ -444,3 +444,18 @@ def test_more_sequences_than_shares(gpu, monkeypatch, B, N, Hq, Hkv, D, page):
     check(llima_amd.tree_attention(tree_mask=mask, **s), s, mask)
     buf, n = bufs[0]
     assert (buf[n:] == 0x7F).all()
+
+
+def test_commit_of_drafts_behind_the_cached_tokens(gpu):
+    """One buffer per step: the drafts stand behind each sequence's cached tokens, K and V side by side."""
+    import llima_amd
+    buf = torch.randn(3, 2, 24, 2, 2, 64, device=gpu).to(torch.bfloat16)   # [layers, B, tokens + drafts, K or V, heads, D]
+    k, v, kc, vc = buf[:, :, 20:, 0], buf[:, :, 20:, 1], buf[:, :, :20, 0], buf[:, :, :20, 1]
+    want = buf.clone()
+    for b, (n, path) in enumerate(((3, [0, 2]), (17, [1, 2, 3]))):
+        for j, node in enumerate(path):
+            want[:, b, n + j] = buf[:, b, 20 + node]
+    nodes = torch.tensor([[0, 2, 0], [1, 2, 3]], dtype=torch.int32, device=gpu)
+    new = llima_amd.tree_commit(k, v, nodes, torch.tensor([2, 3], dtype=torch.int32, device=gpu), kc, vc,
+                                torch.tensor([3, 17], dtype=torch.int32, device=gpu))
+    assert new.tolist() == [5, 20] and torch.equal(buf, want)

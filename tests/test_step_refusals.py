@@ -269,3 +269,45 @@ def test_attention_workspace_is_bounded_by_the_shares():
     row = 33 * 64 * (128 + 2) * 4
     assert size[0] < size[1] <= 2 * size[0]
     assert size[3:] == [size[3]] * 4 and size[3] <= 64 * row + 256
+
+
+def offsets(t):
+    at = torch.zeros(t.shape, dtype=torch.int64) + t.storage_offset()
+    for d, (n, s) in enumerate(zip(t.shape, t.stride())):
+        at += (torch.arange(n) * s).view([-1 if i == d else 1 for i in range(t.dim())])
+    return set(at.flatten().tolist())
+
+
+def test_drafts_beside_the_cache_in_one_storage_are_apart():
+    """Drafted tokens behind or between the cached ones of the same storage, without a value in common, are not refused."""
+    from llima_amd.attention import _shared
+    bf = torch.bfloat16
+    buf = torch.empty(3, 2, 20 + 4, 2, 8, dtype=bf)           # [layers, B, tokens + drafts, heads, D]
+    assert not _shared(buf[:, :, 20:], buf[:, :, :20])
+    assert _shared(buf[:, :, 19:23], buf[:, :, :20]) and _shared(buf[1:2, :, 5:9], buf[:, :, :20])
+    assert not _shared(buf[:, :, 20:].transpose(2, 3), buf[:, :, :20]) and not _shared(buf[:1], buf[1:])
+    both = torch.empty(2, 24, 2, 2, 8, dtype=bf)              # K and V side by side per token
+    for k, c in ((0, 1), (1, 0)):
+        assert not _shared(both[:, 20:, k], both[:, :20, c]) and not _shared(both[:, 20:, k], both[:, :20, k])
+        assert not _shared(both[:, :, k], both[:, :, c]) and _shared(both[:, :, k], both[:, :, k])
+    heads = torch.empty(2, 6, 30, 8, dtype=bf)                # K's heads, then V's, tokens inside
+    assert not _shared(heads[:, :3].transpose(1, 2), heads[:, 3:].transpose(1, 2))
+    assert _shared(heads[:, :3].transpose(1, 2), heads[:, 2:5].transpose(1, 2))
+    assert not _shared(torch.empty(2, 3), torch.empty(2, 3)) and not _shared(buf[:, :0], buf)
+
+
+def test_whether_two_views_share_values_is_never_denied_wrongly():
+    from llima_amd.attention import _shared
+    g = torch.Generator().manual_seed(3)
+    base = torch.empty(4000, dtype=torch.bfloat16)
+    r = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))
+    apart = 0
+    for _ in range(3000):
+        views = []
+        for _ in range(2):
+            shape = [r(1, 5) for _ in range(3)]
+            views.append(base.as_strided(shape, [r(0, 60), r(0, 40), r(0, 12)], r(0, 400)))
+        common = bool(offsets(views[0]) & offsets(views[1]))
+        assert _shared(*views) or not common, views
+        apart += not _shared(*views)
+    assert apart > 100
