@@ -49,7 +49,9 @@ def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
     have none.  Either the spans from their first to their last value do not meet, or, for one of
     the strides, the places of a's values modulo that stride (an interval) are not those of b's,
     as in views that differ in one index or range of a dimension of a larger tensor."""
-    if not a.numel() or not b.numel():
+    sa, sb = a.untyped_storage(), b.untyped_storage()        # first, as the usual case: 0.6 us
+    ba, bb = sa.data_ptr(), sb.data_ptr()
+    if ba >= bb + sb.nbytes() or bb >= ba + sa.nbytes() or not a.numel() or not b.numel():
         return False
 
     def span(t, period=0):
