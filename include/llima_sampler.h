@@ -565,8 +565,9 @@ int llima_tree_attention(const llima_tree_attention_args* args, void* workspace,
  * page, token, head).  A sequence with a count outside [0, L], a node outside [0, N),
  * a length below 0, no room for its path or a page outside [0, pages) among those it
  * would write is left as it is, and new_lens[b] is LLIMA_E_RANGE.  Nothing else of
- * the cache is written.  new_lens may not be cache_lens; the caches may not overlap k
- * or v, and no two sequences may write to one page's token. */
+ * the cache is written.  new_lens may not be cache_lens; the caches may not overlap k,
+ * v or each other (nor themselves, by a stride of 0), and no two sequences may write to
+ * one page's token: the copies are made in no order. */
 typedef struct llima_tree_commit_args {
     const void *k, *v;
     void *k_cache, *v_cache;

@@ -70,6 +70,22 @@ def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+
+
+def _folded(t: torch.Tensor) -> bool:
+    """Whether values of a tensor may share memory: a stride less than what the smaller ones span."""
+    if t.is_contiguous():
+        return False
+    end = 1
+    for s, n in sorted([(s, n) for n, s in zip(t.shape, t.stride()) if n > 1]):
+        if s < end:
+            return t.numel() > 0
+        end += (n - 1) * s
+    return False
+
+
 def _cache(k_cache, v_cache, Hkv, D, dtype, block_table, B, dev):
     """Checks of a cache [..., page_size, Hkv, D] and its table -> (page size, pages, blocks per
     sequence, table)."""
@@ -176,10 +192,11 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     [B, tokens, Hkv, D] or [pages, page_size, Hkv, D] (and the layers' dimension in front);
     bf16 or fp16, D a multiple of 8.  nodes int32 [B, L], counts int32 [B] (a row of
     Eagle3DraftTree's retrieve indices and the accept length + 1; arange and accepted_len + 1
-    for a chain).  k and v may stand beside the caches in one storage, but not in them.  A
-    sequence with a count, node, length or page out of range, or no room for its path, is left
-    as it is and its new length is -2 (LLIMA_E_RANGE).  Nothing waits for the device, and the
-    call can be captured into a graph."""
+    for a chain).  k and v may stand beside the caches in one storage, but not in them, and the
+    caches not in each other (unless keys and values are the same tensors).  A sequence with a
+    count, node, length or page out of range, or no room for its path, is left as it is and its
+    new length is -2 (LLIMA_E_RANGE).  Nothing waits for the device, and the call can be captured
+    into a graph."""
     if k.dim() == 4:
         if k_cache.dim() != 4 or v_cache.dim() != 4 or v.dim() != 4:
             raise ValueError("k and v [B, N, Hkv, D] need 4-dimensional caches")
@@ -202,10 +219,15 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, k.dtype, block_table, B, dev)
     counts, lens = _ints(counts, B, "counts", dev), _ints(cache_lens, B, "cache_lens", dev)
     nodes = nodes if nodes.stride(1) == 1 or nodes.shape[1] == 1 else nodes.contiguous()
+    tied = _same(k, v)
     k, v = _heads(k), _heads(v)
     kc, vc = _in_place(k_cache, "k_cache"), _in_place(v_cache, "v_cache")
     if _shared(k, kc) or _shared(k, vc) or _shared(v, kc) or _shared(v, vc):
         raise ValueError("tree_commit: k and v must not overlap the caches (copy them first)")
+    if _folded(kc) or _folded(vc):
+        raise ValueError("tree_commit: a cache's own values must not overlap (expanded dimensions)")
+    if _shared(kc, vc) and not (tied and _same(kc, vc)):
+        raise ValueError("tree_commit: k_cache and v_cache must not overlap")
     new = torch.empty(B, dtype=torch.int32, device=dev)
     if B == 0:
         return new

@@ -311,3 +311,34 @@ def test_whether_two_views_share_values_is_never_denied_wrongly():
         assert _shared(*views) or not common, views
         apart += not _shared(*views)
     assert apart > 100
+
+
+def test_commit_refuses_caches_in_one_memory(monkeypatch):
+    """Two writes to one place in no order: K's and V's cache the same, or overlapping, or one that repeats its memory."""
+    import llima_amd
+    from llima_amd import attention
+    monkeypatch.setattr(attention, "_on_gpu", lambda *t: None)
+    launched = []
+    monkeypatch.setattr(attention, "lib", lambda: launched.append(1) or (_ for _ in ()).throw(AssertionError("launched")))
+    bf = torch.bfloat16
+    k, v = torch.zeros(2, 3, 4, 64, dtype=bf), torch.zeros(2, 3, 4, 64, dtype=bf)
+    c, o = torch.zeros(2, 10, 4, 64, dtype=bf), torch.zeros(2, 10, 4, 64, dtype=bf)
+    wide = torch.zeros(2, 15, 4, 64, dtype=bf)
+    p, m, n = torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    one = torch.zeros(1, 10, 4, 64, dtype=bf)
+    for kc, vc in ((c, c), (wide[:, :10], wide[:, 5:]), (one.expand(2, 10, 4, 64), o), (c, one.expand(2, 10, 4, 64)),
+                   (c, o[:, :, :1].expand(2, 10, 4, 64)), (o.view(-1).as_strided((2, 10, 4, 64), (2048, 128, 64, 1)), c)):
+        with pytest.raises(ValueError, match="overlap"):
+            llima_amd.tree_commit(k, v, p, m, kc, vc, n)
+    layers = torch.zeros(1, 2, 10, 4, 64, dtype=bf).expand(3, 2, 10, 4, 64)
+    k3 = torch.zeros(3, 2, 3, 4, 64, dtype=bf)
+    with pytest.raises(ValueError, match="overlap"):
+        llima_amd.tree_commit(k3, k3, p, m, layers, torch.zeros(3, 2, 10, 4, 64, dtype=bf), n)
+    assert not launched
+    both = torch.zeros(2, 10, 4, 128, dtype=bf)               # K and V of a head side by side, head-major caches, tied K and V
+    major = torch.zeros(2, 2, 4, 10, 64, dtype=bf).transpose(2, 3)
+    odd = torch.zeros(2, 3, 4, 65, dtype=bf)[..., 1:]         # (copied to aligned rows)
+    for kc, vc, w, x in ((both[..., :64], both[..., 64:], k, v), (major[0], major[1], k, v), (major[:, 0], major[:, 1], k, v),
+                         (c, c, k, k), (c, c, odd, odd)):
+        with pytest.raises((AssertionError, RuntimeError)):   # (past the checks: no GPU here)
+            llima_amd.tree_commit(w, x, p, m, kc, vc, n)
