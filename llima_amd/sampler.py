@@ -200,6 +200,8 @@ def _rows16(x: torch.Tensor, name: str) -> torch.Tensor:
     H = x.shape[-1]
     if H == 0 or H % 8 or H > 65536:
         raise ValueError(f"{name} needs rows of a multiple of 8 values (at most 65536)")
+    if x.numel() // H >= 1 << 31:
+        raise ValueError(f"{name} takes fewer than 2^31 rows")
     if x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0:
         return x if x.shape[0] != 1 else x.as_strided((1, H), (H, 1))
     x = x.reshape(-1, H)

@@ -342,3 +342,28 @@ def test_commit_refuses_caches_in_one_memory(monkeypatch):
                          (c, c, k, k), (c, c, odd, odd)):
         with pytest.raises((AssertionError, RuntimeError)):   # (past the checks: no GPU here)
             llima_amd.tree_commit(w, x, p, m, kc, vc, n)
+
+
+def test_more_rows_than_a_count_holds_are_refused(monkeypatch):
+    """2^32 + 5 rows of 8 (69 GB): the count given to the library has 32 bits, and 5 rows would be computed."""
+    import llima_amd
+    from llima_amd import sampler
+    monkeypatch.setattr(sampler, "_on_gpu", lambda *t: None)
+    counts = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: counts.append(ctypes.c_int32(a[2 if "quantize" in name else 4]).value) or 0
+    monkeypatch.setattr(sampler, "lib", Library)
+    monkeypatch.setattr(sampler, "_on", lambda dev: __import__("contextlib").nullcontext())
+    monkeypatch.setattr(sampler, "_stream", lambda dev: 0)
+    for rows in ((1 << 32) + 5, 1 << 31):
+        x = torch.empty(rows, 8, dtype=torch.bfloat16, device="meta")
+        w = torch.empty(8, dtype=torch.bfloat16, device="meta")
+        for call in (lambda: llima_amd.quantize_rows(x), lambda: llima_amd.add_rms_norm(x, w),
+                     lambda: llima_amd.add_rms_norm(x, w, x, out="fp8")):
+            with pytest.raises(ValueError, match="rows"):
+                call()
+    assert not counts
+    llima_amd.quantize_rows(torch.empty((1 << 31) - 1, 8, dtype=torch.bfloat16, device="meta"))
+    assert counts == [(1 << 31) - 1]
