@@ -200,6 +200,20 @@ __device__ __forceinline__ bool at_find(const AttnParams& P, int64_t at, int len
     return false;
 }
 
+// One over the sum l of a row's weights.  The largest weight is 1 (2^10 in fp16), so a sum of 0
+// is a row that sees nothing, which is 0, or one whose visible scores are all minus
+// infinity, which is NaN.
+template <class Params>
+__device__ __forceinline__ float at_inverse(const Params* P, float l, int b, int n, int len) {
+    if (l != 0.0f) return 1.0f / l;
+    bool sees = len > 0 || !P->mask;
+    for (int m = 0; m < P->N && !sees; ++m) {
+        const int64_t at = b * P->ms[0] + n * P->ms[1] + m;
+        sees = P->mask_f32 ? ((const float*)P->mask)[at] > 0.0f : ((const uint8_t*)P->mask)[at] != 0;
+    }
+    return sees ? __builtin_nanf("") : 0.0f;
+}
+
 __device__ __forceinline__ void at_dma(const void* src, uint8_t* dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                      (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
@@ -608,7 +622,7 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
     }
     if (flag[0]) l = __builtin_nanf("");
     if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing seen: 0
+        const float inv = at_inverse(A, l, b, n, len);
         uint16_t* op = (uint16_t*)A->out + b * A->os[0] + n * A->os[1] + hq * A->os[2] + 4 * g;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
@@ -653,7 +667,8 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
     }
-    const int64_t last = first + at_tiles<T>(P, b < 64 ? (int)readlane((uint32_t)len0, (uint32_t)b) : at_len(P, b, bad)) - 1 - AT_EXTRA;
+    const int len = b < 64 ? (int)readlane((uint32_t)len0, (uint32_t)b) : at_len(P, b, bad);
+    const int64_t last = first + at_tiles<T>(P, len) - 1 - AT_EXTRA;
     const int x0 = (int)(first / share), np = (int)(last / share) - x0 + 1;
     if (np <= 1) return;                                     // the same for a row's waves
     const int h = hq / P.G, row = n * P.G + hq % P.G;
@@ -703,7 +718,7 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
             o[e] = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = at_inverse(&P, l, b, n, len);
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= inv;
     uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + lane * E;

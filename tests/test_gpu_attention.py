@@ -459,3 +459,28 @@ def test_commit_of_drafts_behind_the_cached_tokens(gpu):
     new = llima_amd.tree_commit(k, v, nodes, torch.tensor([2, 3], dtype=torch.int32, device=gpu), kc, vc,
                                 torch.tensor([3, 17], dtype=torch.int32, device=gpu))
     assert new.tolist() == [5, 20] and torch.equal(buf, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [0, 5, 6000])
+def test_scores_that_are_all_minus_infinity(gpu, n, dtype):
+    """The softmax over visible scores of minus infinity alone is NaN, as by the formula (0 / 0), not the 0 of a row that sees
+    nothing; beside a finite score they weigh nothing."""
+    import llima_amd
+    s, g = make(gpu, 2, 4, 4, 2, 64, [n, n], 0, dtype, seed=n + 1)
+    mask = tree_mask(g, 2, 4).to(gpu)
+    mask[1, 2] = False
+    s["q"][:, :, 0] = s["q"][:, :, 0].abs() + 1.0             # head 0 of key head 0: positive, times -inf
+    s["k"][0, :, 0, 7] = -math.inf
+    s["k_cache"][0, :n, 0, 7] = -math.inf
+    got = llima_amd.tree_attention(tree_mask=mask, **s)
+    ref, tol = definition(s, mask)
+    assert torch.isnan(ref[0, :, 0]).all() and torch.isnan(got[0, :, 0]).all()
+    assert torch.isfinite(got[1]).all() and ((got[1].double() - ref[1]).abs() <= tol[1] + 1e-30).all()
+    assert ((got[0, :, 2:].double() - ref[0, :, 2:]).abs() <= tol[0, :, 2:] + 1e-30).all()
+    if n == 0:
+        assert (got[1, 2] == 0).all()
+    s["k"][0, 0, 0, 7] = 0.5                                  # node 0, which all see, has a finite score
+    got = llima_amd.tree_attention(tree_mask=mask, **s)
+    want = s["v"][0, 0, 0].expand(4, 64)
+    assert torch.equal(got[0, :, 0], want)
