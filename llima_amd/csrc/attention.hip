@@ -645,9 +645,9 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
 }
 
 // Joins the parts of each row (a sequence's node and query head), WPR waves a
-// row, which take every WPR-th part each in rounds of 8 loads.  Four waves where rows
-// are few (512 rows of 44 parts 7.4 -> 6.0 us), one where they fill the device
-// (12288 rows: 33 us with four, 11 with one).
+// row, which take every WPR-th part each in rounds of 8 loads.  Four waves up to 1024 rows,
+// one where they fill the device (the call, 16 nodes over 8192 tokens, four / one: 512 rows
+// 26.8 / 29.0 us, 1024 30.3 / 31.5, 2048 40.6 / 38.6, 4096 76.4 / 70.3, 12288 203 / 179).
 template <int DT, int D, int T, int WPR>
 __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
     constexpr int E = D / 64;                                // values per lane
@@ -814,7 +814,7 @@ static void at_launch(const AttnParams& P, hipStream_t st) {
         hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8, GEN>), g, dim3(512), 0, st, P);
     }
     const int64_t rows = (int64_t)P.B * P.N * P.Hq;
-    if (rows <= 2048) hipLaunchKernelGGL((tree_attn_join<DT, D, T, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, P);
+    if (rows <= 1024) hipLaunchKernelGGL((tree_attn_join<DT, D, T, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, P);
     else hipLaunchKernelGGL((tree_attn_join<DT, D, T, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, P);
 }
 
@@ -952,8 +952,9 @@ extern "C" int llima_tree_commit(const llima_tree_commit_args* a, void* stream) 
     P.cap = a->pages > 0 ? (int64_t)a->page_size * a->max_blocks : 0;
     P.B = a->B; P.N = a->N; P.L = a->L; P.Hkv = a->Hkv; P.U = a->D / 8;
     P.page = a->page_size; P.pages = a->pages;
-    // a layer to a workgroup where there are few, 8 where they fill the device
-    // (64 paths in 32 layers: 36 us with one)
+    // a layer to a workgroup where there are few, 8 where they fill the device (one / 8
+    // layers: 1280 and 4096 tokens' layers 17.1 / 17.0 us and 17.3 / 17.2, 8192 19.1 / 17.3,
+    // 16384 33.1 / 19.7)
     const int per = (int64_t)a->B * a->L * a->layers <= 2048 ? 1 : 8;
     hipLaunchKernelGGL(tree_commit, dim3((uint32_t)(a->B * a->L), (uint32_t)((a->layers + per - 1) / per)),
                        dim3(LLIMA_WG), 0, (hipStream_t)stream, P, a->layers, per);
