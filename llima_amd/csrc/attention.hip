@@ -15,8 +15,10 @@
 // order is the one the lane holds (16 s + e % 4 + 8 (e / 4) + 4 g for element e of
 // half g), and V is read from LDS through the transposing loads in that order.
 // P is rounded to the cache's type for that product (by 2^-8 of a weight at most
-// in bf16, 2^-11 in fp16: the precision of the values it multiplies); the row's
-// sum takes the weights before the rounding.  In fp16 the weights carry a factor
+// in bf16, 2^-11 in fp16: the precision of the values it multiplies; the outputs' error
+// grows by 4 to 10 % by it, and each weight in two parts, which avoids that, takes 532 ->
+// 665 us for 33 nodes over 4 x 131072 tokens); the row's sum takes the weights before the
+// rounding.  In fp16 the weights carry a factor
 // of 2^10, so that they become subnormal below 2^-24 of the row's largest.
 //
 // Bound: reading K and V once for all N Hq / Hkv rows of a key head.  Up to 128 such
@@ -25,7 +27,8 @@
 // is added, and as long with the products left out); some 25 us are the call's start, the
 // masked tile, the partial sums and the join.  From five row tiles on the waves' chain
 // of LDS reads, product, softmax and product bounds (4 x 131072 tokens, 33 nodes: 2.15 GB in
-// 555 us, requests alone 408).
+// 528-552 us, requests alone 408).  Heads of 256 with five row tiles and more spill 64 to 69
+// registers.
 #include <type_traits>
 
 #include "common.hpp"

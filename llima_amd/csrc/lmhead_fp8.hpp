@@ -181,11 +181,12 @@ __device__ __forceinline__ void lmh8_slot_out(const LmhParams& P, float (&x)[NX]
 // Shapes <RWV, VB, CWV, MB, S>: <8, 1, 1, 1, 4> up to 32 rows, <4, 2, 2, 1, 4> up to 64,
 // <4, 2, 2, 2, 3> up to 128, and larger batches in passes of 128.  The waves' split along the
 // hidden rows halves what each converts of the weight; along the vocab rows alone
-// (8 waves) the LDS reads bound (64 / 128 rows 130 / 199 us against 101 / 151).
+// (8 waves) the LDS reads bound (64 / 128 rows 130 / 199 us, this 101 / 151 in that build).
 //
-// Bound: reading the weight up to 64 rows (H 4096, V 128256, 0.53 GB: 1 row 92 us,
-// 32 rows 96, 64 101; the requests alone 88), from 128 on (151, 500 rows 600) the issue of
-// the vector instructions that widen, scale and add.
+// Bound: reading the weight up to 64 rows (H 4096, V 128256, 0.53 GB: 1 row 94 us,
+// 32 rows 96, 64 106-112; the requests alone 88), from 128 on (155-160, 500 rows 630) the issue
+// of the vector instructions that widen, scale and add.  256 registers: 33 to 64 rows spill 3
+// (10 with SC), 65 and more 4 (19).
 #define LMH8_NV 256                    // vocab rows per tile
 #define LMH8_CUS 256                   // workgroups: one per CU (its LDS)
 
