@@ -105,6 +105,11 @@ SIGNATURES = {
     "llima_tree_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "llima_tree_attention": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
     "llima_tree_commit": (ctypes.c_int, [_vp, _vp]),
+    "llima_tree_attention_fp8_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "llima_tree_attention_fp8": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
+    "llima_cache_write_fp8": (ctypes.c_int, [_vp, _vp]),
+    "llima_cache_read_fp8": (ctypes.c_int, [_vp, _vp]),
+    "llima_sandwich_norm": (ctypes.c_int, [_vp, _vp]),
     "llima_topk": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i64, _i32, _vp, _vp, _vp]),
     "llima_eagle3_tree_bytes": (_sz, [_i32, _i32]),
     "llima_eagle3_tree_split_bytes": (_sz, [_i32, _i32, _i32]),
@@ -166,9 +171,50 @@ class TreeCommitArgsC(ctypes.Structure):
                                      "max_blocks")])
 
 
-# the same two as bytes in one call (a ctypes structure is filled field by field: 6 us)
+class TreeAttentionFp8ArgsC(ctypes.Structure):
+    """Mirror of llima_tree_attention_fp8_args."""
+    _fields_ = [("a", TreeAttentionArgsC), ("k_scales", _vp), ("v_scales", _vp),
+                ("k_scale_strides", _i64x3), ("v_scale_strides", _i64x3)]
+
+
+class CacheWriteFp8ArgsC(ctypes.Structure):
+    """Mirror of llima_cache_write_fp8_args."""
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_cache", "v_cache", "k_scales", "v_scales", "nodes",
+                                    "counts", "cache_lens", "block_table", "new_lens")] +
+                [(n, _i64x4) for n in ("k_strides", "v_strides", "k_cache_strides", "v_cache_strides",
+                                       "k_scale_strides", "v_scale_strides")] +
+                [("nodes_stride", _i64), ("table_stride", _i64)] +
+                [(n, _i32) for n in ("dtype", "layers", "B", "N", "L", "Hkv", "D", "page_size", "pages",
+                                     "max_blocks")])
+
+
+class CacheReadFp8ArgsC(ctypes.Structure):
+    """Mirror of llima_cache_read_fp8_args."""
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_cache", "v_cache", "k_scales", "v_scales",
+                                    "cache_lens", "block_table")] +
+                [(n, _i64x4) for n in ("k_strides", "v_strides", "k_cache_strides", "v_cache_strides",
+                                       "k_scale_strides", "v_scale_strides")] +
+                [("table_stride", _i64)] +
+                [(n, _i32) for n in ("dtype", "layers", "B", "L", "Hkv", "D", "page_size", "pages",
+                                     "max_blocks")])
+
+
+class SandwichNormArgsC(ctypes.Structure):
+    """Mirror of llima_sandwich_norm_args."""
+    _fields_ = ([(n, _vp) for n in ("x", "residual", "gate", "post_weight", "pre_weight", "out",
+                                    "out_scales", "out_residual")] +
+                [(n, _i64) for n in ("x_stride", "residual_stride", "gate_stride")] +
+                [(n, _i32) for n in ("dtype", "B", "H")] +
+                [(n, ctypes.c_float) for n in ("eps", "weight_offset", "residual_scale", "gate_scale")])
+
+
+# the same as bytes in one call (a ctypes structure is filled field by field: 6 us)
 TREE_ATTENTION_ARGS = struct.Struct("@9P3q3q3q3q3q3q2qq10if0q")
 TREE_COMMIT_ARGS = struct.Struct("@9P4q4q4q4q2q9i0q")
+TREE_ATTENTION_FP8_ARGS = struct.Struct("@9P3q3q3q3q3q3q2qq10if0q2P3q3q")
+CACHE_WRITE_FP8_ARGS = struct.Struct("@11P4q4q4q4q4q4q2q10i0q")
+CACHE_READ_FP8_ARGS = struct.Struct("@8P4q4q4q4q4q4qq9i0q")
+SANDWICH_NORM_ARGS = struct.Struct("@8P3q3i4f0q")
 
 _lib = None
 

@@ -2,10 +2,13 @@
 
   tree_attention(q, k, v, k_cache, v_cache, cache_lens, tree_mask, block_table)
   tree_commit(k, v, nodes, counts, k_cache, v_cache, cache_lens, block_table)
+  Fp8Cache(values, scales), cache_write(k, v, k_cache, v_cache, cache_lens, counts, block_table)
+  cache_read(k_cache, v_cache, cache_lens, block_table, dtype, tokens)
 
 The step of a draft tree around the token selection: the attention reads the mask
 that Eagle3DraftTree.finish makes, the commit keeps the path that verify_tree or
-lm_head_verify_tree accepted.  No counterpart in the reference, whose attention and
+lm_head_verify_tree accepted.  The caches are in 16 bits, or Fp8Cache: in e4m3 with a
+scale per token and head, quantised as they are written.  No counterpart in the reference, whose attention and
 caches are on the NPU.
 """
 from __future__ import annotations
@@ -18,30 +21,82 @@ from . import _lib
 from ._lib import check, lib
 from .sampler import FLOAT_CODES, _on, _on_gpu, _scratch, _stream
 
-__all__ = ["tree_attention", "tree_commit"]
+__all__ = ["Fp8Cache", "cache_read", "cache_write", "tree_attention", "tree_commit"]
 
 
-def _heads(t: torch.Tensor) -> torch.Tensor:
+class Fp8Cache:
+    """The keys or the values of an 8-bit KV cache: `values` float8_e4m3fn [..., tokens, Hkv, D]
+    (D 64, 128 or 256) and `scales` float32 [..., tokens, Hkv], one per token and head: a head's
+    row is values * scales.  In front stand B or, with a block table, pages, and in front of those
+    the layers where every layer's cache is one tensor; cache[i] is layer i's.  tree_attention,
+    tree_commit, cache_write and cache_read take it; a scale is max(max |x|, 2^-100) / 448 of the
+    row that was written.  Strides are free where values of a head are adjacent; `empty` gives
+    the order that is read fastest."""
+    __slots__ = ("values", "scales")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+            raise ValueError("Fp8Cache: values must be float8_e4m3fn and scales float32")
+        if values.dim() < 4 or values.shape[:-1] != scales.shape or values.shape[-1] not in (64, 128, 256):
+            raise ValueError("Fp8Cache: values [..., tokens, Hkv, D], D 64, 128 or 256, and scales [..., tokens, Hkv] are needed")
+        _on_gpu(values, scales)
+        if values.device != scales.device:
+            raise ValueError("Fp8Cache: values and scales must be on one device")
+        self.values, self.scales = values, scales
+
+    @classmethod
+    def empty(cls, *shape: int, device=None) -> "Fp8Cache":
+        """A cache [..., tokens, Hkv, D] whose values are not set; in memory a head's tokens follow
+        each other: [..., Hkv, tokens, D]."""
+        if len(shape) < 4:
+            raise ValueError("Fp8Cache.empty takes [..., tokens, Hkv, D]")
+        n = (*shape[:-3], shape[-2], shape[-3])
+        dev = device if device is not None else "cuda"
+        return cls(torch.empty((*n, shape[-1]), dtype=torch.float8_e4m3fn, device=dev).transpose(-3, -2),
+                   torch.empty(n, dtype=torch.float32, device=dev).transpose(-2, -1))
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    def dim(self) -> int:
+        return self.values.dim()
+
+    def __getitem__(self, layer) -> "Fp8Cache":
+        if self.values.dim() < 5:
+            raise ValueError("Fp8Cache: only a cache of layers is indexed")
+        return Fp8Cache(self.values[layer], self.scales[layer])
+
+
+def _heads(t: torch.Tensor, align: int = 8) -> torch.Tensor:
     """[..., D] that 16-byte accesses can read: D adjacent, the other strides multiples
-    of 8 and not negative, 16-byte aligned (copied when it is not)."""
-    if t.is_contiguous() and t.shape[-1] % 8 == 0 and t.data_ptr() % 16 == 0:
+    of 8 (of 16 for bytes) and not negative, 16-byte aligned (copied when it is not)."""
+    if t.is_contiguous() and t.shape[-1] % align == 0 and t.data_ptr() % 16 == 0:
         return t
     st = t.stride()
     if st[-1] == 1 and t.data_ptr() % 16 == 0:
-        if not any([s % 8 for s in st[:-1]]):
+        if not any([s % align for s in st[:-1]]):
             return t
-        if not any([s % 8 and n > 1 for s, n in zip(st[:-1], t.shape[:-1])]):
+        if not any([s % align and n > 1 for s, n in zip(st[:-1], t.shape[:-1])]):
             return t.as_strided(t.shape, [0 if n <= 1 else s for s, n in zip(st[:-1], t.shape[:-1])] + [1])
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _in_place(t: torch.Tensor, name: str) -> torch.Tensor:
+def _in_place(t: torch.Tensor, name: str, align: int = 8) -> torch.Tensor:
     """A cache as the kernels can use it where it is (it is never copied)."""
-    h = _heads(t)
+    h = _heads(t, align)
     if h is not t and h.data_ptr() != t.data_ptr():
-        raise ValueError(f"{name}: head values must be adjacent, other strides multiples of 8, "
+        raise ValueError(f"{name}: head values must be adjacent, other strides multiples of {align}, "
                          "and the first 16-byte aligned")
     return h
+
+
+def _eight_bits(k_cache, v_cache) -> bool:
+    """Whether both caches are Fp8Cache; one alone is refused."""
+    f = isinstance(k_cache, Fp8Cache)
+    if f != isinstance(v_cache, Fp8Cache):
+        raise ValueError("k_cache and v_cache must both be tensors, or both Fp8Cache")
+    return f
 
 
 def _shared(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -125,7 +180,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
 
     q [B, N, Hq, D], k and v [B, N, Hkv, D] (the drafted tokens' own, not in the cache yet;
     Hq a multiple of Hkv), bf16 or fp16, D 64, 128 or 256.  k_cache, v_cache: [B, tokens, Hkv,
-    D], or pages [pages, page_size, Hkv, D] with block_table int32 [B, blocks]; cache_lens
+    D], or pages [pages, page_size, Hkv, D] with block_table int32 [B, blocks], of q's type or
+    both Fp8Cache (llima_tree_attention_fp8); cache_lens
     int32 [B]: the cached tokens, which every node sees.  tree_mask [N, N] or [B, N, N],
     bool (or uint8, nonzero) or float32 (above 0, as Eagle3DraftTree.finish's): node n sees
     drafted token m where mask[n, m]; None: m <= n, the chain of drafts, or with N = 1 a
@@ -133,6 +189,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     range is NaN.  scale defaults to D^-0.5.  Strides are free where values of a head are
     adjacent (head-major caches as transposed views).  Nothing waits for the device, and the
     call can be captured into a graph."""
+    k8 = v8 = None
+    if _eight_bits(k_cache, v_cache):
+        k8, v8, k_cache, v_cache = k_cache.scales, v_cache.scales, k_cache.values, v_cache.values
     if q.dim() != 4 or k.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("q [B, N, Hq, D], k and v [B, N, Hkv, D] and 4-dimensional caches are needed")
     B, N, Hq, D = q.shape
@@ -149,7 +208,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     dev = q.device
     if not (k.device == v.device == k_cache.device == v_cache.device == dev):
         raise ValueError("tree_attention: tensors must be on one device")
-    page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, q.dtype, block_table, B, dev)
+    page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, q.dtype if k8 is None else torch.float8_e4m3fn,
+                                        block_table, B, dev)
     lens = _ints(cache_lens, B, "cache_lens", dev)
     mask, mask_dtype, ms = tree_mask, _lib.LLIMA_MASK_U8, (0, 0)
     if mask is not None:
@@ -163,21 +223,28 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
             mask_dtype = _lib.LLIMA_MASK_F32
         ms = (mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
     q, k, v = _heads(q), _heads(k), _heads(v)
-    kc, vc = _in_place(k_cache, "k_cache"), _in_place(v_cache, "v_cache")
+    align = 8 if k8 is None else 16
+    kc, vc = _in_place(k_cache, "k_cache", align), _in_place(v_cache, "v_cache", align)
     out = torch.empty((B, N, Hq, D), dtype=q.dtype, device=dev)
     if B == 0:
         return out
     L = lib()
-    ws = _scratch(dev, "tree_attention", L.llima_tree_attention_workspace_bytes(B, N, Hq, Hkv, D))
+    ws = _scratch(dev, "tree_attention", (L.llima_tree_attention_workspace_bytes if k8 is None else
+                                          L.llima_tree_attention_fp8_workspace_bytes)(B, N, Hq, Hkv, D))
     # a table of no blocks is not read
     tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
-    a = _lib.TREE_ATTENTION_ARGS.pack(
+    args = (
         q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), lens.data_ptr(),
         0 if mask is None else mask.data_ptr(), tp, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
         *out.stride()[:3], *kc.stride()[:3], *vc.stride()[:3], *ms, ts, FLOAT_CODES[q.dtype], mask_dtype, B, N, Hq,
         Hkv, D, page, pages, blocks, D ** -0.5 if scale is None else float(scale))
     with _on(dev):
-        check(L.llima_tree_attention(a, ws.data_ptr(), ws.numel(), _stream(dev)), "llima_tree_attention")
+        if k8 is None:
+            check(L.llima_tree_attention(_lib.TREE_ATTENTION_ARGS.pack(*args), ws.data_ptr(), ws.numel(), _stream(dev)),
+                  "llima_tree_attention")
+        else:
+            a = _lib.TREE_ATTENTION_FP8_ARGS.pack(*args, k8.data_ptr(), v8.data_ptr(), *k8.stride(), *v8.stride())
+            check(L.llima_tree_attention_fp8(a, ws.data_ptr(), ws.numel(), _stream(dev)), "llima_tree_attention_fp8")
     return out
 
 
@@ -190,13 +257,18 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
 
     k, v [B, N, Hkv, D] or, for every layer at once, [layers, B, N, Hkv, D], with caches
     [B, tokens, Hkv, D] or [pages, page_size, Hkv, D] (and the layers' dimension in front);
-    bf16 or fp16, D a multiple of 8.  nodes int32 [B, L], counts int32 [B] (a row of
+    bf16 or fp16, D a multiple of 8; or both Fp8Cache, which the path is quantised into
+    (llima_cache_write_fp8).  nodes int32 [B, L], counts int32 [B] (a row of
     Eagle3DraftTree's retrieve indices and the accept length + 1; arange and accepted_len + 1
     for a chain).  k and v may stand beside the caches in one storage, but not in them, and the
     caches not in each other (unless keys and values are the same tensors).  A sequence with a
     count, node, length or page out of range, or no room for its path, is left as it is and its
     new length is -2 (LLIMA_E_RANGE).  Nothing waits for the device, and the call can be captured
     into a graph."""
+    if _eight_bits(k_cache, v_cache):
+        if nodes.dim() != 2 or nodes.shape[1] == 0 or nodes.dtype != torch.int32:
+            raise ValueError("nodes must be int32 [B, L], L at least 1")
+        return _write8("tree_commit", k, v, k_cache, v_cache, cache_lens, nodes, counts, block_table)
     if k.dim() == 4:
         if k_cache.dim() != 4 or v_cache.dim() != 4 or v.dim() != 4:
             raise ValueError("k and v [B, N, Hkv, D] need 4-dimensional caches")
@@ -239,3 +311,125 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     with _on(dev):
         check(lib().llima_tree_commit(a, _stream(dev)), "llima_tree_commit")
     return new
+
+
+def _layers(k_cache: Fp8Cache, v_cache: Fp8Cache, four: bool):
+    """Values and scales of both caches with the layers' dimension in front."""
+    ts = (k_cache.values, v_cache.values, k_cache.scales, v_cache.scales)
+    return [t[None] for t in ts] if four else ts
+
+
+def _write8(name, k, v, k_cache, v_cache, cache_lens, nodes, counts, block_table):
+    """Keys and values into an Fp8Cache (llima_cache_write_fp8)."""
+    four = k.dim() == 4
+    if (k.dim() != 5 and not four) or k_cache.dim() != k.dim() or v_cache.dim() != k.dim() or v.dim() != k.dim():
+        raise ValueError("k and v must be [B, N, Hkv, D] or [layers, B, N, Hkv, D], the caches likewise")
+    kq, vq, ks, vs = _layers(k_cache, v_cache, four)
+    if four:
+        k, v = k[None], v[None]
+    layers, B, N, Hkv, D = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("k and v must have one shape and type, bfloat16 or float16")
+    if kq.shape[0] != layers or vq.shape[0] != layers:
+        raise ValueError("k, v and the caches must have the same number of layers")
+    if N == 0 or Hkv == 0 or Hkv > 1024 or layers == 0 or layers > 65535:
+        raise ValueError("1 to 65535 layers, tokens, and 1 to 1024 heads are needed")
+    _on_gpu(k, v, nodes, counts, cache_lens, block_table)
+    dev = k.device
+    if not (v.device == kq.device == vq.device == dev):
+        raise ValueError(f"{name}: tensors must be on one device")
+    page, pages, blocks, table = _cache(kq, vq, Hkv, D, torch.float8_e4m3fn, block_table, B, dev)
+    lens = _ints(cache_lens, B, "cache_lens", dev)
+    if counts is not None:
+        counts = _ints(counts, B, "counts", dev)
+    L, ns = N, 0
+    if nodes is not None:
+        if nodes.shape[0] != B or nodes.device != dev:
+            raise ValueError("nodes must be int32 [B, L] on the cache's device")
+        nodes = nodes if nodes.stride(1) == 1 or nodes.shape[1] == 1 else nodes.contiguous()
+        L, ns = nodes.shape[1], nodes.stride(0)
+    tied = _same(k, v)
+    k, v = _heads(k), _heads(v)
+    kq, vq = _in_place(kq, "k_cache", 16), _in_place(vq, "v_cache", 16)
+    outs = (kq, vq, ks, vs)
+    if any([_shared(a, o) for a in (k, v) for o in outs]):
+        raise ValueError(f"{name}: k and v must not overlap the caches (copy them first)")
+    if any([_folded(o) for o in outs]):
+        raise ValueError(f"{name}: a cache's own values must not overlap (expanded dimensions)")
+    if not (tied and _same(kq, vq) and _same(ks, vs)) and (_shared(kq, vq) or _shared(ks, vs)) or \
+            _shared(kq, ks) or _shared(vq, vs) or _shared(kq, vs) or _shared(vq, ks):
+        raise ValueError(f"{name}: k_cache and v_cache, values and scales, must not overlap")
+    new = torch.empty(B, dtype=torch.int32, device=dev)
+    if B == 0:
+        return new
+    tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
+    a = _lib.CACHE_WRITE_FP8_ARGS.pack(
+        k.data_ptr(), v.data_ptr(), kq.data_ptr(), vq.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+        0 if nodes is None else nodes.data_ptr(), 0 if counts is None else counts.data_ptr(), lens.data_ptr(), tp,
+        new.data_ptr(), *k.stride()[:4], *v.stride()[:4], *kq.stride()[:4], *vq.stride()[:4], *ks.stride(), *vs.stride(),
+        ns, ts, FLOAT_CODES[k.dtype], layers, B, N, L, Hkv, D, page, pages, blocks)
+    with _on(dev):
+        check(lib().llima_cache_write_fp8(a, _stream(dev)), "llima_cache_write_fp8")
+    return new
+
+
+def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: Fp8Cache, v_cache: Fp8Cache, cache_lens: torch.Tensor,
+                counts: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Quantises the first counts[b] (None: all) of N new tokens' keys and values into 8-bit caches,
+    in place, behind the cache_lens[b] tokens that they hold (llima_cache_write_fp8), and returns the
+    new lengths int32 [B].  For prompts, chunks of them, and decoded tokens; tree_commit keeps an
+    accepted path.
+
+    k, v [B, N, Hkv, D] or [layers, B, N, Hkv, D], bf16 or fp16, D 64, 128 or 256; the caches
+    [B, tokens, Hkv, D] or pages [pages, page_size, Hkv, D] with block_table int32 [B, blocks] (and the
+    layers' dimension in front).  A sequence with a count outside [0, N], a length or page out of range,
+    or no room is left as it is and its new length is -2 (LLIMA_E_RANGE).  The caches may not overlap k,
+    v or each other, and no two sequences may write to one page's token.  Nothing waits for the
+    device, and the call can be captured into a graph."""
+    if not _eight_bits(k_cache, v_cache):
+        raise ValueError("cache_write takes Fp8Cache")
+    return _write8("cache_write", k, v, k_cache, v_cache, cache_lens, None, counts, block_table)
+
+
+def cache_read(k_cache: Fp8Cache, v_cache: Fp8Cache, cache_lens: torch.Tensor,
+               block_table: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
+               tokens: Optional[int] = None):
+    """The first `tokens` tokens (None: all that there is room for) of B sequences of 8-bit caches, in
+    16 bits and in order (llima_cache_read_fp8) -> keys and values [B, tokens, Hkv, D], or [layers, B,
+    tokens, Hkv, D] of caches with the layers' dimension: round(values * scales) of the cache_lens[b]
+    cached tokens, 0 behind them.  dtype bfloat16 or float16.  A sequence with a length or a page out
+    of range is NaN.  For programs that know no 8-bit cache.  Nothing waits for the device, and
+    the call can be captured into a graph."""
+    if not _eight_bits(k_cache, v_cache):
+        raise ValueError("cache_read takes Fp8Cache")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("cache_read gives bfloat16 or float16")
+    if k_cache.dim() not in (4, 5) or v_cache.shape != k_cache.shape:
+        raise ValueError("both caches must be [B, tokens, Hkv, D] or pages, with or without layers, of one shape")
+    four = k_cache.dim() == 4
+    kq, vq, ks, vs = _layers(k_cache, v_cache, four)
+    layers, Hkv, D = kq.shape[0], kq.shape[3], kq.shape[4]
+    if layers == 0 or layers > 65535 or Hkv == 0 or Hkv > 1024:
+        raise ValueError("1 to 65535 layers and 1 to 1024 heads are needed")
+    _on_gpu(cache_lens, block_table)
+    dev = kq.device
+    if vq.device != dev:
+        raise ValueError("cache_read: tensors must be on one device")
+    B = cache_lens.shape[0] if cache_lens.dim() == 1 else -1
+    page, pages, blocks, table = _cache(kq, vq, Hkv, D, torch.float8_e4m3fn, block_table, B, dev)
+    lens = _ints(cache_lens, B, "cache_lens", dev)
+    n = page * blocks if tokens is None else int(tokens)
+    if n < 0 or n > 1 << 30:
+        raise ValueError("0 to 2^30 tokens can be read")
+    kq, vq = _in_place(kq, "k_cache", 16), _in_place(vq, "v_cache", 16)
+    k = torch.empty((layers, B, n, Hkv, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if k.numel():
+        tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
+        a = _lib.CACHE_READ_FP8_ARGS.pack(
+            k.data_ptr(), v.data_ptr(), kq.data_ptr(), vq.data_ptr(), ks.data_ptr(), vs.data_ptr(), lens.data_ptr(), tp,
+            *k.stride()[:4], *v.stride()[:4], *kq.stride()[:4], *vq.stride()[:4], *ks.stride(), *vs.stride(), ts,
+            FLOAT_CODES[dtype], layers, B, n, Hkv, D, page, pages, blocks)
+        with _on(dev):
+            check(lib().llima_cache_read_fp8(a, _stream(dev)), "llima_cache_read_fp8")
+    return (k[0], v[0]) if four else (k, v)

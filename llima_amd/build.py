@@ -24,8 +24,9 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libllima_sampler.so")
 SOURCES = ["argmax.hip", "sample.hip", "verify.hip", "score.hip", "lmhead.hip", "tree.hip", "stop.hip",
-           "norm.hip", "attention.hip"]
+           "norm.hip", "sandwich.hip", "attention.hip", "attention_fp8.hip", "cache.hip"]
 HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "lmhead_fp8.hpp"),
+           os.path.join(CSRC, "attention.hpp"), os.path.join(CSRC, "norm.hpp"), os.path.join(CSRC, "quant.hpp"),
            os.path.join(ROOT, "include", "llima_sampler.h")]
 ARCH = os.environ.get("LLIMA_OFFLOAD_ARCH", "gfx950")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

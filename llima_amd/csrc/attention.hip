@@ -29,198 +29,9 @@
 // of LDS reads, product, softmax and product bounds (4 x 131072 tokens, 33 nodes: 2.15 GB in
 // 528-552 us, requests alone 408).  Heads of 256 with five row tiles and more spill 64 to 69
 // registers.
-#include <type_traits>
-
-#include "common.hpp"
-#include "../../include/llima_sampler.h"
+#include "attention.hpp"
 
 namespace llima {
-
-struct AttnParams {
-    const void *q, *k, *v, *kc, *vc;
-    void* out;
-    const int32_t* lens;                                     // [B]
-    const void* mask;                                        // [B][N][N] or null (m <= n)
-    const int32_t* table;                                    // [B][max_blocks] or null
-    float* part_o;                                           // [slots][Hkv][R][D]
-    float2* part_ml;                                         // [slots][Hkv][R]
-    int64_t qs[3], ks[3], vs[3], os[3];                      // batch, token and head strides (elements)
-    int64_t kcs[3], vcs[3];                                  // page, token and head strides
-    int64_t ms[2];                                           // mask: batch and row strides
-    int64_t ts;                                              // table row stride
-    int64_t cap;                                             // tokens a sequence has room for
-    int32_t mask_f32;
-    int32_t B, N, Hq, Hkv, G, R;                             // R = N G rows of a key head
-    int32_t page, pages;                                     // tokens of a page; pages of the cache
-    uint32_t page_mul, page_shift;                           // j / page = j page_mul >> page_shift, j < 2^30
-    int32_t slots, parts;                                    // partial sums per key head at most; shares of the keys
-    int32_t pairs;                                           // partial sums stand two to a share (at_slot)
-    int32_t RG, RT;                                          // row groups, row tiles of a group
-    float scale2;                                            // |scale| log2(e)
-    int32_t flip;                                            // scale < 0
-    int32_t mode;                                            // AT_TILE, AT_REQUEST or AT_LANE
-};
-
-#define AT_KEYS (1 << 30)              // keys of a sequence at most
-#define AT_TILE 0
-#define AT_REQUEST 1
-#define AT_LANE 2
-
-__device__ __forceinline__ uint32_t at_page(uint32_t mul, uint32_t shift, int j) {
-    return (uint32_t)(((uint64_t)(uint32_t)j * mul) >> shift);
-}
-
-// The kernel's arguments, loaded anew where they are used: held in registers
-// from the start, those of the parts that run seldom push out the others.
-typedef const __attribute__((address_space(4))) AttnParams* AttnArgs;
-__device__ __forceinline__ AttnArgs at_args() {
-    AttnArgs a = (AttnArgs)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(a));
-    return a;
-}
-
-__device__ __forceinline__ uint64_t readfirstlane64(uint64_t v) {
-    return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-           (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-}
-
-typedef float at_acc __attribute__((ext_vector_type(16)));
-typedef short at_s4 __attribute__((ext_vector_type(4)));
-typedef short at_s8 __attribute__((ext_vector_type(8)));
-
-template <int DT> __device__ __forceinline__ at_acc at_mfma(at_s8 a, at_s8 b, at_acc c) {
-    if constexpr (DT == LLIMA_BF16) {
-        typedef __bf16 t8 __attribute__((ext_vector_type(8)));
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
-    } else {
-        typedef _Float16 t8 __attribute__((ext_vector_type(8)));
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
-    }
-}
-
-// Two fp32 rounded to the type (to nearest, ties to even).
-template <int DT> __device__ __forceinline__ uint32_t at_pack(float a, float b) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    const f2 v = {a, b};
-    if constexpr (DT == LLIMA_BF16) {
-        typedef __bf16 t2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
-    } else {
-        typedef _Float16 t2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
-    }
-}
-
-template <int DT> __device__ __forceinline__ float at_f32(uint16_t h) {
-    if constexpr (DT == LLIMA_BF16) return __uint_as_float((uint32_t)h << 16);
-    else return (float)__builtin_bit_cast(_Float16, h);
-}
-
-// Exponent all ones: an infinity or NaN of the type.
-template <int DT> __device__ __forceinline__ bool at_special(uint16_t h) {
-    constexpr uint32_t e = DT == LLIMA_BF16 ? 0x7F80u : 0x7C00u;
-    return (h & e) == e;
-}
-
-// Sequence b's cached length; a length outside [0, cap] is 0 and bad.
-__device__ __forceinline__ int at_len(const AttnParams& P, int b, bool& bad) {
-    const int l = P.lens[b];
-    bad = l < 0 || l > P.cap;
-    return bad ? 0 : l;
-}
-
-// The partition of the keys: each sequence's are tiles of T, all sequences'
-// tiles stand in a row, and P.parts workgroups (per key head and row group)
-// take equal shares of it.  A share may hold parts of several sequences (at_slot:
-// where a part leaves its sums).
-// at_tiles: sequence b's tiles; at_share: the length of a share (every lane of
-// a wave calls it and gets the same).  len0: the length of sequence lane.
-// A sequence counts for AT_EXTRA tiles more than it has, at its end: the time that
-// its mask, its sums' exchange and the next sequence's start take (3 / 6 / 8: 24 ragged
-// sequences of up to 16384 tokens, 16 nodes, 151 / 140 / 140 us; 48 of up to 3000, one
-// node, 75 / 67 / 62; 100 of up to 500 49 / 52 / 59).
-#define AT_EXTRA 6
-template <int T>
-__device__ __forceinline__ int at_tiles(const AttnParams& P, int len) { return (len + P.N + T - 1) / T + AT_EXTRA; }
-
-template <int T>
-__device__ __forceinline__ int64_t at_share(const AttnParams& P, int len0) {
-    const int lane = (int)lane_id();
-    if (P.B == 1)                                            // uniform; a step of one stream waits for this
-        return ((uint32_t)__builtin_amdgcn_readfirstlane(at_tiles<T>(P, len0)) + (uint32_t)P.parts - 1u) / (uint32_t)P.parts;
-    int64_t total = lane < P.B ? at_tiles<T>(P, len0) : 0;
-    for (int b = 64 + lane; b < P.B; b += 64) {
-        bool bad;
-        total += at_tiles<T>(P, at_len(P, b, bad));
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
-    return (total + P.parts - 1) / P.parts;
-}
-
-// The slot of the partial sums that share x has of sequence b (begins: from the
-// sequence's first tile on).  Slot x + b is one that no other pair has; with more
-// sequences than shares, two slots to a share: its first sequence may come from the
-// share before, its last may go on in the next, and the others it has whole.
-__device__ __forceinline__ int at_slot(int pairs, int x, int b, bool begins) {
-    return pairs ? 2 * x + (begins ? 1 : 0) : x + b;
-}
-
-// The sequence that has tile `at` of the row, its length, and its first tile's
-// place in the row; false past the last tile.
-template <int T>
-__device__ __forceinline__ bool at_find(const AttnParams& P, int64_t at, int len0, int& b, int& len,
-                                        int64_t& first) {
-    const int lane = (int)lane_id();
-    if (P.B == 1) {                                          // uniform
-        b = 0;
-        len = __builtin_amdgcn_readfirstlane(len0);
-        first = 0;
-        return at < at_tiles<T>(P, len);
-    }
-    int64_t before = 0;
-    for (int b0 = 0; b0 < P.B; b0 += 64) {
-        bool bad;
-        const bool in = b0 + lane < P.B;
-        const int ln = !in ? 0 : b0 ? at_len(P, b0 + lane, bad) : len0;
-        const int64_t n = in ? at_tiles<T>(P, ln) : 0;
-        int64_t incl = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t up = __shfl_up(incl, o, 64);
-            incl += lane >= o ? up : 0;
-        }
-        const uint64_t past = ballot(in && before + incl > at);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            b = b0 + l;
-            first = before + (int64_t)readlane64((uint64_t)(incl - n), l);
-            len = (int)readlane((uint32_t)ln, l);
-            return true;
-        }
-        before += (int64_t)readlane64((uint64_t)incl, 63);
-    }
-    return false;
-}
-
-// One over the sum l of a row's weights.  The largest weight is 1 (2^10 in fp16), so a sum of 0
-// is a row that sees nothing, which is 0, or one whose visible scores are all minus
-// infinity, which is NaN.
-template <class Params>
-__device__ __forceinline__ float at_inverse(const Params* P, float l, int b, int n, int len) {
-    if (l != 0.0f) return 1.0f / l;
-    bool sees = len > 0 || !P->mask;
-    for (int m = 0; m < P->N && !sees; ++m) {
-        const int64_t at = b * P->ms[0] + n * P->ms[1] + m;
-        sees = P->mask_f32 ? ((const float*)P->mask)[at] > 0.0f : ((const uint8_t*)P->mask)[at] != 0;
-    }
-    return sees ? __builtin_nanf("") : 0.0f;
-}
-
-__device__ __forceinline__ void at_dma(const void* src, uint8_t* dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-}
 
 // Keys KEY + (0 .. 3, 8 .. 11) + 4 g of every block of 32 columns, by the transposing
 // loads from the lane's places.  In one piece with their wait: as builtins, the
@@ -286,17 +97,17 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
     const int part = (int)(blockIdx.x / (uint32_t)(P.Hkv * P.RG));
     bool bad = false;
     const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
-    const int64_t share = (int64_t)readfirstlane64((uint64_t)at_share<T>(P, len0));
+    const int64_t share = (int64_t)readfirstlane64((uint64_t)at_share<KeyTiles<T>>(P, len0));
     const int64_t end = (part + 1) * share;
     for (int64_t from = part * share; from < end;) {         // the share's sequences
     int b, len;
     int64_t first;
-    if (!at_find<T>(P, from, len0, b, len, first)) return;   // uniform: past the last tile
+    if (!at_find<KeyTiles<T>>(P, from, len0, b, len, first)) return;   // uniform: past the last tile
     b = __builtin_amdgcn_readfirstlane(b);
     len = __builtin_amdgcn_readfirstlane(len);
     first = (int64_t)readfirstlane64((uint64_t)first);
     const int nkeys = len + P.N;
-    const int64_t last = first + at_tiles<T>(P, len), upto = last < end ? last : end;
+    const int64_t last = first + KeyTiles<T>::count(P, len), upto = last < end ? last : end;
     const int64_t je = (upto - first) * T;
     const int j0 = (int)(from - first) * T, j1 = je < nkeys ? (int)je : nkeys;
     const bool whole = from == first && upto >= last - AT_EXTRA;   // the sequence has no other part
@@ -647,89 +458,6 @@ __global__ __launch_bounds__(64 * NW, (D == 256 || NW == 2) ? 1 : 2) void tree_a
 #endif
 }
 
-// Joins the parts of each row (a sequence's node and query head), WPR waves a
-// row, which take every WPR-th part each in rounds of 8 loads.  Four waves up to 1024 rows,
-// one where they fill the device (the call, 16 nodes over 8192 tokens, four / one: 512 rows
-// 26.8 / 29.0 us, 1024 30.3 / 31.5, 2048 40.6 / 38.6, 4096 76.4 / 70.3, 12288 203 / 179).
-template <int DT, int D, int T, int WPR>
-__global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
-    constexpr int E = D / 64;                                // values per lane
-    static_assert(WPR == 1 || WPR == LLIMA_WAVES, "one row or four to a workgroup");
-    __shared__ float so[WPR][D], sl[WPR];
-    const int lane = (int)lane_id(), sub = (int)wave_id() % WPR;
-    const int w = (int)(blockIdx.x * (LLIMA_WAVES / WPR) + wave_id() / WPR);
-    if (w >= P.B * P.N * P.Hq) return;                       // (WPR = 1)
-    const int b = w / (P.N * P.Hq), n = w / P.Hq % P.N, hq = w % P.Hq;
-    bool bad;
-    const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
-    const int64_t share = at_share<T>(P, len0);
-    int64_t first = 0;                                       // the sequence's first tile
-    if (b > 0) {                                             // uniform
-        first = lane < b ? at_tiles<T>(P, len0) : 0;
-        for (int i = 64 + lane; i < b; i += 64) first += at_tiles<T>(P, at_len(P, i, bad));
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
-    }
-    const int len = b < 64 ? (int)readlane((uint32_t)len0, (uint32_t)b) : at_len(P, b, bad);
-    const int64_t last = first + at_tiles<T>(P, len) - 1 - AT_EXTRA;
-    const int x0 = (int)(first / share), np = (int)(last / share) - x0 + 1;
-    if (np <= 1) return;                                     // the same for a row's waves
-    const int h = hq / P.G, row = n * P.G + hq % P.G;
-    const size_t slot = (size_t)P.Hkv * P.R, step = P.pairs ? 2 * slot : slot;
-    const size_t at1 = (size_t)at_slot(P.pairs, x0 + 1, b, false) * slot + (size_t)h * P.R + row;
-    const size_t at0 = (size_t)at_slot(P.pairs, x0, b, true) * slot + (size_t)h * P.R + row;
-    auto place = [&](int c) { return c == 0 ? at0 : at1 + (size_t)(c - 1) * step; };
-    float m = -__builtin_inff(), l = 0.0f, o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    // the greatest maximum first (a lane per part), then one pass of weighted sums
-    for (int c = lane; c < np; c += 64) m = __builtin_fmaxf(m, P.part_ml[place(c)].x);
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, x, 64));
-    const float mu = m > -__builtin_inff() ? m : 0.0f;
-    for (int c0 = sub; c0 < np; c0 += 8 * WPR) {
-        float2 ml[8];
-        float po[8][E];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = c0 + i * WPR;
-            const size_t at = place(c < np ? c : c0);
-            ml[i] = P.part_ml[at];
-#pragma unroll
-            for (int e = 0; e < E; ++e) po[i][e] = P.part_o[at * D + lane * E + e];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (c0 + i * WPR < np) {                         // uniform
-                const float a = __builtin_amdgcn_exp2f(ml[i].x - mu);
-                l += ml[i].y * a;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] += po[i][e] * a;
-            }
-        }
-    }
-    if constexpr (WPR > 1) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) so[sub][lane * E + e] = o[e];
-        if (lane == 0) sl[sub] = l;
-        __syncthreads();
-        if (sub != 0) return;
-        l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = lane * E + e;
-            o[e] = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
-        }
-    }
-    const float inv = at_inverse(&P, l, b, n, len);
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= inv;
-    uint16_t* op = (uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + lane * E;
-    if constexpr (E == 1) op[0] = (uint16_t)at_pack<DT>(o[0], 0.0f);
-#pragma unroll
-    for (int e = 0; e + 1 < E; e += 2) *(uint32_t*)(op + e) = at_pack<DT>(o[e], o[e + 1]);
-}
-
 struct CommitParams {
     const uint8_t *k, *v;
     uint8_t *kc, *vc;
@@ -817,8 +545,8 @@ static void at_launch(const AttnParams& P, hipStream_t st) {
         hipLaunchKernelGGL((tree_attn<DT, D, 8, 1, T, S8, GEN>), g, dim3(512), 0, st, P);
     }
     const int64_t rows = (int64_t)P.B * P.N * P.Hq;
-    if (rows <= 1024) hipLaunchKernelGGL((tree_attn_join<DT, D, T, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, P);
-    else hipLaunchKernelGGL((tree_attn_join<DT, D, T, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, P);
+    if (rows <= 1024) hipLaunchKernelGGL((tree_attn_join<DT, D, KeyTiles<T>, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, P);
+    else hipLaunchKernelGGL((tree_attn_join<DT, D, KeyTiles<T>, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, P);
 }
 
 template <int DT>
@@ -834,18 +562,12 @@ static int at_dispatch(const AttnParams& P, int D, hipStream_t st) {
 
 using namespace llima;
 
-static bool at_sizes_ok(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D) {
-    if (B < 0 || N <= 0 || N > 1024 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq > 1024) return false;
-    if (D != 64 && D != 128 && D != 256) return false;
-    return (int64_t)B * N * Hq < (1 << 26);                  // (the join's launch: fewer than 2^32 threads)
-}
 
 static void at_plan(AttnParams& P, int D) {
     P.R = P.N * P.G;
     P.RT = at_row_tiles(P.R, P.RG);
     P.parts = at_parts(P.Hkv, P.RG, P.RT, D);
-    P.pairs = P.parts < P.B;
-    P.slots = P.pairs ? 2 * P.parts : P.parts + P.B;
+    at_slots(P);
 }
 
 extern "C" size_t llima_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq,
@@ -854,72 +576,23 @@ extern "C" size_t llima_tree_attention_workspace_bytes(int32_t B, int32_t N, int
     AttnParams P = {};
     P.B = B; P.N = N; P.Hkv = Hkv; P.G = Hq / Hkv;
     at_plan(P, D);
-    const size_t rows = (size_t)P.slots * Hkv * P.R;
-    return (rows * D * sizeof(float) + 255) / 256 * 256 + rows * sizeof(float2);
-}
-
-// Strides are multiples of 8 elements (16 bytes), so every row is aligned as
-// its base pointer is.
-static bool at_strides_ok(const int64_t* s, int n) {
-    for (int i = 0; i < n; ++i)
-        if (s[i] < 0 || s[i] % 8 != 0) return false;
-    return true;
+    return at_parts_bytes(P, D);
 }
 
 extern "C" int llima_tree_attention(const llima_tree_attention_args* a, void* workspace,
                                     size_t workspace_bytes, void* stream) {
-    if (!a || !at_sizes_ok(a->B, a->N, a->Hq, a->Hkv, a->D)) return LLIMA_E_INVAL;
-    if (a->dtype != LLIMA_BF16 && a->dtype != LLIMA_F16) return LLIMA_E_INVAL;
-    if (!(a->scale == a->scale) || __builtin_isinf(a->scale)) return LLIMA_E_INVAL;
-    if (a->page_size <= 0 || a->pages < 0 || a->max_blocks < 0) return LLIMA_E_INVAL;
-    if (!a->block_table && (a->pages < a->B || a->max_blocks != 1)) return LLIMA_E_INVAL;
-    if ((int64_t)a->page_size * a->max_blocks + a->N > AT_KEYS) return LLIMA_E_INVAL;
-    if (a->mask_dtype != LLIMA_MASK_U8 && a->mask_dtype != LLIMA_MASK_F32) return LLIMA_E_INVAL;
-    if (!at_strides_ok(a->q_strides, 3) || !at_strides_ok(a->k_strides, 3) || !at_strides_ok(a->v_strides, 3) ||
-        !at_strides_ok(a->out_strides, 3) || !at_strides_ok(a->k_cache_strides, 3) ||
-        !at_strides_ok(a->v_cache_strides, 3))
-        return LLIMA_E_INVAL;
-    if (a->mask && (a->mask_strides[0] < 0 || a->mask_strides[1] < 0)) return LLIMA_E_INVAL;
-    if (a->block_table && a->table_stride < 0) return LLIMA_E_INVAL;
-    if (a->B == 0) return LLIMA_OK;
-    const bool cached = a->pages > 0 && a->max_blocks > 0;   // else no sequence may have a cached token
-    if (!a->q || !a->k || !a->v || !a->out || !a->cache_lens || (cached && (!a->k_cache || !a->v_cache)))
-        return LLIMA_E_INVAL;
-    const void* ptrs[] = {a->q, a->k, a->v, a->out, a->k_cache, a->v_cache};
-    for (const void* p : ptrs)
-        if ((uintptr_t)p % 16) return LLIMA_E_INVAL;
+    AttnParams P = {};
+    const int ok = at_fill(a, 8, P);
+    if (ok != LLIMA_OK || a->B == 0) return ok;
     if (!workspace || workspace_bytes < llima_tree_attention_workspace_bytes(a->B, a->N, a->Hq, a->Hkv, a->D))
         return LLIMA_E_WORKSPACE;
     if ((uintptr_t)workspace % 16) return LLIMA_E_INVAL;
-    AttnParams P = {};
-    P.q = a->q; P.k = a->k; P.v = a->v; P.kc = a->k_cache; P.vc = a->v_cache; P.out = a->out;
-    P.lens = a->cache_lens; P.mask = a->mask; P.table = a->block_table;
-    for (int i = 0; i < 3; ++i) {
-        P.qs[i] = a->q_strides[i]; P.ks[i] = a->k_strides[i]; P.vs[i] = a->v_strides[i];
-        P.os[i] = a->out_strides[i]; P.kcs[i] = a->k_cache_strides[i]; P.vcs[i] = a->v_cache_strides[i];
-    }
-    P.ms[0] = a->mask_strides[0]; P.ms[1] = a->mask_strides[1];
-    P.ts = a->table_stride;
-    P.cap = cached ? (int64_t)a->page_size * a->max_blocks : 0;
-    P.mask_f32 = a->mask_dtype == LLIMA_MASK_F32;
-    P.B = a->B; P.N = a->N; P.Hq = a->Hq; P.Hkv = a->Hkv; P.G = a->Hq / a->Hkv;
-    P.page = a->page_size; P.pages = a->pages;
-    // l = ceil(log2 page): mul = ceil(2^(30 + l) / page) <= 2^31 + 1 exceeds the
-    // quotient by less than page / 2^(30 + l) <= 2^-30 of j
-    uint32_t l = 0;
-    while ((1ll << l) < P.page) ++l;
-    P.page_mul = (uint32_t)(((1ull << (30 + l)) + P.page - 1) / (uint64_t)P.page);
-    P.page_shift = 30 + l;
-    P.scale2 = __builtin_fabsf(a->scale) * 1.44269504088896340736f;
-    P.flip = a->scale < 0.0f;
     // offsets within a tile (64 keys) or a request have 31 bits
     const int64_t ts = P.kcs[1] > P.vcs[1] ? P.kcs[1] : P.vcs[1];
     P.mode = ts <= (1 << 23) && (!P.table || P.page % 64 == 0) ? AT_TILE
            : ts <= (1 << 26) && (!P.table || P.page % 8 == 0) ? AT_REQUEST : AT_LANE;
     at_plan(P, a->D);
-    const size_t rows = (size_t)P.slots * P.Hkv * P.R;
-    P.part_o = (float*)workspace;
-    P.part_ml = (float2*)((uint8_t*)workspace + (rows * a->D * sizeof(float) + 255) / 256 * 256);
+    at_parts_at(P, a->D, workspace);
     return a->dtype == LLIMA_BF16 ? at_dispatch<LLIMA_BF16>(P, a->D, (hipStream_t)stream)
                                   : at_dispatch<LLIMA_F16>(P, a->D, (hipStream_t)stream);
 }
@@ -932,8 +605,8 @@ extern "C" int llima_tree_commit(const llima_tree_commit_args* a, void* stream) 
     if (!a->block_table && (a->pages < a->B || a->max_blocks != 1)) return LLIMA_E_INVAL;
     if ((int64_t)a->page_size * a->max_blocks > (int64_t)INT32_MAX) return LLIMA_E_INVAL;
     if ((int64_t)a->B * a->L >= (1 << 24)) return LLIMA_E_INVAL;   // (the launch: fewer than 2^32 threads)
-    if (!at_strides_ok(a->k_strides, 4) || !at_strides_ok(a->v_strides, 4) || !at_strides_ok(a->k_cache_strides, 4) ||
-        !at_strides_ok(a->v_cache_strides, 4) || a->nodes_stride < 0 || (a->block_table && a->table_stride < 0))
+    if (!at_strides_ok(a->k_strides, 4, 8) || !at_strides_ok(a->v_strides, 4, 8) || !at_strides_ok(a->k_cache_strides, 4, 8) ||
+        !at_strides_ok(a->v_cache_strides, 4, 8) || a->nodes_stride < 0 || (a->block_table && a->table_stride < 0))
         return LLIMA_E_INVAL;
     if (a->B == 0) return LLIMA_OK;
     const bool cached = a->pages > 0 && a->max_blocks > 0;

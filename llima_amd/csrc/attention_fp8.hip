@@ -1,0 +1,761 @@
+// attention_fp8.hip -- attention of drafted tokens (or of one new token) over an 8-bit KV
+// cache under a tree mask (gfx950).
+//
+//   out[b][n][h] = sum_j p_j v_j,  p = softmax over the visible j of scale q . k_j
+//   cached tokens:  k_j = kq_j ks_j,  v_j = vq_j vs_j  (e4m3 values, a scale per token and head)
+//
+// One pass over the keys with the running maximum and sum of the softmax (fp32, base 2).
+// bf16 and fp16 hold every e4m3 value, so the values go into the 16-bit matrix cores by a
+// conversion without rounding; a key's scale multiplies its score, a value's scale its
+// weight, both in fp32.  The products are taken transposed in tiles of 16 rows:
+// S^T = K Q^T leaves 4 keys of a query row in a lane (lane l: row l % 16, keys 4 (l / 16)
+// + 0 .. 3), which are at once the operand of O^T = V^T P^T; V's transposing loads fetch the
+// keys in that order.
+//
+// The waves of a workgroup share no tile: each takes its own keys for all rows (up to 64) of
+// its row group, so that a value is read from memory, from LDS and converted once, and no
+// wave waits for another before the end of a sequence's part, where their sums are joined.
+//
+// The reference of the softmax moves only when a row's maximum passes it, and then 2^8
+// beyond: weights are at most 1, and the sums are rescaled seldom.  P is rounded to q's type
+// for its product with V; in fp16 the weights carry a factor of 2^15 and the values' scales
+// the inverse of the largest so far (a power of two), so that the product with a scale
+// neither overflows nor, down to 2^-29 of the largest, becomes subnormal.
+#include "attention.hpp"
+
+namespace llima {
+
+struct At8Params : AttnParams {
+    const float *ksc, *vsc;
+    int64_t kss[3], vss[3];                                  // scales: page, token and head strides (elements)
+};
+
+template <int D> struct A8 {
+    static constexpr int NW = 4;                             // waves
+    static constexpr int KT = D == 256 ? 16 : 32;            // cached keys of a wave's tile
+    static constexpr int DK = KT / 2;                        // drafted keys of one (16-bit values: the same bytes)
+    static constexpr int S = D == 64 ? 3 : 2;                // stages of a wave's ring
+    static constexpr int ST = 2 * KT * D + 256;              // bytes of a stage: K, V, their scales
+    static constexpr int T = NW * KT, TD = NW * DK;          // keys of a tile of the workgroup
+    static constexpr int MAXM = D == 256 ? 2 : 4;            // row tiles of 16
+    static constexpr int QL = D == 256 ? 1 : D == 128 ? 3 : 4;   // of them in LDS at most (two workgroups per CU), the rest in registers
+};
+
+#define A8_HEAD 8.0f                                         // the reference moves to a maximum and this much beyond
+
+// The partition's unit: tiles of T cached keys, then tiles of TD drafted ones.
+template <int D>
+struct Fp8Tiles {
+    static __device__ __forceinline__ int cached(int len) { return (len + A8<D>::T - 1) / A8<D>::T; }
+    static __device__ __forceinline__ int drafted(int N) { return (N + A8<D>::TD - 1) / A8<D>::TD; }
+    static __device__ __forceinline__ int count(const AttnParams& P, int len) { return cached(len) + drafted(P.N) + AT_EXTRA; }
+};
+
+typedef float a8_acc __attribute__((ext_vector_type(4)));
+typedef int a8_i2 __attribute__((ext_vector_type(2)));
+
+// 16 x 16 += 16 x 32 * 32 x 16, and 16 x 16 * 16 x 16.
+template <int DT> __device__ __forceinline__ a8_acc a8_mfma(at_s8 a, at_s8 b, a8_acc c) {
+    if constexpr (DT == LLIMA_BF16) {
+        typedef __bf16 t8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
+    } else {
+        typedef _Float16 t8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
+    }
+}
+template <int DT> __device__ __forceinline__ a8_acc a8_mfma(at_s4 a, at_s4 b, a8_acc c) {
+    if constexpr (DT == LLIMA_BF16) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+    else {
+        typedef _Float16 t4 __attribute__((ext_vector_type(4)));
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(t4, a), __builtin_bit_cast(t4, b), c, 0, 0, 0);
+    }
+}
+
+// 8 e4m3 values as 16-bit ones, exactly.
+template <int DT> __device__ __forceinline__ at_s8 a8_wide(uint32_t lo, uint32_t hi) {
+    llima_u32x4 w;
+    if constexpr (DT == LLIMA_BF16) {
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+    } else {
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+    }
+    return __builtin_bit_cast(at_s8, w);
+}
+
+// The maximum, or the sum, over the four lanes of a query row (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float a8_max4(float x) {
+    auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __builtin_fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __builtin_fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float a8_sum4(float x) {
+    auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// N pieces of V by the transposing loads, from a[i] on, in one piece with their wait (as builtins, the
+// compiler waits for all the requests into LDS before them).
+__device__ __forceinline__ void a8_tr8(const uint32_t (&a)[4], a8_i2 (&v)[4]) {
+    asm volatile("ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\tds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]) : "memory");
+}
+__device__ __forceinline__ void a8_tr16(const uint32_t (&a)[4], at_s4 (&v)[4]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]) : "memory");
+}
+
+template <int N> __device__ __forceinline__ void a8_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// Rows of D bytes (cached) or 2 D bytes (drafted) in LDS: 16-byte unit u of key k stands at unit
+// u ^ swz(k), so that 16 or 32 keys' same unit lie in different banks (256 bytes).
+template <int ROW> __device__ __forceinline__ uint32_t a8_swz(uint32_t key) {
+    return (ROW < 256 ? key / (256 / ROW) : key) & (ROW / 16 - 1) & 15;
+}
+
+// One workgroup: four waves over one share of the keys, one key head and M row tiles of 16.
+// A wave's cached tile lies in one page (contiguous caches, pages of a multiple of its keys):
+// its address comes from the scalar unit; or each 1 KB request of it does (AT_REQUEST), or
+// every lane computes its own (AT_LANE).  GEN: the last two modes.
+template <int DT, int D, int M, bool GEN>
+__global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
+#ifdef __HIP_DEVICE_COMPILE__                               // (the host pass drops the launch stub over the descriptors)
+    using C = A8<D>;
+    constexpr int NW = C::NW, KT = C::KT, DK = C::DK, S = C::S, ST = C::ST, T = C::T, TD = C::TD;
+    constexpr int NB = KT / 16;                              // blocks of 16 keys
+    constexpr int U = D / 16, U2 = D / 8;                    // 16-byte units of a cached and of a drafted row
+    constexpr int KQ = 64 / U, NQ = KT / KQ;                 // keys of a 1 KB request, requests of K or V
+    constexpr int KQ2 = U2 < 64 ? 64 / U2 : 1;
+    constexpr int QL = M < C::QL ? M : C::QL, QR = M - QL;
+    constexpr int NR = 2 * NQ + 2;                           // requests of a cached tile
+    constexpr int DB = D / 16;                               // column blocks
+    constexpr int QT = 16 * 2 * D;                           // bytes of a row tile of Q
+    constexpr int RING = NW * S * ST, XB = NW * DB * 1024;   // a row tile's sums of all waves
+    constexpr int XN = 2 * XB + NW * M * 128 <= RING ? 2 : 1;
+    static_assert(XB + NW * M * 128 <= RING, "room for the waves' sums");
+    static_assert(DK * 2 * D == KT * D && NQ * 1024 == KT * D, "tiles are whole requests");
+    __shared__ __align__(1024) uint8_t sm[RING + QL * QT + 16];
+    uint8_t* const sq = sm + RING;
+    uint32_t* const flag = (uint32_t*)(sq + QL * QT);        // a bad page or length; special values
+    const int t = (int)threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int part = (int)(blockIdx.x / (uint32_t)(P.Hkv * P.RG)), hr = (int)(blockIdx.x % (uint32_t)(P.Hkv * P.RG));
+    const int h = hr / P.RG, rg = hr % P.RG;
+    uint8_t* const ring = sm + wave * (S * ST);
+    bool bad = false, miss = false;
+    const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
+    const int64_t share = (int64_t)readfirstlane64((uint64_t)at_share<Fp8Tiles<D>>(P, len0));
+    const int64_t end = (part + 1) * share;
+    const int nd = Fp8Tiles<D>::drafted(P.N);
+    const int kq = lane / U, unit = lane % U, kq2 = lane / U2, unit2 = lane % U2;
+    uint32_t okv[NQ], ovv[NQ];                               // the lane's offsets within a tile of one page
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const uint32_t key = (uint32_t)(i * KQ + kq), u = (uint32_t)(unit ^ a8_swz<D>(key)) * 16;
+        okv[i] = key * (uint32_t)P.kcs[1] + u;
+        ovv[i] = key * (uint32_t)P.vcs[1] + u;
+    }
+    for (int64_t from = part * share; from < end;) {         // the share's sequences
+    int b, len;
+    int64_t first;
+    if (!at_find<Fp8Tiles<D>>(P, from, len0, b, len, first)) return;   // uniform: past the last tile
+    b = __builtin_amdgcn_readfirstlane(b);
+    len = __builtin_amdgcn_readfirstlane(len);
+    first = (int64_t)readfirstlane64((uint64_t)first);
+    const int nc = Fp8Tiles<D>::cached(len), nt = nc + nd;
+    const int64_t last = first + nt + AT_EXTRA, upto = last < end ? last : end;
+    const int c0 = (int)(from - first), c1 = upto - first < nt ? (int)(upto - first) : nt;
+    const bool whole = from == first && upto >= last - AT_EXTRA;   // the sequence has no other part
+    from = upto;
+    if (c0 >= nt) continue;                                  // uniform: nothing of it but the extra tiles
+    // the wave's tiles: cached ones c0 .., then drafted ones d0 ..
+    const int cend = c1 < nc ? c1 : nc;
+    int nC = cend > c0 ? cend - c0 : 0;
+    if (nC > 0 && (cend - 1) * T + wave * KT >= len) --nC;
+    const int d0 = (c0 > nc ? c0 : nc) - nc, dend = c1 - nc;
+    int nD = dend > d0 ? dend - d0 : 0;
+    if (nD > 0 && (dend - 1) * TD + wave * DK >= P.N) --nD;
+    const int ntile = nC + nD;
+    __syncthreads();                                         // (the sequence before is done with LDS)
+    if (t == 0) {
+        bool wrong;
+        at_len(P, b, wrong);
+        flag[0] = wrong ? 1u : 0u;
+        flag[1] = 0u;
+    }
+    auto key_of = [&](int tile) { return (c0 + tile) * T + wave * KT; };         // a cached tile's first key
+    auto draft_of = [&](int tile) { return (d0 + tile - nC) * TD + wave * DK; };   // a drafted tile's first token
+    // ---------------------------------------------------------------- requests
+    auto page_of = [&](int j) {                              // the page of key j (uniform), by the scalar unit
+        const __attribute__((address_space(4))) int32_t* tab = (const __attribute__((address_space(4))) int32_t*)(P.table + b * P.ts);
+        return tab[at_page(P.page_mul, P.page_shift, j)];
+    };
+    auto pages_of = [&](int j, int n) {                      // the page of key j + lane % KT, the last of n for those behind
+        const int e = (lane & (KT - 1)) < n ? (lane & (KT - 1)) : n - 1;
+        return P.table ? P.table[b * P.ts + at_page(P.page_mul, P.page_shift, j + e)] : b;
+    };
+    auto known = [&](int p) {                                // a page that exists; others are noted
+        if (!P.table) return b;                              // uniform
+        const bool out = p < 0 || p >= P.pages;
+        miss |= out;
+        return out ? 0 : p;
+    };
+    auto inside = [&](int j) { return P.table ? j - (int)at_page(P.page_mul, P.page_shift, j) * P.page : j; };
+    auto lds = [](uint8_t* p) { return (__attribute__((address_space(3))) void*)p; };
+    auto rsrc = [](const void* p) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7FFFFFFF, 0x00027000); };
+    int pg = 0;                                              // the page of the next tile to request; GEN: of the lane's key
+    auto lookup = [&](int tile) {
+        if (tile >= nC) return;                              // uniform
+        const int j = key_of(tile);
+        if constexpr (GEN) pg = pages_of(j, len - j);
+        else if (P.table) pg = page_of(j);                   // uniform
+    };
+    // a cached tile, the lane's own addresses; its n keys, the last of them again behind it
+    auto issue_lanes = [&](int j, int n, int pgl, uint8_t* st) {
+#pragma unroll 1
+        for (int i = 0; i < 2 * NQ; ++i) {
+            const int ki = (i % NQ) * KQ + kq, k = ki < n ? ki : n - 1;
+            const int p = known(__shfl(pgl, k, 64)), o = inside(j + k);
+            const uint32_t u = (uint32_t)(unit ^ a8_swz<D>((uint32_t)ki)) * 16;
+            const uint8_t* src = i < NQ ? (const uint8_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2]
+                                        : (const uint8_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2];
+            at_dma(src + u, st + i * 1024);
+            if (i % NQ == NQ - 1) {                          // uniform: K's or V's scales
+                const int ks = (lane & (KT - 1)) < n ? (lane & (KT - 1)) : n - 1, ps = known(pgl), os = inside(j + ks);
+                const float* sc = i < NQ ? P.ksc + ps * P.kss[0] + os * P.kss[1] + h * P.kss[2]
+                                         : P.vsc + ps * P.vss[0] + os * P.vss[1] + h * P.vss[2];
+                if (lane < KT)
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)sc,
+                                                     (__attribute__((address_space(3))) void*)(st + 2 * KT * D + i / NQ * (KT * 4)), 4, 0, 0);
+            }
+        }
+    };
+    auto issue = [&](int tile, uint8_t* st) {
+        if (tile < nC) {                                     // uniform
+            const int j = key_of(tile), n = len - j < KT ? len - j : KT;
+            if constexpr (!GEN) {
+                if (n == KT) {                               // uniform
+                    const int p = known(pg), o = inside(j);
+                    const auto rk = rsrc((const uint8_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2]);
+                    const auto rv = rsrc((const uint8_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2]);
+                    const auto sk = rsrc(P.ksc + p * P.kss[0] + o * P.kss[1] + h * P.kss[2]);
+                    const auto sv = rsrc(P.vsc + p * P.vss[0] + o * P.vss[1] + h * P.vss[2]);
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i)
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds(st + i * 1024), 16, (int)okv[i], 0, 0, 0);
+                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sk, lds(st + 2 * KT * D), 4, lane * (int)(4 * P.kss[1]), 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i)
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds(st + KT * D + i * 1024), 16, (int)ovv[i], 0, 0, 0);
+                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sv, lds(st + 2 * KT * D + KT * 4), 4, lane * (int)(4 * P.vss[1]), 0, 0, 0);
+                } else {
+                    issue_lanes(j, n, pages_of(j, n), st);
+                }
+            } else if (P.mode == AT_REQUEST && n == KT) {    // uniform
+                const int pgl = pg;
+                lookup(tile + 1);
+                int p[NQ], o[NQ];
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    p[i] = known((int)readlane((uint32_t)pgl, (uint32_t)(i * KQ)));
+                    o[i] = inside(j + i * KQ);
+                }
+                // the lane's key of the scales
+                int pl = p[0], ol = o[0];
+#pragma unroll
+                for (int i = 1; i < NQ; ++i)
+                    if ((lane & (KT - 1)) >= i * KQ) { pl = p[i]; ol = o[i]; }
+                ol += lane & (KQ - 1);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc((const uint8_t*)P.kc + p[i] * P.kcs[0] + o[i] * P.kcs[1] + h * P.kcs[2]),
+                        lds(st + i * 1024), 16, (int)(okv[i] - (uint32_t)(i * KQ) * (uint32_t)P.kcs[1]), 0, 0, 0);
+                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(P.ksc + h * P.kss[2]), lds(st + 2 * KT * D), 4,
+                        (pl * (int)P.kss[0] + ol * (int)P.kss[1]) * 4, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc((const uint8_t*)P.vc + p[i] * P.vcs[0] + o[i] * P.vcs[1] + h * P.vcs[2]),
+                        lds(st + KT * D + i * 1024), 16, (int)(ovv[i] - (uint32_t)(i * KQ) * (uint32_t)P.vcs[1]), 0, 0, 0);
+                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(P.vsc + h * P.vss[2]), lds(st + 2 * KT * D + KT * 4), 4,
+                        (pl * (int)P.vss[0] + ol * (int)P.vss[1]) * 4, 0, 0, 0);
+                return;
+            } else {
+                const int pgl = pg;
+                lookup(tile + 1);
+                issue_lanes(j, n, pgl, st);
+                return;
+            }
+            lookup(tile + 1);
+        } else {
+            const int m0 = draft_of(tile), n = P.N - m0 < DK ? P.N - m0 : DK;
+#pragma unroll 1
+            for (int i = 0; i < 2 * NQ; ++i) {
+                const int ki = (i % NQ) * KQ2 + kq2, k = ki < n ? ki : n - 1;
+                const uint32_t u = (uint32_t)(unit2 ^ a8_swz<2 * D>((uint32_t)ki)) * 16;
+                const uint16_t* src = i < NQ ? (const uint16_t*)P.k + b * P.ks[0] + (int64_t)(m0 + k) * P.ks[1] + h * P.ks[2]
+                                             : (const uint16_t*)P.v + b * P.vs[0] + (int64_t)(m0 + k) * P.vs[1] + h * P.vs[2];
+                at_dma((const uint8_t*)src + u, st + i * 1024);
+            }
+        }
+    };
+    // ---------------------------------------------------------------- Q, loaded before the first requests
+    const int row0 = rg * M * 16;
+    auto row_of = [&](int m) { const int row = row0 + m * 16 + r; return row < P.R ? row : P.R - 1; };
+    auto q_at = [&](int row, int col) {
+        row = row < P.R ? row : P.R - 1;
+        return (const uint16_t*)P.q + b * P.qs[0] + (int64_t)(row / P.G) * P.qs[1] + (h * P.G + row % P.G) * P.qs[2] + col;
+    };
+    constexpr int QI = (QL * 16 * U2 + 255) / 256;
+    llima_u32x4 ql[QI];
+#pragma unroll
+    for (int e = 0; e < QI; ++e) {
+        const int i = t + e * 256;
+        ql[e] = *(const llima_u32x4*)q_at(row0 + i / U2, i % U2 * 8);
+    }
+    at_s8 qr[QR > 0 ? QR : 1][D / 32];
+#pragma unroll
+    for (int m = 0; m < QR; ++m)
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) qr[m][s] = *(const at_s8*)q_at(row_of(QL + m), (s >> 1) * 64 + g * 16 + (s & 1) * 8);
+    asm volatile("" ::: "memory");
+    lookup(0);
+    for (int e = 0; e < S - 1 && e < ntile; ++e) issue(e, ring + e * ST);
+#pragma unroll
+    for (int e = 0; e < QI; ++e) {
+        const int i = t + e * 256, rw = i / U2;
+        if (P.flip) ql[e] ^= 0x80008000u;                    // uniform: a negative scale's sign goes to q
+        if (QL * 16 * U2 % 256 == 0 || rw < QL * 16)
+            *(llima_u32x4*)(sq + rw * 2 * D + ((uint32_t)(i % U2) ^ a8_swz<2 * D>((uint32_t)(rw & 15))) * 16) = ql[e];
+    }
+#pragma unroll
+    for (int m = 0; m < QR; ++m)
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s)
+            if (P.flip) qr[m][s] ^= (short)0x8000;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // step s of a product takes columns 64 (s / 2) + 16 g + 8 (s % 2) + 0 .. 7 of the lane
+    auto qread = [&](int m, int s) {
+        if (m < QL) return *(const at_s8*)(sq + m * QT + r * 2 * D + ((uint32_t)((s >> 1) * 8 + 2 * g + (s & 1)) ^ a8_swz<2 * D>((uint32_t)r)) * 16);
+        return qr[m < QL ? 0 : m - QL][s];
+    };
+    // ---------------------------------------------------------------- products
+    a8_acc o[M][DB];
+    float ref[M], l[M], vref = DT == LLIMA_F16 ? 0.0f : 1.0f, vinv = DT == LLIMA_F16 ? 0.0f : 1.0f;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        ref[m] = -__builtin_inff();
+        l[m] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[m][d] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // fp16: the sums' unit is a power of two that no scale so far exceeds (an infinite one but for)
+    auto unit_for = [&](float top) {
+        top = __builtin_fminf(top, 8.507059173023462e37f);   // 2^126
+        if (DT == LLIMA_F16 && __any(top > vref)) {
+            const float nr = __uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u), a = vref / nr;
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[m][d] *= a;
+            vref = nr;
+            vinv = 1.0f / nr;
+        }
+    };
+    // The softmax of B blocks of scores x (base 2), in place: x becomes the weights.
+    auto softmax = [&](auto& x, auto blocks) {
+        constexpr int BL = decltype(blocks)::value;
+        float mt[M];
+        bool up = false;
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            float a = __builtin_fmaxf(__builtin_fmaxf(x[m][0][0], x[m][0][1]), __builtin_fmaxf(x[m][0][2], x[m][0][3]));
+#pragma unroll
+            for (int k = 1; k < BL; ++k)
+                a = __builtin_fmaxf(a, __builtin_fmaxf(__builtin_fmaxf(x[m][k][0], x[m][k][1]), __builtin_fmaxf(x[m][k][2], x[m][k][3])));
+            mt[m] = a8_max4(a);
+            up |= mt[m] > ref[m];
+        }
+        if (__any(up)) {
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const float nr = mt[m] > ref[m] ? mt[m] + A8_HEAD : ref[m];
+                const float a = mt[m] > ref[m] ? __builtin_amdgcn_exp2f(ref[m] - nr) : 1.0f;
+                ref[m] = nr;
+                l[m] *= a;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[m][d] *= a;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const float mu = (ref[m] > -__builtin_inff() ? ref[m] : 0.0f) - (DT == LLIMA_F16 ? 15.0f : 0.0f);
+#pragma unroll
+            for (int k = 0; k < BL; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[m][k][i] = __builtin_amdgcn_exp2f(x[m][k][i] - mu);
+                    l[m] += x[m][k][i];
+                }
+        }
+    };
+    auto lds_at = [](const uint8_t* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p; };
+    // A staged tile of n cached keys; K has landed, `more` waits for V.
+    auto math8 = [&](const uint8_t* st, int n, auto more) __attribute__((always_inline)) {
+        a8_acc x[M][NB], ks[NB];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            ks[k] = *(const a8_acc*)(st + 2 * KT * D + k * 64 + g * 16) * P.scale2;
+#pragma unroll
+            for (int m = 0; m < M; ++m) x[m][k] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+            llima_u32x4 kr[NB];
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+                kr[k] = *(const llima_u32x4*)(st + (k * 16 + r) * D + ((uint32_t)(4 * c + g) ^ a8_swz<D>((uint32_t)(k * 16 + r))) * 16);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                at_s8 kf[NB];
+#pragma unroll
+                for (int k = 0; k < NB; ++k) kf[k] = a8_wide<DT>(kr[k][2 * s], kr[k][2 * s + 1]);
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    const at_s8 q = qread(m, 2 * c + s);
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) x[m][k] = a8_mfma<DT>(kf[k], q, x[m][k]);
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                x[m][k] *= ks[k];
+                if (n < KT) {                                // uniform: the sequence's last cached keys
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[m][k][i] = k * 16 + 4 * g + i < n ? x[m][k][i] : -__builtin_inff();
+                }
+            }
+        softmax(x, std::integral_constant<int, NB>{});
+        more();
+        a8_acc vs[NB];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) vs[k] = *(const a8_acc*)(st + 2 * KT * D + KT * 4 + k * 64 + g * 16);
+        if constexpr (DT == LLIMA_F16) {
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fmaxf(vs[k][0], vs[k][1]), __builtin_fmaxf(vs[k][2], vs[k][3])));
+            unit_for(a8_max4(top));
+#pragma unroll
+            for (int k = 0; k < NB; ++k) vs[k] *= vinv;
+        }
+        uint32_t pw[M][2 * NB];
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                const a8_acc y = x[m][k] * vs[k];
+                pw[m][2 * k] = at_pack<DT>(y[0], y[1]);
+                pw[m][2 * k + 1] = at_pack<DT>(y[2], y[3]);
+            }
+        // V: a transposing load takes 8 rows of 16 bytes from 16 lanes (row i / 2 of lane i, half i % 2)
+        const int e = r >> 1;
+        if constexpr (NB == 2) {                             // keys 4 g + 0 .. 3 and 16 more of a column block
+            const uint32_t key = (uint32_t)(4 * g + (e & 3) + (e >> 2) * 16);
+            const uint32_t base = lds_at(st) + KT * D + key * D + (uint32_t)(r & 1) * 8, z = a8_swz<D>(key);
+#pragma unroll
+            for (int d = 0; d < DB; d += 4) {
+                uint32_t a[4];
+                a8_i2 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = base + (((uint32_t)(d + i) ^ z) << 4);
+                a8_tr8(a, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const at_s8 vf = a8_wide<DT>((uint32_t)v[i][0], (uint32_t)v[i][1]);
+#pragma unroll
+                    for (int m = 0; m < M; ++m)
+                        o[m][d + i] = a8_mfma<DT>(vf, __builtin_bit_cast(at_s8, (llima_u32x4){pw[m][0], pw[m][1], pw[m][2 * NB - 2], pw[m][2 * NB - 1]}), o[m][d + i]);
+                }
+            }
+        } else {                                             // keys 4 g + 0 .. 3 of two column blocks
+            const uint32_t key = (uint32_t)(4 * g + (e & 3));
+            const uint32_t base = lds_at(st) + KT * D + key * D + (uint32_t)(r & 1) * 8, z = a8_swz<D>(key);
+#pragma unroll
+            for (int d = 0; d < DB; d += 8) {
+                uint32_t a[4];
+                a8_i2 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = base + (((uint32_t)(d + 2 * i + (e >> 2)) ^ z) << 4);
+                a8_tr8(a, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const at_s8 vf = a8_wide<DT>((uint32_t)v[i][0], (uint32_t)v[i][1]);
+#pragma unroll
+                    for (int m = 0; m < M; ++m) {
+                        const at_s4 pf = __builtin_bit_cast(at_s4, (a8_i2){(int)pw[m][0], (int)pw[m][1]});
+                        o[m][d + 2 * i] = a8_mfma<DT>(__builtin_shufflevector(vf, vf, 0, 1, 2, 3), pf, o[m][d + 2 * i]);
+                        o[m][d + 2 * i + 1] = a8_mfma<DT>(__builtin_shufflevector(vf, vf, 4, 5, 6, 7), pf, o[m][d + 2 * i + 1]);
+                    }
+                }
+            }
+        }
+    };
+    auto seen = [&](int n, int mm) {                         // node n sees drafted token mm
+        if (!P.mask) return mm <= n;
+        if (P.mask_f32) return ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
+        return ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
+    };
+    // A staged tile of n drafted tokens from m0 on.
+    auto math16 = [&](uint8_t* st, int m0, int n) __attribute__((always_inline)) {
+        a8_acc x[M][1];
+        bool sees[M][4];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const int node = row_of(m) / P.G;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = 4 * g + i;
+                sees[m][i] = seen(node, m0 + (e < n ? e : n - 1)) && e < n;
+            }
+            x[m][0] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        a8_wait<0>();
+        // Values that not every row sees: infinities and NaN become 0 (0 times them would be NaN
+        // for the rows that do not see them; at the end they are added to the rows that do).
+        for (int p = lane; p < DK * U2; p += 64) {
+            llima_u32x4* const at = (llima_u32x4*)(st + KT * D + p * 16);
+            llima_u32x4 y = *at;
+            bool put = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t w = y[e];
+                if (at_special<DT>((uint16_t)w)) { w &= 0xFFFF0000u; put = true; }
+                if (at_special<DT>((uint16_t)(w >> 16))) { w &= 0xFFFFu; put = true; }
+                y[e] = w;
+            }
+            if (put) { *at = y; flag[1] = 1u; }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const uint32_t kr = (uint32_t)r & (DK - 1);
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            const at_s8 kf = *(const at_s8*)(st + kr * 2 * D + ((uint32_t)((s >> 1) * 8 + 2 * g + (s & 1)) ^ a8_swz<2 * D>(kr)) * 16);
+#pragma unroll
+            for (int m = 0; m < M; ++m) x[m][0] = a8_mfma<DT>(kf, qread(m, s), x[m][0]);
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[m][0][i] = sees[m][i] ? x[m][0][i] * P.scale2 : -__builtin_inff();
+        softmax(x, std::integral_constant<int, 1>{});
+        unit_for(1.0f);
+        at_s4 pf[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const a8_acc y = x[m][0] * vinv;
+            pf[m] = __builtin_bit_cast(at_s4, (a8_i2){(int)at_pack<DT>(y[0], y[1]), (int)at_pack<DT>(y[2], y[3])});
+        }
+        // a transposing load takes 4 rows of 32 bytes from 16 lanes (row i / 4 of lane i, 8 bytes i % 4)
+        const uint32_t key = (uint32_t)(4 * g + (r >> 2)) & (DK - 1);
+        const uint32_t base = lds_at(st) + KT * D + key * 2 * D + (uint32_t)(r & 1) * 8, z = a8_swz<2 * D>(key), half = (uint32_t)(r >> 1 & 1);
+#pragma unroll
+        for (int d = 0; d < DB; d += 4) {
+            uint32_t a[4];
+            at_s4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = base + (((uint32_t)(2 * (d + i)) + half ^ z) << 4);
+            a8_tr16(a, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int m = 0; m < M; ++m) o[m][d + i] = a8_mfma<DT>(v[i], pf[m], o[m][d + i]);
+        }
+    };
+    int slot = 0;
+    for (int tile = 0; tile < nC; ++tile) {
+        const int ahead = tile + S - 1;
+        uint8_t* const st = ring + slot * ST;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot's last tile has been read
+        if (ahead < ntile) issue(ahead, ring + (slot == 0 ? S - 1 : slot - 1) * ST);   // uniform
+        const int n = len - key_of(tile) < KT ? len - key_of(tile) : KT;
+        // cached tiles behind this one count NR requests each, drafted ones fewer: then everything is waited for
+        if (ahead < nC) {                                    // uniform
+            a8_wait<(S - 1) * NR + NQ + 1>();
+            math8(st, n, [] { a8_wait<(S - 1) * NR>(); });
+        } else {
+            a8_wait<0>();
+            math8(st, n, [] {});
+        }
+        slot = slot + 1 < S ? slot + 1 : 0;
+    }
+    for (int tile = nC; tile < ntile; ++tile) {
+        const int ahead = tile + S - 1;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (ahead < ntile) issue(ahead, ring + (slot == 0 ? S - 1 : slot - 1) * ST);   // uniform
+        const int m0 = draft_of(tile);
+        math16(ring + slot * ST, m0, P.N - m0 < DK ? P.N - m0 : DK);
+        slot = slot + 1 < S ? slot + 1 : 0;
+    }
+    // ---------------------------------------------------------------- the waves' sums
+    if (__any(miss) && lane == 0) flag[0] = 1u;
+    __syncthreads();                                         // no wave reads or fills its ring any more
+    float2* const ml = (float2*)(sm + XN * XB);              // [wave][row]
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        l[m] = a8_sum4(l[m]);
+        if (g == 0) ml[wave * M * 16 + m * 16 + r] = make_float2(ref[m], l[m]);
+    }
+    __syncthreads();
+    const bool nan = flag[0] != 0, special = flag[1] != 0;
+    const int drow0 = (c0 > nc ? c0 - nc : 0) * TD, drow1 = c1 - nc <= 0 ? 0 : (c1 - nc) * TD < P.N ? (c1 - nc) * TD : P.N;   // the part's drafted tokens
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        float2 x[NW];
+        float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            x[w] = ml[w * M * 16 + m * 16 + r];
+            top = __builtin_fmaxf(top, x[w].x);
+        }
+        const float mu = top > -__builtin_inff() ? top : 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) sum += x[w].y * __builtin_amdgcn_exp2f(x[w].x - mu);
+        const float a = __builtin_amdgcn_exp2f(ref[m] - mu) * (DT == LLIMA_F16 ? vref : 1.0f);
+        uint8_t* const xb = sm + (XN == 2 ? (m & 1) * XB : 0);
+        if (XN == 1 && m > 0) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DB; ++d) *(a8_acc*)(xb + (wave * DB + d) * 1024 + lane * 16) = o[m][d] * a;
+        __syncthreads();
+        const int row = row0 + m * 16 + r;
+        if (nan) sum = __builtin_nanf("");
+        if (row < P.R) {
+            const int n = row / P.G, hq = h * P.G + row % P.G;
+            const float inv = whole ? at_inverse(&P, sum, b, n, len) : 1.0f;
+            const size_t at = ((size_t)at_slot(P.pairs, part, b, c0 == 0) * P.Hkv + h) * P.R + row;
+            if (!whole && wave == 0 && g == 0) P.part_ml[at] = make_float2(top, sum);
+#pragma unroll
+            for (int i = 0; i < DB / NW; ++i) {
+                const int d = wave + NW * i;
+                a8_acc y = *(const a8_acc*)(xb + d * 1024 + lane * 16);
+#pragma unroll
+                for (int w = 1; w < NW; ++w) y += *(const a8_acc*)(xb + (w * DB + d) * 1024 + lane * 16);
+                if (special) {                               // uniform: infinities and NaN of drafted tokens in this part
+                    for (int mm = drow0; mm < drow1; ++mm) {
+                        if (!seen(n, mm)) continue;          // (of the loop over mm)
+                        const uint2 v = *(const uint2*)((const uint16_t*)P.v + b * P.vs[0] + (int64_t)mm * P.vs[1] + h * P.vs[2] + d * 16 + 4 * g);
+                        auto add = [&](int e, uint32_t u) { y[e] += at_special<DT>((uint16_t)u) ? at_f32<DT>((uint16_t)u) : 0.0f; };
+                        add(0, v.x); add(1, v.x >> 16); add(2, v.y); add(3, v.y >> 16);
+                    }
+                }
+                if (whole) {
+                    y *= inv;
+                    *(uint2*)((uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + d * 16 + 4 * g) =
+                        make_uint2(at_pack<DT>(y[0], y[1]), at_pack<DT>(y[2], y[3]));
+                } else {
+                    *(a8_acc*)(P.part_o + at * D + d * 16 + 4 * g) = y;
+                }
+            }
+        }
+    }
+    }
+#endif
+}
+
+// Shares of the keys: as many workgroups as the device holds at a time, two per CU.
+static int a8_parts(int Hkv, int RG) {
+    const int n = 512 / (Hkv * RG);
+    return n < 1 ? 1 : n;
+}
+
+static void a8_plan(AttnParams& P, int D) {                  // RT: row tiles of 16 of a group
+    const int most = D == 256 ? A8<256>::MAXM : D == 128 ? A8<128>::MAXM : A8<64>::MAXM;
+    P.R = P.N * P.G;
+    const int tiles = (P.R + 15) / 16;
+    P.RG = (tiles + most - 1) / most;
+    P.RT = (tiles + P.RG - 1) / P.RG;
+    P.parts = a8_parts(P.Hkv, P.RG);
+    at_slots(P);
+}
+
+template <int DT, int D, bool GEN>
+static void a8_launch(const At8Params& P, hipStream_t st) {
+    const dim3 g((uint32_t)P.parts * P.RG * P.Hkv), w(64 * A8<D>::NW);
+    if (P.RT == 1) hipLaunchKernelGGL((tree_attn8<DT, D, 1, GEN>), g, w, 0, st, P);
+    else if (P.RT == 2) hipLaunchKernelGGL((tree_attn8<DT, D, 2, GEN>), g, w, 0, st, P);
+    else if constexpr (A8<D>::MAXM > 2) {
+        if (P.RT == 3) hipLaunchKernelGGL((tree_attn8<DT, D, 3, GEN>), g, w, 0, st, P);
+        else hipLaunchKernelGGL((tree_attn8<DT, D, 4, GEN>), g, w, 0, st, P);
+    }
+    const int64_t rows = (int64_t)P.B * P.N * P.Hq;
+    const AttnParams& J = P;
+    if (rows <= 1024) hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, J);
+    else hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, J);
+}
+
+template <int DT>
+static int a8_dispatch(const At8Params& P, int D, hipStream_t st) {
+    const bool gen = P.mode != AT_TILE;
+    if (D == 64) gen ? a8_launch<DT, 64, true>(P, st) : a8_launch<DT, 64, false>(P, st);
+    else if (D == 128) gen ? a8_launch<DT, 128, true>(P, st) : a8_launch<DT, 128, false>(P, st);
+    else gen ? a8_launch<DT, 256, true>(P, st) : a8_launch<DT, 256, false>(P, st);
+    return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
+}
+
+}  // namespace llima
+
+using namespace llima;
+
+extern "C" size_t llima_tree_attention_fp8_workspace_bytes(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D) {
+    if (B <= 0 || !at_sizes_ok(B, N, Hq, Hkv, D)) return 0;
+    AttnParams P = {};
+    P.B = B; P.N = N; P.Hkv = Hkv; P.G = Hq / Hkv;
+    a8_plan(P, D);
+    return at_parts_bytes(P, D);
+}
+
+extern "C" int llima_tree_attention_fp8(const llima_tree_attention_fp8_args* x, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+    if (!x) return LLIMA_E_INVAL;
+    const llima_tree_attention_args* a = &x->a;
+    At8Params P = {};
+    const int ok = at_fill(a, 16, P);
+    if (ok != LLIMA_OK) return ok;
+    if (!at_strides_ok(x->k_scale_strides, 3, 1) || !at_strides_ok(x->v_scale_strides, 3, 1)) return LLIMA_E_INVAL;
+    if (a->B == 0) return LLIMA_OK;
+    if (P.cap > 0 && (!x->k_scales || !x->v_scales)) return LLIMA_E_INVAL;
+    if ((uintptr_t)x->k_scales % 4 || (uintptr_t)x->v_scales % 4) return LLIMA_E_INVAL;
+    if (!workspace || workspace_bytes < llima_tree_attention_fp8_workspace_bytes(a->B, a->N, a->Hq, a->Hkv, a->D))
+        return LLIMA_E_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return LLIMA_E_INVAL;
+    P.ksc = x->k_scales; P.vsc = x->v_scales;
+    int64_t span = 0;                                        // of the scales from a head's first on, in elements
+    for (int i = 0; i < 3; ++i) {
+        P.kss[i] = x->k_scale_strides[i]; P.vss[i] = x->v_scale_strides[i];
+    }
+    for (const int64_t* s : {P.kss, P.vss}) {
+        const int64_t e = (s[0] > (1 << 29) ? 1 << 29 : s[0]) * (int64_t)P.pages + (s[1] > (1 << 29) ? 1 << 29 : s[1]) * (int64_t)P.page;
+        span = e > span ? e : span;
+    }
+    // offsets within a tile (32 keys) or a request, and of the scales, have 31 bits
+    const int64_t ts = P.kcs[1] > P.vcs[1] ? P.kcs[1] : P.vcs[1], ss = P.kss[1] > P.vss[1] ? P.kss[1] : P.vss[1];
+    const int kt = a->D == 256 ? A8<256>::KT : A8<128>::KT, kq = 1024 / a->D;
+    P.mode = ts <= (1 << 25) && ss <= (1 << 23) && (!P.table || P.page % kt == 0) ? AT_TILE
+           : ts <= (1 << 25) && span < (1 << 29) && P.page % kq == 0 ? AT_REQUEST : AT_LANE;
+    a8_plan(P, a->D);
+    at_parts_at(P, a->D, workspace);
+    return a->dtype == LLIMA_BF16 ? a8_dispatch<LLIMA_BF16>(P, a->D, (hipStream_t)stream)
+                                  : a8_dispatch<LLIMA_F16>(P, a->D, (hipStream_t)stream);
+}

@@ -1,0 +1,281 @@
+// cache.hip -- an 8-bit KV cache: keys and values quantised as they are written, and read
+// back in 16 bits (gfx950).
+//
+//   per token and key head:  m = max(max |x|, 2^-100),  scale = m / 448,
+//                            q = e4m3(448 x / m),  back: round(q scale)
+//
+// One scale for a head's D values: the attention over the cache multiplies a key's score
+// and a value's weight by it once, and 4 bytes stand beside 64 to 256.
+#include "attention.hpp"
+#include "quant.hpp"
+
+namespace llima {
+
+struct CacheParams {
+    const uint8_t *k, *v;                                    // written from (write); or null
+    uint8_t *ok, *ov;                                        // read into (read); or null
+    uint8_t *kq, *vq;                                        // the cache's values
+    float *ksc, *vsc;                                        // and scales
+    const int32_t *nodes, *counts, *lens, *table;            // nodes, counts, table: or null
+    int32_t* new_lens;
+    int64_t ks[4], vs[4];                                    // layer, batch, token and head strides (bytes; 16-bit side)
+    int64_t kqs[4], vqs[4];                                  // layer, page, token and head strides (bytes)
+    int64_t kss[4], vss[4];                                  // the same of the scales (elements)
+    int64_t ns, ts, cap;
+    int32_t B, N, L, Hkv;
+    int32_t page, pages;
+    uint32_t page_mul, page_shift, row_mul, row_shift;       // / page; / (2 Hkv)
+    int32_t tok, chunks;                                     // tokens of a workgroup; workgroups of a sequence
+};
+
+// The maximum of non-negative floats' bits over N adjacent lanes, in all of them.
+template <int N>
+__device__ __forceinline__ uint32_t ca_max(uint32_t m) {
+    m = q8_umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));   // lane ^ 1
+    m = q8_umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));   // lane ^ 2
+    m = q8_umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));  // 7 - lane of 8
+    if constexpr (N >= 16) m = q8_umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xF, 0xF, false));   // 15 - lane of 16
+    if constexpr (N >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+        m = q8_umax(s[0], s[1]);
+    }
+    return m;
+}
+
+template <int DT> __device__ __forceinline__ void ca_load8(const llima_u32x4& q, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = at_f32<DT>((uint16_t)q[i]);
+        v[2 * i + 1] = at_f32<DT>((uint16_t)(q[i] >> 16));
+    }
+}
+
+// Every page of tokens [from, to) of sequence b in range (the same in all threads).
+__device__ __forceinline__ bool ca_pages_ok(const CacheParams& P, int b, int from, int to) {
+    bool ok = true;
+    if (P.table && to > from) {                              // uniform
+        const int e1 = (int)at_page(P.page_mul, P.page_shift, to - 1);
+        for (int e = (int)at_page(P.page_mul, P.page_shift, from) + (int)threadIdx.x; e <= e1; e += LLIMA_WG) {
+            const int p = P.table[b * P.ts + e];
+            ok = ok && p >= 0 && p < P.pages;
+        }
+    }
+    return ok;
+}
+
+// Token at of sequence b: its page and place in it.
+__device__ __forceinline__ void ca_place(const CacheParams& P, int b, int at, int64_t& p, int64_t& o) {
+    p = b;
+    o = at;
+    if (P.table) {                                           // uniform
+        const uint32_t e = at_page(P.page_mul, P.page_shift, at);
+        o = at - (int)e * P.page;
+        p = P.table[b * P.ts + e];
+    }
+}
+
+// One workgroup per `tok` places of a sequence and layer.  It checks the sequence's whole
+// path and room (every workgroup of a sequence comes to the same answer); then D / 8 lanes
+// take a row of D values each: 16 bytes in, 8 out, the maximum over the row's lanes.
+template <int DT, int D>
+__global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
+    constexpr int U = D / 8, RW = LLIMA_WG / U, F = 4;       // lanes of a row; rows of a pass; passes in flight
+    const int c = (int)(blockIdx.x % (uint32_t)P.chunks), b = (int)(blockIdx.x / (uint32_t)P.chunks), t = (int)threadIdx.x;
+    const int64_t layer = blockIdx.y;
+    const int len = P.lens[b], cnt = P.counts ? P.counts[b] : P.L;
+    bool ok = len >= 0 && cnt >= 0 && cnt <= P.L && len <= P.cap && (int64_t)len + cnt <= P.cap;
+    if (ok) {                                                // uniform
+        bool all = ca_pages_ok(P, b, len, len + cnt);
+        if (P.nodes)
+            for (int i = t; i < cnt; i += LLIMA_WG) {
+                const int node = P.nodes[b * P.ns + i];
+                all = all && node >= 0 && node < P.N;
+            }
+        ok = __syncthreads_and(all);
+    }
+    if (c == 0 && layer == 0 && t == 0) P.new_lens[b] = ok ? len + cnt : LLIMA_E_RANGE;
+    const int j0 = c * P.tok, j1 = j0 + P.tok < cnt ? j0 + P.tok : cnt;
+    if (!ok || j0 >= cnt) return;                            // uniform
+    const int rows = (j1 - j0) * 2 * P.Hkv, u = t % U;
+    for (int i0 = t / U; i0 < rows; i0 += RW * F) {
+        llima_u32x4 x[F];
+        int j[F], h[F];
+        bool isv[F];
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1;
+            const int e = (int)at_page(P.row_mul, P.row_shift, i), w = i - e * 2 * P.Hkv;
+            j[f] = j0 + e;
+            isv[f] = w >= P.Hkv;
+            h[f] = isv[f] ? w - P.Hkv : w;
+            const int64_t node = P.nodes ? P.nodes[b * P.ns + j[f]] : j[f];
+            const uint8_t* src = isv[f] ? P.v + layer * P.vs[0] + b * P.vs[1] + node * P.vs[2] + h[f] * P.vs[3]
+                                        : P.k + layer * P.ks[0] + b * P.ks[1] + node * P.ks[2] + h[f] * P.ks[3];
+            x[f] = *(const llima_u32x4*)(src + u * 16);
+        }
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            float v[8];
+            ca_load8<DT>(x[f], v);
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = q8_umax(m, q8_abs(v[i]));
+            const float mf = __uint_as_float(q8_umax(ca_max<U>(m), __float_as_uint(Q8_TINY)));
+            const uint2 q = q8_pack8(v, mf);
+            if (i0 + f * RW < rows) {
+                int64_t p, o;
+                ca_place(P, b, len + j[f], p, o);
+                uint8_t* dst = isv[f] ? P.vq + layer * P.vqs[0] + p * P.vqs[1] + o * P.vqs[2] + h[f] * P.vqs[3]
+                                      : P.kq + layer * P.kqs[0] + p * P.kqs[1] + o * P.kqs[2] + h[f] * P.kqs[3];
+                *(uint2*)(dst + u * 8) = q;
+                float* sc = isv[f] ? P.vsc + layer * P.vss[0] + p * P.vss[1] + o * P.vss[2] + h[f] * P.vss[3]
+                                   : P.ksc + layer * P.kss[0] + p * P.kss[1] + o * P.kss[2] + h[f] * P.kss[3];
+                if (u == 0) *sc = mf / 448.0f;
+            }
+        }
+    }
+}
+
+// One workgroup per `tok` tokens of a sequence and layer, D / 8 lanes a row: 8 bytes in, 16
+// out.  Rows past the sequence's length are 0; a sequence with a bad length or page is NaN.
+template <int DT, int D>
+__global__ __launch_bounds__(LLIMA_WG) void cache_read8(CacheParams P) {
+    constexpr int U = D / 8, RW = LLIMA_WG / U, F = 4;
+    const int c = (int)(blockIdx.x % (uint32_t)P.chunks), b = (int)(blockIdx.x / (uint32_t)P.chunks), t = (int)threadIdx.x;
+    const int64_t layer = blockIdx.y;
+    const int len = P.lens[b];
+    bool ok = len >= 0 && len <= P.cap;
+    if (ok) ok = __syncthreads_and(ca_pages_ok(P, b, 0, len));   // uniform
+    const int j0 = c * P.tok, j1 = j0 + P.tok < P.L ? j0 + P.tok : P.L;
+    const int rows = (j1 - j0) * 2 * P.Hkv, u = t % U;
+    for (int i0 = t / U; i0 < rows; i0 += RW * F) {
+        uint2 x[F];
+        float sc[F];
+        uint8_t* dst[F];
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1;
+            const int e = (int)at_page(P.row_mul, P.row_shift, i), w = i - e * 2 * P.Hkv, j = j0 + e;
+            const bool isv = w >= P.Hkv;
+            const int h = isv ? w - P.Hkv : w;
+            dst[f] = (isv ? P.ov + layer * P.vs[0] + b * P.vs[1] + j * P.vs[2] + h * P.vs[3]
+                          : P.ok + layer * P.ks[0] + b * P.ks[1] + j * P.ks[2] + h * P.ks[3]) + u * 16;
+            x[f] = make_uint2(0u, 0u);
+            sc[f] = ok ? 0.0f : __builtin_nanf("");
+            if (ok && j < len) {
+                int64_t p, o;
+                ca_place(P, b, j, p, o);
+                x[f] = *(const uint2*)((isv ? P.vq + layer * P.vqs[0] + p * P.vqs[1] + o * P.vqs[2] + h * P.vqs[3]
+                                            : P.kq + layer * P.kqs[0] + p * P.kqs[1] + o * P.kqs[2] + h * P.kqs[3]) + u * 8);
+                sc[f] = isv ? P.vsc[layer * P.vss[0] + p * P.vss[1] + o * P.vss[2] + h * P.vss[3]]
+                            : P.ksc[layer * P.kss[0] + p * P.kss[1] + o * P.kss[2] + h * P.kss[3]];
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            const uint32_t w[2] = {x[f].x, x[f].y};
+            llima_u32x4 y;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+                y[2 * i] = at_pack<DT>(a[0] * sc[f], a[1] * sc[f]);
+                y[2 * i + 1] = at_pack<DT>(d[0] * sc[f], d[1] * sc[f]);
+            }
+            if (i0 + f * RW < rows) *(llima_u32x4*)dst[f] = y;
+        }
+    }
+}
+
+// Tokens of a workgroup: up to 8 passes of its rows, fewer where that leaves the device idle.
+static void ca_plan(CacheParams& P, int layers, int D) {
+    const int64_t rw = LLIMA_WG / (D / 8), rows = (int64_t)layers * P.B * P.L * 2 * P.Hkv;
+    int64_t passes = rows / (rw * 2048);
+    passes = passes < 1 ? 1 : passes > 8 ? 8 : passes;
+    const int64_t tok = passes * rw / (2 * P.Hkv);
+    P.tok = tok < 1 ? 1 : (int)tok;
+    P.chunks = (P.L + P.tok - 1) / P.tok;
+}
+
+template <int DT, bool WRITE>
+static int ca_launch(const CacheParams& P, int layers, int D, hipStream_t st) {
+    if ((int64_t)P.B * P.chunks >= 1 << 24) return LLIMA_E_INVAL;   // (a launch: fewer than 2^32 threads)
+    const dim3 g((uint32_t)(P.B * P.chunks), (uint32_t)layers), w(LLIMA_WG);
+    auto go = [&](auto d) {
+        constexpr int DD = decltype(d)::value;
+        if constexpr (WRITE) hipLaunchKernelGGL((cache_write8<DT, DD>), g, w, 0, st, P);
+        else hipLaunchKernelGGL((cache_read8<DT, DD>), g, w, 0, st, P);
+    };
+    if (D == 64) go(std::integral_constant<int, 64>{});
+    else if (D == 128) go(std::integral_constant<int, 128>{});
+    else go(std::integral_constant<int, 256>{});
+    return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
+}
+
+// The arguments that writing and reading share: sizes, the cache and its strides.
+template <class Args>
+static int ca_fill(const Args* a, CacheParams& P) {
+    if (!a || (a->dtype != LLIMA_BF16 && a->dtype != LLIMA_F16)) return LLIMA_E_INVAL;
+    if (a->layers <= 0 || a->layers > 65535 || a->B < 0 || a->Hkv <= 0 || a->Hkv > 1024) return LLIMA_E_INVAL;
+    if (a->D != 64 && a->D != 128 && a->D != 256) return LLIMA_E_INVAL;
+    if (a->page_size <= 0 || a->pages < 0 || a->max_blocks < 0) return LLIMA_E_INVAL;
+    if (!a->block_table && (a->pages < a->B || a->max_blocks != 1)) return LLIMA_E_INVAL;
+    if ((int64_t)a->page_size * a->max_blocks > AT_KEYS) return LLIMA_E_INVAL;
+    if (!at_strides_ok(a->k_strides, 4, 8) || !at_strides_ok(a->v_strides, 4, 8) || !at_strides_ok(a->k_cache_strides, 4, 16) ||
+        !at_strides_ok(a->v_cache_strides, 4, 16) || !at_strides_ok(a->k_scale_strides, 4, 1) || !at_strides_ok(a->v_scale_strides, 4, 1))
+        return LLIMA_E_INVAL;
+    if (a->block_table && a->table_stride < 0) return LLIMA_E_INVAL;
+    if (a->B == 0) return LLIMA_OK;
+    const bool cached = a->pages > 0 && a->max_blocks > 0;
+    if (!a->cache_lens || !a->k || !a->v) return LLIMA_E_INVAL;
+    if (cached && (!a->k_cache || !a->v_cache || !a->k_scales || !a->v_scales)) return LLIMA_E_INVAL;
+    const void* ptrs[] = {a->k, a->v, a->k_cache, a->v_cache};
+    for (const void* p : ptrs)
+        if ((uintptr_t)p % 16) return LLIMA_E_INVAL;
+    if ((uintptr_t)a->k_scales % 4 || (uintptr_t)a->v_scales % 4) return LLIMA_E_INVAL;
+    P.kq = (uint8_t*)a->k_cache; P.vq = (uint8_t*)a->v_cache;
+    P.ksc = (float*)a->k_scales; P.vsc = (float*)a->v_scales;
+    P.lens = a->cache_lens; P.table = a->block_table;
+    for (int i = 0; i < 4; ++i) {
+        P.ks[i] = 2 * a->k_strides[i]; P.vs[i] = 2 * a->v_strides[i];
+        P.kqs[i] = a->k_cache_strides[i]; P.vqs[i] = a->v_cache_strides[i];
+        P.kss[i] = a->k_scale_strides[i]; P.vss[i] = a->v_scale_strides[i];
+    }
+    P.ts = a->table_stride;
+    P.cap = cached ? (int64_t)a->page_size * a->max_blocks : 0;
+    P.B = a->B; P.Hkv = a->Hkv;
+    P.page = a->page_size; P.pages = a->pages;
+    at_divisor(P.page, P.page_mul, P.page_shift);
+    at_divisor(2 * P.Hkv, P.row_mul, P.row_shift);
+    return LLIMA_OK;
+}
+
+}  // namespace llima
+
+using namespace llima;
+
+extern "C" int llima_cache_write_fp8(const llima_cache_write_fp8_args* a, void* stream) {
+    CacheParams P = {};
+    if (a && (a->N <= 0 || a->L <= 0 || a->L > AT_KEYS || (!a->nodes && a->L != a->N) || a->nodes_stride < 0)) return LLIMA_E_INVAL;
+    const int ok = ca_fill(a, P);
+    if (ok != LLIMA_OK || a->B == 0) return ok;
+    if (!a->new_lens) return LLIMA_E_INVAL;
+    P.k = (const uint8_t*)a->k; P.v = (const uint8_t*)a->v;
+    P.nodes = a->nodes; P.counts = a->counts; P.new_lens = a->new_lens;
+    P.ns = a->nodes_stride;
+    P.N = a->N; P.L = a->L;
+    ca_plan(P, a->layers, a->D);
+    return a->dtype == LLIMA_BF16 ? ca_launch<LLIMA_BF16, true>(P, a->layers, a->D, (hipStream_t)stream)
+                                  : ca_launch<LLIMA_F16, true>(P, a->layers, a->D, (hipStream_t)stream);
+}
+
+extern "C" int llima_cache_read_fp8(const llima_cache_read_fp8_args* a, void* stream) {
+    CacheParams P = {};
+    if (a && (a->L < 0 || a->L > AT_KEYS)) return LLIMA_E_INVAL;
+    const int ok = ca_fill(a, P);
+    if (ok != LLIMA_OK || a->B == 0 || a->L == 0) return ok;
+    P.ok = (uint8_t*)a->k; P.ov = (uint8_t*)a->v;
+    P.L = a->L;
+    ca_plan(P, a->layers, a->D);
+    return a->dtype == LLIMA_BF16 ? ca_launch<LLIMA_BF16, false>(P, a->layers, a->D, (hipStream_t)stream)
+                                  : ca_launch<LLIMA_F16, false>(P, a->layers, a->D, (hipStream_t)stream);
+}

@@ -15,15 +15,10 @@
 // most below the normal range.  A block holding a NaN or an infinity has that
 // as its scale (and NaN where an infinity stood, 0 where a number did, or NaN
 // throughout for a NaN).
-#include <hip/hip_fp16.h>
-
-#include "common.hpp"
-#include "../../include/llima_sampler.h"
+#include "norm.hpp"
+#include "quant.hpp"
 
 namespace llima {
-
-#define NRM_BLK 128
-#define NRM_TINY 7.8886090522101181e-31f                     // 2^-100
 
 struct NormParams {
     const void* x;
@@ -36,82 +31,6 @@ struct NormParams {
     int32_t B, H, NK;
     float eps, offset;
 };
-
-// 8 values of a row as fp32 (16 bytes of a 16-bit type, 32 of fp32), and back
-// rounded to nearest, ties to even.
-template <int DT> struct NormType;
-template <> struct NormType<LLIMA_BF16> {
-    static constexpr int E = 2;
-    static __device__ __forceinline__ void load(const void* p, float (&v)[8]) {
-        const llima_u32x4 q = *(const llima_u32x4*)p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(q[i] << 16);
-            v[2 * i + 1] = __uint_as_float(q[i] & 0xFFFF0000u);
-        }
-    }
-    static __device__ __forceinline__ void store(void* p, const float (&v)[8]) {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        typedef __bf16 h2 __attribute__((ext_vector_type(2)));
-        llima_u32x4 q;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f2 a = {v[2 * i], v[2 * i + 1]};
-            q[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(a, h2));
-        }
-        *(llima_u32x4*)p = q;
-    }
-    static __device__ __forceinline__ float round(float f) { return (float)(__bf16)f; }
-};
-template <> struct NormType<LLIMA_F16> {
-    static constexpr int E = 2;
-    static __device__ __forceinline__ void load(const void* p, float (&v)[8]) {
-        typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-        const h8 q = *(const h8*)p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)q[i];
-    }
-    static __device__ __forceinline__ void store(void* p, const float (&v)[8]) {
-        typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-        h8 q;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = (_Float16)v[i];
-        *(h8*)p = q;
-    }
-    static __device__ __forceinline__ float round(float f) { return (float)(_Float16)f; }
-};
-template <> struct NormType<LLIMA_F32> {
-    static constexpr int E = 4;
-    static __device__ __forceinline__ void load(const void* p, float (&v)[8]) {
-        const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    }
-    static __device__ __forceinline__ void store(void* p, const float (&v)[8]) {
-        ((float4*)p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        ((float4*)p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-    static __device__ __forceinline__ float round(float f) { return f; }
-};
-
-// The greatest of non-negative floats by their bits: NaN above infinity above
-// every number.
-__device__ __forceinline__ uint32_t nrm_abs(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
-__device__ __forceinline__ uint32_t nrm_umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-
-// e4m3 of 448 v / m, 8 values: 448 v / m as (0.875 v) / (m / 512), the same
-// value with no overflow on the way.
-__device__ __forceinline__ uint2 nrm_pack8(const float (&v)[8], float m) {
-    const float d = m * 0.001953125f;
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = v[i] * 0.875f / d;
-    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
-    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
-    return make_uint2((uint32_t)lo, (uint32_t)hi);
-}
 
 // One workgroup of 64 NWV threads per row; thread t holds the pieces of 8
 // values t + 64 NWV j, j < NP, of the row in registers between the two passes
@@ -192,14 +111,14 @@ __global__ __launch_bounds__(64 * NWV) void rms_rows(NormParams P) {
             uint32_t m = 0;
             if (in) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = nrm_umax(m, nrm_abs(w[i]));
+                for (int i = 0; i < 8; ++i) m = q8_umax(m, q8_abs(w[i]));
             }
 #pragma unroll
-            for (int o = 8; o >= 1; o >>= 1) m = nrm_umax(m, (uint32_t)__shfl_xor((int)m, o, 64));
-            m = nrm_umax(m, __float_as_uint(NRM_TINY));
+            for (int o = 8; o >= 1; o >>= 1) m = q8_umax(m, (uint32_t)__shfl_xor((int)m, o, 64));
+            m = q8_umax(m, __float_as_uint(Q8_TINY));
             const float mf = __uint_as_float(m);
             if (in) {
-                *(uint2*)((uint8_t*)P.out + (size_t)b * P.H + (size_t)p * 8) = nrm_pack8(w, mf);
+                *(uint2*)((uint8_t*)P.out + (size_t)b * P.H + (size_t)p * 8) = q8_pack8(w, mf);
                 if ((p & 15) == 0) P.scales[(size_t)b * P.NK + p / 16] = mf / 448.0f;
             }
         } else {
@@ -235,21 +154,21 @@ __global__ __launch_bounds__(LLIMA_WG) void fp8_blocks(const uint16_t* w, uint8_
         if (n < V && h < H) {                                // H % 8 == 0: a piece is inside or outside
             NormType<LLIMA_BF16>::load(w + (size_t)n * H + h, v[j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = nrm_umax(m, nrm_abs(v[j][i]));
+            for (int i = 0; i < 8; ++i) m = q8_umax(m, q8_abs(v[j][i]));
         }
     }
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) m = nrm_umax(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    for (int o = 32; o >= 1; o >>= 1) m = q8_umax(m, (uint32_t)__shfl_xor((int)m, o, 64));
     if ((t & 63) == 0) part[t >> 6] = m;
     __syncthreads();
-    m = nrm_umax(nrm_umax(part[0], part[1]), nrm_umax(part[2], part[3]));
-    m = nrm_umax(m, __float_as_uint(NRM_TINY));
+    m = q8_umax(q8_umax(part[0], part[1]), q8_umax(part[2], part[3]));
+    m = q8_umax(m, __float_as_uint(Q8_TINY));
     const float mf = __uint_as_float(m);
     if (t == 0) scales[(size_t)vb * NK + kb] = mf / 448.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int n = r0 + 16 * j;
-        if (n < V && h < H) *(uint2*)(out + (size_t)n * H + h) = nrm_pack8(v[j], mf);
+        if (n < V && h < H) *(uint2*)(out + (size_t)n * H + h) = q8_pack8(v[j], mf);
     }
 }
 
@@ -265,9 +184,6 @@ static void nrm_launch_np(const NormParams& P, hipStream_t st) {
         default: hipLaunchKernelGGL((rms_rows<DT, NWV, 0, Q8, NORM>), g, blk, 0, st, P); break;
     }
 }
-
-// A launch holds fewer than 2^32 threads.
-#define NRM_ROWS (1 << 23)
 
 template <int DT, bool Q8, bool NORM>
 static int nrm_launch(const NormParams& P, hipStream_t st) {
@@ -290,16 +206,6 @@ static int nrm_dispatch(const NormParams& P, int32_t dtype, hipStream_t st) {
     if (dtype == LLIMA_BF16) return nrm_launch<LLIMA_BF16, Q8, NORM>(P, st);
     if (dtype == LLIMA_F16) return nrm_launch<LLIMA_F16, Q8, NORM>(P, st);
     return nrm_launch<LLIMA_F32, Q8, NORM>(P, st);
-}
-
-static bool nrm_aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
-
-static int nrm_check(const void* x, int32_t dtype, int32_t B, int32_t H, int64_t stride) {
-    if (dtype != LLIMA_BF16 && dtype != LLIMA_F16 && dtype != LLIMA_F32) return LLIMA_E_INVAL;
-    if (B < 0 || H <= 0 || H % 8 != 0 || H > 65536) return LLIMA_E_INVAL;
-    const int64_t e = dtype == LLIMA_F32 ? 4 : 2;
-    if (B > 0 && (!x || !nrm_aligned(x) || stride * e % 16 != 0 || (B > 1 && stride < H))) return LLIMA_E_INVAL;
-    return LLIMA_OK;
 }
 
 }  // namespace llima

@@ -19,8 +19,9 @@ the buffers handed to it (inputs must already be on the GPU).
   topk(x, k)                          utils.hpp:216-281
   stop_check(tokens, stop_mask, V)    language_model.cpp:643-671 (the decode loops' stop rule)
   Eagle3DraftTree                     language_model_eagle3.cpp:808-1164 (topk_generate's selection)
-  add_rms_norm, quantize_rows,        no reference counterpart: the residual's addition and norm, and
-  Fp8LmHead, lm_head_quantize         the LM head over an 8-bit weight
+  add_rms_norm, sandwich_norm,        no reference counterpart: the residual's addition and norms, and
+  quantize_rows,                      the LM head over an 8-bit weight
+  Fp8LmHead, lm_head_quantize
 
 Errors: the reference throws std::invalid_argument / std::runtime_error; here
 ValueError / RuntimeError are raised for the same conditions.
@@ -46,7 +47,7 @@ __all__ = [
     "Workspace", "score_logits", "select_candidate_tokens", "argmax_gemma4_mtp_masked_rows",
     "argmax_gemma4_mtp_masked_row", "topk", "Eagle3DraftTree", "stop_mask", "stop_check",
     "lm_head_argmax", "lm_head_pack", "PackedLmHead", "Fp8LmHead", "Fp8Rows", "add_rms_norm",
-    "quantize_rows", "lm_head_quantize",
+    "quantize_rows", "lm_head_quantize", "sandwich_norm",
 ]
 
 
@@ -770,6 +771,63 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
                                        float(weight_offset), o.data_ptr(), sc, _ptr(r),
                                        _stream(dev)), "llima_add_rms_norm")
     return y, r
+
+
+def sandwich_norm(x: torch.Tensor, post_weight: Optional[torch.Tensor], residual: torch.Tensor,
+                  pre_weight: torch.Tensor, gate=None, residual_scale: float = 1.0, eps: float = 1e-6,
+                  weight_offset: float = 0.0, out: str = "same"):
+    """The norms on both sides of the residual stream between two blocks (llima_sandwich_norm) ->
+    (y, new residual stream).  The block's output x is normalised with post_weight (None: taken as it is),
+    multiplied by the gate and added to residual_scale * residual, rounded to the type: the new stream,
+    whose norm with pre_weight is y.  Norms as add_rms_norm's: (r * f) * (weight + weight_offset), f = 1 /
+    sqrt(mean(r^2) + eps).
+
+    x [..., H] and residual (the same shape) in bf16, fp16 or fp32, the weights [H] of that type; gate
+    None, a number, or a tensor of that type: [H] (a gate per channel) or x's shape.  out "same"
+    rounds y to the type; "fp8" returns Fp8Rows [rows, H].  H a multiple of 8, at most 65536."""
+    if out not in ("same", "fp8"):
+        raise ValueError("out must be 'same' or 'fp8'")
+    shape, H, dt = x.shape, x.shape[-1] if x.dim() else 0, x.dtype
+    if residual.shape != shape or residual.dtype != dt:
+        raise ValueError("residual must have x's shape and type")
+    a, r = _rows16(x, "sandwich_norm"), _rows16(residual, "sandwich_norm")
+    dev, B = a.device, a.shape[0]
+    ws = []
+    for w in (post_weight, pre_weight):
+        if w is not None:
+            if w.dim() != 1 or w.shape[0] != H or w.dtype != dt or w.device != dev:
+                raise ValueError("weights must be [H] of x's type, on its device")
+            w = w.contiguous()
+            w = w if w.data_ptr() % 16 == 0 else w.clone()
+        ws.append(w)
+    if ws[1] is None:
+        raise ValueError("pre_weight is needed")
+    g, gs, gp = None, 0, 1.0
+    if torch.is_tensor(gate):
+        if gate.shape not in (shape, shape[-1:]) or gate.dtype != dt:
+            raise ValueError("gate must be a number, [H] or of x's shape, of x's type")
+        g = _rows16(gate, "sandwich_norm")
+        gs = g.stride(0) if gate.shape == shape and B > 1 else 0
+    elif gate is not None:
+        gp = float(gate)
+    if r.device != dev or (g is not None and g.device != dev):
+        raise ValueError("sandwich_norm: tensors must be on one device")
+    if out == "fp8":
+        y = Fp8Rows.__new__(Fp8Rows)
+        y.values = torch.empty((B, H), dtype=torch.float8_e4m3fn, device=dev)
+        y.scales = torch.empty((B, -(-H // FP8_BLOCK)), dtype=torch.float32, device=dev)
+        o, sc = y.values.data_ptr(), y.scales.data_ptr()
+    else:
+        y = torch.empty(shape, dtype=dt, device=dev)
+        o, sc = y.data_ptr(), 0
+    s = torch.empty(shape, dtype=dt, device=dev)
+    args = _lib.SANDWICH_NORM_ARGS.pack(
+        a.data_ptr(), r.data_ptr(), 0 if g is None else g.data_ptr(), 0 if ws[0] is None else ws[0].data_ptr(),
+        ws[1].data_ptr(), o, sc, s.data_ptr(), a.stride(0), r.stride(0), gs, FLOAT_CODES[dt], B, H, float(eps),
+        float(weight_offset), float(residual_scale), gp)
+    with _on(dev):
+        check(lib().llima_sandwich_norm(args, _stream(dev)), "llima_sandwich_norm")
+    return y, s
 
 
 def _bf16_rows(hidden) -> None:
