@@ -13,6 +13,7 @@ caches are on the NPU.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -20,6 +21,8 @@ import torch
 from . import _lib
 from ._lib import check, lib
 from .sampler import FLOAT_CODES, _on, _on_gpu, _scratch, _stream
+
+F8 = torch.float8_e4m3fn
 
 __all__ = ["Fp8Cache", "cache_read", "cache_write", "tree_attention", "tree_commit"]
 
@@ -35,9 +38,10 @@ class Fp8Cache:
     __slots__ = ("values", "scales")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
-        if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        if values.dtype != F8 or scales.dtype != torch.float32:
             raise ValueError("Fp8Cache: values must be float8_e4m3fn and scales float32")
-        if values.dim() < 4 or values.shape[:-1] != scales.shape or values.shape[-1] not in (64, 128, 256):
+        shape = values.shape
+        if len(shape) < 4 or shape[:-1] != scales.shape or shape[-1] not in (64, 128, 256):
             raise ValueError("Fp8Cache: values [..., tokens, Hkv, D], D 64, 128 or 256, and scales [..., tokens, Hkv] are needed")
         _on_gpu(values, scales)
         if values.device != scales.device:
@@ -52,7 +56,7 @@ class Fp8Cache:
             raise ValueError("Fp8Cache.empty takes [..., tokens, Hkv, D]")
         n = (*shape[:-3], shape[-2], shape[-3])
         dev = device if device is not None else "cuda"
-        return cls(torch.empty((*n, shape[-1]), dtype=torch.float8_e4m3fn, device=dev).transpose(-3, -2),
+        return cls(torch.empty((*n, shape[-1]), dtype=F8, device=dev).transpose(-3, -2),
                    torch.empty(n, dtype=torch.float32, device=dev).transpose(-2, -1))
 
     @property
@@ -131,14 +135,23 @@ def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _folded(t: torch.Tensor) -> bool:
     """Whether values of a tensor may share memory: a stride less than what the smaller ones span."""
-    if t.is_contiguous():
-        return False
+    return not t.is_contiguous() and _folds(t.shape, t.stride())
+
+
+@lru_cache(256)
+def _folds(shape, stride) -> bool:
     end = 1
-    for s, n in sorted([(s, n) for n, s in zip(t.shape, t.stride()) if n > 1]):
+    for s, n in sorted([(s, n) for n, s in zip(shape, stride) if n > 1]):
         if s < end:
-            return t.numel() > 0
+            return 0 not in shape
         end += (n - 1) * s
     return False
+
+
+def _apart(ts) -> bool:
+    """Whether no two of the tensors' storages meet (then none shares memory with another)."""
+    spans = sorted([(s.data_ptr(), s.nbytes()) for s in [t.untyped_storage() for t in ts]])
+    return all([a + n <= b for (a, n), (b, _) in zip(spans, spans[1:])])
 
 
 def _cache(k_cache, v_cache, Hkv, D, dtype, block_table, B, dev):
@@ -208,8 +221,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     dev = q.device
     if not (k.device == v.device == k_cache.device == v_cache.device == dev):
         raise ValueError("tree_attention: tensors must be on one device")
-    page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, q.dtype if k8 is None else torch.float8_e4m3fn,
-                                        block_table, B, dev)
+    page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, q.dtype if k8 is None else F8, block_table, B, dev)
     lens = _ints(cache_lens, B, "cache_lens", dev)
     mask, mask_dtype, ms = tree_mask, _lib.LLIMA_MASK_U8, (0, 0)
     if mask is not None:
@@ -338,7 +350,7 @@ def _write8(name, k, v, k_cache, v_cache, cache_lens, nodes, counts, block_table
     dev = k.device
     if not (v.device == kq.device == vq.device == dev):
         raise ValueError(f"{name}: tensors must be on one device")
-    page, pages, blocks, table = _cache(kq, vq, Hkv, D, torch.float8_e4m3fn, block_table, B, dev)
+    page, pages, blocks, table = _cache(kq, vq, Hkv, D, F8, block_table, B, dev)
     lens = _ints(cache_lens, B, "cache_lens", dev)
     if counts is not None:
         counts = _ints(counts, B, "counts", dev)
@@ -352,12 +364,14 @@ def _write8(name, k, v, k_cache, v_cache, cache_lens, nodes, counts, block_table
     k, v = _heads(k), _heads(v)
     kq, vq = _in_place(kq, "k_cache", 16), _in_place(vq, "v_cache", 16)
     outs = (kq, vq, ks, vs)
-    if any([_shared(a, o) for a in (k, v) for o in outs]):
+    apart = _apart((k, v, *outs))                            # the usual case
+    if not apart and any([_shared(a, o) for a in (k, v) for o in outs]):
         raise ValueError(f"{name}: k and v must not overlap the caches (copy them first)")
     if any([_folded(o) for o in outs]):
         raise ValueError(f"{name}: a cache's own values must not overlap (expanded dimensions)")
-    if not (tied and _same(kq, vq) and _same(ks, vs)) and (_shared(kq, vq) or _shared(ks, vs)) or \
-            _shared(kq, ks) or _shared(vq, vs) or _shared(kq, vs) or _shared(vq, ks):
+    if not apart and (
+            not (tied and _same(kq, vq) and _same(ks, vs)) and (_shared(kq, vq) or _shared(ks, vs)) or
+            _shared(kq, ks) or _shared(vq, vs) or _shared(kq, vs) or _shared(vq, ks)):
         raise ValueError(f"{name}: k_cache and v_cache, values and scales, must not overlap")
     new = torch.empty(B, dtype=torch.int32, device=dev)
     if B == 0:
@@ -416,7 +430,7 @@ def cache_read(k_cache: Fp8Cache, v_cache: Fp8Cache, cache_lens: torch.Tensor,
     if vq.device != dev:
         raise ValueError("cache_read: tensors must be on one device")
     B = cache_lens.shape[0] if cache_lens.dim() == 1 else -1
-    page, pages, blocks, table = _cache(kq, vq, Hkv, D, torch.float8_e4m3fn, block_table, B, dev)
+    page, pages, blocks, table = _cache(kq, vq, Hkv, D, F8, block_table, B, dev)
     lens = _ints(cache_lens, B, "cache_lens", dev)
     n = page * blocks if tokens is None else int(tokens)
     if n < 0 or n > 1 << 30:

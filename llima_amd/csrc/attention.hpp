@@ -116,6 +116,7 @@ __device__ __forceinline__ int at_len(const AttnParams& P, int b, bool& bad) {
 #define AT_EXTRA 6
 template <int T>
 struct KeyTiles {
+    static constexpr int EXTRA = AT_EXTRA;
     static __device__ __forceinline__ int count(const AttnParams& P, int len) { return (len + P.N + T - 1) / T + AT_EXTRA; }
 };
 
@@ -129,9 +130,7 @@ __device__ __forceinline__ int64_t at_share(const AttnParams& P, int len0) {
         bool bad;
         total += TL::count(P, at_len(P, b, bad));
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
-    return (total + P.parts - 1) / P.parts;
+    return ((int64_t)wave_sum_u64((uint64_t)total) + P.parts - 1) / P.parts;
 }
 
 // The slot of the partial sums that share x has of sequence b (begins: from the
@@ -159,22 +158,17 @@ __device__ __forceinline__ bool at_find(const AttnParams& P, int64_t at, int len
         bool bad;
         const bool in = b0 + lane < P.B;
         const int ln = !in ? 0 : b0 ? at_len(P, b0 + lane, bad) : len0;
-        const int64_t n = in ? TL::count(P, ln) : 0;
-        int64_t incl = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t up = __shfl_up(incl, o, 64);
-            incl += lane >= o ? up : 0;
-        }
+        const uint32_t n = in ? (uint32_t)TL::count(P, ln) : 0u;   // 64 times 2^25 + 70 at most
+        const uint32_t incl = wave_incl_scan_u32(n);
         const uint64_t past = ballot(in && before + incl > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             b = b0 + l;
-            first = before + (int64_t)readlane64((uint64_t)(incl - n), l);
+            first = before + readlane(incl - n, l);
             len = (int)readlane((uint32_t)ln, l);
             return true;
         }
-        before += (int64_t)readlane64((uint64_t)incl, 63);
+        before += readlane63(incl);
     }
     return false;
 }
@@ -218,11 +212,10 @@ __global__ __launch_bounds__(LLIMA_WG) void tree_attn_join(AttnParams P) {
     if (b > 0) {                                             // uniform
         first = lane < b ? TL::count(P, len0) : 0;
         for (int i = 64 + lane; i < b; i += 64) first += TL::count(P, at_len(P, i, bad));
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, 64);
+        first = (int64_t)wave_sum_u64((uint64_t)first);
     }
     const int len = b < 64 ? (int)readlane((uint32_t)len0, (uint32_t)b) : at_len(P, b, bad);
-    const int64_t last = first + TL::count(P, len) - 1 - AT_EXTRA;
+    const int64_t last = first + TL::count(P, len) - 1 - TL::EXTRA;
     const int x0 = (int)(first / share), np = (int)(last / share) - x0 + 1;
     if (np <= 1) return;                                     // the same for a row's waves
     const int h = hq / P.G, row = n * P.G + hq % P.G;

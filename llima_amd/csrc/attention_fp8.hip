@@ -17,10 +17,12 @@
 // wave waits for another before the end of a sequence's part, where their sums are joined.
 //
 // The reference of the softmax moves only when a row's maximum passes it, and then 2^8
-// beyond: weights are at most 1, and the sums are rescaled seldom.  P is rounded to q's type
-// for its product with V; in fp16 the weights carry a factor of 2^15 and the values' scales
-// the inverse of the largest so far (a power of two), so that the product with a scale
-// neither overflows nor, down to 2^-29 of the largest, becomes subnormal.
+// beyond: weights are at most 1, and the sums are rescaled seldom.  For the product with V a
+// weight times its value's scale is rounded to fp16 whatever q's type (11 bits; in bf16 the
+// outputs' error against 64 bits was 0.0023 of their size, now 0.0017, that of the output's own
+// rounding); it carries a factor of 2^15 and the inverse of the largest scale so far (a power
+// of two), so that it neither overflows nor, down to 2^-29 of the largest, becomes subnormal.
+// The drafted tokens' values are of q's type, and so are their weights.
 #include "attention.hpp"
 
 namespace llima {
@@ -28,7 +30,12 @@ namespace llima {
 struct At8Params : AttnParams {
     const float *ksc, *vsc;
     int64_t kss[3], vss[3];                                  // scales: page, token and head strides (elements)
+    uint32_t g_mul, g_shift;                                 // row / G
 };
+
+// The arguments, loaded anew where they are used (at_args).
+typedef const __attribute__((address_space(4))) At8Params* At8Args;
+__device__ __forceinline__ At8Args a8_args() { return (At8Args)at_args(); }
 
 template <int D> struct A8 {
     static constexpr int NW = 4;                             // waves
@@ -37,7 +44,7 @@ template <int D> struct A8 {
     static constexpr int S = D == 64 ? 3 : 2;                // stages of a wave's ring
     static constexpr int ST = 2 * KT * D + 256;              // bytes of a stage: K, V, their scales
     static constexpr int T = NW * KT, TD = NW * DK;          // keys of a tile of the workgroup
-    static constexpr int MAXM = D == 256 ? 2 : 4;            // row tiles of 16
+    static constexpr int MAXM = D == 256 ? 2 : 4;            // row tiles of 16 of a workgroup at most
     static constexpr int QL = D == 256 ? 1 : D == 128 ? 3 : 4;   // of them in LDS at most (two workgroups per CU), the rest in registers
 };
 
@@ -46,9 +53,10 @@ template <int D> struct A8 {
 // The partition's unit: tiles of T cached keys, then tiles of TD drafted ones.
 template <int D>
 struct Fp8Tiles {
-    static __device__ __forceinline__ int cached(int len) { return (len + A8<D>::T - 1) / A8<D>::T; }
-    static __device__ __forceinline__ int drafted(int N) { return (N + A8<D>::TD - 1) / A8<D>::TD; }
-    static __device__ __forceinline__ int count(const AttnParams& P, int len) { return cached(len) + drafted(P.N) + AT_EXTRA; }
+    static constexpr int EXTRA = 4;                          // what a sequence's start and end take, as AT_EXTRA
+    static __device__ __forceinline__ int cached(int len) { return (int)((uint32_t)(len + A8<D>::T - 1) / (uint32_t)A8<D>::T); }
+    static __device__ __forceinline__ int drafted(int N) { return (int)((uint32_t)(N + A8<D>::TD - 1) / (uint32_t)A8<D>::TD); }
+    static __device__ __forceinline__ int count(const AttnParams& P, int len) { return cached(len) + drafted(P.N) + EXTRA; }
 };
 
 typedef float a8_acc __attribute__((ext_vector_type(4)));
@@ -89,12 +97,20 @@ template <int DT> __device__ __forceinline__ at_s8 a8_wide(uint32_t lo, uint32_t
     return __builtin_bit_cast(at_s8, w);
 }
 
+// The greatest of three; NaN is left out.  (As builtins, every operand is
+// canonicalised first.)
+__device__ __forceinline__ float a8_max(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
 // The maximum, or the sum, over the four lanes of a query row (l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float a8_max4(float x) {
     auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __builtin_fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    x = a8_max(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[1]));
     s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __builtin_fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    return a8_max(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[1]));
 }
 __device__ __forceinline__ float a8_sum4(float x) {
     auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -129,7 +145,7 @@ template <int ROW> __device__ __forceinline__ uint32_t a8_swz(uint32_t key) {
 // its address comes from the scalar unit; or each 1 KB request of it does (AT_REQUEST), or
 // every lane computes its own (AT_LANE).  GEN: the last two modes.
 template <int DT, int D, int M, bool GEN>
-__global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
+__global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #ifdef __HIP_DEVICE_COMPILE__                               // (the host pass drops the launch stub over the descriptors)
     using C = A8<D>;
     constexpr int NW = C::NW, KT = C::KT, DK = C::DK, S = C::S, ST = C::ST, T = C::T, TD = C::TD;
@@ -150,22 +166,17 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
     uint32_t* const flag = (uint32_t*)(sq + QL * QT);        // a bad page or length; special values
     const int t = (int)threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int part = (int)(blockIdx.x / (uint32_t)(P.Hkv * P.RG)), hr = (int)(blockIdx.x % (uint32_t)(P.Hkv * P.RG));
-    const int h = hr / P.RG, rg = hr % P.RG;
+    // workgroups go to the 8 XCDs in turn: the row groups of a share and head on one of them, side by side, so
+    // that its keys come from memory once and from that XCD's L2 for the other groups
+    const uint32_t turn = blockIdx.x / 8u, pair = turn / (uint32_t)P.RG * 8u + blockIdx.x % 8u;
+    const int rg = (int)(turn % (uint32_t)P.RG), part = (int)(pair / (uint32_t)P.Hkv), h = (int)(pair % (uint32_t)P.Hkv);
+    if (part >= P.parts) return;                             // (the grid is a multiple of 8)
     uint8_t* const ring = sm + wave * (S * ST);
     bool bad = false, miss = false;
     const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
     const int64_t share = (int64_t)readfirstlane64((uint64_t)at_share<Fp8Tiles<D>>(P, len0));
     const int64_t end = (part + 1) * share;
     const int nd = Fp8Tiles<D>::drafted(P.N);
-    const int kq = lane / U, unit = lane % U, kq2 = lane / U2, unit2 = lane % U2;
-    uint32_t okv[NQ], ovv[NQ];                               // the lane's offsets within a tile of one page
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-        const uint32_t key = (uint32_t)(i * KQ + kq), u = (uint32_t)(unit ^ a8_swz<D>(key)) * 16;
-        okv[i] = key * (uint32_t)P.kcs[1] + u;
-        ovv[i] = key * (uint32_t)P.vcs[1] + u;
-    }
     for (int64_t from = part * share; from < end;) {         // the share's sequences
     int b, len;
     int64_t first;
@@ -174,9 +185,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
     len = __builtin_amdgcn_readfirstlane(len);
     first = (int64_t)readfirstlane64((uint64_t)first);
     const int nc = Fp8Tiles<D>::cached(len), nt = nc + nd;
-    const int64_t last = first + nt + AT_EXTRA, upto = last < end ? last : end;
-    const int c0 = (int)(from - first), c1 = upto - first < nt ? (int)(upto - first) : nt;
-    const bool whole = from == first && upto >= last - AT_EXTRA;   // the sequence has no other part
+    const int64_t last = first + nt + Fp8Tiles<D>::EXTRA, upto = last < end ? last : end;
+    const int c0 = __builtin_amdgcn_readfirstlane((int)(from - first));
+    const int c1 = __builtin_amdgcn_readfirstlane(upto - first < nt ? (int)(upto - first) : nt);
+    const bool whole = from == first && upto >= last - Fp8Tiles<D>::EXTRA;   // the sequence has no other part
     from = upto;
     if (c0 >= nt) continue;                                  // uniform: nothing of it but the extra tiles
     // the wave's tiles: cached ones c0 .., then drafted ones d0 ..
@@ -186,7 +198,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
     const int d0 = (c0 > nc ? c0 : nc) - nc, dend = c1 - nc;
     int nD = dend > d0 ? dend - d0 : 0;
     if (nD > 0 && (dend - 1) * TD + wave * DK >= P.N) --nD;
-    const int ntile = nC + nD;
+    nC = __builtin_amdgcn_readfirstlane(nC);
+    const int ntile = nC + __builtin_amdgcn_readfirstlane(nD);
     __syncthreads();                                         // (the sequence before is done with LDS)
     if (t == 0) {
         bool wrong;
@@ -212,6 +225,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         return out ? 0 : p;
     };
     auto inside = [&](int j) { return P.table ? j - (int)at_page(P.page_mul, P.page_shift, j) * P.page : j; };
+    // a head's first row of page p, place o (uniform)
+    const uint8_t* const kh = (const uint8_t*)P.kc + h * P.kcs[2];
+    const uint8_t* const vh = (const uint8_t*)P.vc + h * P.vcs[2];
+    const float *const ksh = P.ksc + h * P.kss[2], *const vsh = P.vsc + h * P.vss[2];
     auto lds = [](uint8_t* p) { return (__attribute__((address_space(3))) void*)p; };
     auto rsrc = [](const void* p) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7FFFFFFF, 0x00027000); };
     int pg = 0;                                              // the page of the next tile to request; GEN: of the lane's key
@@ -221,121 +238,130 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         if constexpr (GEN) pg = pages_of(j, len - j);
         else if (P.table) pg = page_of(j);                   // uniform
     };
+    // lane numbers that the compiler does not know to be the same in every tile: what is made from them is not
+    // kept in registers, nor spilled
+    auto fresh = [&](int x) {
+        if constexpr (M * D > 256) asm volatile("" : "+v"(x));
+        return (uint32_t)x;
+    };
     // a cached tile, the lane's own addresses; its n keys, the last of them again behind it
     auto issue_lanes = [&](int j, int n, int pgl, uint8_t* st) {
+        const At8Args A = a8_args();
+        const int ln = (int)fresh(lane), kq = ln / U, unit = ln % U;
 #pragma unroll 1
         for (int i = 0; i < 2 * NQ; ++i) {
             const int ki = (i % NQ) * KQ + kq, k = ki < n ? ki : n - 1;
             const int p = known(__shfl(pgl, k, 64)), o = inside(j + k);
             const uint32_t u = (uint32_t)(unit ^ a8_swz<D>((uint32_t)ki)) * 16;
-            const uint8_t* src = i < NQ ? (const uint8_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2]
-                                        : (const uint8_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2];
+            const uint8_t* src = i < NQ ? kh + p * A->kcs[0] + o * A->kcs[1] : vh + p * A->vcs[0] + o * A->vcs[1];
             at_dma(src + u, st + i * 1024);
             if (i % NQ == NQ - 1) {                          // uniform: K's or V's scales
                 const int ks = (lane & (KT - 1)) < n ? (lane & (KT - 1)) : n - 1, ps = known(pgl), os = inside(j + ks);
-                const float* sc = i < NQ ? P.ksc + ps * P.kss[0] + os * P.kss[1] + h * P.kss[2]
-                                         : P.vsc + ps * P.vss[0] + os * P.vss[1] + h * P.vss[2];
+                const float* sc = i < NQ ? ksh + ps * A->kss[0] + os * A->kss[1] : vsh + ps * A->vss[0] + os * A->vss[1];
                 if (lane < KT)
                     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)sc,
                                                      (__attribute__((address_space(3))) void*)(st + 2 * KT * D + i / NQ * (KT * 4)), 4, 0, 0);
             }
         }
     };
-    auto issue = [&](int tile, uint8_t* st) {
+    auto issue = [&](int tile, uint8_t* st) __attribute__((always_inline)) {
         if (tile < nC) {                                     // uniform
             const int j = key_of(tile), n = len - j < KT ? len - j : KT;
-            if constexpr (!GEN) {
-                if (n == KT) {                               // uniform
-                    const int p = known(pg), o = inside(j);
-                    const auto rk = rsrc((const uint8_t*)P.kc + p * P.kcs[0] + o * P.kcs[1] + h * P.kcs[2]);
-                    const auto rv = rsrc((const uint8_t*)P.vc + p * P.vcs[0] + o * P.vcs[1] + h * P.vcs[2]);
-                    const auto sk = rsrc(P.ksc + p * P.kss[0] + o * P.kss[1] + h * P.kss[2]);
-                    const auto sv = rsrc(P.vsc + p * P.vss[0] + o * P.vss[1] + h * P.vss[2]);
+            const int pgl = pg;
+            lookup(tile + 1);
+            const uint32_t ln = fresh(lane), kq = ln / U;
+            auto unit_at = [&](int i) { return ((ln % U) ^ a8_swz<D>((uint32_t)(i * KQ) + kq)) * 16; };   // of request i
+            if (!GEN && n == KT) {                           // uniform
+                const int p = known(pgl), o = inside(j);
+                const auto rk = rsrc(kh + p * P.kcs[0] + o * P.kcs[1]), rv = rsrc(vh + p * P.vcs[0] + o * P.vcs[1]);
+                const auto sk = rsrc(ksh + p * P.kss[0] + o * P.kss[1]), sv = rsrc(vsh + p * P.vss[0] + o * P.vss[1]);
+                auto requests = [&](auto nt) {
+                    constexpr int AUX = decltype(nt)::value;
 #pragma unroll
                     for (int i = 0; i < NQ; ++i)
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds(st + i * 1024), 16, (int)okv[i], 0, 0, 0);
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds(st + i * 1024), 16, (int)(kq * (uint32_t)P.kcs[1] + unit_at(i)), i * KQ * (int)P.kcs[1], 0, AUX);
                     if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sk, lds(st + 2 * KT * D), 4, lane * (int)(4 * P.kss[1]), 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < NQ; ++i)
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds(st + KT * D + i * 1024), 16, (int)ovv[i], 0, 0, 0);
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds(st + KT * D + i * 1024), 16, (int)(kq * (uint32_t)P.vcs[1] + unit_at(i)), i * KQ * (int)P.vcs[1], 0, AUX);
                     if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sv, lds(st + 2 * KT * D + KT * 4), 4, lane * (int)(4 * P.vss[1]), 0, 0, 0);
-                } else {
-                    issue_lanes(j, n, pages_of(j, n), st);
-                }
-            } else if (P.mode == AT_REQUEST && n == KT) {    // uniform
-                const int pgl = pg;
-                lookup(tile + 1);
+                };
+                // values that one workgroup reads pass by L2; those of several row groups stay in it
+                if (P.RG == 1) requests(std::integral_constant<int, 2>{});   // uniform
+                else requests(std::integral_constant<int, 0>{});
+            } else if (GEN && P.mode == AT_REQUEST && n == KT) {   // uniform
                 int p[NQ], o[NQ];
 #pragma unroll
                 for (int i = 0; i < NQ; ++i) {
                     p[i] = known((int)readlane((uint32_t)pgl, (uint32_t)(i * KQ)));
                     o[i] = inside(j + i * KQ);
                 }
-                // the lane's key of the scales
-                int pl = p[0], ol = o[0];
+                int pl = p[0], ol = o[0];                    // the lane's key of the scales
 #pragma unroll
                 for (int i = 1; i < NQ; ++i)
                     if ((lane & (KT - 1)) >= i * KQ) { pl = p[i]; ol = o[i]; }
                 ol += lane & (KQ - 1);
 #pragma unroll
                 for (int i = 0; i < NQ; ++i)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc((const uint8_t*)P.kc + p[i] * P.kcs[0] + o[i] * P.kcs[1] + h * P.kcs[2]),
-                        lds(st + i * 1024), 16, (int)(okv[i] - (uint32_t)(i * KQ) * (uint32_t)P.kcs[1]), 0, 0, 0);
-                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(P.ksc + h * P.kss[2]), lds(st + 2 * KT * D), 4,
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(kh + p[i] * P.kcs[0] + o[i] * P.kcs[1]), lds(st + i * 1024), 16,
+                        (int)(kq * (uint32_t)P.kcs[1] + unit_at(i)), 0, 0, 0);
+                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(ksh), lds(st + 2 * KT * D), 4,
                         (pl * (int)P.kss[0] + ol * (int)P.kss[1]) * 4, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < NQ; ++i)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc((const uint8_t*)P.vc + p[i] * P.vcs[0] + o[i] * P.vcs[1] + h * P.vcs[2]),
-                        lds(st + KT * D + i * 1024), 16, (int)(ovv[i] - (uint32_t)(i * KQ) * (uint32_t)P.vcs[1]), 0, 0, 0);
-                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(P.vsc + h * P.vss[2]), lds(st + 2 * KT * D + KT * 4), 4,
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(vh + p[i] * P.vcs[0] + o[i] * P.vcs[1]), lds(st + KT * D + i * 1024), 16,
+                        (int)(kq * (uint32_t)P.vcs[1] + unit_at(i)), 0, 0, 0);
+                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(vsh), lds(st + 2 * KT * D + KT * 4), 4,
                         (pl * (int)P.vss[0] + ol * (int)P.vss[1]) * 4, 0, 0, 0);
-                return;
             } else {
-                const int pgl = pg;
-                lookup(tile + 1);
-                issue_lanes(j, n, pgl, st);
-                return;
+                issue_lanes(j, n, GEN ? pgl : pages_of(j, n), st);
             }
-            lookup(tile + 1);
         } else {
-            const int m0 = draft_of(tile), n = P.N - m0 < DK ? P.N - m0 : DK;
+            const At8Args A = a8_args();
+            const int m0 = draft_of(tile), n = A->N - m0 < DK ? A->N - m0 : DK;
+            const int ln = (int)fresh(lane), kq2 = ln / U2, unit2 = ln % U2;
 #pragma unroll 1
             for (int i = 0; i < 2 * NQ; ++i) {
                 const int ki = (i % NQ) * KQ2 + kq2, k = ki < n ? ki : n - 1;
                 const uint32_t u = (uint32_t)(unit2 ^ a8_swz<2 * D>((uint32_t)ki)) * 16;
-                const uint16_t* src = i < NQ ? (const uint16_t*)P.k + b * P.ks[0] + (int64_t)(m0 + k) * P.ks[1] + h * P.ks[2]
-                                             : (const uint16_t*)P.v + b * P.vs[0] + (int64_t)(m0 + k) * P.vs[1] + h * P.vs[2];
+                const uint16_t* src = i < NQ ? (const uint16_t*)A->k + b * A->ks[0] + (int64_t)(m0 + k) * A->ks[1] + h * A->ks[2]
+                                             : (const uint16_t*)A->v + b * A->vs[0] + (int64_t)(m0 + k) * A->vs[1] + h * A->vs[2];
                 at_dma((const uint8_t*)src + u, st + i * 1024);
             }
         }
     };
     // ---------------------------------------------------------------- Q, loaded before the first requests
     const int row0 = rg * M * 16;
-    auto row_of = [&](int m) { const int row = row0 + m * 16 + r; return row < P.R ? row : P.R - 1; };
-    auto q_at = [&](int row, int col) {
-        row = row < P.R ? row : P.R - 1;
-        return (const uint16_t*)P.q + b * P.qs[0] + (int64_t)(row / P.G) * P.qs[1] + (h * P.G + row % P.G) * P.qs[2] + col;
+    auto last_row = [&](int row) { return row < P.R ? row : P.R - 1; };
+    auto node_of = [&](At8Args A, int row) { return (int)at_page(A->g_mul, A->g_shift, row); };   // row's node; its query head
+    auto head_of = [&](At8Args A, int row, int n) { return h * A->G + row - n * A->G; };
+    auto q_at = [&](At8Args A, int row, int col) {
+        row = last_row(row);
+        const int n = node_of(A, row);
+        return (const uint16_t*)A->q + b * A->qs[0] + (int64_t)n * A->qs[1] + (int64_t)head_of(A, row, n) * A->qs[2] + col;
     };
-    constexpr int QI = (QL * 16 * U2 + 255) / 256;
+    const At8Args AQ = a8_args();
+    const int tq = (int)fresh(t);
+    constexpr int QI = (QL * 16 * U2 + 64 * NW - 1) / (64 * NW);
     llima_u32x4 ql[QI];
 #pragma unroll
     for (int e = 0; e < QI; ++e) {
-        const int i = t + e * 256;
-        ql[e] = *(const llima_u32x4*)q_at(row0 + i / U2, i % U2 * 8);
+        const int i = tq + e * 64 * NW;
+        ql[e] = *(const llima_u32x4*)q_at(AQ, row0 + i / U2, i % U2 * 8);
     }
     at_s8 qr[QR > 0 ? QR : 1][D / 32];
 #pragma unroll
     for (int m = 0; m < QR; ++m)
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s) qr[m][s] = *(const at_s8*)q_at(row_of(QL + m), (s >> 1) * 64 + g * 16 + (s & 1) * 8);
+        for (int s = 0; s < D / 32; ++s) qr[m][s] = *(const at_s8*)q_at(AQ, row0 + (QL + m) * 16 + (tq & 15), (s >> 1) * 64 + (tq >> 4 & 3) * 16 + (s & 1) * 8);
     asm volatile("" ::: "memory");
     lookup(0);
     for (int e = 0; e < S - 1 && e < ntile; ++e) issue(e, ring + e * ST);
 #pragma unroll
     for (int e = 0; e < QI; ++e) {
-        const int i = t + e * 256, rw = i / U2;
+        const int i = tq + e * 64 * NW, rw = i / U2;
         if (P.flip) ql[e] ^= 0x80008000u;                    // uniform: a negative scale's sign goes to q
-        if (QL * 16 * U2 % 256 == 0 || rw < QL * 16)
+        if (QL * 16 * U2 % (64 * NW) == 0 || rw < QL * 16)
             *(llima_u32x4*)(sq + rw * 2 * D + ((uint32_t)(i % U2) ^ a8_swz<2 * D>((uint32_t)(rw & 15))) * 16) = ql[e];
     }
 #pragma unroll
@@ -345,13 +371,15 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
             if (P.flip) qr[m][s] ^= (short)0x8000;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     // step s of a product takes columns 64 (s / 2) + 16 g + 8 (s % 2) + 0 .. 7 of the lane
-    auto qread = [&](int m, int s) {
-        if (m < QL) return *(const at_s8*)(sq + m * QT + r * 2 * D + ((uint32_t)((s >> 1) * 8 + 2 * g + (s & 1)) ^ a8_swz<2 * D>((uint32_t)r)) * 16);
+    auto qread = [&](int m, int s, uint32_t base) {
+        if (m < QL) return *(const at_s8*)(sq + m * QT + (base ^ (uint32_t)((s >> 1) * 128 + (s & 1) * 16)));
         return qr[m < QL ? 0 : m - QL][s];
     };
+    // the lane's place of step 0 in a row tile of Q
+    auto qplace = [&](uint32_t rr, uint32_t gg) { return rr * 2 * D + ((2 * gg) ^ a8_swz<2 * D>(rr)) * 16; };
     // ---------------------------------------------------------------- products
     a8_acc o[M][DB];
-    float ref[M], l[M], vref = DT == LLIMA_F16 ? 0.0f : 1.0f, vinv = DT == LLIMA_F16 ? 0.0f : 1.0f;
+    float ref[M], l[M], vref = 0.0f, vinv = 0.0f;            // the unit of the sums over 2^15, and its inverse
 #pragma unroll
     for (int m = 0; m < M; ++m) {
         ref[m] = -__builtin_inff();
@@ -359,10 +387,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[m][d] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // fp16: the sums' unit is a power of two that no scale so far exceeds (an infinite one but for)
+    // the sums' unit is a power of two that no scale so far exceeds (an infinite one but for)
     auto unit_for = [&](float top) {
         top = __builtin_fminf(top, 8.507059173023462e37f);   // 2^126
-        if (DT == LLIMA_F16 && __any(top > vref)) {
+        if (__any(top > vref)) {
             const float nr = __uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u), a = vref / nr;
 #pragma unroll
             for (int m = 0; m < M; ++m)
@@ -379,10 +407,9 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         bool up = false;
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            float a = __builtin_fmaxf(__builtin_fmaxf(x[m][0][0], x[m][0][1]), __builtin_fmaxf(x[m][0][2], x[m][0][3]));
+            float a = a8_max(x[m][0][0], x[m][0][1], a8_max(x[m][0][2], x[m][0][3], x[m][0][3]));
 #pragma unroll
-            for (int k = 1; k < BL; ++k)
-                a = __builtin_fmaxf(a, __builtin_fmaxf(__builtin_fmaxf(x[m][k][0], x[m][k][1]), __builtin_fmaxf(x[m][k][2], x[m][k][3])));
+            for (int k = 1; k < BL; ++k) a = a8_max(x[m][k][0], x[m][k][1], a8_max(x[m][k][2], x[m][k][3], a));
             mt[m] = a8_max4(a);
             up |= mt[m] > ref[m];
         }
@@ -399,7 +426,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            const float mu = (ref[m] > -__builtin_inff() ? ref[m] : 0.0f) - (DT == LLIMA_F16 ? 15.0f : 0.0f);
+            const float mu = (ref[m] > -__builtin_inff() ? ref[m] : 0.0f) - 15.0f;
 #pragma unroll
             for (int k = 0; k < BL; ++k)
 #pragma unroll
@@ -410,8 +437,9 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         }
     };
     auto lds_at = [](const uint8_t* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p; };
-    // A staged tile of n cached keys; K has landed, `more` waits for V.
-    auto math8 = [&](const uint8_t* st, int n, auto more) __attribute__((always_inline)) {
+    // A staged tile of n cached keys; K has landed, and V too unless there are requests of more tiles.
+    auto math8 = [&](const uint8_t* st, int n, bool more) __attribute__((always_inline)) {
+        const uint32_t rr = fresh(r), gg = fresh(g), qb = qplace(rr, gg);
         a8_acc x[M][NB], ks[NB];
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
@@ -419,12 +447,13 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
 #pragma unroll
             for (int m = 0; m < M; ++m) x[m][k] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
         }
+        __builtin_amdgcn_s_setprio(1);                       // the wave with products to issue goes before the one in the softmax
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
             llima_u32x4 kr[NB];
 #pragma unroll
             for (int k = 0; k < NB; ++k)
-                kr[k] = *(const llima_u32x4*)(st + (k * 16 + r) * D + ((uint32_t)(4 * c + g) ^ a8_swz<D>((uint32_t)(k * 16 + r))) * 16);
+                kr[k] = *(const llima_u32x4*)(st + k * 16 * D + ((rr * D + (gg ^ a8_swz<D>(rr)) * 16) ^ (uint32_t)(c * 64)));
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 at_s8 kf[NB];
@@ -432,104 +461,133 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
                 for (int k = 0; k < NB; ++k) kf[k] = a8_wide<DT>(kr[k][2 * s], kr[k][2 * s + 1]);
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
-                    const at_s8 q = qread(m, 2 * c + s);
+                    const at_s8 q = qread(m, 2 * c + s, qb);
 #pragma unroll
                     for (int k = 0; k < NB; ++k) x[m][k] = a8_mfma<DT>(kf[k], q, x[m][k]);
                 }
+                __builtin_amdgcn_sched_barrier(0);           // (else the reads of Q come all at once)
             }
         }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int k = 0; k < NB; ++k) {
-                x[m][k] *= ks[k];
-                if (n < KT) {                                // uniform: the sequence's last cached keys
+            for (int k = 0; k < NB; ++k) x[m][k] *= ks[k];
+        if (n < KT) {                                        // uniform: the sequence's last cached keys
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[m][k][i] = k * 16 + 4 * g + i < n ? x[m][k][i] : -__builtin_inff();
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = k * 16 + 4 * (int)gg + i < n;
+#pragma unroll
+                    for (int m = 0; m < M; ++m) x[m][k][i] = in ? x[m][k][i] : -__builtin_inff();
                 }
-            }
+        }
         softmax(x, std::integral_constant<int, NB>{});
-        more();
+        if (more) a8_wait<(S - 1) * NR>();                   // uniform
         a8_acc vs[NB];
 #pragma unroll
         for (int k = 0; k < NB; ++k) vs[k] = *(const a8_acc*)(st + 2 * KT * D + KT * 4 + k * 64 + g * 16);
-        if constexpr (DT == LLIMA_F16) {
-            float top = 0.0f;
+        float top = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NB; ++k) top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fmaxf(vs[k][0], vs[k][1]), __builtin_fmaxf(vs[k][2], vs[k][3])));
-            unit_for(a8_max4(top));
+        for (int k = 0; k < NB; ++k) top = a8_max(vs[k][0], vs[k][1], a8_max(vs[k][2], vs[k][3], top));
+        unit_for(a8_max4(top));
 #pragma unroll
-            for (int k = 0; k < NB; ++k) vs[k] *= vinv;
-        }
+        for (int k = 0; k < NB; ++k) vs[k] *= vinv;
         uint32_t pw[M][2 * NB];
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
                 const a8_acc y = x[m][k] * vs[k];
-                pw[m][2 * k] = at_pack<DT>(y[0], y[1]);
-                pw[m][2 * k + 1] = at_pack<DT>(y[2], y[3]);
+                pw[m][2 * k] = at_pack<LLIMA_F16>(y[0], y[1]);
+                pw[m][2 * k + 1] = at_pack<LLIMA_F16>(y[2], y[3]);
             }
+        __builtin_amdgcn_s_setprio(1);
         // V: a transposing load takes 8 rows of 16 bytes from 16 lanes (row i / 2 of lane i, half i % 2)
-        const int e = r >> 1;
+        const uint32_t e = rr >> 1;
         if constexpr (NB == 2) {                             // keys 4 g + 0 .. 3 and 16 more of a column block
-            const uint32_t key = (uint32_t)(4 * g + (e & 3) + (e >> 2) * 16);
-            const uint32_t base = lds_at(st) + KT * D + key * D + (uint32_t)(r & 1) * 8, z = a8_swz<D>(key);
+            const uint32_t key = 4 * gg + (e & 3) + (e >> 2) * 16;
+            const uint32_t base = KT * D + ((key * D + (rr & 1) * 8) | (a8_swz<D>(key) << 4)), at = lds_at(st);
 #pragma unroll
             for (int d = 0; d < DB; d += 4) {
                 uint32_t a[4];
                 a8_i2 v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = base + (((uint32_t)(d + i) ^ z) << 4);
+                for (int i = 0; i < 4; ++i) a[i] = at + (base ^ (uint32_t)((d + i) << 4));
                 a8_tr8(a, v);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const at_s8 vf = a8_wide<DT>((uint32_t)v[i][0], (uint32_t)v[i][1]);
+                    const at_s8 vf = a8_wide<LLIMA_F16>((uint32_t)v[i][0], (uint32_t)v[i][1]);
 #pragma unroll
                     for (int m = 0; m < M; ++m)
-                        o[m][d + i] = a8_mfma<DT>(vf, __builtin_bit_cast(at_s8, (llima_u32x4){pw[m][0], pw[m][1], pw[m][2 * NB - 2], pw[m][2 * NB - 1]}), o[m][d + i]);
+                        o[m][d + i] = a8_mfma<LLIMA_F16>(vf, __builtin_bit_cast(at_s8, (llima_u32x4){pw[m][0], pw[m][1], pw[m][2 * NB - 2], pw[m][2 * NB - 1]}), o[m][d + i]);
                 }
             }
         } else {                                             // keys 4 g + 0 .. 3 of two column blocks
-            const uint32_t key = (uint32_t)(4 * g + (e & 3));
-            const uint32_t base = lds_at(st) + KT * D + key * D + (uint32_t)(r & 1) * 8, z = a8_swz<D>(key);
+            const uint32_t key = 4 * gg + (e & 3);
+            const uint32_t base = KT * D + ((key * D + (rr & 1) * 8) | (a8_swz<D>(key) ^ (e >> 2)) << 4), at = lds_at(st);
 #pragma unroll
             for (int d = 0; d < DB; d += 8) {
                 uint32_t a[4];
                 a8_i2 v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = base + (((uint32_t)(d + 2 * i + (e >> 2)) ^ z) << 4);
+                for (int i = 0; i < 4; ++i) a[i] = at + (base ^ (uint32_t)((d + 2 * i) << 4));
                 a8_tr8(a, v);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const at_s8 vf = a8_wide<DT>((uint32_t)v[i][0], (uint32_t)v[i][1]);
+                    const at_s8 vf = a8_wide<LLIMA_F16>((uint32_t)v[i][0], (uint32_t)v[i][1]);
 #pragma unroll
                     for (int m = 0; m < M; ++m) {
                         const at_s4 pf = __builtin_bit_cast(at_s4, (a8_i2){(int)pw[m][0], (int)pw[m][1]});
-                        o[m][d + 2 * i] = a8_mfma<DT>(__builtin_shufflevector(vf, vf, 0, 1, 2, 3), pf, o[m][d + 2 * i]);
-                        o[m][d + 2 * i + 1] = a8_mfma<DT>(__builtin_shufflevector(vf, vf, 4, 5, 6, 7), pf, o[m][d + 2 * i + 1]);
+                        o[m][d + 2 * i] = a8_mfma<LLIMA_F16>(__builtin_shufflevector(vf, vf, 0, 1, 2, 3), pf, o[m][d + 2 * i]);
+                        o[m][d + 2 * i + 1] = a8_mfma<LLIMA_F16>(__builtin_shufflevector(vf, vf, 4, 5, 6, 7), pf, o[m][d + 2 * i + 1]);
                     }
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     };
-    auto seen = [&](int n, int mm) {                         // node n sees drafted token mm
-        if (!P.mask) return mm <= n;
-        if (P.mask_f32) return ((const float*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] > 0.0f;
-        return ((const uint8_t*)P.mask)[b * P.ms[0] + n * P.ms[1] + mm] != 0;
+    auto seen = [&](At8Args A, int n, int mm) {              // node n sees drafted token mm
+        if (!A->mask) return mm <= n;
+        if (A->mask_f32) return ((const float*)A->mask)[b * A->ms[0] + n * A->ms[1] + mm] > 0.0f;
+        return ((const uint8_t*)A->mask)[b * A->ms[0] + n * A->ms[1] + mm] != 0;
     };
     // A staged tile of n drafted tokens from m0 on.
     auto math16 = [&](uint8_t* st, int m0, int n) __attribute__((always_inline)) {
+        const At8Args A = a8_args();
+        const int r = (int)fresh(t) & 15, g = (int)fresh(t) >> 4 & 3;
         a8_acc x[M][1];
-        bool sees[M][4];
+        uint32_t sees[M];                                    // bit i: the row sees token m0 + 4 g + i
+        auto masks = [&](auto at) {                          // every load before the first use
+            decltype(at(0)) v[M][4];
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[m][i] = at(b * A->ms[0] + node_of(A, last_row(row0 + m * 16 + r)) * A->ms[1] + m0 + (4 * g + i < n ? 4 * g + i : n - 1));
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                sees[m] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sees[m] |= v[m][i] > 0 ? 1u << i : 0u;
+            }
+        };
+        if (!A->mask) {                                      // uniform
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const int c = node_of(A, last_row(row0 + m * 16 + r)) - m0 - 4 * g + 1;
+                sees[m] = c <= 0 ? 0u : c >= 4 ? 15u : (1u << c) - 1;
+            }
+        } else if (A->mask_f32) {                            // uniform
+            masks([&](int64_t i) { return ((const float*)A->mask)[i]; });
+        } else {
+            masks([&](int64_t i) { return ((const uint8_t*)A->mask)[i]; });
+        }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            const int node = row_of(m) / P.G;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int e = 4 * g + i;
-                sees[m][i] = seen(node, m0 + (e < n ? e : n - 1)) && e < n;
-            }
+            const int c = n - 4 * g;                         // tokens behind the last are nobody's
+            sees[m] &= c <= 0 ? 0u : c >= 4 ? 15u : (1u << c) - 1;
             x[m][0] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
         }
         a8_wait<0>();
@@ -554,14 +612,14 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         for (int s = 0; s < D / 32; ++s) {
             const at_s8 kf = *(const at_s8*)(st + kr * 2 * D + ((uint32_t)((s >> 1) * 8 + 2 * g + (s & 1)) ^ a8_swz<2 * D>(kr)) * 16);
 #pragma unroll
-            for (int m = 0; m < M; ++m) x[m][0] = a8_mfma<DT>(kf, qread(m, s), x[m][0]);
+            for (int m = 0; m < M; ++m) x[m][0] = a8_mfma<DT>(kf, qread(m, s, qplace((uint32_t)r, (uint32_t)g)), x[m][0]);
         }
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[m][0][i] = sees[m][i] ? x[m][0][i] * P.scale2 : -__builtin_inff();
+            for (int i = 0; i < 4; ++i) x[m][0][i] = sees[m] >> i & 1 ? x[m][0][i] * P.scale2 : -__builtin_inff();
         softmax(x, std::integral_constant<int, 1>{});
-        unit_for(1.0f);
+        unit_for(DT == LLIMA_BF16 ? 32768.0f : 1.0f);        // weights in units that keep a product with any value of the type finite
         at_s4 pf[M];
 #pragma unroll
         for (int m = 0; m < M; ++m) {
@@ -591,14 +649,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot's last tile has been read
         if (ahead < ntile) issue(ahead, ring + (slot == 0 ? S - 1 : slot - 1) * ST);   // uniform
         const int n = len - key_of(tile) < KT ? len - key_of(tile) : KT;
-        // cached tiles behind this one count NR requests each, drafted ones fewer: then everything is waited for
-        if (ahead < nC) {                                    // uniform
-            a8_wait<(S - 1) * NR + NQ + 1>();
-            math8(st, n, [] { a8_wait<(S - 1) * NR>(); });
-        } else {
-            a8_wait<0>();
-            math8(st, n, [] {});
-        }
+        // cached tiles behind this one have NR requests each, drafted ones fewer: then everything is waited for
+        const bool more = ahead < nC;                        // uniform
+        if (more) a8_wait<(S - 1) * NR + NQ + 1>();
+        else a8_wait<0>();
+        math8(st, n, more);
         slot = slot + 1 < S ? slot + 1 : 0;
     }
     for (int tile = nC; tile < ntile; ++tile) {
@@ -610,15 +665,17 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         slot = slot + 1 < S ? slot + 1 : 0;
     }
     // ---------------------------------------------------------------- the waves' sums
-    if (__any(miss) && lane == 0) flag[0] = 1u;
+    if (miss) flag[0] = 1u;
     __syncthreads();                                         // no wave reads or fills its ring any more
+    const int r = (int)fresh(t) & 15, g = (int)fresh(t) >> 4 & 3, lane = (int)fresh(t) & 63;
     float2* const ml = (float2*)(sm + XN * XB);              // [wave][row]
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-        l[m] = a8_sum4(l[m]);
+        l[m] = a8_sum4(l[m]) * 3.0517578125e-5f;             // 2^-15
         if (g == 0) ml[wave * M * 16 + m * 16 + r] = make_float2(ref[m], l[m]);
     }
     __syncthreads();
+    const At8Args A = a8_args();
     const bool nan = flag[0] != 0, special = flag[1] != 0;
     const int drow0 = (c0 > nc ? c0 - nc : 0) * TD, drow1 = c1 - nc <= 0 ? 0 : (c1 - nc) * TD < P.N ? (c1 - nc) * TD : P.N;   // the part's drafted tokens
 #pragma unroll
@@ -633,7 +690,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         const float mu = top > -__builtin_inff() ? top : 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) sum += x[w].y * __builtin_amdgcn_exp2f(x[w].x - mu);
-        const float a = __builtin_amdgcn_exp2f(ref[m] - mu) * (DT == LLIMA_F16 ? vref : 1.0f);
+        const float a = __builtin_amdgcn_exp2f(ref[m] - mu) * (vref * 3.0517578125e-5f);
         uint8_t* const xb = sm + (XN == 2 ? (m & 1) * XB : 0);
         if (XN == 1 && m > 0) __syncthreads();
 #pragma unroll
@@ -642,10 +699,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
         const int row = row0 + m * 16 + r;
         if (nan) sum = __builtin_nanf("");
         if (row < P.R) {
-            const int n = row / P.G, hq = h * P.G + row % P.G;
-            const float inv = whole ? at_inverse(&P, sum, b, n, len) : 1.0f;
-            const size_t at = ((size_t)at_slot(P.pairs, part, b, c0 == 0) * P.Hkv + h) * P.R + row;
-            if (!whole && wave == 0 && g == 0) P.part_ml[at] = make_float2(top, sum);
+            const int n = node_of(A, row), hq = head_of(A, row, n);
+            const float inv = whole ? at_inverse(A, sum, b, n, len) : 1.0f;
+            const size_t at = ((size_t)at_slot(A->pairs, part, b, c0 == 0) * A->Hkv + h) * P.R + row;
+            if (!whole && wave == 0 && g == 0) A->part_ml[at] = make_float2(top, sum);
 #pragma unroll
             for (int i = 0; i < DB / NW; ++i) {
                 const int d = wave + NW * i;
@@ -654,18 +711,18 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
                 for (int w = 1; w < NW; ++w) y += *(const a8_acc*)(xb + (w * DB + d) * 1024 + lane * 16);
                 if (special) {                               // uniform: infinities and NaN of drafted tokens in this part
                     for (int mm = drow0; mm < drow1; ++mm) {
-                        if (!seen(n, mm)) continue;          // (of the loop over mm)
-                        const uint2 v = *(const uint2*)((const uint16_t*)P.v + b * P.vs[0] + (int64_t)mm * P.vs[1] + h * P.vs[2] + d * 16 + 4 * g);
+                        if (!seen(A, n, mm)) continue;          // (of the loop over mm)
+                        const uint2 v = *(const uint2*)((const uint16_t*)A->v + b * A->vs[0] + (int64_t)mm * A->vs[1] + h * A->vs[2] + d * 16 + 4 * g);
                         auto add = [&](int e, uint32_t u) { y[e] += at_special<DT>((uint16_t)u) ? at_f32<DT>((uint16_t)u) : 0.0f; };
                         add(0, v.x); add(1, v.x >> 16); add(2, v.y); add(3, v.y >> 16);
                     }
                 }
                 if (whole) {
                     y *= inv;
-                    *(uint2*)((uint16_t*)P.out + b * P.os[0] + n * P.os[1] + hq * P.os[2] + d * 16 + 4 * g) =
+                    *(uint2*)((uint16_t*)A->out + b * A->os[0] + n * A->os[1] + hq * A->os[2] + d * 16 + 4 * g) =
                         make_uint2(at_pack<DT>(y[0], y[1]), at_pack<DT>(y[2], y[3]));
                 } else {
-                    *(a8_acc*)(P.part_o + at * D + d * 16 + 4 * g) = y;
+                    *(a8_acc*)(A->part_o + at * D + d * 16 + 4 * g) = y;
                 }
             }
         }
@@ -674,35 +731,44 @@ __global__ __launch_bounds__(256, 2) void tree_attn8(At8Params P) {
 #endif
 }
 
-// Shares of the keys: as many workgroups as the device holds at a time, two per CU.
-static int a8_parts(int Hkv, int RG) {
-    const int n = 512 / (Hkv * RG);
-    return n < 1 ? 1 : n;
+// f(M) with the number of row tiles as a constant.
+template <int D, class F>
+static void a8_tiles(int RT, F f) {
+    if (RT == 1) f(std::integral_constant<int, 1>{});
+    else if (RT == 2) f(std::integral_constant<int, 2>{});
+    else if constexpr (A8<D>::MAXM > 2) {
+        if (RT == 3) f(std::integral_constant<int, 3>{});
+        else f(std::integral_constant<int, 4>{});
+    }
 }
 
-static void a8_plan(AttnParams& P, int D) {                  // RT: row tiles of 16 of a group
-    const int most = D == 256 ? A8<256>::MAXM : D == 128 ? A8<128>::MAXM : A8<64>::MAXM;
+template <int D>
+static void a8_plan_at(AttnParams& P) {                      // RT: row tiles of 16 of a group
     P.R = P.N * P.G;
     const int tiles = (P.R + 15) / 16;
-    P.RG = (tiles + most - 1) / most;
+    P.RG = (tiles + A8<D>::MAXM - 1) / A8<D>::MAXM;
     P.RT = (tiles + P.RG - 1) / P.RG;
-    P.parts = a8_parts(P.Hkv, P.RG);
+    P.parts = 512 / (P.Hkv * P.RG);                          // as many workgroups as the device holds at a time, two per CU
+    if (P.parts < 1) P.parts = 1;
     at_slots(P);
+}
+
+static void a8_plan(AttnParams& P, int D) {
+    if (D == 64) a8_plan_at<64>(P);
+    else if (D == 128) a8_plan_at<128>(P);
+    else a8_plan_at<256>(P);
 }
 
 template <int DT, int D, bool GEN>
 static void a8_launch(const At8Params& P, hipStream_t st) {
-    const dim3 g((uint32_t)P.parts * P.RG * P.Hkv), w(64 * A8<D>::NW);
-    if (P.RT == 1) hipLaunchKernelGGL((tree_attn8<DT, D, 1, GEN>), g, w, 0, st, P);
-    else if (P.RT == 2) hipLaunchKernelGGL((tree_attn8<DT, D, 2, GEN>), g, w, 0, st, P);
-    else if constexpr (A8<D>::MAXM > 2) {
-        if (P.RT == 3) hipLaunchKernelGGL((tree_attn8<DT, D, 3, GEN>), g, w, 0, st, P);
-        else hipLaunchKernelGGL((tree_attn8<DT, D, 4, GEN>), g, w, 0, st, P);
-    }
-    const int64_t rows = (int64_t)P.B * P.N * P.Hq;
-    const AttnParams& J = P;
-    if (rows <= 1024) hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, J);
-    else hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, J);
+    a8_tiles<D>(P.RT, [&](auto m) {
+        constexpr int M = decltype(m)::value;
+        const int64_t rows = (int64_t)P.B * P.N * P.Hq;
+        const AttnParams& J = P;
+        hipLaunchKernelGGL((tree_attn8<DT, D, M, GEN>), dim3(((uint32_t)P.parts * P.Hkv + 7) / 8 * 8 * P.RG), dim3(64 * A8<D>::NW), 0, st, P);
+        if (rows <= 1024) hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, J);
+        else hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, J);
+    });
 }
 
 template <int DT>
@@ -754,6 +820,7 @@ extern "C" int llima_tree_attention_fp8(const llima_tree_attention_fp8_args* x, 
     const int kt = a->D == 256 ? A8<256>::KT : A8<128>::KT, kq = 1024 / a->D;
     P.mode = ts <= (1 << 25) && ss <= (1 << 23) && (!P.table || P.page % kt == 0) ? AT_TILE
            : ts <= (1 << 25) && span < (1 << 29) && P.page % kq == 0 ? AT_REQUEST : AT_LANE;
+    at_divisor(P.G, P.g_mul, P.g_shift);
     a8_plan(P, a->D);
     at_parts_at(P, a->D, workspace);
     return a->dtype == LLIMA_BF16 ? a8_dispatch<LLIMA_BF16>(P, a->D, (hipStream_t)stream)

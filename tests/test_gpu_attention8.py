@@ -1,12 +1,12 @@
 """tree_attention over an Fp8Cache against its definition in 64 bits, over the values that the cache holds.
 
-Tolerance of an output, u = 2^-8 (bf16) or 2^-11 (fp16): a weight times its value's scale is rounded for the product
-with v (u of sum p |v|), the output once (u of it); a score of D exact products, its key's scale and the scaling is off
-by (D + 6) 2^-23 of scale sum |q k|, which moves its weight by as much again in the sum it is divided by; the sums over n
-keys, the exponentials, the scales' products and the rescaling add (n + 64) 2^-23.  fp16: a weight is held in units of
-2^-15 times a power of two that is at most twice the largest scale, or 1 where a drafted token was multiplied; below 2^-14 of
-that its absolute error is 2^-25, which times the largest value it multiplies is 2^-40 2 max(1, scale) max(448, |v|) a key;
-an output is subnormal below 2^-14 (2^-25).
+Tolerance of an output, u = 2^-8 (bf16) or 2^-11 (fp16): a weight times its value's scale is rounded to fp16, a drafted
+token's weight to the type, for the product with v (u of sum p |v| at most), the output once (u of it); a score of D exact
+products, its key's scale and the scaling is off by (D + 6) 2^-23 of scale sum |q k|, which moves its weight by as much
+again in the sum it is divided by; the sums over n keys, the exponentials, the scales' products and the rescaling add
+(n + 64) 2^-23.  A weight in fp16 is held in units of 2^-15 times a power of two that is at most twice the largest scale, or 1
+where a drafted token in fp16 was multiplied; below 2^-14 of that its absolute error is 2^-25, which times the largest
+value it multiplies is 2^-40 2 max(1, scale) max(448, |v|) a key; an output in fp16 is subnormal below 2^-14 (2^-25).
 """
 import math
 
@@ -73,9 +73,11 @@ def definition(s, mask, scale=None):
             mag = p @ seen.abs()
             es = (D + 6) * 2.0 ** -23 * abs(scale) * (q[b, :, h].abs() @ torch.where(see.any(0)[:, None], kh, 0.0).abs().t()).amax(1, keepdim=True)
             a = (u + 2 * es + (n + N + 64) * 2.0 ** -23) * mag + u * o.abs()
+            top = float(seen.abs().max()) if seen.numel() else 0.0
             if u < 2.0 ** -8:
-                top = float(seen.abs().max()) if seen.numel() else 0.0
                 a = a + (n + N) * 2.0 ** -39 * max(448.0, top) * max(1.0, top / 448) + 2.0 ** -25
+            else:
+                a = a + n * 2.0 ** -39 * top
             out[b, :, h], tol[b, :, h] = o, a
     return out, tol
 
