@@ -24,7 +24,7 @@ struct CacheParams {
     int64_t ns, ts, cap;
     int32_t B, N, L, Hkv;
     int32_t page, pages;
-    uint32_t page_mul, page_shift, row_mul, row_shift;       // / page; / (2 Hkv)
+    uint32_t page_mul, page_shift, row_mul, row_shift;       // / page; / Hkv
     int32_t tok, chunks;                                     // tokens of a workgroup; workgroups of a sequence
 };
 
@@ -40,6 +40,23 @@ __device__ __forceinline__ uint32_t ca_max(uint32_t m) {
         m = q8_umax(s[0], s[1]);
     }
     return m;
+}
+
+// The largest magnitude of 8 values, as bits of fp32.  16-bit floats without their sign are in
+// the order of the numbers they are, NaN above infinity.
+typedef uint16_t ca_h2 __attribute__((ext_vector_type(2)));
+template <int DT> __device__ __forceinline__ uint32_t ca_top8(const llima_u32x4& q) {
+    ca_h2 m = __builtin_bit_cast(ca_h2, q[0] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(ca_h2, q[i] & 0x7FFF7FFFu));
+    return __float_as_uint(at_f32<DT>(m[0] > m[1] ? m[0] : m[1]));
+}
+
+// m / 448 rounded to nearest (as Q8Divisor's quotients).
+__device__ __forceinline__ float ca_scale(float m) {
+    constexpr float r = 1.0f / 448.0f;
+    const float q = m * r;
+    return m < __builtin_inff() ? __builtin_fmaf(__builtin_fmaf(-q, 448.0f, m), r, q) : q;
 }
 
 template <int DT> __device__ __forceinline__ void ca_load8(const llima_u32x4& q, float (&v)[8]) {
@@ -64,20 +81,28 @@ __device__ __forceinline__ bool ca_pages_ok(const CacheParams& P, int b, int fro
 }
 
 // Token at of sequence b: its page and place in it.
-__device__ __forceinline__ void ca_place(const CacheParams& P, int b, int at, int64_t& p, int64_t& o) {
-    p = b;
-    o = at;
+__device__ __forceinline__ void ca_place(const CacheParams& P, int b, int at, uint32_t& p, uint32_t& o) {
+    p = (uint32_t)b;
+    o = (uint32_t)at;
     if (P.table) {                                           // uniform
         const uint32_t e = at_page(P.page_mul, P.page_shift, at);
-        o = at - (int)e * P.page;
-        p = P.table[b * P.ts + e];
+        o = (uint32_t)at - e * (uint32_t)P.page;
+        p = (uint32_t)P.table[b * P.ts + e];
     }
+}
+
+// i s.  W: strides past 32 bits (one multiplication instead of three where there are none: the
+// addresses' products took as long as the rest of a row).
+template <bool W> __device__ __forceinline__ int64_t ca_mul(uint32_t i, int64_t s) {
+    if constexpr (W) return (int64_t)i * s;
+    else return (int64_t)((uint64_t)i * (uint32_t)s);
 }
 
 // One workgroup per `tok` places of a sequence and layer.  It checks the sequence's whole
 // path and room (every workgroup of a sequence comes to the same answer); then D / 8 lanes
-// take a row of D values each: 16 bytes in, 8 out, the maximum over the row's lanes.
-template <int DT, int D>
+// take a row of D values each: 16 bytes in, 8 out, the maximum over the row's lanes.  Keys
+// first, then values: what they do not share of a row's address is the workgroup's.
+template <int DT, int D, bool W>
 __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
     constexpr int U = D / 8, RW = LLIMA_WG / U, F = 4;       // lanes of a row; rows of a pass; passes in flight
     const int c = (int)(blockIdx.x % (uint32_t)P.chunks), b = (int)(blockIdx.x / (uint32_t)P.chunks), t = (int)threadIdx.x;
@@ -96,49 +121,44 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
     if (c == 0 && layer == 0 && t == 0) P.new_lens[b] = ok ? len + cnt : LLIMA_E_RANGE;
     const int j0 = c * P.tok, j1 = j0 + P.tok < cnt ? j0 + P.tok : cnt;
     if (!ok || j0 >= cnt) return;                            // uniform
-    const int rows = (j1 - j0) * 2 * P.Hkv, u = t % U;
-    for (int i0 = t / U; i0 < rows; i0 += RW * F) {
-        llima_u32x4 x[F];
-        int j[F], h[F];
-        bool isv[F];
+    const int rows = (j1 - j0) * P.Hkv, u = t % U;
+    auto write = [&](const uint8_t* x, const int64_t* xs, uint8_t* q, const int64_t* qs, float* s, const int64_t* ss) __attribute__((always_inline)) {
+        const uint8_t* const src = x + layer * xs[0] + b * xs[1];
+        uint8_t* const dst = q + layer * qs[0];
+        float* const sc = s + layer * ss[0];
+        for (int i0 = t / U; i0 < rows; i0 += RW * F) {
+            llima_u32x4 y[F];
+            int j[F], h[F];
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1;
-            const int e = (int)at_page(P.row_mul, P.row_shift, i), w = i - e * 2 * P.Hkv;
-            j[f] = j0 + e;
-            isv[f] = w >= P.Hkv;
-            h[f] = isv[f] ? w - P.Hkv : w;
-            const int64_t node = P.nodes ? P.nodes[b * P.ns + j[f]] : j[f];
-            const uint8_t* src = isv[f] ? P.v + layer * P.vs[0] + b * P.vs[1] + node * P.vs[2] + h[f] * P.vs[3]
-                                        : P.k + layer * P.ks[0] + b * P.ks[1] + node * P.ks[2] + h[f] * P.ks[3];
-            x[f] = *(const llima_u32x4*)(src + u * 16);
-        }
+            for (int f = 0; f < F; ++f) {
+                const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1, e = (int)at_page(P.row_mul, P.row_shift, i);
+                j[f] = j0 + e;
+                h[f] = i - e * P.Hkv;
+                const int node = P.nodes ? P.nodes[b * P.ns + j[f]] : j[f];
+                y[f] = *(const llima_u32x4*)(src + ca_mul<W>((uint32_t)node, xs[2]) + ca_mul<W>((uint32_t)h[f], xs[3]) + u * 16);
+            }
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            float v[8];
-            ca_load8<DT>(x[f], v);
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = q8_umax(m, q8_abs(v[i]));
-            const float mf = __uint_as_float(q8_umax(ca_max<U>(m), __float_as_uint(Q8_TINY)));
-            const uint2 q = q8_pack8(v, mf);
-            if (i0 + f * RW < rows) {
-                int64_t p, o;
-                ca_place(P, b, len + j[f], p, o);
-                uint8_t* dst = isv[f] ? P.vq + layer * P.vqs[0] + p * P.vqs[1] + o * P.vqs[2] + h[f] * P.vqs[3]
-                                      : P.kq + layer * P.kqs[0] + p * P.kqs[1] + o * P.kqs[2] + h[f] * P.kqs[3];
-                *(uint2*)(dst + u * 8) = q;
-                float* sc = isv[f] ? P.vsc + layer * P.vss[0] + p * P.vss[1] + o * P.vss[2] + h[f] * P.vss[3]
-                                   : P.ksc + layer * P.kss[0] + p * P.kss[1] + o * P.kss[2] + h[f] * P.kss[3];
-                if (u == 0) *sc = mf / 448.0f;
+            for (int f = 0; f < F; ++f) {
+                float v[8];
+                ca_load8<DT>(y[f], v);
+                const float mf = __uint_as_float(q8_umax(ca_max<U>(ca_top8<DT>(y[f])), __float_as_uint(Q8_TINY)));
+                const uint2 z = q8_pack8(v, mf);
+                if (i0 + f * RW < rows) {
+                    uint32_t p, o;
+                    ca_place(P, b, len + j[f], p, o);
+                    *(uint2*)(dst + ca_mul<W>(p, qs[1]) + ca_mul<W>(o, qs[2]) + ca_mul<W>((uint32_t)h[f], qs[3]) + u * 8) = z;
+                    if (u == 0) sc[ca_mul<W>(p, ss[1]) + ca_mul<W>(o, ss[2]) + ca_mul<W>((uint32_t)h[f], ss[3])] = ca_scale(mf);
+                }
             }
         }
-    }
+    };
+    write(P.k, P.ks, P.kq, P.kqs, P.ksc, P.kss);
+    write(P.v, P.vs, P.vq, P.vqs, P.vsc, P.vss);
 }
 
 // One workgroup per `tok` tokens of a sequence and layer, D / 8 lanes a row: 8 bytes in, 16
 // out.  Rows past the sequence's length are 0; a sequence with a bad length or page is NaN.
-template <int DT, int D>
+template <int DT, int D, bool W>
 __global__ __launch_bounds__(LLIMA_WG) void cache_read8(CacheParams P) {
     constexpr int U = D / 8, RW = LLIMA_WG / U, F = 4;
     const int c = (int)(blockIdx.x % (uint32_t)P.chunks), b = (int)(blockIdx.x / (uint32_t)P.chunks), t = (int)threadIdx.x;
@@ -147,43 +167,45 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_read8(CacheParams P) {
     bool ok = len >= 0 && len <= P.cap;
     if (ok) ok = __syncthreads_and(ca_pages_ok(P, b, 0, len));   // uniform
     const int j0 = c * P.tok, j1 = j0 + P.tok < P.L ? j0 + P.tok : P.L;
-    const int rows = (j1 - j0) * 2 * P.Hkv, u = t % U;
-    for (int i0 = t / U; i0 < rows; i0 += RW * F) {
-        uint2 x[F];
-        float sc[F];
-        uint8_t* dst[F];
+    const int rows = (j1 - j0) * P.Hkv, u = t % U;
+    auto read = [&](uint8_t* y, const int64_t* ys, const uint8_t* q, const int64_t* qs, const float* s, const int64_t* ss) __attribute__((always_inline)) {
+        uint8_t* const dst = y + layer * ys[0] + b * ys[1];
+        const uint8_t* const src = q + layer * qs[0];
+        const float* const scs = s + layer * ss[0];
+        for (int i0 = t / U; i0 < rows; i0 += RW * F) {
+            uint2 x[F];
+            float sc[F];
+            uint8_t* to[F];
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1;
-            const int e = (int)at_page(P.row_mul, P.row_shift, i), w = i - e * 2 * P.Hkv, j = j0 + e;
-            const bool isv = w >= P.Hkv;
-            const int h = isv ? w - P.Hkv : w;
-            dst[f] = (isv ? P.ov + layer * P.vs[0] + b * P.vs[1] + j * P.vs[2] + h * P.vs[3]
-                          : P.ok + layer * P.ks[0] + b * P.ks[1] + j * P.ks[2] + h * P.ks[3]) + u * 16;
-            x[f] = make_uint2(0u, 0u);
-            sc[f] = ok ? 0.0f : __builtin_nanf("");
-            if (ok && j < len) {
-                int64_t p, o;
-                ca_place(P, b, j, p, o);
-                x[f] = *(const uint2*)((isv ? P.vq + layer * P.vqs[0] + p * P.vqs[1] + o * P.vqs[2] + h * P.vqs[3]
-                                            : P.kq + layer * P.kqs[0] + p * P.kqs[1] + o * P.kqs[2] + h * P.kqs[3]) + u * 8);
-                sc[f] = isv ? P.vsc[layer * P.vss[0] + p * P.vss[1] + o * P.vss[2] + h * P.vss[3]]
-                            : P.ksc[layer * P.kss[0] + p * P.kss[1] + o * P.kss[2] + h * P.kss[3]];
+            for (int f = 0; f < F; ++f) {
+                const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1;
+                const int e = (int)at_page(P.row_mul, P.row_shift, i), h = i - e * P.Hkv, j = j0 + e;
+                to[f] = dst + ca_mul<W>((uint32_t)j, ys[2]) + ca_mul<W>((uint32_t)h, ys[3]) + u * 16;
+                x[f] = make_uint2(0u, 0u);
+                sc[f] = ok ? 0.0f : __builtin_nanf("");
+                if (ok && j < len) {
+                    uint32_t p, o;
+                    ca_place(P, b, j, p, o);
+                    x[f] = *(const uint2*)(src + ca_mul<W>(p, qs[1]) + ca_mul<W>(o, qs[2]) + ca_mul<W>((uint32_t)h, qs[3]) + u * 8);
+                    sc[f] = scs[ca_mul<W>(p, ss[1]) + ca_mul<W>(o, ss[2]) + ca_mul<W>((uint32_t)h, ss[3])];
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                const uint32_t w[2] = {x[f].x, x[f].y};
+                llima_u32x4 z;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+                    z[2 * i] = at_pack<DT>(a[0] * sc[f], a[1] * sc[f]);
+                    z[2 * i + 1] = at_pack<DT>(d[0] * sc[f], d[1] * sc[f]);
+                }
+                if (i0 + f * RW < rows) *(llima_u32x4*)to[f] = z;
             }
         }
-#pragma unroll
-        for (int f = 0; f < F; ++f) {
-            const uint32_t w[2] = {x[f].x, x[f].y};
-            llima_u32x4 y;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-                y[2 * i] = at_pack<DT>(a[0] * sc[f], a[1] * sc[f]);
-                y[2 * i + 1] = at_pack<DT>(d[0] * sc[f], d[1] * sc[f]);
-            }
-            if (i0 + f * RW < rows) *(llima_u32x4*)dst[f] = y;
-        }
-    }
+    };
+    read(P.ok, P.ks, P.kq, P.kqs, P.ksc, P.kss);
+    read(P.ov, P.vs, P.vq, P.vqs, P.vsc, P.vss);
 }
 
 // Tokens of a workgroup: up to 8 passes of its rows, fewer where that leaves the device idle.
@@ -200,14 +222,19 @@ template <int DT, bool WRITE>
 static int ca_launch(const CacheParams& P, int layers, int D, hipStream_t st) {
     if ((int64_t)P.B * P.chunks >= 1 << 24) return LLIMA_E_INVAL;   // (a launch: fewer than 2^32 threads)
     const dim3 g((uint32_t)(P.B * P.chunks), (uint32_t)layers), w(LLIMA_WG);
-    auto go = [&](auto d) {
+    bool wide = false;                                       // (the layers' and, of k and v, the batch's strides are the workgroup's)
+    for (const int64_t* s : {P.ks, P.vs, P.kqs, P.vqs, P.kss, P.vss})
+        for (int i = 1; i < 4; ++i) wide = wide || s[i] > (int64_t)UINT32_MAX;
+    auto go = [&](auto d, auto w64) {
         constexpr int DD = decltype(d)::value;
-        if constexpr (WRITE) hipLaunchKernelGGL((cache_write8<DT, DD>), g, w, 0, st, P);
-        else hipLaunchKernelGGL((cache_read8<DT, DD>), g, w, 0, st, P);
+        constexpr bool WW = decltype(w64)::value;
+        if constexpr (WRITE) hipLaunchKernelGGL((cache_write8<DT, DD, WW>), g, w, 0, st, P);
+        else hipLaunchKernelGGL((cache_read8<DT, DD, WW>), g, w, 0, st, P);
     };
-    if (D == 64) go(std::integral_constant<int, 64>{});
-    else if (D == 128) go(std::integral_constant<int, 128>{});
-    else go(std::integral_constant<int, 256>{});
+    auto at = [&](auto d) { wide ? go(d, std::true_type{}) : go(d, std::false_type{}); };
+    if (D == 64) at(std::integral_constant<int, 64>{});
+    else if (D == 128) at(std::integral_constant<int, 128>{});
+    else at(std::integral_constant<int, 256>{});
     return hipGetLastError() == hipSuccess ? LLIMA_OK : LLIMA_E_HIP;
 }
 
@@ -245,7 +272,7 @@ static int ca_fill(const Args* a, CacheParams& P) {
     P.B = a->B; P.Hkv = a->Hkv;
     P.page = a->page_size; P.pages = a->pages;
     at_divisor(P.page, P.page_mul, P.page_shift);
-    at_divisor(2 * P.Hkv, P.row_mul, P.row_shift);
+    at_divisor(P.Hkv, P.row_mul, P.row_shift);
     return LLIMA_OK;
 }
 

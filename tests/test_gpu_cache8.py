@@ -233,3 +233,35 @@ def test_overlaps_are_refused(gpu):
             call()
     assert (buf == 0).all() and (sc == 0).all()
     assert llima_amd.cache_write(k, k, kc, kc, lens).tolist() == [3, 3]           # keys that are the values
+
+
+def test_strides_and_places_past_32_bits(gpu):
+    """Sequences 4.5 GB apart, and a page behind as many bytes."""
+    import llima_amd
+    L, Hkv, D = 2_200_000, 8, 256
+
+    def cache():
+        return llima_amd.Fp8Cache(torch.empty(2, L, Hkv, D, dtype=torch.uint8, device=gpu).view(F8), torch.empty(2, L, Hkv, device=gpu))
+    kc, vc = cache(), cache()
+    k, v = (torch.randn(2, 3, Hkv, D, device=gpu).bfloat16() for _ in range(2))
+    lens = torch.tensor([0, L - 3], dtype=torch.int32, device=gpu)
+    assert llima_amd.cache_write(k, v, kc, vc, lens).tolist() == [3, L]
+    for c, x in ((kc, k), (vc, v)):
+        q, s = quantize(x)
+        assert same(c.values[0, :3], q[0]) and same(c.values[1, -3:], q[1])
+        assert torch.equal(c.scales[0, :3], s[0]) and torch.equal(c.scales[1, -3:], s[1])
+    page = 100
+    kp, vp = (llima_amd.Fp8Cache(c.values.view(torch.uint8).view(2 * L // page, page, Hkv, D).view(F8), c.scales.view(2 * L // page, page, Hkv))
+              for c in (kc, vc))
+    table = torch.tensor([[5, 2 * L // page - 1]], dtype=torch.int32, device=gpu)
+    kp.values.view(torch.uint8)[5].zero_()
+    kp.scales[5].zero_()
+    vp.values.view(torch.uint8)[5].zero_()
+    vp.scales[5].zero_()
+    n = torch.tensor([197], dtype=torch.int32, device=gpu)
+    new = llima_amd.cache_write(k[:1], v[:1], kp, vp, n, block_table=table)
+    assert new.tolist() == [200]
+    rk, rv = llima_amd.cache_read(kp, vp, new, block_table=table)
+    for r, c, x in ((rk, kp, k), (rv, vp, v)):
+        q, s = quantize(x[0])
+        assert same(c.values[-1, -3:], q) and torch.equal(r[0, 197:], (q.float() * s[..., None]).bfloat16()) and (r[0, :100] == 0).all()
