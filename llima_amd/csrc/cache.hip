@@ -98,10 +98,11 @@ template <bool W> __device__ __forceinline__ int64_t ca_mul(uint32_t i, int64_t 
     else return (int64_t)((uint64_t)i * (uint32_t)s);
 }
 
-// One workgroup per `tok` places of a sequence and layer.  It checks the sequence's whole
-// path and room (every workgroup of a sequence comes to the same answer); then D / 8 lanes
-// take a row of D values each: 16 bytes in, 8 out, the maximum over the row's lanes.  Keys
-// first, then values: what they do not share of a row's address is the workgroup's.
+// One workgroup per `tok` places of a sequence and layer; D / 8 lanes take a row of D values
+// each: 16 bytes in, 8 out, the maximum over the row's lanes.  The first rows are requested
+// before the sequence's whole path and room are checked (every workgroup of a sequence comes
+// to the same answer, and nothing is written before it), keys and values together, so that
+// half of them are still on their way while the others are computed.
 template <int DT, int D, bool W>
 __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
     constexpr int U = D / 8, RW = LLIMA_WG / U, F = 4;       // lanes of a row; rows of a pass; passes in flight
@@ -109,6 +110,26 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
     const int64_t layer = blockIdx.y;
     const int len = P.lens[b], cnt = P.counts ? P.counts[b] : P.L;
     bool ok = len >= 0 && cnt >= 0 && cnt <= P.L && len <= P.cap && (int64_t)len + cnt <= P.cap;
+    const int j0 = c * P.tok, j1 = j0 + P.tok < cnt ? j0 + P.tok : cnt;
+    const int rows = (j1 - j0) * P.Hkv, u = t % U;           // 0 and less: nothing of this workgroup's
+    llima_u32x4 y[2][F];
+    uint32_t h[F], p[F], o[F];                               // head, page and place in it (a wait for a load behind
+    auto load = [&](int i0) {                                // a store is one for the store, so these come first too)
+#pragma unroll
+        for (int f = 0; f < F; ++f) {                        // the last row again behind it
+            const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1, e = (int)at_page(P.row_mul, P.row_shift, i), j = j0 + e;
+            h[f] = (uint32_t)(i - e * P.Hkv);
+            ca_place(P, b, len + j, p[f], o[f]);
+            int node = j;
+            if (P.nodes) {                                   // uniform
+                node = P.nodes[b * P.ns + j];
+                node = node >= 0 && node < P.N ? node : 0;   // (not written then)
+            }
+            y[0][f] = *(const llima_u32x4*)(P.k + layer * P.ks[0] + b * P.ks[1] + ca_mul<W>((uint32_t)node, P.ks[2]) + ca_mul<W>(h[f], P.ks[3]) + u * 16);
+            y[1][f] = *(const llima_u32x4*)(P.v + layer * P.vs[0] + b * P.vs[1] + ca_mul<W>((uint32_t)node, P.vs[2]) + ca_mul<W>(h[f], P.vs[3]) + u * 16);
+        }
+    };
+    if (ok && rows > 0) load(t / U);                         // uniform
     if (ok) {                                                // uniform
         bool all = ca_pages_ok(P, b, len, len + cnt);
         if (P.nodes)
@@ -119,41 +140,27 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
         ok = __syncthreads_and(all);
     }
     if (c == 0 && layer == 0 && t == 0) P.new_lens[b] = ok ? len + cnt : LLIMA_E_RANGE;
-    const int j0 = c * P.tok, j1 = j0 + P.tok < cnt ? j0 + P.tok : cnt;
-    if (!ok || j0 >= cnt) return;                            // uniform
-    const int rows = (j1 - j0) * P.Hkv, u = t % U;
-    auto write = [&](const uint8_t* x, const int64_t* xs, uint8_t* q, const int64_t* qs, float* s, const int64_t* ss) __attribute__((always_inline)) {
-        const uint8_t* const src = x + layer * xs[0] + b * xs[1];
-        uint8_t* const dst = q + layer * qs[0];
-        float* const sc = s + layer * ss[0];
-        for (int i0 = t / U; i0 < rows; i0 += RW * F) {
-            llima_u32x4 y[F];
-            int j[F], h[F];
+    if (!ok || rows <= 0) return;                            // uniform
+    for (int i0 = t / U;;) {
 #pragma unroll
-            for (int f = 0; f < F; ++f) {
-                const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1, e = (int)at_page(P.row_mul, P.row_shift, i);
-                j[f] = j0 + e;
-                h[f] = i - e * P.Hkv;
-                const int node = P.nodes ? P.nodes[b * P.ns + j[f]] : j[f];
-                y[f] = *(const llima_u32x4*)(src + ca_mul<W>((uint32_t)node, xs[2]) + ca_mul<W>((uint32_t)h[f], xs[3]) + u * 16);
-            }
-#pragma unroll
-            for (int f = 0; f < F; ++f) {
+        for (int f = 0; f < F; ++f) {
+            auto put = [&](const llima_u32x4& x, uint8_t* q, const int64_t* qs, float* s, const int64_t* ss) __attribute__((always_inline)) {
                 float v[8];
-                ca_load8<DT>(y[f], v);
-                const float mf = __uint_as_float(q8_umax(ca_max<U>(ca_top8<DT>(y[f])), __float_as_uint(Q8_TINY)));
+                ca_load8<DT>(x, v);
+                const float mf = __uint_as_float(q8_umax(ca_max<U>(ca_top8<DT>(x)), __float_as_uint(Q8_TINY)));
                 const uint2 z = q8_pack8(v, mf);
                 if (i0 + f * RW < rows) {
-                    uint32_t p, o;
-                    ca_place(P, b, len + j[f], p, o);
-                    *(uint2*)(dst + ca_mul<W>(p, qs[1]) + ca_mul<W>(o, qs[2]) + ca_mul<W>((uint32_t)h[f], qs[3]) + u * 8) = z;
-                    if (u == 0) sc[ca_mul<W>(p, ss[1]) + ca_mul<W>(o, ss[2]) + ca_mul<W>((uint32_t)h[f], ss[3])] = ca_scale(mf);
+                    *(uint2*)(q + layer * qs[0] + ca_mul<W>(p[f], qs[1]) + ca_mul<W>(o[f], qs[2]) + ca_mul<W>(h[f], qs[3]) + u * 8) = z;
+                    if (u == 0) s[layer * ss[0] + ca_mul<W>(p[f], ss[1]) + ca_mul<W>(o[f], ss[2]) + ca_mul<W>(h[f], ss[3])] = ca_scale(mf);
                 }
-            }
+            };
+            put(y[0][f], P.kq, P.kqs, P.ksc, P.kss);
+            put(y[1][f], P.vq, P.vqs, P.vsc, P.vss);
         }
-    };
-    write(P.k, P.ks, P.kq, P.kqs, P.ksc, P.kss);
-    write(P.v, P.vs, P.vq, P.vqs, P.vsc, P.vss);
+        i0 += RW * F;
+        if (i0 - t / U >= rows) break;                       // uniform
+        load(i0);
+    }
 }
 
 // One workgroup per `tok` tokens of a sequence and layer, D / 8 lanes a row: 8 bytes in, 16
@@ -168,28 +175,33 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_read8(CacheParams P) {
     if (ok) ok = __syncthreads_and(ca_pages_ok(P, b, 0, len));   // uniform
     const int j0 = c * P.tok, j1 = j0 + P.tok < P.L ? j0 + P.tok : P.L;
     const int rows = (j1 - j0) * P.Hkv, u = t % U;
-    auto read = [&](uint8_t* y, const int64_t* ys, const uint8_t* q, const int64_t* qs, const float* s, const int64_t* ss) __attribute__((always_inline)) {
-        uint8_t* const dst = y + layer * ys[0] + b * ys[1];
-        const uint8_t* const src = q + layer * qs[0];
-        const float* const scs = s + layer * ss[0];
-        for (int i0 = t / U; i0 < rows; i0 += RW * F) {
-            uint2 x[F];
-            float sc[F];
-            uint8_t* to[F];
+    for (int i0 = t / U; i0 < rows; i0 += RW * F) {
+        uint32_t h[F], p[F], o[F];
+        int j[F];
+#pragma unroll
+        for (int f = 0; f < F; ++f) {                        // the last row again behind it
+            const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1, e = (int)at_page(P.row_mul, P.row_shift, i);
+            j[f] = j0 + e;
+            h[f] = (uint32_t)(i - e * P.Hkv);
+            p[f] = o[f] = 0;
+            if (ok && j[f] < len) ca_place(P, b, j[f], p[f], o[f]);
+        }
+        uint2 x[2][F];
+        float sc[2][F];
+        auto load = [&](uint2 (&x)[F], float (&sc)[F], const uint8_t* q, const int64_t* qs, const float* s, const int64_t* ss) __attribute__((always_inline)) {
 #pragma unroll
             for (int f = 0; f < F; ++f) {
-                const int i = i0 + f * RW < rows ? i0 + f * RW : rows - 1;
-                const int e = (int)at_page(P.row_mul, P.row_shift, i), h = i - e * P.Hkv, j = j0 + e;
-                to[f] = dst + ca_mul<W>((uint32_t)j, ys[2]) + ca_mul<W>((uint32_t)h, ys[3]) + u * 16;
                 x[f] = make_uint2(0u, 0u);
                 sc[f] = ok ? 0.0f : __builtin_nanf("");
-                if (ok && j < len) {
-                    uint32_t p, o;
-                    ca_place(P, b, j, p, o);
-                    x[f] = *(const uint2*)(src + ca_mul<W>(p, qs[1]) + ca_mul<W>(o, qs[2]) + ca_mul<W>((uint32_t)h, qs[3]) + u * 8);
-                    sc[f] = scs[ca_mul<W>(p, ss[1]) + ca_mul<W>(o, ss[2]) + ca_mul<W>((uint32_t)h, ss[3])];
+                if (ok && j[f] < len) {
+                    x[f] = *(const uint2*)(q + layer * qs[0] + ca_mul<W>(p[f], qs[1]) + ca_mul<W>(o[f], qs[2]) + ca_mul<W>(h[f], qs[3]) + u * 8);
+                    sc[f] = s[layer * ss[0] + ca_mul<W>(p[f], ss[1]) + ca_mul<W>(o[f], ss[2]) + ca_mul<W>(h[f], ss[3])];
                 }
             }
+        };
+        load(x[0], sc[0], P.kq, P.kqs, P.ksc, P.kss);
+        load(x[1], sc[1], P.vq, P.vqs, P.vsc, P.vss);
+        auto put = [&](const uint2 (&x)[F], const float (&sc)[F], uint8_t* y, const int64_t* ys) __attribute__((always_inline)) {
 #pragma unroll
             for (int f = 0; f < F; ++f) {
                 const uint32_t w[2] = {x[f].x, x[f].y};
@@ -200,12 +212,13 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_read8(CacheParams P) {
                     z[2 * i] = at_pack<DT>(a[0] * sc[f], a[1] * sc[f]);
                     z[2 * i + 1] = at_pack<DT>(d[0] * sc[f], d[1] * sc[f]);
                 }
-                if (i0 + f * RW < rows) *(llima_u32x4*)to[f] = z;
+                if (i0 + f * RW < rows)
+                    *(llima_u32x4*)(y + layer * ys[0] + b * ys[1] + ca_mul<W>((uint32_t)j[f], ys[2]) + ca_mul<W>(h[f], ys[3]) + u * 16) = z;
             }
-        }
-    };
-    read(P.ok, P.ks, P.kq, P.kqs, P.ksc, P.kss);
-    read(P.ov, P.vs, P.vq, P.vqs, P.vsc, P.vss);
+        };
+        put(x[0], sc[0], P.ok, P.ks);
+        put(x[1], sc[1], P.ov, P.vs);
+    }
 }
 
 // Tokens of a workgroup: up to 8 passes of its rows, fewer where that leaves the device idle.
