@@ -165,6 +165,8 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
 
 // One workgroup per `tok` tokens of a sequence and layer, D / 8 lanes a row: 8 bytes in, 16
 // out.  Rows past the sequence's length are 0; a sequence with a bad length or page is NaN.
+// Bound: the outputs' bytes, five sixths of all (16 sequences of up to 8192 tokens: 638 MB).  Stores
+// that pass by L2 leave it to the reads: 132 -> 106 us.
 template <int DT, int D, bool W>
 __global__ __launch_bounds__(LLIMA_WG) void cache_read8(CacheParams P) {
     constexpr int U = D / 8, RW = LLIMA_WG / U, F = 4;
@@ -213,7 +215,8 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_read8(CacheParams P) {
                     z[2 * i + 1] = at_pack<DT>(d[0] * sc[f], d[1] * sc[f]);
                 }
                 if (i0 + f * RW < rows)
-                    *(llima_u32x4*)(y + layer * ys[0] + b * ys[1] + ca_mul<W>((uint32_t)j[f], ys[2]) + ca_mul<W>(h[f], ys[3]) + u * 16) = z;
+                    __builtin_nontemporal_store(z, (llima_u32x4*)(y + layer * ys[0] + b * ys[1] + ca_mul<W>((uint32_t)j[f], ys[2]) +
+                                                                  ca_mul<W>(h[f], ys[3]) + u * 16));
             }
         };
         put(x[0], sc[0], P.ok, P.ks);

@@ -26,6 +26,15 @@ struct SandwichParams {
     float eps, offset, rs, gs;
 };
 
+// A piece that nobody reads again: it passes by L2 (8000 x 5760 bf16: 75 -> 69 us).
+template <class Raw> __device__ __forceinline__ Raw sw_once(const void* p) {
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Raw) / 16); ++i)
+        ((llima_u32x4*)&r)[i] = __builtin_nontemporal_load((const llima_u32x4*)p + i);
+    return r;
+}
+
 // 1 / sqrt of the mean of the squares whose sums the threads hold, rounded once to fp32.
 template <int NWV>
 __device__ __forceinline__ float sw_factor(double s, double* part, int H, float eps) {
@@ -97,8 +106,8 @@ __global__ __launch_bounds__(64 * NWV) void sandwich_rows(SandwichParams P) {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int p = t + NT * j < np ? t + NT * j : np - 1;
-            rx[j] = *(const typename T::Raw*)at(x, p);
-            ra[j] = *(const typename T::Raw*)at(res, p);
+            rx[j] = sw_once<typename T::Raw>(at(x, p));
+            ra[j] = sw_once<typename T::Raw>(at(res, p));
             if (P.post) r1[j] = *(const typename T::Raw*)at(P.post, p);   // uniform
             if (P.gate) rg[j] = *(const typename T::Raw*)at(gate, p);     // uniform
             r2[j] = *(const typename T::Raw*)at(P.pre, p);
