@@ -208,12 +208,18 @@ class SandwichNormArgsC(ctypes.Structure):
                 [(n, ctypes.c_float) for n in ("eps", "weight_offset", "residual_scale", "gate_scale")])
 
 
-# the same as bytes in one call (a ctypes structure is filled field by field: 6 us)
+# the same as bytes (a ctypes structure is filled field by field: 6 us): in one call, or the pointers and,
+# packed once for calls of one form, what follows them
 TREE_ATTENTION_ARGS = struct.Struct("@9P3q3q3q3q3q3q2qq10if0q")
 TREE_COMMIT_ARGS = struct.Struct("@9P4q4q4q4q2q9i0q")
 TREE_ATTENTION_FP8_ARGS = struct.Struct("@9P3q3q3q3q3q3q2qq10if0q2P3q3q")
 CACHE_WRITE_FP8_ARGS = struct.Struct("@11P4q4q4q4q4q4q2q10i0q")
 CACHE_READ_FP8_ARGS = struct.Struct("@8P4q4q4q4q4q4qq9i0q")
+TREE_ATTENTION_SIZES = struct.Struct("@3q3q3q3q3q3q2qq10if0q")
+CACHE_WRITE_FP8_SIZES = struct.Struct("@4q4q4q4q4q4q2q10i0q")
+CACHE_READ_FP8_SIZES = struct.Struct("@4q4q4q4q4q4qq9i0q")
+TWO_POINTERS, EIGHT_POINTERS, NINE_POINTERS, ELEVEN_POINTERS = (struct.Struct(f"@{n}P") for n in (2, 8, 9, 11))
+SIX_STRIDES = struct.Struct("@6q")
 SANDWICH_NORM_ARGS = struct.Struct("@8P3q3i4f0q")
 
 _lib = None

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .sampler import FLOAT_CODES, _on, _on_gpu, _scratch, _stream
+from .sampler import _PLANS, FLOAT_CODES, _form, _on, _on_gpu, _planned, _scratch, _stream
 
 F8 = torch.float8_e4m3fn
 
@@ -202,9 +202,41 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     range is NaN.  scale defaults to D^-0.5.  Strides are free where values of a head are
     adjacent (head-major caches as transposed views).  Nothing waits for the device, and the
     call can be captured into a graph."""
-    k8 = v8 = None
     if _eight_bits(k_cache, v_cache):
-        k8, v8, k_cache, v_cache = k_cache.scales, v_cache.scales, k_cache.values, v_cache.values
+        return _attend(q, k, v, k_cache.values, v_cache.values, cache_lens, tree_mask, block_table, k_cache.scales,
+                       v_cache.scales, scale)
+    return _attend(q, k, v, k_cache, v_cache, cache_lens, tree_mask, block_table, None, None, scale)
+
+
+def _attend(q, k, v, kc, vc, lens, mask, table, k8, v8, scale):
+    form = (scale, _form(q), _form(k), _form(v), _form(kc), _form(vc), _form(lens), _form(mask), _form(table), _form(k8), _form(v8))
+    plan = _PLANS.get(form)
+    if plan is None:
+        given = (q, k, v, kc, vc, lens, mask, table)
+        used = _attend_checks(*given, k8, v8)
+        if any([x is not y for x, y in zip(given, used)]):   # copies, or views with other strides
+            return _attend(*used, k8, v8, scale)
+        plan = _planned(form, _attend_plan(*given, k8, v8, scale))
+    like, dev, nbytes, sizes, scales = plan
+    out = torch.empty_like(q) if like else torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if nbytes == 0:                                          # no sequences
+        return out
+    ws = _scratch(dev, "tree_attention", nbytes)
+    ptrs = _lib.NINE_POINTERS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), lens.data_ptr(),
+        0 if mask is None else mask.data_ptr(),
+        0 if table is None else table.data_ptr() or lens.data_ptr())     # a table of no blocks is not read
+    with _on(dev):
+        if k8 is None:
+            check(lib().llima_tree_attention(ptrs + sizes, ws.data_ptr(), ws.numel(), _stream(dev)), "llima_tree_attention")
+        else:
+            a = ptrs + sizes + _lib.TWO_POINTERS.pack(k8.data_ptr(), v8.data_ptr()) + scales
+            check(lib().llima_tree_attention_fp8(a, ws.data_ptr(), ws.numel(), _stream(dev)), "llima_tree_attention_fp8")
+    return out
+
+
+def _attend_checks(q, k, v, k_cache, v_cache, cache_lens, mask, block_table, k8, v8):
+    """The call's tensors as the kernels can read them, or ValueError."""
     if q.dim() != 4 or k.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("q [B, N, Hq, D], k and v [B, N, Hkv, D] and 4-dimensional caches are needed")
     B, N, Hq, D = q.shape
@@ -217,47 +249,41 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
         raise ValueError("the head size must be 64, 128 or 256")
     if N == 0 or N > 1024 or Hkv == 0 or Hq == 0 or Hq % Hkv or Hq > 1024:
         raise ValueError("1 to 1024 drafted tokens and query heads, a multiple of the key heads, are supported")
-    _on_gpu(q, k, v, k_cache, v_cache, cache_lens, tree_mask, block_table)
+    _on_gpu(q, k, v, k_cache, v_cache, cache_lens, mask, block_table)
     dev = q.device
     if not (k.device == v.device == k_cache.device == v_cache.device == dev):
         raise ValueError("tree_attention: tensors must be on one device")
-    page, pages, blocks, table = _cache(k_cache, v_cache, Hkv, D, q.dtype if k8 is None else F8, block_table, B, dev)
+    if k8 is not None and not (k8.shape == v8.shape == k_cache.shape[:-1] and k8.device == v8.device == dev):
+        raise ValueError("tree_attention: an Fp8Cache's scales must be [..., tokens, Hkv] beside its values")
+    table = _cache(k_cache, v_cache, Hkv, D, q.dtype if k8 is None else F8, block_table, B, dev)[3]
     lens = _ints(cache_lens, B, "cache_lens", dev)
-    mask, mask_dtype, ms = tree_mask, _lib.LLIMA_MASK_U8, (0, 0)
     if mask is not None:
         if tuple(mask.shape) not in ((N, N), (B, N, N)) or mask.device != dev:
             raise ValueError("tree_mask must be [N, N] or [B, N, N] on q's device")
         if mask.dtype not in (torch.bool, torch.uint8, torch.float32):
             raise ValueError("tree_mask must be bool, uint8 or float32")
         if mask.stride(-1) != 1:
-            mask = mask.contiguous()
-        if mask.dtype == torch.float32:
-            mask_dtype = _lib.LLIMA_MASK_F32
-        ms = (mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
-    q, k, v = _heads(q), _heads(k), _heads(v)
+            mask = mask.clone(memory_format=torch.contiguous_format)
     align = 8 if k8 is None else 16
-    kc, vc = _in_place(k_cache, "k_cache", align), _in_place(v_cache, "v_cache", align)
-    out = torch.empty((B, N, Hq, D), dtype=q.dtype, device=dev)
-    if B == 0:
-        return out
-    L = lib()
-    ws = _scratch(dev, "tree_attention", (L.llima_tree_attention_workspace_bytes if k8 is None else
-                                          L.llima_tree_attention_fp8_workspace_bytes)(B, N, Hq, Hkv, D))
-    # a table of no blocks is not read
-    tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
-    args = (
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), lens.data_ptr(),
-        0 if mask is None else mask.data_ptr(), tp, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-        *out.stride()[:3], *kc.stride()[:3], *vc.stride()[:3], *ms, ts, FLOAT_CODES[q.dtype], mask_dtype, B, N, Hq,
-        Hkv, D, page, pages, blocks, D ** -0.5 if scale is None else float(scale))
-    with _on(dev):
-        if k8 is None:
-            check(L.llima_tree_attention(_lib.TREE_ATTENTION_ARGS.pack(*args), ws.data_ptr(), ws.numel(), _stream(dev)),
-                  "llima_tree_attention")
-        else:
-            a = _lib.TREE_ATTENTION_FP8_ARGS.pack(*args, k8.data_ptr(), v8.data_ptr(), *k8.stride(), *v8.stride())
-            check(L.llima_tree_attention_fp8(a, ws.data_ptr(), ws.numel(), _stream(dev)), "llima_tree_attention_fp8")
-    return out
+    return (_heads(q), _heads(k), _heads(v), _in_place(k_cache, "k_cache", align), _in_place(v_cache, "v_cache", align),
+            lens, mask, table)
+
+
+def _attend_plan(q, k, v, kc, vc, lens, mask, table, k8, v8, scale):
+    """(whether the output is laid out as q, device, workspace bytes, the arguments behind the pointers, the scales' strides)."""
+    B, N, Hq, D = q.shape
+    Hkv, dev = k.shape[2], q.device
+    page, pages, blocks, _ = _cache(kc, vc, Hkv, D, kc.dtype, table, B, dev)
+    bytes_of = lib().llima_tree_attention_workspace_bytes if k8 is None else lib().llima_tree_attention_fp8_workspace_bytes
+    os = (N * Hq * D, Hq * D, D)
+    ms = (0, 0) if mask is None else (mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2))
+    sizes = _lib.TREE_ATTENTION_SIZES.pack(
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *os, *kc.stride()[:3], *vc.stride()[:3], *ms,
+        0 if table is None else table.stride(0), FLOAT_CODES[q.dtype],
+        _lib.LLIMA_MASK_F32 if mask is not None and mask.dtype == torch.float32 else _lib.LLIMA_MASK_U8, B, N, Hq, Hkv, D,
+        page, pages, blocks, D ** -0.5 if scale is None else float(scale))
+    scales = b"" if k8 is None else _lib.SIX_STRIDES.pack(*k8.stride(), *v8.stride())
+    return q.is_contiguous(), dev, bytes_of(B, N, Hq, Hkv, D), sizes, scales
 
 
 def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: torch.Tensor,
@@ -325,20 +351,55 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, nodes: torch.Tensor, counts: t
     return new
 
 
-def _layers(k_cache: Fp8Cache, v_cache: Fp8Cache, four: bool):
+def _layers(k_cache: Fp8Cache, v_cache: Fp8Cache):
     """Values and scales of both caches with the layers' dimension in front."""
     ts = (k_cache.values, v_cache.values, k_cache.scales, v_cache.scales)
-    return [t[None] for t in ts] if four else ts
+    return [t[None] for t in ts] if k_cache.dim() == 4 else ts
 
 
 def _write8(name, k, v, k_cache, v_cache, cache_lens, nodes, counts, block_table):
     """Keys and values into an Fp8Cache (llima_cache_write_fp8)."""
-    four = k.dim() == 4
-    if (k.dim() != 5 and not four) or k_cache.dim() != k.dim() or v_cache.dim() != k.dim() or v.dim() != k.dim():
-        raise ValueError("k and v must be [B, N, Hkv, D] or [layers, B, N, Hkv, D], the caches likewise")
-    kq, vq, ks, vs = _layers(k_cache, v_cache, four)
-    if four:
+    if k.dim() == 4:
+        if k_cache.dim() != 4 or v_cache.dim() != 4 or v.dim() != 4:
+            raise ValueError("k and v [B, N, Hkv, D] need 4-dimensional caches")
         k, v = k[None], v[None]
+    elif k.dim() != 5 or k_cache.dim() != 5 or v_cache.dim() != 5 or v.dim() != 5:
+        raise ValueError("k and v must be [B, N, Hkv, D] or [layers, B, N, Hkv, D], the caches likewise")
+    return _put8(name, k, v, *_layers(k_cache, v_cache), cache_lens, nodes, counts, block_table)
+
+
+def _put8(name, k, v, kq, vq, ks, vs, lens, nodes, counts, table):
+    form = (_form(k), _form(v), _form(kq), _form(vq), _form(ks), _form(vs), _form(lens), _form(nodes), _form(counts), _form(table))
+    plan = _PLANS.get(form)
+    if plan is None:
+        given = (k, v, kq, vq, ks, vs, lens, nodes, counts, table)
+        used = _put8_checks(name, *given)
+        if any([x is not y for x, y in zip(given, used)]):   # copies, or views with other strides
+            return _put8(name, *used)
+        plan = _planned(form, _put8_plan(*given))
+    B, dev, sizes = plan
+    outs = (kq, vq, ks, vs)
+    if not _apart((k, v, *outs)):                            # (the usual case: no two in one storage)
+        if any([_shared(a, o) for a in (k, v) for o in outs]):
+            raise ValueError(f"{name}: k and v must not overlap the caches (copy them first)")
+        tied = _same(k, v) and _same(kq, vq) and _same(ks, vs)
+        if not tied and (_shared(kq, vq) or _shared(ks, vs)) or \
+                _shared(kq, ks) or _shared(vq, vs) or _shared(kq, vs) or _shared(vq, ks):
+            raise ValueError(f"{name}: k_cache and v_cache, values and scales, must not overlap")
+    new = torch.empty(B, dtype=torch.int32, device=dev)
+    if B == 0:
+        return new
+    ptrs = _lib.ELEVEN_POINTERS.pack(
+        k.data_ptr(), v.data_ptr(), kq.data_ptr(), vq.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+        0 if nodes is None else nodes.data_ptr(), 0 if counts is None else counts.data_ptr(), lens.data_ptr(),
+        0 if table is None else table.data_ptr() or lens.data_ptr(), new.data_ptr())
+    with _on(dev):
+        check(lib().llima_cache_write_fp8(ptrs + sizes, _stream(dev)), "llima_cache_write_fp8")
+    return new
+
+
+def _put8_checks(name, k, v, kq, vq, ks, vs, cache_lens, nodes, counts, block_table):
+    """The call's tensors as the kernel can use them, or ValueError."""
     layers, B, N, Hkv, D = k.shape
     if v.shape != k.shape or v.dtype != k.dtype or k.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("k and v must have one shape and type, bfloat16 or float16")
@@ -350,41 +411,31 @@ def _write8(name, k, v, k_cache, v_cache, cache_lens, nodes, counts, block_table
     dev = k.device
     if not (v.device == kq.device == vq.device == dev):
         raise ValueError(f"{name}: tensors must be on one device")
-    page, pages, blocks, table = _cache(kq, vq, Hkv, D, F8, block_table, B, dev)
+    table = _cache(kq, vq, Hkv, D, F8, block_table, B, dev)[3]
     lens = _ints(cache_lens, B, "cache_lens", dev)
     if counts is not None:
         counts = _ints(counts, B, "counts", dev)
-    L, ns = N, 0
     if nodes is not None:
         if nodes.shape[0] != B or nodes.device != dev:
             raise ValueError("nodes must be int32 [B, L] on the cache's device")
         nodes = nodes if nodes.stride(1) == 1 or nodes.shape[1] == 1 else nodes.contiguous()
-        L, ns = nodes.shape[1], nodes.stride(0)
-    tied = _same(k, v)
-    k, v = _heads(k), _heads(v)
     kq, vq = _in_place(kq, "k_cache", 16), _in_place(vq, "v_cache", 16)
-    outs = (kq, vq, ks, vs)
-    apart = _apart((k, v, *outs))                            # the usual case
-    if not apart and any([_shared(a, o) for a in (k, v) for o in outs]):
-        raise ValueError(f"{name}: k and v must not overlap the caches (copy them first)")
-    if any([_folded(o) for o in outs]):
+    if any([_folded(o) for o in (kq, vq, ks, vs)]):
         raise ValueError(f"{name}: a cache's own values must not overlap (expanded dimensions)")
-    if not apart and (
-            not (tied and _same(kq, vq) and _same(ks, vs)) and (_shared(kq, vq) or _shared(ks, vs)) or
-            _shared(kq, ks) or _shared(vq, vs) or _shared(kq, vs) or _shared(vq, ks)):
-        raise ValueError(f"{name}: k_cache and v_cache, values and scales, must not overlap")
-    new = torch.empty(B, dtype=torch.int32, device=dev)
-    if B == 0:
-        return new
-    tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
-    a = _lib.CACHE_WRITE_FP8_ARGS.pack(
-        k.data_ptr(), v.data_ptr(), kq.data_ptr(), vq.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-        0 if nodes is None else nodes.data_ptr(), 0 if counts is None else counts.data_ptr(), lens.data_ptr(), tp,
-        new.data_ptr(), *k.stride()[:4], *v.stride()[:4], *kq.stride()[:4], *vq.stride()[:4], *ks.stride(), *vs.stride(),
-        ns, ts, FLOAT_CODES[k.dtype], layers, B, N, L, Hkv, D, page, pages, blocks)
-    with _on(dev):
-        check(lib().llima_cache_write_fp8(a, _stream(dev)), "llima_cache_write_fp8")
-    return new
+    if not _same(k, v):
+        return _heads(k), _heads(v), kq, vq, ks, vs, lens, nodes, counts, table
+    k = _heads(k)                                            # (keys that are the values stay so)
+    return k, k, kq, vq, ks, vs, lens, nodes, counts, table
+
+
+def _put8_plan(k, v, kq, vq, ks, vs, lens, nodes, counts, table):
+    """(sequences, device, the arguments behind the pointers)."""
+    layers, B, N, Hkv, D = k.shape
+    page, pages, blocks, _ = _cache(kq, vq, Hkv, D, F8, table, B, k.device)
+    L, ns = (N, 0) if nodes is None else (nodes.shape[1], nodes.stride(0))
+    return B, k.device, _lib.CACHE_WRITE_FP8_SIZES.pack(
+        *k.stride()[:4], *v.stride()[:4], *kq.stride()[:4], *vq.stride()[:4], *ks.stride(), *vs.stride(), ns,
+        0 if table is None else table.stride(0), FLOAT_CODES[k.dtype], layers, B, N, L, Hkv, D, page, pages, blocks)
 
 
 def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: Fp8Cache, v_cache: Fp8Cache, cache_lens: torch.Tensor,
@@ -420,9 +471,32 @@ def cache_read(k_cache: Fp8Cache, v_cache: Fp8Cache, cache_lens: torch.Tensor,
         raise ValueError("cache_read gives bfloat16 or float16")
     if k_cache.dim() not in (4, 5) or v_cache.shape != k_cache.shape:
         raise ValueError("both caches must be [B, tokens, Hkv, D] or pages, with or without layers, of one shape")
-    four = k_cache.dim() == 4
-    kq, vq, ks, vs = _layers(k_cache, v_cache, four)
-    layers, Hkv, D = kq.shape[0], kq.shape[3], kq.shape[4]
+    k, v = _get8(*_layers(k_cache, v_cache), cache_lens, block_table, dtype, tokens)
+    return (k[0], v[0]) if k_cache.dim() == 4 else (k, v)
+
+
+def _get8(kq, vq, ks, vs, lens, table, dtype, tokens):
+    form = (dtype, tokens, _form(kq), _form(vq), _form(ks), _form(vs), _form(lens), _form(table))
+    plan = _PLANS.get(form)
+    if plan is None:
+        given = (kq, vq, ks, vs, lens, table)
+        used = _get8_checks(*given, tokens)
+        if any([x is not y for x, y in zip(given, used)]):   # copies, or views with other strides
+            return _get8(*used, dtype, tokens)
+        plan = _planned(form, _get8_plan(*given, dtype, tokens))
+    shape, dev, sizes = plan
+    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+    if sizes:
+        ptrs = _lib.EIGHT_POINTERS.pack(
+            k.data_ptr(), v.data_ptr(), kq.data_ptr(), vq.data_ptr(), ks.data_ptr(), vs.data_ptr(), lens.data_ptr(),
+            0 if table is None else table.data_ptr() or lens.data_ptr())
+        with _on(dev):
+            check(lib().llima_cache_read_fp8(ptrs + sizes, _stream(dev)), "llima_cache_read_fp8")
+    return k, v
+
+
+def _get8_checks(kq, vq, ks, vs, cache_lens, block_table, tokens):
+    layers, Hkv = kq.shape[0], kq.shape[3]
     if layers == 0 or layers > 65535 or Hkv == 0 or Hkv > 1024:
         raise ValueError("1 to 65535 layers and 1 to 1024 heads are needed")
     _on_gpu(cache_lens, block_table)
@@ -430,20 +504,20 @@ def cache_read(k_cache: Fp8Cache, v_cache: Fp8Cache, cache_lens: torch.Tensor,
     if vq.device != dev:
         raise ValueError("cache_read: tensors must be on one device")
     B = cache_lens.shape[0] if cache_lens.dim() == 1 else -1
-    page, pages, blocks, table = _cache(kq, vq, Hkv, D, F8, block_table, B, dev)
+    table = _cache(kq, vq, Hkv, kq.shape[4], F8, block_table, B, dev)[3]
     lens = _ints(cache_lens, B, "cache_lens", dev)
-    n = page * blocks if tokens is None else int(tokens)
-    if n < 0 or n > 1 << 30:
+    if tokens is not None and not 0 <= int(tokens) <= 1 << 30:
         raise ValueError("0 to 2^30 tokens can be read")
-    kq, vq = _in_place(kq, "k_cache", 16), _in_place(vq, "v_cache", 16)
-    k = torch.empty((layers, B, n, Hkv, D), dtype=dtype, device=dev)
-    v = torch.empty_like(k)
-    if k.numel():
-        tp, ts = (0, 0) if table is None else (table.data_ptr() or lens.data_ptr(), table.stride(0))
-        a = _lib.CACHE_READ_FP8_ARGS.pack(
-            k.data_ptr(), v.data_ptr(), kq.data_ptr(), vq.data_ptr(), ks.data_ptr(), vs.data_ptr(), lens.data_ptr(), tp,
-            *k.stride()[:4], *v.stride()[:4], *kq.stride()[:4], *vq.stride()[:4], *ks.stride(), *vs.stride(), ts,
-            FLOAT_CODES[dtype], layers, B, n, Hkv, D, page, pages, blocks)
-        with _on(dev):
-            check(lib().llima_cache_read_fp8(a, _stream(dev)), "llima_cache_read_fp8")
-    return (k[0], v[0]) if four else (k, v)
+    return _in_place(kq, "k_cache", 16), _in_place(vq, "v_cache", 16), ks, vs, lens, table
+
+
+def _get8_plan(kq, vq, ks, vs, lens, table, dtype, tokens):
+    """(outputs' shape, device, the arguments behind the pointers or nothing where there is nothing to read)."""
+    layers, Hkv, D, B = kq.shape[0], kq.shape[3], kq.shape[4], lens.shape[0]
+    page, pages, blocks, _ = _cache(kq, vq, Hkv, D, F8, table, B, kq.device)
+    n = page * blocks if tokens is None else int(tokens)
+    os = (B * n * Hkv * D, n * Hkv * D, Hkv * D, D)
+    sizes = b"" if B * n == 0 else _lib.CACHE_READ_FP8_SIZES.pack(
+        *os, *os, *kq.stride()[:4], *vq.stride()[:4], *ks.stride(), *vs.stride(), 0 if table is None else table.stride(0),
+        FLOAT_CODES[dtype], layers, B, n, Hkv, D, page, pages, blocks)
+    return (layers, B, n, Hkv, D), kq.device, sizes

@@ -192,6 +192,22 @@ FLOAT_CODES = {torch.float32: _lib.LLIMA_F32, torch.bfloat16: _lib.LLIMA_BF16,
                torch.float16: _lib.LLIMA_F16}
 
 
+# What the checks of a call came to, by its tensors' shapes, strides, types, devices and alignment (not their
+# addresses or values): a call like an earlier one goes straight to its launch.
+_PLANS: dict = {}
+
+
+def _form(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device(), t.data_ptr() % 16)
+
+
+def _planned(form, plan):
+    if len(_PLANS) >= 1024:
+        _PLANS.clear()
+    _PLANS[form] = plan
+    return plan
+
+
 def _rows16(x: torch.Tensor, name: str) -> torch.Tensor:
     """x [..., H] as rows [B, H] that the kernels' 16-byte accesses can read: values of
     a row adjacent, rows and the first row 16-byte aligned (copied when they are not)."""
@@ -787,31 +803,17 @@ def sandwich_norm(x: torch.Tensor, post_weight: Optional[torch.Tensor], residual
     rounds y to the type; "fp8" returns Fp8Rows [rows, H].  H a multiple of 8, at most 65536."""
     if out not in ("same", "fp8"):
         raise ValueError("out must be 'same' or 'fp8'")
-    shape, H, dt = x.shape, x.shape[-1] if x.dim() else 0, x.dtype
-    if residual.shape != shape or residual.dtype != dt:
-        raise ValueError("residual must have x's shape and type")
-    a, r = _rows16(x, "sandwich_norm"), _rows16(residual, "sandwich_norm")
-    dev, B = a.device, a.shape[0]
-    ws = []
-    for w in (post_weight, pre_weight):
-        if w is not None:
-            if w.dim() != 1 or w.shape[0] != H or w.dtype != dt or w.device != dev:
-                raise ValueError("weights must be [H] of x's type, on its device")
-            w = w.contiguous()
-            w = w if w.data_ptr() % 16 == 0 else w.clone()
-        ws.append(w)
-    if ws[1] is None:
-        raise ValueError("pre_weight is needed")
-    g, gs, gp = None, 0, 1.0
-    if torch.is_tensor(gate):
-        if gate.shape not in (shape, shape[-1:]) or gate.dtype != dt:
-            raise ValueError("gate must be a number, [H] or of x's shape, of x's type")
-        g = _rows16(gate, "sandwich_norm")
-        gs = g.stride(0) if gate.shape == shape and B > 1 else 0
-    elif gate is not None:
-        gp = float(gate)
-    if r.device != dev or (g is not None and g.device != dev):
-        raise ValueError("sandwich_norm: tensors must be on one device")
+    g, gs = (gate, 1.0) if torch.is_tensor(gate) else (None, 1.0 if gate is None else float(gate))
+    form = ("sandwich_norm", _form(x), _form(post_weight), _form(residual), _form(pre_weight), _form(g))
+    plan = _PLANS.get(form)
+    if plan is None:
+        given = (x, post_weight, residual, pre_weight, g)
+        used = _sandwich_checks(*given)
+        x, post_weight, residual, pre_weight, g = used[:5]
+        plan = (*used[5:], x.device, x.dtype, *x.shape)
+        if all([a is b or a.data_ptr() == b.data_ptr() for a, b in zip(given, used)]):   # no copies
+            _planned(form, plan)
+    shape, sx, sr, sg, dev, dt, B, H = plan
     if out == "fp8":
         y = Fp8Rows.__new__(Fp8Rows)
         y.values = torch.empty((B, H), dtype=torch.float8_e4m3fn, device=dev)
@@ -822,12 +824,40 @@ def sandwich_norm(x: torch.Tensor, post_weight: Optional[torch.Tensor], residual
         o, sc = y.data_ptr(), 0
     s = torch.empty(shape, dtype=dt, device=dev)
     args = _lib.SANDWICH_NORM_ARGS.pack(
-        a.data_ptr(), r.data_ptr(), 0 if g is None else g.data_ptr(), 0 if ws[0] is None else ws[0].data_ptr(),
-        ws[1].data_ptr(), o, sc, s.data_ptr(), a.stride(0), r.stride(0), gs, FLOAT_CODES[dt], B, H, float(eps),
-        float(weight_offset), float(residual_scale), gp)
+        x.data_ptr(), residual.data_ptr(), 0 if g is None else g.data_ptr(),
+        0 if post_weight is None else post_weight.data_ptr(), pre_weight.data_ptr(), o, sc, s.data_ptr(), sx, sr, sg,
+        FLOAT_CODES[dt], B, H, eps, weight_offset, residual_scale, gs)
     with _on(dev):
         check(lib().llima_sandwich_norm(args, _stream(dev)), "llima_sandwich_norm")
     return y, s
+
+
+def _sandwich_checks(x, post_weight, residual, pre_weight, gate):
+    """sandwich_norm's tensors as the kernel can read them (x as rows), the outputs' shape and the rows' strides,
+    or ValueError."""
+    shape, H, dt = x.shape, x.shape[-1] if x.dim() else 0, x.dtype
+    if residual.shape != shape or residual.dtype != dt:
+        raise ValueError("residual must have x's shape and type")
+    a, r = _rows16(x, "sandwich_norm"), _rows16(residual, "sandwich_norm")
+    dev, ws = a.device, []
+    for w in (post_weight, pre_weight):
+        if w is not None:
+            if w.dim() != 1 or w.shape[0] != H or w.dtype != dt or w.device != dev:
+                raise ValueError("weights must be [H] of x's type, on its device")
+            w = w.contiguous()
+            w = w if w.data_ptr() % 16 == 0 else w.clone()
+        ws.append(w)
+    if ws[1] is None:
+        raise ValueError("pre_weight is needed")
+    g, gs = gate, 0
+    if gate is not None:
+        if gate.shape not in (shape, shape[-1:]) or gate.dtype != dt:
+            raise ValueError("gate must be a number, [H] or of x's shape, of x's type")
+        g = _rows16(gate, "sandwich_norm")
+        gs = g.stride(0) if gate.shape == shape and a.shape[0] > 1 else 0
+    if r.device != dev or (g is not None and g.device != dev):
+        raise ValueError("sandwich_norm: tensors must be on one device")
+    return a, ws[0], r, ws[1], g, shape, a.stride(0), r.stride(0), gs
 
 
 def _bf16_rows(hidden) -> None:

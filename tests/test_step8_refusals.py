@@ -127,6 +127,11 @@ def test_packed_arguments_have_the_structures_sizes():
     for packed, c in ((_lib.TREE_ATTENTION_FP8_ARGS, _lib.TreeAttentionFp8ArgsC), (_lib.CACHE_WRITE_FP8_ARGS, _lib.CacheWriteFp8ArgsC),
                       (_lib.CACHE_READ_FP8_ARGS, _lib.CacheReadFp8ArgsC), (_lib.SANDWICH_NORM_ARGS, _lib.SandwichNormArgsC)):
         assert packed.size == ctypes.sizeof(c)
+    whole = _lib.TREE_ATTENTION_ARGS.size
+    assert _lib.NINE_POINTERS.size + _lib.TREE_ATTENTION_SIZES.size == whole == ctypes.sizeof(_lib.TreeAttentionArgsC)
+    assert whole + _lib.TWO_POINTERS.size + _lib.SIX_STRIDES.size == _lib.TREE_ATTENTION_FP8_ARGS.size
+    assert _lib.ELEVEN_POINTERS.size + _lib.CACHE_WRITE_FP8_SIZES.size == _lib.CACHE_WRITE_FP8_ARGS.size
+    assert _lib.EIGHT_POINTERS.size + _lib.CACHE_READ_FP8_SIZES.size == _lib.CACHE_READ_FP8_ARGS.size
 
 
 def test_python_refuses(monkeypatch):
