@@ -216,19 +216,24 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     };
     auto pages_of = [&](int j, int n) {                      // the page of key j + lane % KT, the last of n for those behind
         const int e = (lane & (KT - 1)) < n ? (lane & (KT - 1)) : n - 1;
-        return P.table ? P.table[b * P.ts + at_page(P.page_mul, P.page_shift, j + e)] : b;
+        return P.table ? P.table[b * P.ts + at_page(P.page_mul, P.page_shift, j + e)] : 0;
     };
     auto known = [&](int p) {                                // a page that exists; others are noted
-        if (!P.table) return b;                              // uniform
+        if (!P.table) return 0;                              // uniform
         const bool out = p < 0 || p >= P.pages;
         miss |= out;
         return out ? 0 : p;
     };
     auto inside = [&](int j) { return P.table ? j - (int)at_page(P.page_mul, P.page_shift, j) * P.page : j; };
-    // a head's first row of page p, place o (uniform)
-    const uint8_t* const kh = (const uint8_t*)P.kc + h * P.kcs[2];
-    const uint8_t* const vh = (const uint8_t*)P.vc + h * P.vcs[2];
-    const float *const ksh = P.ksc + h * P.kss[2], *const vsh = P.vsc + h * P.vss[2];
+    // the head's rows: of every page, or of the sequence where there are no pages (its page is 0 then)
+    const int64_t own = P.table ? 0 : b;
+    const uint8_t* const kh = (const uint8_t*)P.kc + own * P.kcs[0] + h * P.kcs[2];
+    const uint8_t* const vh = (const uint8_t*)P.vc + own * P.vcs[0] + h * P.vcs[2];
+    const float *const ksh = P.ksc + own * P.kss[0] + h * P.kss[2], *const vsh = P.vsc + own * P.vss[0] + h * P.vss[2];
+    // page p, place o of it, by strides below 2^32 (AT_TILE, AT_REQUEST)
+    auto at32 = [&](auto* base, int p, int o, const int64_t (&s)[3]) {
+        return base + ((uint64_t)(uint32_t)p * (uint32_t)s[0] + (uint64_t)(uint32_t)o * (uint32_t)s[1]);
+    };
     auto lds = [](uint8_t* p) { return (__attribute__((address_space(3))) void*)p; };
     auto rsrc = [](const void* p) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7FFFFFFF, 0x00027000); };
     int pg = 0;                                              // the page of the next tile to request; GEN: of the lane's key
@@ -241,7 +246,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     // lane numbers that the compiler does not know to be the same in every tile: what is made from them is not
     // kept in registers, nor spilled
     auto fresh = [&](int x) {
-        if constexpr (M * D > 256) asm volatile("" : "+v"(x));
+        if constexpr (M * D > 384) asm volatile("" : "+v"(x));
         return (uint32_t)x;
     };
     // a cached tile, the lane's own addresses; its n keys, the last of them again behind it
@@ -254,7 +259,10 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
             const int p = known(__shfl(pgl, k, 64)), o = inside(j + k);
             const uint32_t u = (uint32_t)(unit ^ a8_swz<D>((uint32_t)ki)) * 16;
             const uint8_t* src = i < NQ ? kh + p * A->kcs[0] + o * A->kcs[1] : vh + p * A->vcs[0] + o * A->vcs[1];
-            at_dma(src + u, st + i * 1024);
+            const auto from = (const __attribute__((address_space(1))) void*)(src + u);
+            const auto to = (__attribute__((address_space(3))) void*)(st + i * 1024);
+            if (A->RG == 1) __builtin_amdgcn_global_load_lds(from, to, 16, 0, 2);   // uniform
+            else __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
             if (i % NQ == NQ - 1) {                          // uniform: K's or V's scales
                 const int ks = (lane & (KT - 1)) < n ? (lane & (KT - 1)) : n - 1, ps = known(pgl), os = inside(j + ks);
                 const float* sc = i < NQ ? ksh + ps * A->kss[0] + os * A->kss[1] : vsh + ps * A->vss[0] + os * A->vss[1];
@@ -273,8 +281,8 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
             auto unit_at = [&](int i) { return ((ln % U) ^ a8_swz<D>((uint32_t)(i * KQ) + kq)) * 16; };   // of request i
             if (!GEN && n == KT) {                           // uniform
                 const int p = known(pgl), o = inside(j);
-                const auto rk = rsrc(kh + p * P.kcs[0] + o * P.kcs[1]), rv = rsrc(vh + p * P.vcs[0] + o * P.vcs[1]);
-                const auto sk = rsrc(ksh + p * P.kss[0] + o * P.kss[1]), sv = rsrc(vsh + p * P.vss[0] + o * P.vss[1]);
+                const auto rk = rsrc(at32(kh, p, o, P.kcs)), rv = rsrc(at32(vh, p, o, P.vcs));
+                const auto sk = rsrc(at32(ksh, p, o, P.kss)), sv = rsrc(at32(vsh, p, o, P.vss));
                 auto requests = [&](auto nt) {
                     constexpr int AUX = decltype(nt)::value;
 #pragma unroll
@@ -301,18 +309,23 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
                 for (int i = 1; i < NQ; ++i)
                     if ((lane & (KT - 1)) >= i * KQ) { pl = p[i]; ol = o[i]; }
                 ol += lane & (KQ - 1);
+                auto requests = [&](auto nt) {
+                    constexpr int AUX = decltype(nt)::value;
 #pragma unroll
-                for (int i = 0; i < NQ; ++i)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(kh + p[i] * P.kcs[0] + o[i] * P.kcs[1]), lds(st + i * 1024), 16,
-                        (int)(kq * (uint32_t)P.kcs[1] + unit_at(i)), 0, 0, 0);
-                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(ksh), lds(st + 2 * KT * D), 4,
-                        (pl * (int)P.kss[0] + ol * (int)P.kss[1]) * 4, 0, 0, 0);
+                    for (int i = 0; i < NQ; ++i)
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(at32(kh, p[i], o[i], P.kcs)), lds(st + i * 1024), 16,
+                            (int)(kq * (uint32_t)P.kcs[1] + unit_at(i)), 0, 0, AUX);
+                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(ksh), lds(st + 2 * KT * D), 4,
+                            (pl * (int)P.kss[0] + ol * (int)P.kss[1]) * 4, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < NQ; ++i)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(vh + p[i] * P.vcs[0] + o[i] * P.vcs[1]), lds(st + KT * D + i * 1024), 16,
-                        (int)(kq * (uint32_t)P.vcs[1] + unit_at(i)), 0, 0, 0);
-                if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(vsh), lds(st + 2 * KT * D + KT * 4), 4,
-                        (pl * (int)P.vss[0] + ol * (int)P.vss[1]) * 4, 0, 0, 0);
+                    for (int i = 0; i < NQ; ++i)
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(at32(vh, p[i], o[i], P.vcs)), lds(st + KT * D + i * 1024), 16,
+                            (int)(kq * (uint32_t)P.vcs[1] + unit_at(i)), 0, 0, AUX);
+                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(vsh), lds(st + 2 * KT * D + KT * 4), 4,
+                            (pl * (int)P.vss[0] + ol * (int)P.vss[1]) * 4, 0, 0, 0);
+                };
+                if (P.RG == 1) requests(std::integral_constant<int, 2>{});   // uniform
+                else requests(std::integral_constant<int, 0>{});
             } else {
                 issue_lanes(j, n, GEN ? pgl : pages_of(j, n), st);
             }
@@ -818,8 +831,11 @@ extern "C" int llima_tree_attention_fp8(const llima_tree_attention_fp8_args* x, 
     // offsets within a tile (32 keys) or a request, and of the scales, have 31 bits
     const int64_t ts = P.kcs[1] > P.vcs[1] ? P.kcs[1] : P.vcs[1], ss = P.kss[1] > P.vss[1] ? P.kss[1] : P.vss[1];
     const int kt = a->D == 256 ? A8<256>::KT : A8<128>::KT, kq = 1024 / a->D;
-    P.mode = ts <= (1 << 25) && ss <= (1 << 23) && (!P.table || P.page % kt == 0) ? AT_TILE
-           : ts <= (1 << 25) && span < (1 << 29) && P.page % kq == 0 ? AT_REQUEST : AT_LANE;
+    int64_t far = 0;                                         // the longest stride of pages
+    for (const int64_t* s : {P.kcs, P.vcs, P.kss, P.vss}) far = P.table && s[0] > far ? s[0] : far;
+    P.mode = ts > (1 << 25) || far > (int64_t)UINT32_MAX ? AT_LANE
+           : ss <= (1 << 23) && (!P.table || P.page % kt == 0) ? AT_TILE
+           : span < (1 << 29) && P.page % kq == 0 ? AT_REQUEST : AT_LANE;
     at_divisor(P.G, P.g_mul, P.g_shift);
     a8_plan(P, a->D);
     at_parts_at(P, a->D, workspace);
