@@ -16,12 +16,13 @@
 // its row group, so that a value is read from memory, from LDS and converted once, and no
 // wave waits for another before the end of a sequence's part, where their sums are joined.
 //
-// The reference of the softmax moves only when a row's maximum passes it, and then 2^8
-// beyond: weights are at most 1, and the sums are rescaled seldom.  For the product with V a
-// weight times its value's scale is rounded to fp16 whatever q's type (11 bits; in bf16 the
-// outputs' error against 64 bits was 0.0023 of their size, now 0.0017, that of the output's own
-// rounding); it carries a factor of 2^15 and the inverse of the largest scale so far (a power
-// of two), so that it neither overflows nor, down to 2^-29 of the largest, becomes subnormal.
+// What a row's scores are taken less moves only when a weight would pass 2^15, and then so
+// far that the greatest is 2^7: the sums are rescaled seldom, and a score's product with its
+// key's scale and the difference are one operation.  For the product with V a weight times its
+// value's scale is rounded to fp16 whatever q's type (11 bits; in bf16 the outputs' error
+// against 64 bits was 0.0023 of their size, now 0.0017, that of the output's own rounding); it
+// carries the inverse of the largest scale so far (a power of two), so that it neither
+// overflows nor, down to 2^-29 of the largest, becomes subnormal.
 // The drafted tokens' values are of q's type, and so are their weights.
 #include "attention.hpp"
 
@@ -48,7 +49,8 @@ template <int D> struct A8 {
     static constexpr int QL = D == 256 ? 1 : D == 128 ? 3 : 4;   // of them in LDS at most (two workgroups per CU), the rest in registers
 };
 
-#define A8_HEAD 8.0f                                         // the reference moves to a maximum and this much beyond
+#define A8_MOST 15.0f                                        // the logarithm of the greatest weight, base 2
+#define A8_HEAD 8.0f                                         // where it is passed, the row's maximum comes this much below it
 
 // The partition's unit: tiles of T cached keys, then tiles of TD drafted ones.
 template <int D>
@@ -392,11 +394,13 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     auto qplace = [&](uint32_t rr, uint32_t gg) { return rr * 2 * D + ((2 * gg) ^ a8_swz<2 * D>(rr)) * 16; };
     // ---------------------------------------------------------------- products
     a8_acc o[M][DB];
-    float ref[M], l[M], vref = 0.0f, vinv = 0.0f;            // the unit of the sums over 2^15, and its inverse
+    // mu: what a row's scores (base 2) are taken less; a score less mu is its weight's logarithm, at most `most`,
+    // which is -inf for a row that has seen nothing yet
+    float mu[M], most[M], l[M], vref = 0.0f, vinv = 0.0f;    // the unit of the sums over 2^15, and its inverse
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-        ref[m] = -__builtin_inff();
-        l[m] = 0.0f;
+        mu[m] = l[m] = 0.0f;
+        most[m] = -__builtin_inff();
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[m][d] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -413,7 +417,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
             vinv = 1.0f / nr;
         }
     };
-    // The softmax of B blocks of scores x (base 2), in place: x becomes the weights.
+    // The softmax of blocks of scores less mu, in place: x becomes the weights.
     auto softmax = [&](auto& x, auto blocks) {
         constexpr int BL = decltype(blocks)::value;
         float mt[M];
@@ -424,30 +428,32 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #pragma unroll
             for (int k = 1; k < BL; ++k) a = a8_max(x[m][k][0], x[m][k][1], a8_max(x[m][k][2], x[m][k][3], a));
             mt[m] = a8_max4(a);
-            up |= mt[m] > ref[m];
+            up |= mt[m] > most[m];
         }
         if (__any(up)) {
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                const float nr = mt[m] > ref[m] ? mt[m] + A8_HEAD : ref[m];
-                const float a = mt[m] > ref[m] ? __builtin_amdgcn_exp2f(ref[m] - nr) : 1.0f;
-                ref[m] = nr;
+                const bool raise = mt[m] > most[m];
+                const float to = raise ? mu[m] + (mt[m] - (A8_MOST - A8_HEAD)) : mu[m], by = to - mu[m];
+                const float a = !raise ? 1.0f : most[m] > 0.0f ? __builtin_amdgcn_exp2f(-by) : 0.0f;
+                mu[m] = to;
+                most[m] = raise ? A8_MOST : most[m];
                 l[m] *= a;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) o[m][d] *= a;
+#pragma unroll
+                for (int k = 0; k < BL; ++k) x[m][k] -= by;
             }
         }
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            const float mu = (ref[m] > -__builtin_inff() ? ref[m] : 0.0f) - 15.0f;
+        for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int k = 0; k < BL; ++k)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[m][k][i] = __builtin_amdgcn_exp2f(x[m][k][i] - mu);
+                    x[m][k][i] = __builtin_amdgcn_exp2f(x[m][k][i]);
                     l[m] += x[m][k][i];
                 }
-        }
     };
     auto lds_at = [](const uint8_t* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p; };
     // A staged tile of n cached keys; K has landed, and V too unless there are requests of more tiles.
@@ -485,7 +491,9 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int k = 0; k < NB; ++k) x[m][k] *= ks[k];
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[m][k][i] = __builtin_fmaf(x[m][k][i], ks[k][i], -mu[m]);
         if (n < KT) {                                        // uniform: the sequence's last cached keys
 #pragma unroll
             for (int k = 0; k < NB; ++k)
@@ -630,7 +638,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[m][0][i] = sees[m] >> i & 1 ? x[m][0][i] * P.scale2 : -__builtin_inff();
+            for (int i = 0; i < 4; ++i) x[m][0][i] = sees[m] >> i & 1 ? __builtin_fmaf(x[m][0][i], P.scale2, -mu[m]) : -__builtin_inff();
         softmax(x, std::integral_constant<int, 1>{});
         unit_for(DT == LLIMA_BF16 ? 32768.0f : 1.0f);        // weights in units that keep a product with any value of the type finite
         at_s4 pf[M];
@@ -685,7 +693,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #pragma unroll
     for (int m = 0; m < M; ++m) {
         l[m] = a8_sum4(l[m]) * 3.0517578125e-5f;             // 2^-15
-        if (g == 0) ml[wave * M * 16 + m * 16 + r] = make_float2(ref[m], l[m]);
+        if (g == 0) ml[wave * M * 16 + m * 16 + r] = make_float2(most[m] > 0.0f ? mu[m] : -__builtin_inff(), l[m]);
     }
     __syncthreads();
     const At8Args A = a8_args();
@@ -700,10 +708,10 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
             x[w] = ml[w * M * 16 + m * 16 + r];
             top = __builtin_fmaxf(top, x[w].x);
         }
-        const float mu = top > -__builtin_inff() ? top : 0.0f;
+        const float zero = top > -__builtin_inff() ? top : 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) sum += x[w].y * __builtin_amdgcn_exp2f(x[w].x - mu);
-        const float a = __builtin_amdgcn_exp2f(ref[m] - mu) * (vref * 3.0517578125e-5f);
+        for (int w = 0; w < NW; ++w) sum += x[w].y * __builtin_amdgcn_exp2f(x[w].x - zero);
+        const float a = (most[m] > 0.0f ? __builtin_amdgcn_exp2f(mu[m] - zero) : 0.0f) * (vref * 3.0517578125e-5f);
         uint8_t* const xb = sm + (XN == 2 ? (m & 1) * XB : 0);
         if (XN == 1 && m > 0) __syncthreads();
 #pragma unroll
