@@ -202,6 +202,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     range is NaN.  scale defaults to D^-0.5.  Strides are free where values of a head are
     adjacent (head-major caches as transposed views).  Nothing waits for the device, and the
     call can be captured into a graph."""
+    scale = None if scale is None else float(scale)
     if _eight_bits(k_cache, v_cache):
         return _attend(q, k, v, k_cache.values, v_cache.values, cache_lens, tree_mask, block_table, k_cache.scales,
                        v_cache.scales, scale)
@@ -281,7 +282,7 @@ def _attend_plan(q, k, v, kc, vc, lens, mask, table, k8, v8, scale):
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *os, *kc.stride()[:3], *vc.stride()[:3], *ms,
         0 if table is None else table.stride(0), FLOAT_CODES[q.dtype],
         _lib.LLIMA_MASK_F32 if mask is not None and mask.dtype == torch.float32 else _lib.LLIMA_MASK_U8, B, N, Hq, Hkv, D,
-        page, pages, blocks, D ** -0.5 if scale is None else float(scale))
+        page, pages, blocks, D ** -0.5 if scale is None else scale)
     scales = b"" if k8 is None else _lib.SIX_STRIDES.pack(*k8.stride(), *v8.stride())
     return q.is_contiguous(), dev, bytes_of(B, N, Hq, Hkv, D), sizes, scales
 
@@ -471,7 +472,7 @@ def cache_read(k_cache: Fp8Cache, v_cache: Fp8Cache, cache_lens: torch.Tensor,
         raise ValueError("cache_read gives bfloat16 or float16")
     if k_cache.dim() not in (4, 5) or v_cache.shape != k_cache.shape:
         raise ValueError("both caches must be [B, tokens, Hkv, D] or pages, with or without layers, of one shape")
-    k, v = _get8(*_layers(k_cache, v_cache), cache_lens, block_table, dtype, tokens)
+    k, v = _get8(*_layers(k_cache, v_cache), cache_lens, block_table, dtype, None if tokens is None else int(tokens))
     return (k[0], v[0]) if k_cache.dim() == 4 else (k, v)
 
 
@@ -506,7 +507,7 @@ def _get8_checks(kq, vq, ks, vs, cache_lens, block_table, tokens):
     B = cache_lens.shape[0] if cache_lens.dim() == 1 else -1
     table = _cache(kq, vq, Hkv, kq.shape[4], F8, block_table, B, dev)[3]
     lens = _ints(cache_lens, B, "cache_lens", dev)
-    if tokens is not None and not 0 <= int(tokens) <= 1 << 30:
+    if tokens is not None and not 0 <= tokens <= 1 << 30:
         raise ValueError("0 to 2^30 tokens can be read")
     return _in_place(kq, "k_cache", 16), _in_place(vq, "v_cache", 16), ks, vs, lens, table
 
@@ -515,7 +516,7 @@ def _get8_plan(kq, vq, ks, vs, lens, table, dtype, tokens):
     """(outputs' shape, device, the arguments behind the pointers or nothing where there is nothing to read)."""
     layers, Hkv, D, B = kq.shape[0], kq.shape[3], kq.shape[4], lens.shape[0]
     page, pages, blocks, _ = _cache(kq, vq, Hkv, D, F8, table, B, kq.device)
-    n = page * blocks if tokens is None else int(tokens)
+    n = page * blocks if tokens is None else tokens
     os = (B * n * Hkv * D, n * Hkv * D, Hkv * D, D)
     sizes = b"" if B * n == 0 else _lib.CACHE_READ_FP8_SIZES.pack(
         *os, *os, *kq.stride()[:4], *vq.stride()[:4], *ks.stride(), *vs.stride(), 0 if table is None else table.stride(0),

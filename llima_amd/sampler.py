@@ -823,6 +823,8 @@ def sandwich_norm(x: torch.Tensor, post_weight: Optional[torch.Tensor], residual
         y = torch.empty(shape, dtype=dt, device=dev)
         o, sc = y.data_ptr(), 0
     s = torch.empty(shape, dtype=dt, device=dev)
+    if not all([abs(f) < 1e38 for f in (eps, weight_offset, residual_scale, gs)]):
+        raise ValueError("eps, weight_offset, residual_scale and a gate's number must be finite")
     args = _lib.SANDWICH_NORM_ARGS.pack(
         x.data_ptr(), residual.data_ptr(), 0 if g is None else g.data_ptr(),
         0 if post_weight is None else post_weight.data_ptr(), pre_weight.data_ptr(), o, sc, s.data_ptr(), sx, sr, sg,

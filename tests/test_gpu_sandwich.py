@@ -141,3 +141,15 @@ def test_captured(gpu):
         gr.replay()
         torch.cuda.synchronize()
         assert torch.equal(q.values.float(), eq.values.float()) and torch.equal(q.scales, eq.scales) and torch.equal(r, er)
+
+
+def test_numbers_out_of_range_are_refused(gpu):
+    import llima_amd
+    x, post, res, pre, _ = (on(gpu, t) for t in inputs(2, 64, torch.bfloat16, 9, "none"))
+    for bad in (dict(eps=-1.0), dict(eps=math.nan), dict(weight_offset=math.inf), dict(residual_scale=1e39), dict(gate=-1e39),
+                dict(gate=math.nan), dict(gate=post[:32]), dict(gate=post.float()), dict(gate=x[:1])):
+        with pytest.raises(ValueError):
+            llima_amd.sandwich_norm(x, post, res, pre, **bad)
+    for args in ((x, post, res, None), (x, post[:32], res, pre), (x, post, res, pre.float()), (x[:, :60], post[:60], res[:, :60], pre[:60])):
+        with pytest.raises(ValueError):
+            llima_amd.sandwich_norm(*args)
