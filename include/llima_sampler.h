@@ -626,8 +626,9 @@ int llima_tree_commit(const llima_tree_commit_args* args, void* stream);
 
 /* llima_tree_attention over such a cache: the same outputs for k_j = q_j scale_j of the
  * cached tokens (a key's scale multiplies its score, a value's scale its weight, in
- * fp32); the drafted tokens' own k and v are of dtype.  In fp16 the weights times the
- * values' scales are kept in units of the largest scale so far, rounded to dtype. */
+ * fp32); the drafted tokens' own k and v are of dtype.  For its product with a cached
+ * value a weight times the value's scale is rounded to fp16, for either dtype, in a unit
+ * of the largest scale so far. */
 typedef struct llima_tree_attention_fp8_args {
     llima_tree_attention_args a;         /* k_cache, v_cache and their strides: bytes */
     const float *k_scales, *v_scales;

@@ -24,6 +24,19 @@
 // carries the inverse of the largest scale so far (a power of two), so that it neither
 // overflows nor, down to 2^-29 of the largest, becomes subnormal.
 // The drafted tokens' values are of q's type, and so are their weights.
+//
+// Bound: up to one row tile (16 rows per key head) reading the cache's D + 4 bytes per key and
+// value once.  64 sequences of one token, 755 MB: 117-126 us, 6.0-6.4 TB/s (requests into LDS alone
+// reach 5.6 TB/s, 6.2 where they pass by L2).  From three row tiles on the issue: a tile of 32 keys takes
+// a wave 413 vector operations with 48 matrix ones among them, of which half widen K and V or are the
+// softmax's, and 157 scalar ones (33 nodes of 4 heads over 4 x 131072 tokens, 1.1 GB: 480-500 us; the
+// vector units busy 60 % of the time, the matrix cores 26 %; requests alone 287).  16 nodes over
+// 24 x up to 16384: 80 us, the memory's 50.  Short calls are a chain of latencies (1 x 1000 tokens: 8.3 us
+// and 4.1 of the join).
+//
+// Why four waves with tiles of their own: waves that share a tile convert it once each or pass it on
+// through LDS.  Eight waves for three and more row tiles: 118 -> 131 us (16 nodes, 24 x 8192); tiles of
+// 16 keys and three workgroups per CU: 142 -> 172 us (64 sequences of one token).
 #include "attention.hpp"
 
 namespace llima {
@@ -55,7 +68,7 @@ template <int D> struct A8 {
 // The partition's unit: tiles of T cached keys, then tiles of TD drafted ones.
 template <int D>
 struct Fp8Tiles {
-    static constexpr int EXTRA = 4;                          // what a sequence's start and end take, as AT_EXTRA
+    static constexpr int EXTRA = 4;                          // tiles that a sequence's start and end take the time of (6: 2 to 8 % longer; 2 and 9: longer)
     static __device__ __forceinline__ int cached(int len) { return (int)((uint32_t)(len + A8<D>::T - 1) / (uint32_t)A8<D>::T); }
     static __device__ __forceinline__ int drafted(int N) { return (int)((uint32_t)(N + A8<D>::TD - 1) / (uint32_t)A8<D>::TD); }
     static __device__ __forceinline__ int count(const AttnParams& P, int len) { return cached(len) + drafted(P.N) + EXTRA; }
@@ -100,7 +113,8 @@ template <int DT> __device__ __forceinline__ at_s8 a8_wide(uint32_t lo, uint32_t
 }
 
 // The greatest of three; NaN is left out.  (As builtins, every operand is
-// canonicalised first.)
+// canonicalised first.)  Its operands are results of ordinary operations, never a matrix
+// instruction's own, and a swap of lanes takes its result only after a copy of it.
 __device__ __forceinline__ float a8_max(float a, float b, float c) {
     float d;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
@@ -169,7 +183,8 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     const int t = (int)threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     // workgroups go to the 8 XCDs in turn: the row groups of a share and head on one of them, side by side, so
-    // that its keys come from memory once and from that XCD's L2 for the other groups
+    // that its keys come from memory once and from that XCD's L2 for the other groups (requests of three row
+    // groups alone over 4 x 131072 tokens: 513 -> 287 us)
     const uint32_t turn = blockIdx.x / 8u, pair = turn / (uint32_t)P.RG * 8u + blockIdx.x % 8u;
     const int rg = (int)(turn % (uint32_t)P.RG), part = (int)(pair / (uint32_t)P.Hkv), h = (int)(pair % (uint32_t)P.Hkv);
     if (part >= P.parts) return;                             // (the grid is a multiple of 8)

@@ -10,7 +10,11 @@
 // Every product and sum is one fp32 operation in this order, as in rms_rows: the outputs do
 // not depend on how a row is spread over lanes.
 //
-// Bound: reading x, the residual and a gate per token once, writing r and y once.
+// Bound: reading x, the residual and a gate per token once, writing r and y once.  8000 rows of
+// 5760 in bf16: 369 MB in 71 us, 5.2 TB/s, what a copy reaches.  16 rows of 4096 into 8 bits:
+// 4.9 us, one wait for memory and two exchanges of sums.
+// One workgroup per row, since a row's factor needs all of it and it fits the registers.  Outputs
+// that pass by L2 too are slower (69 -> 72 us), and the next operator reads them.
 #include "norm.hpp"
 #include "quant.hpp"
 
@@ -26,7 +30,7 @@ struct SandwichParams {
     float eps, offset, rs, gs;
 };
 
-// A piece that nobody reads again: it passes by L2 (8000 x 5760 bf16: 75 -> 69 us).
+// A piece that nobody reads again: it passes by L2 (8000 x 5760 bf16, whole calls: 71.7 -> 70.8 us).
 template <class Raw> __device__ __forceinline__ Raw sw_once(const void* p) {
     Raw r;
 #pragma unroll
