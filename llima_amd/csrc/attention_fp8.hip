@@ -135,12 +135,19 @@ __device__ __forceinline__ float a8_sum4(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// N pieces of V by the transposing loads, from a[i] on, in one piece with their wait (as builtins, the
+// 4 or 8 pieces of V by the transposing loads, from a[i] on, in one piece with their wait (as builtins, the
 // compiler waits for all the requests into LDS before them).
 __device__ __forceinline__ void a8_tr8(const uint32_t (&a)[4], a8_i2 (&v)[4]) {
     asm volatile("ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\tds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\t"
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]) : "memory");
+}
+__device__ __forceinline__ void a8_tr8(const uint32_t (&a)[8], a8_i2 (&v)[8]) {
+    asm volatile("ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %9\n\tds_read_b64_tr_b8 %2, %10\n\tds_read_b64_tr_b8 %3, %11\n\t"
+                 "ds_read_b64_tr_b8 %4, %12\n\tds_read_b64_tr_b8 %5, %13\n\tds_read_b64_tr_b8 %6, %14\n\tds_read_b64_tr_b8 %7, %15\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]) : "memory");
 }
 __device__ __forceinline__ void a8_tr16(const uint32_t (&a)[4], at_s4 (&v)[4]) {
     asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7\n\t"
@@ -172,6 +179,8 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     constexpr int QL = M < C::QL ? M : C::QL, QR = M - QL;
     constexpr int NR = 2 * NQ + 2;                           // requests of a cached tile
     constexpr int DB = D / 16;                               // column blocks
+    constexpr int VG = DB < 8 ? DB : 8;                      // of them read from LDS at a time
+    constexpr bool AHEAD = M * D <= 384;                     // Q's pieces are read a step before their products (registers: else with it)
     constexpr int QT = 16 * 2 * D;                           // bytes of a row tile of Q
     constexpr int RING = NW * S * ST, XB = NW * DB * 1024;   // a row tile's sums of all waves
     constexpr int XN = 2 * XB + NW * M * 128 <= RING ? 2 : 1;
@@ -244,16 +253,39 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     auto inside = [&](int j) { return P.table ? j - (int)at_page(P.page_mul, P.page_shift, j) * P.page : j; };
     // the head's rows: of every page, or of the sequence where there are no pages (its page is 0 then)
     const int64_t own = P.table ? 0 : b;
-    const uint8_t* const kh = (const uint8_t*)P.kc + own * P.kcs[0] + h * P.kcs[2];
-    const uint8_t* const vh = (const uint8_t*)P.vc + own * P.vcs[0] + h * P.vcs[2];
-    const float *const ksh = P.ksc + own * P.kss[0] + h * P.kss[2], *const vsh = P.vsc + own * P.vss[0] + h * P.vss[2];
+    const uint8_t* kh = (const uint8_t*)P.kc + own * P.kcs[0] + h * P.kcs[2];
+    const uint8_t* vh = (const uint8_t*)P.vc + own * P.vcs[0] + h * P.vcs[2];
+    const float *ksh = P.ksc + own * P.kss[0] + h * P.kss[2], *vsh = P.vsc + own * P.vss[0] + h * P.vss[2];
+    // what every tile's addresses are made from; hidden from the compiler, which else loads it anew for each tile, one
+    // wait after the other (a fifth of a tile's time with three row tiles; with `aim` 498 -> 470 us,
+    // 33 nodes over 4 x 131072 tokens)
+    uint32_t kst[2] = {(uint32_t)P.kcs[0], (uint32_t)P.kcs[1]}, vst[2] = {(uint32_t)P.vcs[0], (uint32_t)P.vcs[1]};
+    uint32_t sst[4] = {(uint32_t)P.kss[0], (uint32_t)P.kss[1], (uint32_t)P.vss[0], (uint32_t)P.vss[1]};
+    if constexpr (!GEN) {
+        asm volatile("" : "+s"(kh), "+s"(vh), "+s"(ksh), "+s"(vsh));
+        asm volatile("" : "+s"(kst[0]), "+s"(kst[1]), "+s"(vst[0]), "+s"(vst[1]), "+s"(sst[0]), "+s"(sst[1]), "+s"(sst[2]), "+s"(sst[3]));
+    }
     // page p, place o of it, by strides below 2^32 (AT_TILE, AT_REQUEST)
-    auto at32 = [&](auto* base, int p, int o, const int64_t (&s)[3]) {
-        return base + ((uint64_t)(uint32_t)p * (uint32_t)s[0] + (uint64_t)(uint32_t)o * (uint32_t)s[1]);
+    auto at32 = [&](auto* base, int p, int o, uint32_t s0, uint32_t s1) {
+        return base + ((uint64_t)(uint32_t)p * s0 + (uint64_t)(uint32_t)o * s1);
     };
     auto lds = [](uint8_t* p) { return (__attribute__((address_space(3))) void*)p; };
     auto rsrc = [](const void* p) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7FFFFFFF, 0x00027000); };
     int pg = 0;                                              // the page of the next tile to request; GEN: of the lane's key
+    // the next tile to request (AT_TILE): its addresses are made while the matrix cores are busy
+    const uint8_t *ak = nullptr, *av = nullptr;
+    const float *aks = nullptr, *avs = nullptr;
+    auto aim = [&](int tile) __attribute__((always_inline)) {
+        if constexpr (!GEN) {
+            const int j = key_of(tile);
+            if (tile >= nC || len - j < KT) return;          // uniform
+            const int p = known(pg), o = inside(j);
+            ak = at32(kh, p, o, kst[0], kst[1]);
+            av = at32(vh, p, o, vst[0], vst[1]);
+            aks = at32(ksh, p, o, sst[0], sst[1]);
+            avs = at32(vsh, p, o, sst[2], sst[3]);
+        }
+    };
     auto lookup = [&](int tile) {
         if (tile >= nC) return;                              // uniform
         const int j = key_of(tile);
@@ -263,7 +295,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     // lane numbers that the compiler does not know to be the same in every tile: what is made from them is not
     // kept in registers, nor spilled
     auto fresh = [&](int x) {
-        if constexpr (M * D > 384) asm volatile("" : "+v"(x));
+        if constexpr (M * D >= 384) asm volatile("" : "+v"(x));
         return (uint32_t)x;
     };
     // a cached tile, the lane's own addresses; its n keys, the last of them again behind it
@@ -293,23 +325,23 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
         if (tile < nC) {                                     // uniform
             const int j = key_of(tile), n = len - j < KT ? len - j : KT;
             const int pgl = pg;
-            lookup(tile + 1);
+            if constexpr (GEN) lookup(tile + 1);
             const uint32_t ln = fresh(lane), kq = ln / U;
             auto unit_at = [&](int i) { return ((ln % U) ^ a8_swz<D>((uint32_t)(i * KQ) + kq)) * 16; };   // of request i
             if (!GEN && n == KT) {                           // uniform
-                const int p = known(pgl), o = inside(j);
-                const auto rk = rsrc(at32(kh, p, o, P.kcs)), rv = rsrc(at32(vh, p, o, P.vcs));
-                const auto sk = rsrc(at32(ksh, p, o, P.kss)), sv = rsrc(at32(vsh, p, o, P.vss));
+                const auto rk = rsrc(ak), rv = rsrc(av), sk = rsrc(aks), sv = rsrc(avs);
+                uint32_t k1 = kst[1], v1 = vst[1];           // (not kept multiplied: a value spilled costs more)
+                asm volatile("" : "+s"(k1), "+s"(v1));
                 auto requests = [&](auto nt) {
                     constexpr int AUX = decltype(nt)::value;
 #pragma unroll
                     for (int i = 0; i < NQ; ++i)
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds(st + i * 1024), 16, (int)(kq * (uint32_t)P.kcs[1] + unit_at(i)), i * KQ * (int)P.kcs[1], 0, AUX);
-                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sk, lds(st + 2 * KT * D), 4, lane * (int)(4 * P.kss[1]), 0, 0, 0);
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds(st + i * 1024), 16, (int)(kq * k1 + unit_at(i)), i * KQ * (int)k1, 0, AUX);
+                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sk, lds(st + 2 * KT * D), 4, lane * (int)(4 * sst[1]), 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < NQ; ++i)
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds(st + KT * D + i * 1024), 16, (int)(kq * (uint32_t)P.vcs[1] + unit_at(i)), i * KQ * (int)P.vcs[1], 0, AUX);
-                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sv, lds(st + 2 * KT * D + KT * 4), 4, lane * (int)(4 * P.vss[1]), 0, 0, 0);
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds(st + KT * D + i * 1024), 16, (int)(kq * v1 + unit_at(i)), i * KQ * (int)v1, 0, AUX);
+                    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sv, lds(st + 2 * KT * D + KT * 4), 4, lane * (int)(4 * sst[3]), 0, 0, 0);
                 };
                 // values that one workgroup reads pass by L2; those of several row groups stay in it
                 if (P.RG == 1) requests(std::integral_constant<int, 2>{});   // uniform
@@ -330,13 +362,13 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
                     constexpr int AUX = decltype(nt)::value;
 #pragma unroll
                     for (int i = 0; i < NQ; ++i)
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(at32(kh, p[i], o[i], P.kcs)), lds(st + i * 1024), 16,
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(at32(kh, p[i], o[i], kst[0], kst[1])), lds(st + i * 1024), 16,
                             (int)(kq * (uint32_t)P.kcs[1] + unit_at(i)), 0, 0, AUX);
                     if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(ksh), lds(st + 2 * KT * D), 4,
                             (pl * (int)P.kss[0] + ol * (int)P.kss[1]) * 4, 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < NQ; ++i)
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(at32(vh, p[i], o[i], P.vcs)), lds(st + KT * D + i * 1024), 16,
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(at32(vh, p[i], o[i], vst[0], vst[1])), lds(st + KT * D + i * 1024), 16,
                             (int)(kq * (uint32_t)P.vcs[1] + unit_at(i)), 0, 0, AUX);
                     if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(vsh), lds(st + 2 * KT * D + KT * 4), 4,
                             (pl * (int)P.vss[0] + ol * (int)P.vss[1]) * 4, 0, 0, 0);
@@ -386,7 +418,12 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
         for (int s = 0; s < D / 32; ++s) qr[m][s] = *(const at_s8*)q_at(AQ, row0 + (QL + m) * 16 + (tq & 15), (s >> 1) * 64 + (tq >> 4 & 3) * 16 + (s & 1) * 8);
     asm volatile("" ::: "memory");
     lookup(0);
-    for (int e = 0; e < S - 1 && e < ntile; ++e) issue(e, ring + e * ST);
+    for (int e = 0; e < S - 1 && e < ntile; ++e) {
+        aim(e);
+        if constexpr (!GEN) lookup(e + 1);
+        issue(e, ring + e * ST);
+    }
+    aim(S - 1);
 #pragma unroll
     for (int e = 0; e < QI; ++e) {
         const int i = tq + e * 64 * NW, rw = i / U2;
@@ -419,10 +456,10 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[m][d] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // the sums' unit is a power of two that no scale so far exceeds (an infinite one but for)
+    // the sums' unit is a power of two that no scale so far exceeds (an infinite one but for); top: the lane's greatest
     auto unit_for = [&](float top) {
-        top = __builtin_fminf(top, 8.507059173023462e37f);   // 2^126
-        if (__any(top > vref)) {
+        if (__any(__builtin_fminf(top, 8.507059173023462e37f) > vref)) {   // 2^126
+            top = __builtin_fminf(a8_max4(top), 8.507059173023462e37f);
             const float nr = __uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u), a = vref / nr;
 #pragma unroll
             for (int m = 0; m < M; ++m)
@@ -435,21 +472,22 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     // The softmax of blocks of scores less mu, in place: x becomes the weights.
     auto softmax = [&](auto& x, auto blocks) {
         constexpr int BL = decltype(blocks)::value;
-        float mt[M];
+        float mt[M];                                         // of the lane's keys
         bool up = false;
 #pragma unroll
         for (int m = 0; m < M; ++m) {
             float a = a8_max(x[m][0][0], x[m][0][1], a8_max(x[m][0][2], x[m][0][3], x[m][0][3]));
 #pragma unroll
             for (int k = 1; k < BL; ++k) a = a8_max(x[m][k][0], x[m][k][1], a8_max(x[m][k][2], x[m][k][3], a));
-            mt[m] = a8_max4(a);
-            up |= mt[m] > most[m];
+            mt[m] = a;
+            up |= a > most[m];
         }
         if (__any(up)) {
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                const bool raise = mt[m] > most[m];
-                const float to = raise ? mu[m] + (mt[m] - (A8_MOST - A8_HEAD)) : mu[m], by = to - mu[m];
+                const float top = a8_max4(mt[m]);            // of the row's
+                const bool raise = top > most[m];
+                const float to = raise ? mu[m] + (top - (A8_MOST - A8_HEAD)) : mu[m], by = to - mu[m];
                 const float a = !raise ? 1.0f : most[m] > 0.0f ? __builtin_amdgcn_exp2f(-by) : 0.0f;
                 mu[m] = to;
                 most[m] = raise ? A8_MOST : most[m];
@@ -472,37 +510,50 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     };
     auto lds_at = [](const uint8_t* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p; };
     // A staged tile of n cached keys; K has landed, and V too unless there are requests of more tiles.
-    auto math8 = [&](const uint8_t* st, int n, bool more) __attribute__((always_inline)) {
+    auto math8 = [&](const uint8_t* st, int n, bool more, int next) __attribute__((always_inline)) {
         const uint32_t rr = fresh(r), gg = fresh(g), qb = qplace(rr, gg);
         a8_acc x[M][NB], ks[NB];
 #pragma unroll
-        for (int k = 0; k < NB; ++k) {
-            ks[k] = *(const a8_acc*)(st + 2 * KT * D + k * 64 + g * 16) * P.scale2;
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int m = 0; m < M; ++m) x[m][k] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        __builtin_amdgcn_s_setprio(1);                       // the wave with products to issue goes before the one in the softmax
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            llima_u32x4 kr[NB];
+            for (int k = 0; k < NB; ++k) x[m][k] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
+        // K's pieces of 64 columns, and Q's of 32, are read a step before their products (each waited for where it was
+        // read before: 16 nodes, 24 x 8192 tokens, 118 -> 113 us)
+        llima_u32x4 kr[2][NB];
+        at_s8 q[2][M];
+        auto kread = [&](int c) {
 #pragma unroll
             for (int k = 0; k < NB; ++k)
-                kr[k] = *(const llima_u32x4*)(st + k * 16 * D + ((rr * D + (gg ^ a8_swz<D>(rr)) * 16) ^ (uint32_t)(c * 64)));
+                kr[c & 1][k] = *(const llima_u32x4*)(st + k * 16 * D + ((rr * D + (gg ^ a8_swz<D>(rr)) * 16) ^ (uint32_t)(c * 64)));
+        };
+        auto qreads = [&](int s) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                at_s8 kf[NB];
+            for (int m = 0; m < M; ++m) q[s & 1][m] = qread(m, s, qb);
+        };
+        kread(0);
+        if (AHEAD) qreads(0);
 #pragma unroll
-                for (int k = 0; k < NB; ++k) kf[k] = a8_wide<DT>(kr[k][2 * s], kr[k][2 * s + 1]);
+        for (int k = 0; k < NB; ++k) ks[k] = *(const a8_acc*)(st + 2 * KT * D + k * 64 + g * 16);
+        __builtin_amdgcn_s_setprio(1);                       // the wave with products to issue goes before the one in the softmax
 #pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    const at_s8 q = qread(m, 2 * c + s, qb);
+        for (int s = 0; s < D / 32; ++s) {
+            if (!AHEAD) qreads(s);
+            if (s % 2 == 0 && s + 2 < D / 32) kread(s / 2 + 1);
+            if (AHEAD && s + 1 < D / 32) qreads(s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            at_s8 kf[NB];
 #pragma unroll
-                    for (int k = 0; k < NB; ++k) x[m][k] = a8_mfma<DT>(kf[k], q, x[m][k]);
-                }
-                __builtin_amdgcn_sched_barrier(0);           // (else the reads of Q come all at once)
-            }
+            for (int k = 0; k < NB; ++k) kf[k] = a8_wide<DT>(kr[s >> 1 & 1][k][2 * (s & 1)], kr[s >> 1 & 1][k][2 * (s & 1) + 1]);
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int k = 0; k < NB; ++k) x[m][k] = a8_mfma<DT>(kf[k], q[s & 1][m], x[m][k]);
+            if (s == 0) aim(next);
+            __builtin_amdgcn_sched_barrier(0);               // (else the reads of Q come all at once)
         }
         __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) ks[k] *= P.scale2;
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -519,15 +570,15 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
                     for (int m = 0; m < M; ++m) x[m][k][i] = in ? x[m][k][i] : -__builtin_inff();
                 }
         }
-        softmax(x, std::integral_constant<int, NB>{});
         if (more) a8_wait<(S - 1) * NR>();                   // uniform
         a8_acc vs[NB];
 #pragma unroll
         for (int k = 0; k < NB; ++k) vs[k] = *(const a8_acc*)(st + 2 * KT * D + KT * 4 + k * 64 + g * 16);
+        softmax(x, std::integral_constant<int, NB>{});
         float top = 0.0f;
 #pragma unroll
         for (int k = 0; k < NB; ++k) top = a8_max(vs[k][0], vs[k][1], a8_max(vs[k][2], vs[k][3], top));
-        unit_for(a8_max4(top));
+        unit_for(top);
 #pragma unroll
         for (int k = 0; k < NB; ++k) vs[k] *= vinv;
         uint32_t pw[M][2 * NB];
@@ -546,14 +597,14 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
             const uint32_t key = 4 * gg + (e & 3) + (e >> 2) * 16;
             const uint32_t base = KT * D + ((key * D + (rr & 1) * 8) | (a8_swz<D>(key) << 4)), at = lds_at(st);
 #pragma unroll
-            for (int d = 0; d < DB; d += 4) {
-                uint32_t a[4];
-                a8_i2 v[4];
+            for (int d = 0; d < DB; d += VG) {
+                uint32_t a[VG];
+                a8_i2 v[VG];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = at + (base ^ (uint32_t)((d + i) << 4));
+                for (int i = 0; i < VG; ++i) a[i] = at + (base ^ (uint32_t)((d + i) << 4));
                 a8_tr8(a, v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < VG; ++i) {
                     const at_s8 vf = a8_wide<LLIMA_F16>((uint32_t)v[i][0], (uint32_t)v[i][1]);
 #pragma unroll
                     for (int m = 0; m < M; ++m)
@@ -687,9 +738,10 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
         const int n = len - key_of(tile) < KT ? len - key_of(tile) : KT;
         // cached tiles behind this one have NR requests each, drafted ones fewer: then everything is waited for
         const bool more = ahead < nC;                        // uniform
+        if constexpr (!GEN) lookup(ahead + 1);
         if (more) a8_wait<(S - 1) * NR + NQ + 1>();
         else a8_wait<0>();
-        math8(st, n, more);
+        math8(st, n, more, ahead + 1);
         slot = slot + 1 < S ? slot + 1 : 0;
     }
     for (int tile = nC; tile < ntile; ++tile) {
