@@ -256,12 +256,14 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     const uint8_t* kh = (const uint8_t*)P.kc + own * P.kcs[0] + h * P.kcs[2];
     const uint8_t* vh = (const uint8_t*)P.vc + own * P.vcs[0] + h * P.vcs[2];
     const float *ksh = P.ksc + own * P.kss[0] + h * P.kss[2], *vsh = P.vsc + own * P.vss[0] + h * P.vss[2];
-    // what every tile's addresses are made from; hidden from the compiler, which else loads it anew for each tile, one
-    // wait after the other (a fifth of a tile's time with three row tiles; with `aim` 498 -> 470 us,
-    // 33 nodes over 4 x 131072 tokens)
+    // What every tile's addresses are made from; hidden from the compiler, which else loads it anew for each tile, one
+    // wait after the other: a fifth of a tile's time with three row tiles (with `aim`, 33 nodes over 4 x 131072 tokens 498
+    // -> 470 us).  One row tile waits for memory in any case, and starts sequences more often (64 of one token: hidden
+    // 143 us in a graph, not hidden 141).
+    constexpr bool HIDE = !GEN && M > 1;
     uint32_t kst[2] = {(uint32_t)P.kcs[0], (uint32_t)P.kcs[1]}, vst[2] = {(uint32_t)P.vcs[0], (uint32_t)P.vcs[1]};
     uint32_t sst[4] = {(uint32_t)P.kss[0], (uint32_t)P.kss[1], (uint32_t)P.vss[0], (uint32_t)P.vss[1]};
-    if constexpr (!GEN) {
+    if constexpr (HIDE) {
         asm volatile("" : "+s"(kh), "+s"(vh), "+s"(ksh), "+s"(vsh));
         asm volatile("" : "+s"(kst[0]), "+s"(kst[1]), "+s"(vst[0]), "+s"(vst[1]), "+s"(sst[0]), "+s"(sst[1]), "+s"(sst[2]), "+s"(sst[3]));
     }
@@ -331,7 +333,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
             if (!GEN && n == KT) {                           // uniform
                 const auto rk = rsrc(ak), rv = rsrc(av), sk = rsrc(aks), sv = rsrc(avs);
                 uint32_t k1 = kst[1], v1 = vst[1];           // (not kept multiplied: a value spilled costs more)
-                asm volatile("" : "+s"(k1), "+s"(v1));
+                if constexpr (HIDE) asm volatile("" : "+s"(k1), "+s"(v1));
                 auto requests = [&](auto nt) {
                     constexpr int AUX = decltype(nt)::value;
 #pragma unroll
