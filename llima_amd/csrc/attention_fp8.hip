@@ -166,11 +166,16 @@ template <int ROW> __device__ __forceinline__ uint32_t a8_swz(uint32_t key) {
 // One workgroup: four waves over one share of the keys, one key head and M row tiles of 16.
 // A wave's cached tile lies in one page (contiguous caches, pages of a multiple of its keys):
 // its address comes from the scalar unit; or each 1 KB request of it does (AT_REQUEST), or
-// every lane computes its own (AT_LANE).  GEN: the last two modes.
-template <int DT, int D, int M, bool GEN>
+// every lane computes its own (AT_LANE).  KIND: A8_ONE and A8_MANY for the first mode and one or
+// several row groups, A8_GEN for the last two.
+#define A8_ONE 0
+#define A8_MANY 1
+#define A8_GEN 2
+template <int DT, int D, int M, int KIND>
 __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #ifdef __HIP_DEVICE_COMPILE__                               // (the host pass drops the launch stub over the descriptors)
     using C = A8<D>;
+    constexpr bool GEN = KIND == A8_GEN;
     constexpr int NW = C::NW, KT = C::KT, DK = C::DK, S = C::S, ST = C::ST, T = C::T, TD = C::TD;
     constexpr int NB = KT / 16;                              // blocks of 16 keys
     constexpr int U = D / 16, U2 = D / 8;                    // 16-byte units of a cached and of a drafted row
@@ -345,9 +350,10 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
                         __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds(st + KT * D + i * 1024), 16, (int)(kq * v1 + unit_at(i)), i * KQ * (int)v1, 0, AUX);
                     if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(sv, lds(st + 2 * KT * D + KT * 4), 4, lane * (int)(4 * sst[3]), 0, 0, 0);
                 };
-                // values that one workgroup reads pass by L2; those of several row groups stay in it
-                if (P.RG == 1) requests(std::integral_constant<int, 2>{});   // uniform
-                else requests(std::integral_constant<int, 0>{});
+                // values that one workgroup reads pass by L2 (16 nodes, 24 x 8192 tokens: 114 -> 103 us), those of several
+                // row groups stay in it; as a branch here, its spilled descriptors cost 465 instead of 430 us (33 nodes
+                // over 4 x 131072)
+                requests(std::integral_constant<int, KIND == A8_ONE ? 2 : 0>{});
             } else if (GEN && P.mode == AT_REQUEST && n == KT) {   // uniform
                 int p[NQ], o[NQ];
 #pragma unroll
@@ -855,7 +861,14 @@ static void a8_launch(const At8Params& P, hipStream_t st) {
         constexpr int M = decltype(m)::value;
         const int64_t rows = (int64_t)P.B * P.N * P.Hq;
         const AttnParams& J = P;
-        hipLaunchKernelGGL((tree_attn8<DT, D, M, GEN>), dim3(((uint32_t)P.parts * P.Hkv + 7) / 8 * 8 * P.RG), dim3(64 * A8<D>::NW), 0, st, P);
+        auto go = [&](auto kind) {
+            constexpr int KIND = decltype(kind)::value;
+            hipLaunchKernelGGL((tree_attn8<DT, D, M, KIND>), dim3(((uint32_t)P.parts * P.Hkv + 7) / 8 * 8 * P.RG), dim3(64 * A8<D>::NW), 0, st, P);
+        };
+        if constexpr (GEN) go(std::integral_constant<int, A8_GEN>{});
+        else if constexpr (2 * M <= A8<D>::MAXM) go(std::integral_constant<int, A8_ONE>{});   // (several groups have more tiles each)
+        else if (P.RG == 1) go(std::integral_constant<int, A8_ONE>{});
+        else go(std::integral_constant<int, A8_MANY>{});
         if (rows <= 1024) hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 4>), dim3((uint32_t)rows), dim3(LLIMA_WG), 0, st, J);
         else hipLaunchKernelGGL((tree_attn_join<DT, D, Fp8Tiles<D>, 1>), dim3((uint32_t)((rows + 3) / 4)), dim3(LLIMA_WG), 0, st, J);
     });
