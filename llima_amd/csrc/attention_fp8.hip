@@ -202,7 +202,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     const int rg = (int)(turn % (uint32_t)P.RG), part = (int)(pair / (uint32_t)P.Hkv), h = (int)(pair % (uint32_t)P.Hkv);
     if (part >= P.parts) return;                             // (the grid is a multiple of 8)
     uint8_t* const ring = sm + wave * (S * ST);
-    bool bad = false, miss = false;
+    bool bad = false;
     const int len0 = lane < P.B ? at_len(P, lane, bad) : 0;
     const int64_t share = (int64_t)readfirstlane64((uint64_t)at_share<Fp8Tiles<D>>(P, len0));
     const int64_t end = (part + 1) * share;
@@ -240,6 +240,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     auto key_of = [&](int tile) { return (c0 + tile) * T + wave * KT; };         // a cached tile's first key
     auto draft_of = [&](int tile) { return (d0 + tile - nC) * TD + wave * DK; };   // a drafted tile's first token
     // ---------------------------------------------------------------- requests
+    bool miss = false;                                       // a page of this sequence that does not exist
     auto page_of = [&](int j) {                              // the page of key j (uniform), by the scalar unit
         const __attribute__((address_space(4))) int32_t* tab = (const __attribute__((address_space(4))) int32_t*)(P.table + b * P.ts);
         return tab[at_page(P.page_mul, P.page_shift, j)];
