@@ -114,7 +114,7 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
     const int len = P.lens[b], cnt = P.counts ? P.counts[b] : P.L;
     bool ok = len >= 0 && cnt >= 0 && cnt <= P.L && len <= P.cap && (int64_t)len + cnt <= P.cap;
     const int j0 = c * P.tok, j1 = j0 + P.tok < cnt ? j0 + P.tok : cnt;
-    const int rows = (j1 - j0) * P.Hkv, u = t % U;           // 0 and less: nothing of this workgroup's
+    const int rows = j0 < cnt ? (j1 - j0) * P.Hkv : 0, u = t % U;   // (behind the count the product may pass 32 bits)
     llima_u32x4 y[2][F];
     uint32_t h[F], p[F], o[F];                               // head, page and place in it (a wait for a load behind
     auto load = [&](int i0) {                                // a store is one for the store, so these come first too)
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(LLIMA_WG) void cache_write8(CacheParams P) {
         ok = __syncthreads_and(all);
     }
     if (c == 0 && layer == 0 && t == 0) P.new_lens[b] = ok ? len + cnt : LLIMA_E_RANGE;
-    if (!ok || rows <= 0) return;                            // uniform
+    if (!ok || rows == 0) return;                            // uniform
     for (int i0 = t / U;;) {
 #pragma unroll
         for (int f = 0; f < F; ++f) {
