@@ -627,8 +627,9 @@ int llima_tree_commit(const llima_tree_commit_args* args, void* stream);
 /* llima_tree_attention over such a cache: the same outputs for k_j = q_j scale_j of the
  * cached tokens (a key's scale multiplies its score, a value's scale its weight, in
  * fp32); the drafted tokens' own k and v are of dtype.  For its product with a cached
- * value a weight times the value's scale is rounded to fp16, for either dtype, in a unit
- * of the largest scale so far. */
+ * value a weight times the value's scale is rounded to fp16, for either dtype: by 2^-11
+ * of itself, or by 2^-32 of its row's greatest such product where that is more (scales
+ * below 2^-93 count as that much here). */
 typedef struct llima_tree_attention_fp8_args {
     llima_tree_attention_args a;         /* k_cache, v_cache and their strides: bytes */
     const float *k_scales, *v_scales;

@@ -16,13 +16,15 @@
 // its row group, so that a value is read from memory, from LDS and converted once, and no
 // wave waits for another before the end of a sequence's part, where their sums are joined.
 //
-// What a row's scores are taken less moves only when a weight would pass 2^15, and then so
-// far that the greatest is 2^7: the sums are rescaled seldom, and a score's product with its
-// key's scale and the difference are one operation.  For the product with V a weight times its
-// value's scale is rounded to fp16 whatever q's type (11 bits; in bf16 the outputs' error
-// against 64 bits was 0.0023 of their size, now 0.0017, that of the output's own rounding); it
-// carries the inverse of the largest scale so far (a power of two), so that it neither
-// overflows nor, down to 2^-29 of the largest, becomes subnormal.
+// For the product with V a weight times its value's scale is rounded to fp16 whatever q's type
+// (11 bits; in bf16 the outputs' error against 64 bits was 0.0023 of their size with weights in bf16, now
+// 0.0017, that of the output's own rounding).  What a row's scores are taken less goes by these products, not
+// by the weights: it moves only when one would pass 2^15, and then so far that the row's greatest is 2^7 (the
+// sums are rescaled seldom, and a score's product with its key's scale and the difference are one
+// operation).  So a product is rounded by its own size down to 2^-21 of its row's greatest, whatever the scales
+// of keys that weigh nothing there, and by 2^-32 of the greatest below.  The weights alone, which
+// are summed, run from 2^-120 to 2^100.  A lane's greatest score and greatest scale tell that nothing moves; the
+// logarithms of single scales are taken only where they do not.
 // The drafted tokens' values are of q's type, and so are their weights.
 //
 // Bound: up to one row tile (16 rows per key head) reading the cache's D + 4 bytes per key and
@@ -61,8 +63,10 @@ template <int D> struct A8 {
     static constexpr int QL = D == 256 ? 1 : D == 128 ? 3 : 4;   // of them in LDS at most (two workgroups per CU), the rest in registers
 };
 
-#define A8_MOST 15.0f                                        // the logarithm of the greatest weight, base 2
+#define A8_MOST 15.0f                                        // the logarithm of a row's greatest weight times scale, base 2
 #define A8_HEAD 8.0f                                         // where it is passed, the row's maximum comes this much below it
+#define A8_UNIT 8                                            // scales enter times 2^8 (that of the greatest bf16 value is 2^119)
+#define A8_LEAST -85.0f                                      // and count as 2^-93 at least, so that weights without them stay below 2^100
 
 // The partition's unit: tiles of T cached keys, then tiles of TD drafted ones.
 template <int D>
@@ -117,6 +121,12 @@ template <int DT> __device__ __forceinline__ at_s8 a8_wide(uint32_t lo, uint32_t
 __device__ __forceinline__ float a8_max(float a, float b, float c) {
     float d;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
+__device__ __forceinline__ float a8_max_abs(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
     return d;
 }
 
@@ -454,9 +464,9 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     auto qplace = [&](uint32_t rr, uint32_t gg) { return rr * 2 * D + ((2 * gg) ^ a8_swz<2 * D>(rr)) * 16; };
     // ---------------------------------------------------------------- products
     a8_acc o[M][DB];
-    // mu: what a row's scores (base 2) are taken less; a score less mu is its weight's logarithm, at most `most`,
-    // which is -inf for a row that has seen nothing yet
-    float mu[M], most[M], l[M], vref = 0.0f, vinv = 0.0f;    // the unit of the sums over 2^15, and its inverse
+    // mu: what a row's scores (base 2) are taken less; a score less mu is its weight's logarithm, which with the logarithm of
+    // the value's scale is at most `most`: -inf for a row that has seen nothing yet
+    float mu[M], most[M], l[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
         mu[m] = l[m] = 0.0f;
@@ -464,44 +474,36 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[m][d] = (a8_acc){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // the sums' unit is a power of two that no scale so far exceeds (an infinite one but for); top: the lane's greatest
-    auto unit_for = [&](float top) {
-        if (__any(__builtin_fminf(top, 8.507059173023462e37f) > vref)) {   // 2^126
-            top = __builtin_fminf(a8_max4(top), 8.507059173023462e37f);
-            const float nr = __uint_as_float((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u), a = vref / nr;
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[m][d] *= a;
-            vref = nr;
-            vinv = 1.0f / nr;
-        }
-    };
-    // The softmax of blocks of scores less mu, in place: x becomes the weights.
-    auto softmax = [&](auto& x, auto blocks) {
+    // The softmax of blocks of scores less mu, in place: x becomes the weights.  logs(k, i): the logarithm of what a key's
+    // weight is multiplied by; bound: no less than that of any of the lane's keys.
+    auto softmax = [&](auto& x, auto blocks, float bound, auto logs) {
         constexpr int BL = decltype(blocks)::value;
-        float mt[M];                                         // of the lane's keys
         bool up = false;
 #pragma unroll
         for (int m = 0; m < M; ++m) {
             float a = a8_max(x[m][0][0], x[m][0][1], a8_max(x[m][0][2], x[m][0][3], x[m][0][3]));
 #pragma unroll
             for (int k = 1; k < BL; ++k) a = a8_max(x[m][k][0], x[m][k][1], a8_max(x[m][k][2], x[m][k][3], a));
-            mt[m] = a;
-            up |= a > most[m];
+            up |= a > most[m] - bound;
         }
         if (__any(up)) {
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                const float top = a8_max4(mt[m]);            // of the row's
+                float a0 = -__builtin_inff();
+#pragma unroll
+                for (int k = 0; k < BL; ++k)
+                    a0 = a8_max(x[m][k][0] + logs(k, 0), x[m][k][1] + logs(k, 1), a8_max(x[m][k][2] + logs(k, 2), x[m][k][3] + logs(k, 3), a0));
+                const float top = a8_max4(a0);               // of the row's
                 const bool raise = top > most[m];
+                if (!__any(raise)) continue;                 // (more often than not the bound alone was passed: 455 -> 447 us, 33 nodes over 4 x 131072 tokens)
                 const float to = raise ? mu[m] + (top - (A8_MOST - A8_HEAD)) : mu[m], by = to - mu[m];
-                const float a = !raise ? 1.0f : most[m] > 0.0f ? __builtin_amdgcn_exp2f(-by) : 0.0f;
+                // (half of it, twice: a sum of weights without their scales may be 2^230 above what is added to it next)
+                const float a = !raise ? 1.0f : most[m] > 0.0f ? __builtin_amdgcn_exp2f(-0.5f * by) : 0.0f;
                 mu[m] = to;
                 most[m] = raise ? A8_MOST : most[m];
-                l[m] *= a;
+                l[m] = l[m] * a * a;
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[m][d] *= a;
+                for (int d = 0; d < DB; ++d) o[m][d] *= a * a;
 #pragma unroll
                 for (int k = 0; k < BL; ++k) x[m][k] -= by;
             }
@@ -582,13 +584,15 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
         a8_acc vs[NB];
 #pragma unroll
         for (int k = 0; k < NB; ++k) vs[k] = *(const a8_acc*)(st + 2 * KT * D + KT * 4 + k * 64 + g * 16);
-        softmax(x, std::integral_constant<int, NB>{});
         float top = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NB; ++k) top = a8_max(vs[k][0], vs[k][1], a8_max(vs[k][2], vs[k][3], top));
-        unit_for(top);
-#pragma unroll
-        for (int k = 0; k < NB; ++k) vs[k] *= vinv;
+        for (int k = 0; k < NB; ++k) {
+            vs[k] *= (float)(1 << A8_UNIT);
+            top = a8_max_abs(vs[k][0], vs[k][1], a8_max_abs(vs[k][2], vs[k][3], top));
+        }
+        // (an infinite scale's logarithm is 127, its bound 129)
+        softmax(x, std::integral_constant<int, NB>{}, __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_logf(top) + 0.001f, A8_LEAST), 129.0f),
+                [&](int k, int i) { return __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_logf(__builtin_fabsf(vs[k][i])), A8_LEAST), 127.0f); });
         uint32_t pw[M][2 * NB];
 #pragma unroll
         for (int m = 0; m < M; ++m)
@@ -713,12 +717,13 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
         for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[m][0][i] = sees[m] >> i & 1 ? __builtin_fmaf(x[m][0][i], P.scale2, -mu[m]) : -__builtin_inff();
-        softmax(x, std::integral_constant<int, 1>{});
-        unit_for(DT == LLIMA_BF16 ? 32768.0f : 1.0f);        // weights in units that keep a product with any value of the type finite
+        // bf16: weights of at most 2^-11, which keep the sum of 1024 products with any values of the type finite
+        constexpr float LG = DT == LLIMA_BF16 ? A8_UNIT + A8_MOST + 11.0f : A8_UNIT;
+        softmax(x, std::integral_constant<int, 1>{}, LG, [](int, int) { return LG; });
         at_s4 pf[M];
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            const a8_acc y = x[m][0] * vinv;
+            const a8_acc y = x[m][0] * (float)(1 << A8_UNIT);
             pf[m] = __builtin_bit_cast(at_s4, (a8_i2){(int)at_pack<DT>(y[0], y[1]), (int)at_pack<DT>(y[2], y[3])});
         }
         // a transposing load takes 4 rows of 32 bytes from 16 lanes (row i / 4 of lane i, 8 bytes i % 4)
@@ -767,8 +772,13 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
     float2* const ml = (float2*)(sm + XN * XB);              // [wave][row]
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-        l[m] = a8_sum4(l[m]) * 3.0517578125e-5f;             // 2^-15
-        if (g == 0) ml[wave * M * 16 + m * 16 + r] = make_float2(most[m] > 0.0f ? mu[m] : -__builtin_inff(), l[m]);
+        // the sum's exponent goes into mu: sums of other waves and parts may have had far smaller or larger scales; sums of
+        // less than 2^-11, which keep those of four waves in 512 parts times any values finite
+        const float sum = a8_sum4(l[m]);
+        const int e = __builtin_amdgcn_frexp_expf(sum) + 11; // (of 0, infinities and NaN: 0)
+        mu[m] += (float)e;
+        l[m] = __int_as_float(-e - A8_UNIT);                 // the exponent of what o is multiplied by
+        if (g == 0) ml[wave * M * 16 + m * 16 + r] = make_float2(most[m] > 0.0f ? mu[m] : -__builtin_inff(), __builtin_amdgcn_ldexpf(sum, -e));
     }
     __syncthreads();
     const At8Args A = a8_args();
@@ -786,7 +796,7 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
         const float zero = top > -__builtin_inff() ? top : 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) sum += x[w].y * __builtin_amdgcn_exp2f(x[w].x - zero);
-        const float a = (most[m] > 0.0f ? __builtin_amdgcn_exp2f(mu[m] - zero) : 0.0f) * (vref * 3.0517578125e-5f);
+        const float a = __builtin_amdgcn_ldexpf(most[m] > 0.0f ? __builtin_amdgcn_exp2f(mu[m] - zero) : 0.0f, __float_as_int(l[m]));
         uint8_t* const xb = sm + (XN == 2 ? (m & 1) * XB : 0);
         if (XN == 1 && m > 0) __syncthreads();
 #pragma unroll
