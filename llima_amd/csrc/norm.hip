@@ -7,7 +7,8 @@
 //         m = max(max |y|, 2^-100),  scale = m / 448,  q = e4m3(448 y / m)
 //
 // The mean is summed in 64 bits and f rounded once from it, y is three fp32
-// products, and 448 y / m one product and one IEEE division: every step is a
+// products, and 448 y / m one product and the IEEE division's quotient (as
+// Q8Divisor takes it: 8192 x 5760 bf16 rows 31 -> 25 us): every step is a
 // defined operation, so the outputs do not depend on how a row is spread over
 // lanes (a sum of 16-bit squares is exact in 64 bits but for the last place),
 // and a tie of the 8-bit rounding stays one.  Rounding to 8 bits is what the
