@@ -250,6 +250,8 @@ def _attend_checks(q, k, v, k_cache, v_cache, cache_lens, mask, block_table, k8,
         raise ValueError("the head size must be 64, 128 or 256")
     if N == 0 or N > 1024 or Hkv == 0 or Hq == 0 or Hq % Hkv or Hq > 1024:
         raise ValueError("1 to 1024 drafted tokens and query heads, a multiple of the key heads, are supported")
+    if B * N * Hq >= 1 << 26:
+        raise ValueError("fewer than 2^26 rows (sequences, drafted tokens and query heads) are supported")
     _on_gpu(q, k, v, k_cache, v_cache, cache_lens, mask, block_table)
     dev = q.device
     if not (k.device == v.device == k_cache.device == v_cache.device == dev):
