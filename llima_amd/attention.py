@@ -74,12 +74,14 @@ class Fp8Cache:
 
 def _heads(t: torch.Tensor, align: int = 8) -> torch.Tensor:
     """[..., D] that 16-byte accesses can read: D adjacent, the other strides multiples
-    of 8 (of 16 for bytes) and not negative, 16-byte aligned (copied when it is not)."""
-    if t.is_contiguous() and t.shape[-1] % align == 0 and t.data_ptr() % 16 == 0:
-        return t
+    of 8 (of 16 for bytes) and not negative, 16-byte aligned (copied when it is not).  The
+    stride of a dimension of one, which may be any number also where is_contiguous() holds, becomes 0."""
     st = t.stride()
     if st[-1] == 1 and t.data_ptr() % 16 == 0:
-        if not any([s % align for s in st[:-1]]):
+        bits = 0
+        for n in st[:-1]:                                    # align is a power of two
+            bits |= n
+        if not bits % align:
             return t
         if not any([s % align and n > 1 for s, n in zip(st[:-1], t.shape[:-1])]):
             return t.as_strided(t.shape, [0 if n <= 1 else s for s, n in zip(st[:-1], t.shape[:-1])] + [1])
