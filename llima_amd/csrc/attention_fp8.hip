@@ -495,7 +495,9 @@ __global__ __launch_bounds__((64 * A8<D>::NW), 2) void tree_attn8(At8Params P) {
                     a0 = a8_max(x[m][k][0] + logs(k, 0), x[m][k][1] + logs(k, 1), a8_max(x[m][k][2] + logs(k, 2), x[m][k][3] + logs(k, 3), a0));
                 const float top = a8_max4(a0);               // of the row's
                 const bool raise = top > most[m];
-                if (!__any(raise)) continue;                 // (more often than not the bound alone was passed: 455 -> 447 us, 33 nodes over 4 x 131072 tokens)
+                // (more often than not the bound alone was passed: 455 -> 447 us, 33 nodes over 4 x 131072 tokens; with one row
+                // tile, pages of 16: 85 -> 94, 24 x 8192)
+                if (M > 1 && !__any(raise)) continue;
                 const float to = raise ? mu[m] + (top - (A8_MOST - A8_HEAD)) : mu[m], by = to - mu[m];
                 // (half of it, twice: a sum of weights without their scales may be 2^230 above what is added to it next)
                 const float a = !raise ? 1.0f : most[m] > 0.0f ? __builtin_amdgcn_exp2f(-0.5f * by) : 0.0f;
