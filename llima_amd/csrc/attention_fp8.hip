@@ -30,9 +30,9 @@
 // Bound: up to one row tile (16 rows per key head) reading the cache's D + 4 bytes per key and
 // value once.  64 sequences of one token, 755 MB: 117-126 us, 6.0-6.4 TB/s (requests into LDS alone
 // reach 5.6 TB/s, 6.2 where they pass by L2).  From three row tiles on the issue: a tile of 32 keys takes
-// a wave 335 vector operations with 48 matrix ones and 64 that widen K and V among them, and 129 scalar ones
-// (33 nodes of 4 heads over 4 x 131072 tokens, 1.1 GB: 430-450 us; the vector units busy 68 % of the time, the
-// matrix cores 36 %; requests alone 287).  16 nodes over 24 x up to 16384: 72 us, the memory's 50.  Short calls
+// a wave 340 vector operations with 48 matrix ones and 64 that widen K and V among them, and 129 scalar ones
+// (33 nodes of 4 heads over 4 x 131072 tokens, 1.1 GB: 440-453 us; the vector units busy 67 % of the time, the
+// matrix cores 35 %; requests alone 287).  16 nodes over 24 x up to 16384: 72 us, the memory's 50.  Short calls
 // are a chain of latencies (1 x 1000 tokens: 8.7 us and 4.1 of the join).
 //
 // Why four waves with tiles of their own: waves that share a tile convert it once each or pass it on
