@@ -649,7 +649,8 @@ int llima_tree_attention_fp8(const llima_tree_attention_fp8_args* args, void* wo
  *   k, v [layers][B][N][Hkv][D] of dtype LLIMA_BF16 or LLIMA_F16, D 64, 128 or 256
  * A sequence that llima_tree_commit leaves out is left out here, with the same new
  * length; nothing else of the cache is written; the same buffers may not overlap.
- * Hkv at most 1024, page_size * max_blocks and L at most 2^30. */
+ * Hkv at most 1024, page_size * max_blocks and L at most 2^30, B L below 2^24 (above that
+ * as far as a launch holds it: a workgroup takes several tokens where heads are few). */
 typedef struct llima_cache_write_fp8_args {
     const void *k, *v;
     void *k_cache, *v_cache;
